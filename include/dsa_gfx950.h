@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 10
+#define DSA_ABI_VERSION 11
 
 #define DSA_OK 0
 #define DSA_EINVAL (-1)      /* a null pointer or a size out of range */
@@ -421,6 +421,50 @@ int dsa_pool_keys_write(const void* rows, int rows_fp8, const float* rows_scale,
                         const int32_t* positions, const int32_t* page_table, int table_shared, int table_pages,
                         const int64_t* slot_mapping, void* pool_key, int n_rows, int kp, int page_size,
                         long long num_slots, void* stream);
+
+/*
+ * Pages of the paged caches (no counterpart among the reference's kernels: its page pool and prefix caches are host
+ * code, trnrt/engine/kv_pool.py:1-50, and its caches are copied by the framework). A page pool is a use count per page,
+ * ref int32 [num_pages] (0 or less: free; page 0, the null page, is never given out, counted or moved), page tables
+ * [rows, max_pages], and the caches that the tables index: caches (a host array of n_caches device pointers; any
+ * number) with page_bytes (a host array: each cache's bytes per page, num_pages of them). One call moves a page of
+ * every cache. Page ids outside [0, num_pages) read the null page. Every choice is in ascending order, so results do not
+ * vary from run to run. Calls that share a pool must not overlap. Nothing is returned to the host: a pool without enough
+ * free pages shows in `pages`.
+ *
+ * dsa_pages_copy: page src[i] -> page dst[i] of every cache, i < n (int32 [n] each). A pair with an id outside the pool,
+ * with dst the null page or with src == dst is skipped. No dst may be a src or another's dst (their bytes would be
+ * unspecified).
+ *
+ * dsa_pages_fork: n new sequences, child i of table row parents[i] (int32 [n], rows of page_table [B, max_pages] with
+ * ctx_len int32 [B] tokens, clamped to the table): the parent's floor(len / page_size) full pages are shared (their
+ * counts rise by one), a partial last page is copied into the lowest free page (whose count becomes one), and
+ * child_table [n, max_pages] gets the row (0 past its pages). pages int32 [n]: the child's new page, 0 where it needs
+ * none, -1 where there was none left, or parents[i] is no row: such a child's row is 0 and counts nothing. The pages of
+ * the parents' rows must be counted in ref, and no output may overlap an input.
+ *
+ * dsa_pages_release: every row i < n of page_table gives up its ceil(ctx_len[i] / page_size) pages: their counts fall by
+ * one, never below 0 (a row given twice is released twice).
+ *
+ * dsa_pages_compact: the L pages in use (ref > 0) moved to pages 1 .. L: those there already stay, the k-th one past L
+ * goes to the k-th free page up to L, in every cache. new_ref [num_pages] and new_table [B, max_pages] are ref and
+ * page_table in the new places (an entry of a free page becomes 0), remap int32 [num_pages] each page's new place (0: a
+ * free page), for whatever else holds page ids. The outputs must not be the inputs; pages past L keep their bytes.
+ *
+ * workspace: dsa_pages_workspace_bytes(num_pages, n) (n: the children of a fork; no zero fill needed).
+ */
+size_t dsa_pages_workspace_bytes(int num_pages, int n);
+int dsa_pages_copy(void* const* caches, const long long* page_bytes, int n_caches, const int32_t* src,
+                   const int32_t* dst, int n, int num_pages, void* stream);
+int dsa_pages_fork(int32_t* ref, const int32_t* page_table, const int32_t* ctx_len, const int32_t* parents,
+                   int32_t* child_table, int32_t* pages, void* const* caches, const long long* page_bytes,
+                   int n_caches, void* workspace, size_t workspace_bytes, int B, int n, int max_pages, int page_size,
+                   int num_pages, void* stream);
+int dsa_pages_release(int32_t* ref, const int32_t* page_table, const int32_t* ctx_len, int n, int max_pages,
+                      int page_size, int num_pages, void* stream);
+int dsa_pages_compact(const int32_t* ref, const int32_t* page_table, int32_t* new_ref, int32_t* new_table,
+                      int32_t* remap, void* const* caches, const long long* page_bytes, int n_caches, void* workspace,
+                      size_t workspace_bytes, int B, int max_pages, int num_pages, void* stream);
 
 /*
  * Bytes of workspace an entry point needs. kind: DSA_WS_TOPK (B, max_len, keep), DSA_WS_ATTENTION (B, H, keep,

@@ -30,7 +30,7 @@ DSA_WS_TOPK = 1
 DSA_WS_ATTENTION = 2
 DSA_WS_LAYER = 3
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 P = c_void_p
 # Every entry point of include/dsa_gfx950.h with its ctypes signature (restype, argtypes).
@@ -109,6 +109,11 @@ SIGNATURES: dict[str, tuple] = {
         [P, P, P, P, P, P, P, P, P, P, P, c_size_t, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, P],
     ),
     "dsa_prefill_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "dsa_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "dsa_pages_copy": (c_int, [P, P, c_int, P, P, c_int, c_int, P]),
+    "dsa_pages_fork": (c_int, [P, P, P, P, P, P, P, P, c_int, P, c_size_t, c_int, c_int, c_int, c_int, c_int, P]),
+    "dsa_pages_release": (c_int, [P, P, P, c_int, c_int, c_int, c_int, P]),
+    "dsa_pages_compact": (c_int, [P, P, P, P, P, P, P, c_int, P, c_size_t, c_int, c_int, c_int, P]),
     "dsa_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
     "dsa_default_splits": (c_int, [c_int, c_int, c_int]),
     "dsa_layer_status": (c_int, [P, P, P, c_int, P]),

@@ -113,6 +113,20 @@ hipError_t launch_compact_slots(const int* rows, const float* bias, int B, int N
 hipError_t launch_value_order(const int64_t* pools, const int64_t* cnt, const float* vals, int N, int keep,
                               int64_t* out_pools, float* out_vals, hipStream_t s);
 
+size_t pages_fork_bytes(int n);
+size_t pages_compact_bytes(int num_pages);
+bool pages_units_ok(const long long* page_bytes, int n_caches, long n);
+hipError_t launch_pages_copy(void* const* caches, const long long* page_bytes, int n_caches, const int* src,
+                             const int* dst, int n, int num_pages, hipStream_t s);
+hipError_t launch_pages_fork(int* ref, const int* table, const int* ctx_len, const int* parents, int* child,
+                             int* pages, void* const* caches, const long long* page_bytes, int n_caches, void* ws,
+                             int B, int n, int max_pages, int page_size, int num_pages, hipStream_t s);
+hipError_t launch_pages_release(int* ref, const int* table, const int* ctx_len, int n, int max_pages, int page_size,
+                                int num_pages, hipStream_t s);
+hipError_t launch_pages_compact(const int* ref, const int* table, int* new_ref, int* new_table, int* remap,
+                                void* const* caches, const long long* page_bytes, int n_caches, void* ws,
+                                long table_size, int num_pages, int num_cu, hipStream_t s);
+
 thread_local KernelTimer* g_kernel_timer = nullptr;
 }  // namespace dsa
 
@@ -1249,3 +1263,72 @@ static int pooled_layer(const void* q_idx_bf16, const float* w, const void* pool
                                        static_cast<char*>(workspace) + t_need, B, H, Dqk, keep_sel, max_pages,
                                        page_size, num_pages, scale, plan.splits, s, pf, plan.wide));
 }
+
+// -- pages of the caches -------------------------------------------------------------------------------------------
+
+// DSA_OK where every cache is given with a page of at least a byte.
+static int page_caches_status(void* const* caches, const long long* page_bytes, int n_caches, long n) {
+  if (n_caches < 0 || (n_caches > 0 && (!caches || !page_bytes))) return DSA_EINVAL;
+  for (int i = 0; i < n_caches; ++i)
+    if (!caches[i] || page_bytes[i] < 1) return DSA_EINVAL;
+  return dsa::pages_units_ok(page_bytes, n_caches, n) ? DSA_OK : DSA_EUNSUPPORTED;
+}
+
+extern "C" {
+
+size_t dsa_pages_workspace_bytes(int num_pages, int n) {
+  if (num_pages < 1 || n < 0) return 0;
+  const size_t f = dsa::pages_fork_bytes(n), c = dsa::pages_compact_bytes(num_pages);
+  return align256(f > c ? f : c);
+}
+
+int dsa_pages_copy(void* const* caches, const long long* page_bytes, int n_caches, const int32_t* src,
+                   const int32_t* dst, int n, int num_pages, void* stream) {
+  if (n < 0 || num_pages < 1) return DSA_EINVAL;
+  const int st = page_caches_status(caches, page_bytes, n_caches, n);
+  if (st != DSA_OK || n == 0 || n_caches == 0) return st;
+  if (!src || !dst) return DSA_EINVAL;
+  return status(dsa::launch_pages_copy(caches, page_bytes, n_caches, src, dst, n, num_pages,
+                                       static_cast<hipStream_t>(stream)));
+}
+
+int dsa_pages_fork(int32_t* ref, const int32_t* page_table, const int32_t* ctx_len, const int32_t* parents,
+                   int32_t* child_table, int32_t* pages, void* const* caches, const long long* page_bytes,
+                   int n_caches, void* workspace, size_t workspace_bytes, int B, int n, int max_pages, int page_size,
+                   int num_pages, void* stream) {
+  if (B < 0 || n < 0 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
+  const int st = page_caches_status(caches, page_bytes, n_caches, n);
+  if (st != DSA_OK || n == 0) return st;
+  if (!ref || !page_table || !ctx_len || !parents || !child_table || !pages) return DSA_EINVAL;
+  if (!workspace || workspace_bytes < dsa::pages_fork_bytes(n)) return DSA_EWORKSPACE;
+  return status(dsa::launch_pages_fork(ref, page_table, ctx_len, parents, child_table, pages, caches, page_bytes,
+                                       n_caches, workspace, B, n, max_pages, page_size, num_pages,
+                                       static_cast<hipStream_t>(stream)));
+}
+
+int dsa_pages_release(int32_t* ref, const int32_t* page_table, const int32_t* ctx_len, int n, int max_pages,
+                      int page_size, int num_pages, void* stream) {
+  if (n < 0 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
+  if (n == 0) return DSA_OK;
+  if (!ref || !page_table || !ctx_len) return DSA_EINVAL;
+  if (n > 0xffffff) return DSA_EUNSUPPORTED;
+  return status(dsa::launch_pages_release(ref, page_table, ctx_len, n, max_pages, page_size, num_pages,
+                                          static_cast<hipStream_t>(stream)));
+}
+
+int dsa_pages_compact(const int32_t* ref, const int32_t* page_table, int32_t* new_ref, int32_t* new_table,
+                      int32_t* remap, void* const* caches, const long long* page_bytes, int n_caches, void* workspace,
+                      size_t workspace_bytes, int B, int max_pages, int num_pages, void* stream) {
+  if (B < 0 || max_pages < 1 || num_pages < 1) return DSA_EINVAL;
+  const int st = page_caches_status(caches, page_bytes, n_caches, 1);
+  if (st != DSA_OK) return st;
+  if (!ref || !new_ref || !remap || (B > 0 && (!page_table || !new_table))) return DSA_EINVAL;
+  if (ref == new_ref || (B > 0 && page_table == new_table)) return DSA_EINVAL;  // read after the first are written
+  if (num_pages > 0x1fffffff) return DSA_EUNSUPPORTED;
+  if (!workspace || workspace_bytes < dsa::pages_compact_bytes(num_pages)) return DSA_EWORKSPACE;
+  return status(dsa::launch_pages_compact(ref, page_table, new_ref, new_table, remap, caches, page_bytes, n_caches,
+                                          workspace, (long)B * max_pages, num_pages, num_cu(),
+                                          static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"

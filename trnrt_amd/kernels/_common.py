@@ -32,6 +32,15 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def call(device: torch.device, fn, *args) -> int:
+    """fn(*args, stream): a C entry point on device's current stream, with device the current one (a launch goes to the
+    current device, whichever the tensors are on)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return fn(*args, stream_ptr(device))
+    with torch.cuda.device(device):
+        return fn(*args, stream_ptr(device))
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
