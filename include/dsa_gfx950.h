@@ -423,6 +423,26 @@ int dsa_pool_keys_write(const void* rows, int rows_fp8, const float* rows_scale,
                         long long num_slots, void* stream);
 
 /*
+ * Absorbed latent attention over every cached token (the reference's `attention` below its selection's reach,
+ * trnrt/models/mla.py:420-482, with the arithmetic of trnrt/kernels/dsa_decode.py:26-43): a decode batch, or S new
+ * tokens a sequence (a speculative step, a short append), causal. For sequence b, query i < S and head h, over the
+ * tokens t < n = ctx_len[b] - S + i + 1 (ctx_len counts the new tokens, whose rows are in the cache):
+ *   K[t] = kv_fp8[slot(b, t)] * kv_scale[slot(b, t)], V[t] = K[t][:512]
+ *   s[t] = scale * q[b, i, h, :] . K[t],  p = softmax_t(s),  out[b, i, h, :] = sum_t p[t] V[t],  lse = log sum_t exp(s[t])
+ * n <= 0: out 0, lse NEG_INF (-1e30).
+ *   q bf16 [B, S, H, Dqk], Dqk 576 (512 latent + 64 rope) or 512 (NoPE); any H; kv_fp8 uint8 e4m3fn [num_pages *
+ *   page_size, Dqk], kv_scale fp32 per slot or null (every scale 1); page_table int32 [B, max_pages], any page_size;
+ *   ctx_len int32 [B] (clamped to [0, max_pages * page_size]); out_bf16 [B, S, H, 512] and / or out_f32 (either may be
+ *   null), lse fp32 [B, S, H] or null. Only slots of tokens t < ctx_len[b] are read.
+ *   workspace: dsa_dense_workspace_bytes(S, H) bytes whatever B (no zero fill needed).
+ */
+size_t dsa_dense_workspace_bytes(int S, int H);
+int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table,
+                  const int32_t* ctx_len, void* out_bf16, float* out_f32, float* lse, void* workspace,
+                  size_t workspace_bytes, int B, int S, int H, int Dqk, int max_pages, int page_size, int num_pages,
+                  float scale, void* stream);
+
+/*
  * Pages of the paged caches (no counterpart among the reference's kernels: its page pool and prefix caches are host
  * code, trnrt/engine/kv_pool.py:1-50, and its caches are copied by the framework). A page pool is a use count per page,
  * ref int32 [num_pages] (0 or less: free; page 0, the null page, is never given out, counted or moved), page tables

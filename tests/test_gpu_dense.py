@@ -1,0 +1,213 @@
+"""Absorbed latent attention without a selection (trnrt_amd/kernels/dsa_dense.py) against the definition in float64, with
+the caches' unused slots full of NaN.
+
+Tolerances, from the arithmetic: the kernel rounds each softmax weight (times its token's scale) to bf16, off by at most
+2^-8 of it, so an output by at most 2^-8 of A = sum_t p[t] |V[t]|; a bf16 output is rounded once more, 2^-8 of its size;
+scores are fp32 sums of D products, off by less than D 2^-24 sum |q K| (E below, their largest over the tokens), which moves
+weights by that much relative, and the log-sum-exp by that much, plus the roundings of the exponential and the logarithm
+(a few 2^-23 each, and 2^-23 of the maximum)."""
+
+import pytest
+import torch
+
+from tests._helpers import say
+from trnrt_amd.kernels import dsa_decode, dsa_dense
+
+pytestmark = pytest.mark.gpu
+FP8 = torch.float8_e4m3fn
+
+
+def make(lens, S, H, D, ps, seed, q_gain=1.0, scaled=True, spread=0.5):
+    """CPU inputs: pages in random order, every slot that holds no token NaN."""
+    g = torch.Generator().manual_seed(seed)
+    B = len(lens)
+    npg = [-(-n // ps) for n in lens]
+    mp = max(max(npg), 1) + 1
+    pages = 1 + sum(npg)
+    table = torch.full((B, mp), -7, dtype=torch.int32)  # entries past a row's pages are not read
+    perm = (torch.randperm(pages - 1, generator=g) + 1).to(torch.int32)
+    kv = torch.full((pages * ps, D), 0x7F, dtype=torch.uint8)
+    sc = torch.full((pages * ps,), float("nan"))
+    at = 0
+    for b, n in enumerate(lens):
+        table[b, :npg[b]] = perm[at:at + npg[b]]
+        at += npg[b]
+        t = torch.arange(n)
+        slot = table[b][t // ps].long() * ps + t % ps
+        x = torch.randn(n, D, generator=g) * torch.exp(spread * torch.randn(n, 1, generator=g))
+        s = x.abs().amax(-1).clamp(min=1e-30) / 448 if n else torch.ones(0)
+        kv[slot] = (x / s[:, None]).clamp(-448, 448).to(FP8).view(torch.uint8)
+        sc[slot] = s
+    q = (torch.randn(B, S, H, D, generator=g) * q_gain).to(torch.bfloat16)
+    return q, kv, sc if scaled else None, table, torch.tensor(lens, dtype=torch.int32)
+
+
+def reference(q, kv, sc, table, lens, ps, scale):
+    """(out, lse, A, E) in float64 on the GPU's float64 units."""
+    B, S, H, D = q.shape
+    dev = "cuda"
+    out = torch.zeros(B, S, H, 512, dtype=torch.float64)
+    lse = torch.full((B, S, H), -1e30, dtype=torch.float64)
+    A, E = torch.zeros_like(out), torch.zeros(B, S, H, dtype=torch.float64)
+    for b in range(B):
+        n = min(max(int(lens[b]), 0), table.shape[1] * ps)
+        t = torch.arange(n)
+        slot = table[b][t // ps].long() * ps + t % ps
+        K = kv[slot].view(FP8).to(torch.float64).to(dev)
+        if sc is not None:
+            K = K * sc[slot].to(torch.float64).to(dev)[:, None]
+        for i in range(S):
+            m = n - S + i + 1
+            if m <= 0:
+                continue
+            x = q[b, i].to(torch.float64).to(dev)
+            s = x @ K[:m].T.contiguous() * scale
+            w = torch.softmax(s, -1)
+            out[b, i] = (w @ K[:m, :512].contiguous()).cpu()
+            A[b, i] = (w @ K[:m, :512].abs().contiguous()).cpu()
+            lse[b, i] = torch.logsumexp(s, -1).cpu()
+            E[b, i] = (x.abs() @ K[:m].abs().T.contiguous()).amax(-1).cpu() * scale * D * 2.0 ** -24
+    return out, lse, A, E
+
+
+def check(inp, ps, scale=192 ** -0.5, out_dtype=torch.bfloat16, squeeze=False):
+    q, kv, sc, table, lens = inp
+    ref, lref, A, E = reference(q, kv, sc, table, lens, ps, scale)
+    g = [None if x is None else x.cuda() for x in (q[:, 0] if squeeze else q, kv, sc, table, lens)]
+    out, lse = dsa_dense.attend(*g, ps, scale, out_dtype=out_dtype)
+    assert out.dtype == out_dtype
+    out, lse = out.double().cpu().view(ref.shape), lse.double().cpu().view(lref.shape)
+    rel = 2.0 ** -8 + 2 * E[..., None] + 2.0 ** -20
+    tol = A * rel + (2.0 ** -8 * (ref.abs() + A * rel) if out_dtype == torch.bfloat16 else 0) + 1e-30
+    bad = ~((out - ref).abs() <= tol)
+    assert not bad.any(), f"{int(bad.sum())} outputs off, the worst {float(((out - ref).abs() / tol).max())} of the tolerance"
+    ltol = E + 2.0 ** -21 + 2.0 ** -22 * lref.abs()
+    bad = ~((lse - lref).abs() <= ltol)
+    assert not bad.any(), f"lse off by {float(((lse - lref).abs() / ltol).max())} of the tolerance"
+    return out, lse
+
+
+@pytest.mark.parametrize("D", [576, 512])
+@pytest.mark.parametrize("H,S", [(16, 1), (64, 1), (1, 1), (24, 1), (128, 1), (16, 4), (40, 3), (8, 7)])
+def test_heads_and_new_tokens(H, S, D):
+    say("dense", H, S, D)
+    check(make([300, 1, 64, 65, 63, 0, 129, 777], S, H, D, 64, seed=H + S), 64)
+
+
+@pytest.mark.parametrize("ps", [1, 16, 33, 48, 128, 1000])
+def test_page_sizes(ps):
+    say("dense pages of", ps)
+    check(make([500, 31, 2], 2, 20, 576, ps, seed=ps), ps)
+
+
+def test_one_new_token_without_its_dimension():
+    say("dense [B, H, D]")
+    check(make([100, 200], 1, 32, 512, 64, seed=1), 64, squeeze=True)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("scaled", [True, False])
+def test_unscaled_cache_and_fp32_outputs(scaled, out_dtype):
+    say("dense scaled", scaled, out_dtype)
+    inp = make([700, 90], 1, 64, 576, 64, seed=3, scaled=scaled, q_gain=1.0 if scaled else 0.01)
+    check(inp, 64, out_dtype=out_dtype)
+
+
+@pytest.mark.parametrize("gain", [0.0, 8.0, 40.0])
+def test_flat_and_steep_softmax(gain):
+    """All weights alike; maxima that move far between chunks; rows whose scores all lie far below zero."""
+    say("dense gain", gain)
+    inp = make([1500, 640, 70], 1, 48, 576, 64, seed=5, q_gain=gain)
+    check(inp, 64)
+    q, kv, sc, table, lens = inp
+    kv[:] = torch.where(kv == 0x7F, kv, 0x38)  # every value 1: scores - |q| scale
+    check((-q.abs(), kv, sc, table, lens), 64)
+
+
+@pytest.mark.parametrize("H", [16, 64])
+def test_long_and_ragged(H):
+    """Row tiles shared by many workgroups, several tiles in one workgroup, sequences without tokens between."""
+    say("dense long", H)
+    check(make([40000, 0, 3, 0, 0, 9000, 128, 20001], 1, H, 576, 64, seed=H), 64)
+
+
+def test_many_short_sequences():
+    say("dense 1,100 sequences")
+    g = torch.Generator().manual_seed(0)
+    lens = torch.randint(0, 130, (1100,), generator=g).tolist()
+    check(make(lens, 1, 16, 512, 16, seed=2), 16)
+
+
+def test_all_empty_and_no_sequence():
+    say("dense empty")
+    out, lse = check(make([0, 0, 0], 2, 16, 576, 64, seed=2), 64)
+    assert not out.any() and (lse.float() == -1e30).all()  # (as fp32, which has no -1e30 exactly)
+    q, kv, sc, table, lens = (x.cuda() for x in make([4], 1, 16, 576, 64, seed=2))
+    o, l = dsa_dense.attend(q[:0], kv, sc, table[:0], lens[:0], 64, 0.1)
+    assert o.shape == (0, 1, 16, 512) and l.shape == (0, 1, 16)
+
+
+def test_lengths_past_the_table_and_foreign_pages():
+    """A length past the table is the table's; a page id outside the cache reads the null page."""
+    say("dense clamps")
+    q, kv, sc, table, lens = make([200, 128], 1, 16, 576, 64, seed=9)
+    table[0, 4], lens[0] = 0, 10 ** 9  # five pages, the last the null page
+    table[1, 1] = 10 ** 6
+    kv[:64], sc[:64] = 0x30, 0.5
+    want = table.clone()
+    want[1, 1] = 0
+    kv[table[0, 3].long() * 64 + 8:table[0, 3].long() * 64 + 64] = 0x28
+    sc[table[0, 3].long() * 64 + 8:table[0, 3].long() * 64 + 64] = 0.25
+    ref, lref, A, _ = reference(q, kv, sc, want, lens, 64, 0.07)
+    out, lse = dsa_dense.attend(q.cuda(), kv.cuda(), sc.cuda(), table.cuda(), lens.cuda(), 64, 0.07)
+    assert ((out.double().cpu() - ref).abs() <= 2.0 ** -7 * A + 1e-6).all()
+    assert (lse.double().cpu() - lref).abs().max() < 1e-4
+
+
+def test_selecting_every_token_agrees():
+    """dsa_decode.attend_tokens over all positions is the same attention: both within two weight roundings of it."""
+    say("dense against the selected form")
+    q, kv, sc, table, lens = (x.cuda() for x in make([1000, 512, 77], 1, 64, 576, 64, seed=4))
+    idx = torch.arange(1000, dtype=torch.int32, device="cuda").repeat(3, 1)
+    out, lse = dsa_dense.attend(q[:, 0], kv, sc, table, lens, 64, 192 ** -0.5)
+    o2, l2 = dsa_decode.attend_tokens(q[:, 0].contiguous(), kv, sc, idx, lens, table, 64, 192 ** -0.5)
+    torch.testing.assert_close(out.float(), o2.float(), atol=2e-2, rtol=2e-2)
+    torch.testing.assert_close(lse, l2, atol=1e-5, rtol=1e-6)
+
+
+def test_graph_replays_and_another_stream():
+    say("dense in a graph, on another stream")
+    inps = [make([900, 64, 1300], 2, 16, 576, 64, seed=30 + i) for i in range(3)]
+    q, kv, sc, table, lens = (x.cuda() for x in inps[0])
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        eager = dsa_dense.attend(q, kv, sc, table, lens, 64, 0.07, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = dsa_dense.attend(q, kv, sc, table, lens, 64, 0.07, workspace=ws)
+    for i in (0, 1, 2):
+        for a, b in zip((q, kv, sc, table, lens), inps[i]):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = dsa_dense.attend(q, kv, sc, table, lens, 64, 0.07)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        if i == 0:
+            assert torch.equal(out, eager[0])
+
+
+def test_refusals():
+    q, kv, sc, table, lens = (x.cuda() for x in make([100, 5], 1, 16, 576, 64, seed=0))
+    ok = dict(q=q, kv_cache=kv, kv_scale=sc, table=table, ctx_len=lens, page_size=64, scale=0.1)
+    for bad in (dict(q=q[..., :500]), dict(q=q[0, 0]), dict(page_size=60), dict(page_size=0), dict(kv_scale=sc[:-1]),
+                dict(table=table[:1]), dict(table=table[0]), dict(ctx_len=lens[:1]), dict(kv_cache=kv.float()),
+                dict(kv_cache=kv.t()), dict(out=torch.empty(2, 1, 16, 500, device="cuda")),
+                dict(out=torch.empty(2, 1, 16, 512, dtype=torch.float16, device="cuda")),
+                dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))):
+        with pytest.raises(ValueError):
+            dsa_dense.attend(**{**ok, **bad})
+    with pytest.raises(RuntimeError, match="GPU only"):
+        dsa_dense.attend(**{**ok, "q": q.cpu()})

@@ -113,6 +113,11 @@ hipError_t launch_compact_slots(const int* rows, const float* bias, int B, int N
 hipError_t launch_value_order(const int64_t* pools, const int64_t* cnt, const float* vals, int N, int keep,
                               int64_t* out_pools, float* out_vals, hipStream_t s);
 
+size_t dense_workspace_bytes(int M, int num_cu);
+hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* kvs, const int* table,
+                            const int* ctx_len, uint16_t* out, float* out_f32, float* lse, void* ws, int B, int S,
+                            int H, int Dqk, int max_pages, int page_size, int num_pages, float scale, int num_cu,
+                            hipStream_t s);
 size_t pages_fork_bytes(int n);
 size_t pages_compact_bytes(int num_pages);
 bool pages_units_ok(const long long* page_bytes, int n_caches, long n);
@@ -1263,6 +1268,34 @@ static int pooled_layer(const void* q_idx_bf16, const float* w, const void* pool
                                        static_cast<char*>(workspace) + t_need, B, H, Dqk, keep_sel, max_pages,
                                        page_size, num_pages, scale, plan.splits, s, pf, plan.wide));
 }
+
+// -- latent attention without a selection ---------------------------------------------------------------------------
+
+extern "C" {
+
+size_t dsa_dense_workspace_bytes(int S, int H) {
+  if (S < 1 || H < 1 || (long)S * H > 0x7fffffffL) return 0;
+  return align256(dsa::dense_workspace_bytes(S * H, num_cu()));
+}
+
+int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table,
+                  const int32_t* ctx_len, void* out_bf16, float* out_f32, float* lse, void* workspace,
+                  size_t workspace_bytes, int B, int S, int H, int Dqk, int max_pages, int page_size, int num_pages,
+                  float scale, void* stream) {
+  if (B < 0 || S < 1 || H < 1 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
+  if (Dqk != 512 && Dqk != 576) return DSA_EUNSUPPORTED;
+  // a cache of less than 2^31 slots; rows within a launch's 2^32 threads
+  if ((long)num_pages * page_size > 0x7fffffffL || (long)B * S > 0x7fffffffL / H / 128) return DSA_EUNSUPPORTED;
+  if (B == 0) return DSA_OK;
+  if (!q_bf16 || !kv_fp8 || !page_table || !ctx_len || (!out_bf16 && !out_f32)) return DSA_EINVAL;
+  if (!workspace || workspace_bytes < dsa::dense_workspace_bytes(S * H, num_cu())) return DSA_EWORKSPACE;
+  return status(dsa::launch_dense_mla(static_cast<const uint16_t*>(q_bf16), kv_fp8, kv_scale, page_table, ctx_len,
+                                      static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, S, H, Dqk,
+                                      max_pages, page_size, num_pages, scale, num_cu(),
+                                      static_cast<hipStream_t>(stream)));
+}
+
+}  // extern "C"
 
 // -- pages of the caches -------------------------------------------------------------------------------------------
 

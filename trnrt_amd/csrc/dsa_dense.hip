@@ -1,0 +1,595 @@
+// Absorbed latent attention over every cached token of a paged FP8 latent cache for gfx950: decode rows and the S new
+// tokens of a speculative step, with no selection (the arithmetic of dsa_attention.hip, whose slots are chosen).
+//
+//   s[r, t] = scale x sigma_t x (q_r . c_t),  p = softmax_t(s),  out_r = sum_t p sigma_t c_t[:512],  lse
+//
+// for the M = S x H rows r (query, head) of a sequence over its tokens t: e4m3 rows c_t with a scale sigma_t.
+//
+// What bounds it: a token is 580 bytes for 2 x M x 1,088 FLOP, so up to about 64 rows the cache's stream through HBM is the
+// bound, above it the matrix units. One workgroup a CU has a tile of 32 or 64 rows of one sequence and a range of its
+// chunks of 64 tokens; its 8 waves have two kinds of work, one of each on every SIMD, a chunk apart, with one barrier a
+// chunk (products of one kind run under the other's conversions and exponentials):
+//   - scoring waves 0-3, interval c: chunk c's scores S^T = K . Q^T, 32 tokens x 32 rows a wave, the queries in registers,
+//     then P = 2^(s - m) x the tokens' scales in bf16 into LDS;
+//   - value waves 4-7, interval c: chunk c - 1's O^T += V^T . P, 128 dims of all rows a wave, in registers, and the loads
+//     of a later chunk: asynchronous 16-byte loads straight into LDS, which wait for nothing until their chunk's turn.
+// Both products are v_mfma_f32_32x32x16_bf16 with the e4m3 operand converted on the way (exact). The chunks of all
+// sequences and row tiles form one list that the workgroups share evenly, whatever the lengths: each takes a stretch of it
+// and writes a row tile's outputs where it holds all its chunks, else a partial (the rows x 512 in fp32, their maxima and
+// sums) that dense_combine_kernel joins. Neighbouring stretches lie on one XCD, so that the row tiles of a sequence read its
+// cache through the same L2.
+// The online softmax rescales lazily without waiting for the chunk's maximum: P is taken against the running maximum as it
+// stands; a wave that meets a score past its slack raises a flag, and before the chunk's values are multiplied every wave
+// sees the flags and, when one is up, the maxima are exchanged, P is taken again and O rescaled (a stretch's chunk 0 always
+// does, with O still zero).
+#include "dsa_common.h"
+
+namespace dsa {
+
+constexpr int DN_DV = 512;
+constexpr int DN_CHUNK = 64;
+constexpr int DN_THREADS = 512;
+constexpr float DN_SLACK = 11.5f;      // lazy rescaling (base 2): p = 2^(s - m) <= 2^11.5 between moves of m
+constexpr float DN_LOG2E = 1.44269504088896341f;
+constexpr float DN_LOG2E_LO = (float)(1.44269504088896341 - (double)DN_LOG2E);
+constexpr int DN_PROW = DN_CHUNK + 8;  // P row stride (bf16)
+constexpr int DN_KAHEAD = 3;           // score steps whose key reads are in flight
+constexpr int DN_VAHEAD = 3;           // value steps whose operand reads are in flight
+
+typedef int dn_v2i __attribute__((ext_vector_type(2)));
+
+// A chunk's LDS layout: the rows' first 512 bytes at r x 512, 16-byte piece p of row r (token) at p ^ (r & 7); then, of
+// 576-byte rows, the last 64 at r x 64, piece p at p ^ ((r >> 1) & 3). With it the reads of one piece of 8 consecutive rows
+// (key operand, and value operand, read transposed) cover the 32 banks once.
+__device__ __forceinline__ int dn_swizzle(int r) { return r & 7; }
+
+// RB: blocks of 32 rows in a tile. Buffers: chunk c being scored, c - 1 whose values are multiplied, and the rest arriving.
+template <int DQK, int RB>
+struct DnShared {
+  static constexpr int BUFS = RB == 1 ? 4 : 3;  // (160 KiB of LDS)
+  alignas(1024) uint8_t tile[BUFS][DN_CHUNK * DQK];
+  alignas(16) uint16_t p[2][32 * RB * DN_PROW];  // P[row][token] of two chunks
+  alignas(16) float ksc[BUFS][DN_CHUNK];         // the chunks' token scales
+  alignas(16) float kfac[BUFS][DN_CHUNK];        // x softmax scale x log2 e
+  float cmax[2][32 * RB];                        // [token half][row]: a chunk's maxima when one moves
+  float al[32 * RB];                             // and its rescale factors
+  alignas(16) int flag[2][4];                    // per chunk parity and wave: a score past the running maximum's slack
+  float lsum[2][32 * RB];                        // [token half][row]: a stretch's sums
+  float mfin[32 * RB];                           // and maxima (base 2)
+  int tot[DN_THREADS / WAVE];
+  int found[3];
+};
+
+// t / page_size for 0 <= t < 2^31: t x mul >> shift (mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size)).
+struct DnPage {
+  uint32_t mul;
+  int shift;
+  int size;
+};
+
+// Every wave of the workgroup, whichever its role: LDS accesses before it are visible after it; global loads stay in
+// flight.
+__device__ __forceinline__ void dn_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A sequence's tokens and chunks of them.
+__device__ __forceinline__ int dn_len(int ctx_len, int max_pages, int page_size) {
+  const long cap = (long)max_pages * page_size;
+  return (int)min(max((long)ctx_len, 0L), min(cap, 0x7fffff00L));
+}
+__device__ __forceinline__ int dn_chunks(int len) { return (len + DN_CHUNK - 1) / DN_CHUNK; }
+
+// The inclusive prefix sum of v over the workgroup's THREADS threads and its total.
+template <int THREADS>
+__device__ __forceinline__ int dn_scan(int v, int* tot, int& total) {
+  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+  const int x = wave_incl_scan(v);
+  __syncthreads();
+  if (lane == WAVE - 1) tot[wave] = x;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / WAVE; ++w) {
+    const int s = tot[w];
+    before += w < wave ? s : 0;
+    total += s;
+  }
+  return before + x;
+}
+
+// The number of units (sequence, row tile, chunk of tokens). Every thread of the workgroup calls this.
+template <int THREADS>
+__device__ __forceinline__ long dn_total(const int* __restrict__ ctx_len, int B, int tiles, int max_pages,
+                                         int page_size, int* tot) {
+  long units = 0;
+  for (int b0 = 0; b0 < B; b0 += THREADS) {
+    const int b = b0 + (int)threadIdx.x;
+    int total;
+    dn_scan<THREADS>(b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, page_size)) : 0, tot, total);
+    units += (long)total * tiles;
+  }
+  return units;
+}
+
+// The first unit of workgroup w of G, and the workgroup that has unit u.
+__device__ __forceinline__ long dn_start(long w, long units, int G) { return w * units / G; }
+__device__ __forceinline__ long dn_owner(long u, long units, int G) { return ((u + 1) * G - 1) / units; }
+
+template <int DQK, int RB>
+__global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
+    const uint16_t* __restrict__ q, const uint8_t* __restrict__ kv, const float* __restrict__ kvs,
+    const int* __restrict__ table, const int* __restrict__ ctx_len, uint16_t* __restrict__ out,
+    float* __restrict__ out_f32, float* __restrict__ lse_out, float* __restrict__ ws_o, float* __restrict__ ws_ml,
+    int B, int S, int H, int max_pages, DnPage pg, int num_pages, float scale) {
+  typedef DnShared<DQK, RB> Sh;
+  constexpr int ROWS = 32 * RB, BUFS = Sh::BUFS;
+  constexpr int STEPS = DQK / 32;           // 32 dims: one 16-byte read of a key row per lane, two products
+  constexpr int TAIL = DN_CHUNK * 512;      // where the rows' last 64 bytes lie
+  constexpr int LOADS = DQK == 576 ? 9 : 8;  // a chunk's asynchronous loads per value wave
+  __shared__ Sh sh;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int j = lane & 31, h = lane >> 5;
+  const int M = S * H, tiles = (M + ROWS - 1) / ROWS;
+  const int G = gridDim.x;
+  const int wg = (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3);  // (workgroup x runs on XCD x % 8; G a multiple of 8)
+
+  const long units = dn_total<DN_THREADS>(ctx_len, B, tiles, max_pages, pg.size, sh.tot);
+  const long u0 = dn_start(wg, units, G), u1 = dn_start(wg + 1, units, G);
+  if (u0 >= u1) return;
+  {  // the sequence of unit u0
+    long before = 0;
+    for (int b0 = 0; b0 < B; b0 += DN_THREADS) {
+      const int b = b0 + tid;
+      const int n = b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, pg.size)) : 0;
+      int total;
+      const int incl = dn_scan<DN_THREADS>(n, sh.tot, total);
+      const long lo = (before + incl - n) * tiles, hi = (before + incl) * tiles;
+      if (lo <= u0 && u0 < hi) {
+        sh.found[0] = b;
+        sh.found[1] = (int)((u0 - lo) / n);
+        sh.found[2] = (int)((u0 - lo) % n);
+      }
+      before += total;
+      if (u0 < before * tiles) break;
+    }
+    if (tid < 8) sh.flag[tid >> 2][tid & 3] = 0;
+    __syncthreads();
+  }
+  // scale x log2 e to twice fp32's digits: rounded, its error would be the same for every score, and so the lse's
+  const float sl2 = scale * DN_LOG2E, sl2_lo = fmaf(scale, DN_LOG2E, -sl2) + scale * DN_LOG2E_LO;
+  // the stretch at hand: chunks c0 .. of row tile mt of sequence b
+  int b = __builtin_amdgcn_readfirstlane(sh.found[0]), mt = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
+
+  for (long u = u0; u < u1;) {
+    const int len = dn_len(ctx_len[b], max_pages, pg.size), all = dn_chunks(len);
+    const int nch = (int)min((long)(all - c0), u1 - u);  // this stretch's chunks
+    const bool whole = nch == all;
+    const int t0 = c0 * DN_CHUNK, r0 = mt * ROWS;  // its first token and row
+
+    // the outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x & 7)), so that a
+    // row's pieces in order and a piece's rows in order both cover the banks once; a wave writes whole rows
+    f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
+    auto write = [&](int half) __attribute__((always_inline)) {
+      const size_t slot = 2 * (size_t)wg + (u > u0);
+      const int dim = 256 * half + 4 * lane;
+#pragma unroll 1
+      for (int r = wave; r < ROWS && r0 + r < M; r += DN_THREADS / WAVE) {
+        f32x4 v = area[64 * lane + (r ^ (lane & 7))];
+        const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
+        if (whole) {
+          const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= inv;
+          const size_t at = (size_t)b * M + r0 + r;
+          if (out)
+            *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+          if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
+          if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+        } else {
+          *reinterpret_cast<f32x4*>(ws_o + (slot * ROWS + r) * DN_DV + dim) = v;
+          if (half == 0 && lane == 0) {
+            ws_ml[2 * (slot * ROWS + r)] = m;
+            ws_ml[2 * (slot * ROWS + r) + 1] = l;
+          }
+        }
+      }
+    };
+
+    if (wave < 4) {
+      // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
+      const int th = wave >> 1, hh = wave & 1;
+      const bool works = hh < RB;
+      const int row = min(r0 + 32 * (works ? hh : 0) + j, M - 1);
+      const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
+      const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
+      bf16x8 qb[2 * STEPS];  // row 32 hh + j: step s holds dims 32 s + 16 h .. + 15
+      if (works) {
+        const uint16_t* qr = q + ((size_t)b * M + row) * DQK + 16 * h;
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          qb[2 * s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s));
+          qb[2 * s + 1] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s + 8));
+        }
+      }
+      dn_barrier();  // chunk 0 is in place
+      float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
+                           // always up
+      float l_run = 0.0f;  // this lane's share of its running sum
+      float psum = 0.0f;   // and of the last chunk's, not yet in l_run
+      f32x16 sv = {};      // the last chunk's scores - m_run: row 32 hh + j, tokens 32 th + 8 (r / 4) + 4 h + r % 4
+      const int kr = 32 * th + j;
+      int koff[4], ktail[2];  // byte offsets of a row's pieces in a chunk (they repeat after 4 steps of 32 dims)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) koff[i] = kr * 512 + 16 * ((2 * i | h) ^ dn_swizzle(kr));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) ktail[i] = TAIL + kr * 64 + 16 * ((2 * i | h) ^ ((kr >> 1) & 3));
+      uint16_t* const pw = &sh.p[0][(32 * (works ? hh : 0) + j) * DN_PROW + 32 * th + 4 * h];
+      int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
+      auto four = [&](const float* a, int g) __attribute__((always_inline)) {
+        return *reinterpret_cast<const f32x4*>(a + 32 * th + 8 * g + 4 * h);
+      };
+      // four tokens (group g of the lane's 16) of P from their scores and scales
+      auto p_group = [&](int c, int g, const f32x4& ks) __attribute__((always_inline)) {
+        float pv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[4 * g + e]);
+        psum += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+        // (bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded)
+        *reinterpret_cast<uint2*>(pw + (c & 1) * ROWS * DN_PROW + 8 * g) =
+            make_uint2(bf16_pack(pv[0] * ks[0], pv[1] * ks[1]), bf16_pack(pv[2] * ks[2], pv[3] * ks[3]));
+      };
+      // a chunk whose flags (fl) are up: its maxima over both token halves, the moved running maxima, P again
+      auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
+        if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+          float cm = sv[0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) cm = max_nonan(cm, sv[r]);
+          cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
+          if (works && h == 0) sh.cmax[th][32 * hh + j] = cm;
+          dn_barrier();
+          cm = max_nonan(cm, sh.cmax[th ^ 1][32 * (works ? hh : 0) + j]);
+          // a row that sees none of chunk 0 sees none of the stretch: its maximum stays finite
+          const float up = c == 0 ? max_nonan(cm, -1e30f) : cm > DN_SLACK ? cm : 0.0f;
+          // chunk 0 has nothing to rescale, and its factor would be infinite where every score is at or below -128
+          const float alpha = c == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+          m_run += up;
+          l_run *= alpha;
+          psum = 0.0f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sv[r] -= up;
+          if (works) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
+            if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
+          }
+          dn_barrier();
+        }
+        l_run += psum;
+        psum = 0.0f;
+      };
+      auto flags = [&](int c) __attribute__((always_inline)) { return *reinterpret_cast<const int4*>(sh.flag[c & 1]); };
+      __builtin_amdgcn_s_setprio(1);  // these waves bound the interval: their products go before the value products
+      for (int c = 0; c < nch; ++c) {
+        const uint8_t* tile = sh.tile[buf];
+        auto k_read = [&](int s) __attribute__((always_inline)) {
+          return *reinterpret_cast<const u32x4*>(tile + (s < 16 ? koff[s & 3] + 128 * (s >> 2) : ktail[s & 1]));
+        };
+        int4 fl = make_int4(0, 0, 0, 0);
+        if (c > 0) fl = flags(c - 1);
+        f32x16 sa = {};
+        u32x4 kk[DN_KAHEAD + 1];
+        bf16x8 ka[2], kb[2];
+        f32x4 ks[2], kx[2];
+#pragma unroll
+        for (int s = 0; s < DN_KAHEAD; ++s) kk[s] = k_read(s);
+        __builtin_amdgcn_sched_barrier(0);
+        settle(c - 1, fl);
+        if (works) {
+          ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
+          kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
+#pragma unroll
+          for (int s = 0; s < STEPS; ++s) {
+            if (s + DN_KAHEAD < STEPS) kk[(s + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(s + DN_KAHEAD);
+            sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[s & 1], qb[2 * s], sa, 0, 0, 0);
+            sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[s & 1], qb[2 * s + 1], sa, 0, 0, 0);
+            if (s + 1 < STEPS) {
+              const u32x4 k1 = kk[(s + 1) % (DN_KAHEAD + 1)];
+              ka[(s + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
+              kb[(s + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
+            }
+            if (s == STEPS - 2) {
+              ks[0] = four(sh.ksc[buf], 0);
+              kx[0] = four(sh.kfac[buf], 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (g < 3) kx[(g + 1) & 1] = four(sh.kfac[buf], g + 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sv[4 * g + e] = fmaf(sa[4 * g + e], kx[g & 1][e], -m_run);
+          }
+          if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
+            const int lim = seen - t0 - c * DN_CHUNK - 32 * th - 4 * h;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sv[4 * g + e] = 8 * g + e < lim ? sv[4 * g + e] : -INFINITY;
+          }
+          float cm = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            if (g < 3) ks[(g + 1) & 1] = four(sh.ksc[buf], g + 1);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) cm = max_nonan(cm, sv[4 * g + e]);
+            p_group(c, g, ks[g & 1]);
+          }
+          const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
+          if (lane == 0) sh.flag[c & 1][wave] = any;
+        }
+        last = buf;
+        buf = buf == BUFS - 1 ? 0 : buf + 1;
+        dn_barrier();
+      }
+      __builtin_amdgcn_s_setprio(0);
+      settle(nch - 1, flags(nch - 1));
+      const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
+      if (works && h == 0) sh.lsum[th][32 * hh + j] = lw;
+      if (works && th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
+      dn_barrier();  // the tiles are free
+      dn_barrier();  // the first 256 dims' outputs are in LDS
+      write(0);
+      dn_barrier();
+      dn_barrier();  // and the others'
+      write(1);
+    } else {
+      // -- the loads and the values: wave w brings rows 16 w .. + 15 of a chunk, takes dims 128 w .. + 127 of all rows --
+      const int w = wave - 4;
+      const int* trow = table + (size_t)b * max_pages;
+      // token `lane` of chunk c, the sequence's last one past its end (a slot behind it may never have been written, and
+      // its NaN x weight 0 is NaN)
+      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + lane, len - 1); };
+      auto page_of = [&](int t) __attribute__((always_inline)) { return (int)((uint64_t)t * pg.mul >> pg.shift); };
+      const int mrow = 4 * (16 * w + h), trw = 4 * (16 * w + (lane >> 2));
+      int mcol[4];  // load k < 8 brings rows 16 w + 2 k and + 1, load 8 the last pieces of all 16
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mcol[k] = 16 * (j ^ dn_swizzle(2 * k | h));
+      const int tcol = 512 + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
+      int page = trow[page_of(token(0))];  // of this lane's token in the chunk to bring next
+      auto issue = [&](int c, int to) __attribute__((always_inline)) {  // chunk c's loads into buffer `to`
+        const int t = token(c);
+        const int slot = safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
+        page = trow[page_of(token(c + 1))];
+        uint8_t* dst = sh.tile[to] + 16 * w * 512;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(mrow + 8 * k, slot);
+          __builtin_amdgcn_global_load_lds(kv + (size_t)s * DQK + mcol[k & 3],
+                                           (__attribute__((address_space(3))) void*)(dst + 1024 * k), 16, 0, 0);
+        }
+        if (DQK == 576) {
+          const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(trw, slot);
+          __builtin_amdgcn_global_load_lds(kv + (size_t)s * DQK + tcol,
+                                           (__attribute__((address_space(3))) void*)(sh.tile[to] + TAIL + 1024 * w),
+                                           16, 0, 0);
+        }
+        if (kvs)  // (every value wave the same: so that their loads count alike)
+          __builtin_amdgcn_global_load_lds(kvs + slot, (__attribute__((address_space(3))) void*)sh.ksc[to], 4, 0, 0);
+        else
+          sh.ksc[to][lane] = 1.0f;
+      };
+      constexpr int AHEAD = BUFS - 2;  // chunks in flight
+      // chunk `to`'s loads have landed, with at most AHEAD - 1 chunks' younger than them out (more: so many are; only the
+      // rows' loads are counted: a count too low only waits longer); then the tokens' factors
+      auto landed = [&](int to, bool more) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (more)
+          __builtin_amdgcn_s_waitcnt(vmcnt_wait((AHEAD - 1) * LOADS));
+        else
+          __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
+        __builtin_amdgcn_sched_barrier(0);
+        if (w == 0) {
+          const float k = sh.ksc[to][lane];
+          sh.kfac[to][lane] = fmaf(k, sl2, k * sl2_lo);
+        }
+      };
+      f32x16 o[4][RB];  // [dim block][row block]: row 32 i + j, dims 128 w + 32 d + 8 (r / 4) + 4 h + r % 4
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
+      const int vr = 8 * h + ((lane & 15) >> 1);  // (value operand: this lane's address is of row vr + 16 t)
+      int voff[4];
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+        voff[d] = vr * 512 + 128 * w + 16 * ((2 * d | ((lane >> 4) & 1)) ^ dn_swizzle(vr)) + 8 * (lane & 1);
+      const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
+      // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed
+      auto v_read = [&](const uint8_t* kt, int i) __attribute__((always_inline)) {
+        return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+            (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 3] + 16 * (i >> 2) * 512));
+      };
+      auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
+        return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * ROWS * DN_PROW + 32 * i * DN_PROW + 16 * t));
+      };
+      // chunk c's weights are final after this (and O on their maxima)
+      auto settle = [&](int c) __attribute__((always_inline)) {
+        const int4 fl = *reinterpret_cast<const int4*>(sh.flag[c & 1]);
+        if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+          dn_barrier();
+          dn_barrier();
+          if (c > 0) {  // O is zero before
+#pragma unroll
+            for (int i = 0; i < RB; ++i) {
+              const float a = sh.al[32 * i + j];
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[d][i][r] *= a;
+            }
+          }
+        }
+      };
+      // a chunk's value product: 16 steps of RB products, the next steps' operands read and converted ahead
+      auto value = [&](const uint8_t* kt, int pb) __attribute__((always_inline)) {
+        dn_v2i vv[DN_VAHEAD + 1];
+        bf16x8 pa[2][RB], vb[2];
+#pragma unroll
+        for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
+#pragma unroll
+        for (int i = 0; i < RB; ++i) pa[0][i] = p_read(pb, 0, i);
+        vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int t = i >> 2, d = i & 3;
+          if (i + DN_VAHEAD < 16) vv[(i + DN_VAHEAD) % (DN_VAHEAD + 1)] = v_read(kt, i + DN_VAHEAD);
+          if (d < RB && t < 3) pa[(t + 1) & 1][d] = p_read(pb, t + 1, d);
+#pragma unroll
+          for (int x = 0; x < RB; ++x)
+            o[d][x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i & 1], pa[t & 1][x], o[d][x], 0, 0, 0);
+          if (i < 15) {
+            const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
+            vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c)
+        if (c < nch) issue(c, c);
+      landed(0, nch >= AHEAD);
+      dn_barrier();  // chunk 0 is in place
+      int buf = 0;   // chunk c's buffer
+      for (int c = 0; c < nch; ++c) {
+        const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
+        if (c > 0) settle(c - 1);
+        // chunk c + AHEAD into the buffer that chunk c - 2 left
+        if (c + AHEAD < nch) issue(c + AHEAD, prev == 0 ? BUFS - 1 : prev - 1);
+        if (c > 0) value(sh.tile[prev], (c - 1) & 1);
+        if (c + 1 < nch) landed(next, c + AHEAD < nch);
+        buf = next;
+        dn_barrier();
+      }
+      settle(nch - 1);
+      value(sh.tile[buf == 0 ? BUFS - 1 : buf - 1], (nch - 1) & 1);
+      dn_barrier();  // the tiles are free
+      auto store = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int x = 32 * (w & 1) + 8 * d + 2 * g + h;
+              area[64 * x + ((32 * i + j) ^ (x & 7))] =
+                  f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
+            }
+      };
+      if (w < 2) store();
+      dn_barrier();
+      write(0);
+      dn_barrier();
+      if (w >= 2) store();
+      dn_barrier();
+      write(1);
+    }
+    dn_barrier();  // (the area's readers, before the next stretch's loads)
+    u += nch;
+    c0 = 0;
+    if (u < u1 && ++mt == tiles) {  // the next sequence with tokens
+      mt = 0;
+      do ++b;
+      while (ctx_len[b] <= 0);
+    }
+  }
+}
+
+constexpr int DC_THREADS = 128;  // a workgroup: one row's 512 outputs
+
+// Joins the partials of row blockIdx.x where its row tile was shared: out = sum 2^(m - max) O / sum 2^(m - max) l; and
+// writes the rows of sequences without tokens.
+__global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
+    const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ ctx_len,
+    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H, int rows,
+    int G, int max_pages, int page_size) {
+  __shared__ int tot[DC_THREADS / WAVE];
+  const int M = S * H, tiles = (M + rows - 1) / rows, t = threadIdx.x;
+  const int b = blockIdx.x / M, row = blockIdx.x - b * M, mt = row / rows, j = row - mt * rows;
+  long units = 0, before = 0;
+  for (int b0 = 0; b0 < B; b0 += DC_THREADS) {
+    const int x = b0 + t;
+    const int n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, page_size)) : 0;
+    int total;
+    dn_scan<DC_THREADS>(n, tot, total);
+    units += total;
+    dn_scan<DC_THREADS>(x < b ? n : 0, tot, total);
+    before += total;
+  }
+  units *= tiles;
+  const int nch = dn_chunks(dn_len(ctx_len[b], max_pages, page_size));
+  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+  float lse = NEG_INF;
+  if (nch > 0) {
+    const long first = before * tiles + (long)mt * nch;  // the row tile's units: first .. first + nch - 1
+    const int w0 = (int)dn_owner(first, units, G), w1 = (int)dn_owner(first + nch - 1, units, G);
+    if (w0 == w1) return;  // written by its workgroup
+    // workgroup w0's stretch is its second one where it started before the tile, the others' is their first
+    const size_t slot0 = 2 * (size_t)w0 + (dn_start(w0, units, G) < first);
+    auto slot = [&](int w) __attribute__((always_inline)) { return (w == w0 ? slot0 : 2 * (size_t)w) * rows + j; };
+    float mm = -INFINITY, ll = 0.0f;
+    for (int w = w0; w <= w1; ++w)
+      if (dn_start(w, units, G) < dn_start(w + 1, units, G)) mm = max_nonan(mm, ws_ml[2 * slot(w)]);
+    for (int w = w0; w <= w1; ++w) {
+      if (dn_start(w, units, G) >= dn_start(w + 1, units, G)) continue;  // a workgroup without work
+      const float f = __builtin_amdgcn_exp2f(ws_ml[2 * slot(w)] - mm);
+      ll += f * ws_ml[2 * slot(w) + 1];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(ws_o + slot(w) * DN_DV + 4 * t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+    }
+    const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] *= inv;
+    if (ll > 0.0f) lse = lse_base2(mm, ll);
+  }
+  const size_t at = (size_t)blockIdx.x * DN_DV + 4 * t;
+  if (out) *reinterpret_cast<uint2*>(out + at) = make_uint2(bf16_pack(acc[0], acc[1]), bf16_pack(acc[2], acc[3]));
+  if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at) = acc;
+  if (lse_out && t == 0) lse_out[blockIdx.x] = lse;
+}
+
+// Workgroups: one a CU, a multiple of the 8 XCDs.
+static int dense_grid(int num_cu) { return num_cu < 8 ? 8 : num_cu / 8 * 8; }
+
+static int dense_rows(int M) { return M <= 32 ? 32 : 64; }
+
+size_t dense_workspace_bytes(int M, int num_cu) {
+  return (size_t)2 * dense_grid(num_cu) * dense_rows(M) * (DN_DV + 2) * sizeof(float);
+}
+
+hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* kvs, const int* table,
+                            const int* ctx_len, uint16_t* out, float* out_f32, float* lse, void* ws, int B, int S,
+                            int H, int Dqk, int max_pages, int page_size, int num_pages, float scale, int num_cu,
+                            hipStream_t s) {
+  const int G = dense_grid(num_cu), rows = dense_rows(S * H);
+  int log2 = 0;
+  while ((1L << log2) < page_size) ++log2;
+  const DnPage pg = {(uint32_t)(((1ull << (31 + log2)) + page_size - 1) / page_size), 31 + log2, page_size};
+  float* ws_o = static_cast<float*>(ws);
+  float* ws_ml = ws_o + (size_t)2 * G * rows * DN_DV;
+  const auto kernel = rows == 32 ? Dqk == 512 ? dense_mla_kernel<512, 1> : dense_mla_kernel<576, 1>
+                                 : Dqk == 512 ? dense_mla_kernel<512, 2> : dense_mla_kernel<576, 2>;
+  const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
+                              out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale);
+  if (e != hipSuccess) return e;
+  return launch("dense_combine_kernel", dense_combine_kernel, dim3(B * S * H), dim3(DC_THREADS), s, ws_o, ws_ml,
+                ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+}
+
+}  // namespace dsa
