@@ -443,6 +443,34 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
                   float scale, void* stream);
 
 /*
+ * Expanded latent attention, the form of a prefill (the reference's non-absorbed `attention`, trnrt/models/mla.py:420-482),
+ * in two calls: per pair of tokens and head it costs 192 + 128 multiply-adds where dsa_dense_mla's latent products cost
+ * 576 + 512.
+ *
+ * dsa_expand_latent: the keys and values of every head from the cached latent rows. Sequence b's tokens 0 .. n_b - 1 are
+ * output rows cu_len[b] .. cu_len[b + 1] - 1 (cu_len int32 [B + 1], ascending, cu_len[0] = 0; n_b = cu_len[b + 1] -
+ * cu_len[b]); with c_t = kv_fp8[slot(b, t)] * kv_scale[slot(b, t)]:
+ *   k[row, h, :] = c_t[:512] . w[h, :128, :]^T,  v[row, h, :] = c_t[:512] . w[h, 128:, :]^T,  rope[row, :] = c_t[512:]
+ *   w bf16 [H, 256, 512]; k, v bf16 [total, H, 128]; rope bf16 [total, 64] (Dqk 576; ignored for 512); kv_fp8, kv_scale,
+ *   page_table as dsa_dense_mla (a token past the table reads the null page). Rows from cu_len[B] on are not written,
+ *   nor any from `total` on.
+ *
+ * dsa_expanded_mla: ragged attention over them. Sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 of q, its keys
+ * and values rows cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1] each, clamped to [0, Tq] and [0, Tk]); query i of nq sees keys
+ * t < nk (causal = 0) or t < nk - nq + i + 1 (causal):
+ *   s[t] = scale * (q[i, h, :128] . k[t, h, :] + q[i, h, 128:] . rope[t, :]), p = softmax_t(s), out[i, h, :] = sum_t p[t]
+ *   v[t, h, :], lse = log sum_t exp(s[t]); a query that sees no key: out 0, lse NEG_INF (-1e30).
+ *   q bf16 [Tq, H, 192] with rope bf16 [Tk, 64], or [Tq, H, 128] with rope null; k, v bf16 [Tk, H, 128]; out_bf16 and / or
+ *   out_f32 [Tq, H, 128], lse fp32 [Tq, H] or null. Rows of q outside every sequence have no output written.
+ */
+int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table, const int32_t* cu_len,
+                      const void* w_bf16, void* k_bf16, void* v_bf16, void* rope_bf16, int B, int total, int H,
+                      int Dqk, int max_pages, int page_size, int num_pages, void* stream);
+int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
+                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse, int B,
+                     int Tq, int Tk, int H, int causal, float scale, void* stream);
+
+/*
  * Pages of the paged caches (no counterpart among the reference's kernels: its page pool and prefix caches are host
  * code, trnrt/engine/kv_pool.py:1-50, and its caches are copied by the framework). A page pool is a use count per page,
  * ref int32 [num_pages] (0 or less: free; page 0, the null page, is never given out, counted or moved), page tables

@@ -118,6 +118,13 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
                             const int* ctx_len, uint16_t* out, float* out_f32, float* lse, void* ws, int B, int S,
                             int H, int Dqk, int max_pages, int page_size, int num_pages, float scale, int num_cu,
                             hipStream_t s);
+hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* table, const int* cu,
+                                const uint16_t* w, uint16_t* k, uint16_t* v, uint16_t* r, int B, int total, int H,
+                                int D, int max_pages, int page_size, int num_pages, hipStream_t s);
+bool expanded_grid_ok(int B, int Tq, int H);
+hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
+                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, int B,
+                                  int Tq, int Tk, int H, int causal, float scale, hipStream_t s);
 size_t pages_fork_bytes(int n);
 size_t pages_compact_bytes(int num_pages);
 bool pages_units_ok(const long long* page_bytes, int n_caches, long n);
@@ -1293,6 +1300,37 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
                                       static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, S, H, Dqk,
                                       max_pages, page_size, num_pages, scale, num_cu(),
                                       static_cast<hipStream_t>(stream)));
+}
+
+int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table, const int32_t* cu_len,
+                      const void* w_bf16, void* k_bf16, void* v_bf16, void* rope_bf16, int B, int total, int H,
+                      int Dqk, int max_pages, int page_size, int num_pages, void* stream) {
+  if (B < 0 || total < 0 || H < 1 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
+  if (Dqk != 512 && Dqk != 576) return DSA_EUNSUPPORTED;
+  if ((long)num_pages * page_size > 0x7fffffffL || ((long)total / 256 + 1) * 2 * H > 0xffffffL || total > 0x7fffff00)
+    return DSA_EUNSUPPORTED;
+  if (B == 0 || total == 0) return DSA_OK;
+  if (!kv_fp8 || !page_table || !cu_len || !w_bf16 || !k_bf16 || !v_bf16 || (Dqk == 576 && !rope_bf16))
+    return DSA_EINVAL;
+  return status(dsa::launch_expand_latent(
+      kv_fp8, kv_scale, page_table, cu_len, static_cast<const uint16_t*>(w_bf16), static_cast<uint16_t*>(k_bf16),
+      static_cast<uint16_t*>(v_bf16), Dqk == 576 ? static_cast<uint16_t*>(rope_bf16) : nullptr, B, total, H, Dqk,
+      max_pages, page_size, num_pages, static_cast<hipStream_t>(stream)));
+}
+
+int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
+                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse, int B,
+                     int Tq, int Tk, int H, int causal, float scale, void* stream) {
+  if (B < 0 || Tq < 0 || Tk < 0 || H < 1) return DSA_EINVAL;
+  if (!dsa::expanded_grid_ok(B, Tq, H)) return DSA_EUNSUPPORTED;
+  if (B == 0 || Tq == 0) return DSA_OK;
+  // (no keys: k, v and rope_bf16 may be null, and every query sees nothing)
+  if (!q_bf16 || !cu_q || !cu_k || (!out_bf16 && !out_f32) || (Tk > 0 && (!k_bf16 || !v_bf16))) return DSA_EINVAL;
+  return status(dsa::launch_expanded_attend(
+      static_cast<const uint16_t*>(q_bf16), static_cast<const uint16_t*>(k_bf16),
+      static_cast<const uint16_t*>(rope_bf16), static_cast<const uint16_t*>(v_bf16), cu_q, cu_k,
+      static_cast<uint16_t*>(out_bf16), out_f32, lse, B, Tq, Tk, H, causal != 0, scale,
+      static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

@@ -22,7 +22,8 @@
 // stands; a wave that meets a score past its slack raises a flag, and before the chunk's values are multiplied every wave
 // sees the flags and, when one is up, the maxima are exchanged, P is taken again and O rescaled (a stretch's chunk 0 always
 // does, with O still zero).
-#include "dsa_common.h"
+#include "dsa_async.h"
+#include "dsa_scan.h"
 
 namespace dsa {
 
@@ -51,6 +52,7 @@ struct DnShared {
   alignas(16) uint16_t p[2][32 * RB * DN_PROW];  // P[row][token] of two chunks
   alignas(16) float ksc[BUFS][DN_CHUNK];         // the chunks' token scales
   alignas(16) float kfac[BUFS][DN_CHUNK];        // x softmax scale x log2 e
+  int page[4][DN_CHUNK];                         // and the pages of their tokens, four chunks
   float cmax[2][32 * RB];                        // [token half][row]: a chunk's maxima when one moves
   float al[32 * RB];                             // and its rescale factors
   alignas(16) int flag[2][4];                    // per chunk parity and wave: a score past the running maximum's slack
@@ -67,39 +69,12 @@ struct DnPage {
   int size;
 };
 
-// Every wave of the workgroup, whichever its role: LDS accesses before it are visible after it; global loads stay in
-// flight.
-__device__ __forceinline__ void dn_barrier() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // A sequence's tokens and chunks of them.
 __device__ __forceinline__ int dn_len(int ctx_len, int max_pages, int page_size) {
   const long cap = (long)max_pages * page_size;
   return (int)min(max((long)ctx_len, 0L), min(cap, 0x7fffff00L));
 }
 __device__ __forceinline__ int dn_chunks(int len) { return (len + DN_CHUNK - 1) / DN_CHUNK; }
-
-// The inclusive prefix sum of v over the workgroup's THREADS threads and its total.
-template <int THREADS>
-__device__ __forceinline__ int dn_scan(int v, int* tot, int& total) {
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int x = wave_incl_scan(v);
-  __syncthreads();
-  if (lane == WAVE - 1) tot[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / WAVE; ++w) {
-    const int s = tot[w];
-    before += w < wave ? s : 0;
-    total += s;
-  }
-  return before + x;
-}
 
 // The number of units (sequence, row tile, chunk of tokens). Every thread of the workgroup calls this.
 template <int THREADS>
@@ -109,7 +84,7 @@ __device__ __forceinline__ long dn_total(const int* __restrict__ ctx_len, int B,
   for (int b0 = 0; b0 < B; b0 += THREADS) {
     const int b = b0 + (int)threadIdx.x;
     int total;
-    dn_scan<THREADS>(b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, page_size)) : 0, tot, total);
+    group_incl_scan<THREADS>(b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, page_size)) : 0, tot, total);
     units += (long)total * tiles;
   }
   return units;
@@ -131,9 +106,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   constexpr int TAIL = DN_CHUNK * 512;      // where the rows' last 64 bytes lie
   constexpr int LOADS = DQK == 576 ? 9 : 8;  // a chunk's asynchronous loads per value wave
   __shared__ Sh sh;
-  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
+  const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int j = lane & 31, h = lane >> 5;
   const int M = S * H, tiles = (M + ROWS - 1) / ROWS;
   const int G = gridDim.x;
   const int wg = (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3);  // (workgroup x runs on XCD x % 8; G a multiple of 8)
@@ -147,7 +121,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       const int b = b0 + tid;
       const int n = b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, pg.size)) : 0;
       int total;
-      const int incl = dn_scan<DN_THREADS>(n, sh.tot, total);
+      const int incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
       const long lo = (before + incl - n) * tiles, hi = (before + incl) * tiles;
       if (lo <= u0 && u0 < hi) {
         sh.found[0] = b;
@@ -161,7 +135,11 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     __syncthreads();
   }
   // scale x log2 e to twice fp32's digits: rounded, its error would be the same for every score, and so the lse's
-  const float sl2 = scale * DN_LOG2E, sl2_lo = fmaf(scale, DN_LOG2E, -sl2) + scale * DN_LOG2E_LO;
+  auto uniform = [](float x) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
+  };
+  const float sl2 = uniform(scale * DN_LOG2E);
+  const float sl2_lo = uniform(fmaf(scale, DN_LOG2E, -sl2) + scale * DN_LOG2E_LO);
   // the stretch at hand: chunks c0 .. of row tile mt of sequence b
   int b = __builtin_amdgcn_readfirstlane(sh.found[0]), mt = __builtin_amdgcn_readfirstlane(sh.found[1]);
   int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
@@ -177,7 +155,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
     auto write = [&](int half) __attribute__((always_inline)) {
       const size_t slot = 2 * (size_t)wg + (u > u0);
-      const int dim = 256 * half + 4 * lane;
+      const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
 #pragma unroll 1
       for (int r = wave; r < ROWS && r0 + r < M; r += DN_THREADS / WAVE) {
         f32x4 v = area[64 * lane + (r ^ (lane & 7))];
@@ -204,6 +182,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     if (wave < 4) {
       // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
       const int th = wave >> 1, hh = wave & 1;
+      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
       const bool works = hh < RB;
       const int row = min(r0 + 32 * (works ? hh : 0) + j, M - 1);
       const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
@@ -216,8 +195,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           qb[2 * s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s));
           qb[2 * s + 1] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s + 8));
         }
+        arrive(qb);
       }
-      dn_barrier();  // chunk 0 is in place
+      lds_barrier();  // chunk 0 is in place
       float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
                            // always up
       float l_run = 0.0f;  // this lane's share of its running sum
@@ -252,7 +232,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           for (int r = 1; r < 16; ++r) cm = max_nonan(cm, sv[r]);
           cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
           if (works && h == 0) sh.cmax[th][32 * hh + j] = cm;
-          dn_barrier();
+          lds_barrier();
           cm = max_nonan(cm, sh.cmax[th ^ 1][32 * (works ? hh : 0) + j]);
           // a row that sees none of chunk 0 sees none of the stretch: its maximum stays finite
           const float up = c == 0 ? max_nonan(cm, -1e30f) : cm > DN_SLACK ? cm : 0.0f;
@@ -268,7 +248,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
             if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
           }
-          dn_barrier();
+          lds_barrier();
         }
         l_run += psum;
         psum = 0.0f;
@@ -335,22 +315,23 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         }
         last = buf;
         buf = buf == BUFS - 1 ? 0 : buf + 1;
-        dn_barrier();
+        lds_barrier();
       }
       __builtin_amdgcn_s_setprio(0);
       settle(nch - 1, flags(nch - 1));
       const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
       if (works && h == 0) sh.lsum[th][32 * hh + j] = lw;
       if (works && th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
-      dn_barrier();  // the tiles are free
-      dn_barrier();  // the first 256 dims' outputs are in LDS
+      lds_barrier();  // the tiles are free
+      lds_barrier();  // the first 256 dims' outputs are in LDS
       write(0);
-      dn_barrier();
-      dn_barrier();  // and the others'
+      lds_barrier();
+      lds_barrier();  // and the others'
       write(1);
     } else {
       // -- the loads and the values: wave w brings rows 16 w .. + 15 of a chunk, takes dims 128 w .. + 127 of all rows --
       const int w = wave - 4;
+      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
       const int* trow = table + (size_t)b * max_pages;
       // token `lane` of chunk c, the sequence's last one past its end (a slot behind it may never have been written, and
       // its NaN x weight 0 is NaN)
@@ -361,39 +342,35 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 #pragma unroll
       for (int k = 0; k < 4; ++k) mcol[k] = 16 * (j ^ dn_swizzle(2 * k | h));
       const int tcol = 512 + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
-      int page = trow[page_of(token(0))];  // of this lane's token in the chunk to bring next
-      auto issue = [&](int c, int to) __attribute__((always_inline)) {  // chunk c's loads into buffer `to`
+      const uint32_t tile_lds = lds_address(sh.tile[0] + 16 * w * 512), tail_lds = lds_address(sh.tile[0] + TAIL + 1024 * w);
+      const uint32_t ksc_lds = lds_address(sh.ksc[0]), page_lds = lds_address(sh.page[0]);
+      if (!kvs)
+        for (int i = 0; i < BUFS; ++i) sh.ksc[i][lane] = 1.0f;
+      // chunk c's loads into buffer `to`, and its scales and the pages of chunk c + 2 (every value wave the same ones, so
+      // that each waits for its own); `page`: of this lane's token
+      auto issue = [&](int c, int to, int page) __attribute__((always_inline)) {
         const int t = token(c);
         const int slot = safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
-        page = trow[page_of(token(c + 1))];
-        uint8_t* dst = sh.tile[to] + 16 * w * 512;
+        load_lds4(trow + page_of(token(c + 2)), page_lds + 4 * DN_CHUNK * ((c + 2) & 3));
+        if (kvs) load_lds4(kvs + slot, ksc_lds + 4 * DN_CHUNK * to);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(mrow + 8 * k, slot);
-          __builtin_amdgcn_global_load_lds(kv + (size_t)s * DQK + mcol[k & 3],
-                                           (__attribute__((address_space(3))) void*)(dst + 1024 * k), 16, 0, 0);
+          load_lds16(kv + (size_t)s * DQK + mcol[k & 3], tile_lds + DN_CHUNK * DQK * to + 1024 * k);
         }
         if (DQK == 576) {
           const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(trw, slot);
-          __builtin_amdgcn_global_load_lds(kv + (size_t)s * DQK + tcol,
-                                           (__attribute__((address_space(3))) void*)(sh.tile[to] + TAIL + 1024 * w),
-                                           16, 0, 0);
+          load_lds16(kv + (size_t)s * DQK + tcol, tail_lds + DN_CHUNK * DQK * to);
         }
-        if (kvs)  // (every value wave the same: so that their loads count alike)
-          __builtin_amdgcn_global_load_lds(kvs + slot, (__attribute__((address_space(3))) void*)sh.ksc[to], 4, 0, 0);
-        else
-          sh.ksc[to][lane] = 1.0f;
       };
       constexpr int AHEAD = BUFS - 2;  // chunks in flight
-      // chunk `to`'s loads have landed, with at most AHEAD - 1 chunks' younger than them out (more: so many are; only the
-      // rows' loads are counted: a count too low only waits longer); then the tokens' factors
+      // chunk `to`'s loads have landed (`more`: with those of the AHEAD - 1 chunks after it out), and so the pages two
+      // chunks on; then the tokens' factors
       auto landed = [&](int to, bool more) __attribute__((always_inline)) {
-        __builtin_amdgcn_sched_barrier(0);
         if (more)
-          __builtin_amdgcn_s_waitcnt(vmcnt_wait((AHEAD - 1) * LOADS));
+          wait_loads<(AHEAD - 1) * (LOADS + 1)>();
         else
-          __builtin_amdgcn_s_waitcnt(vmcnt_wait(0));
-        __builtin_amdgcn_sched_barrier(0);
+          wait_loads<0>();
         if (w == 0) {
           const float k = sh.ksc[to][lane];
           sh.kfac[to][lane] = fmaf(k, sl2, k * sl2_lo);
@@ -422,8 +399,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       auto settle = [&](int c) __attribute__((always_inline)) {
         const int4 fl = *reinterpret_cast<const int4*>(sh.flag[c & 1]);
         if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
-          dn_barrier();
-          dn_barrier();
+          lds_barrier();
+          lds_barrier();
           if (c > 0) {  // O is zero before
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
@@ -460,25 +437,28 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-#pragma unroll
-      for (int c = 0; c < AHEAD; ++c)
-        if (c < nch) issue(c, c);
-      landed(0, nch >= AHEAD);
-      dn_barrier();  // chunk 0 is in place
+      {
+        const int p0 = trow[page_of(token(0))], p1 = trow[page_of(token(1))];
+        if (AHEAD == 1) sh.page[1][lane] = p1;
+        issue(0, 0, p0);
+        if (AHEAD == 2 && nch > 1) issue(1, 1, p1);
+      }
+      landed(0, AHEAD == 2 && nch > 1);
+      lds_barrier();  // chunk 0 is in place
       int buf = 0;   // chunk c's buffer
       for (int c = 0; c < nch; ++c) {
         const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
         if (c > 0) settle(c - 1);
         // chunk c + AHEAD into the buffer that chunk c - 2 left
-        if (c + AHEAD < nch) issue(c + AHEAD, prev == 0 ? BUFS - 1 : prev - 1);
+        if (c + AHEAD < nch) issue(c + AHEAD, prev == 0 ? BUFS - 1 : prev - 1, sh.page[(c + AHEAD) & 3][lane]);
         if (c > 0) value(sh.tile[prev], (c - 1) & 1);
         if (c + 1 < nch) landed(next, c + AHEAD < nch);
         buf = next;
-        dn_barrier();
+        lds_barrier();
       }
       settle(nch - 1);
       value(sh.tile[buf == 0 ? BUFS - 1 : buf - 1], (nch - 1) & 1);
-      dn_barrier();  // the tiles are free
+      lds_barrier();  // the tiles are free
       auto store = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < RB; ++i)
@@ -492,14 +472,14 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             }
       };
       if (w < 2) store();
-      dn_barrier();
+      lds_barrier();
       write(0);
-      dn_barrier();
+      lds_barrier();
       if (w >= 2) store();
-      dn_barrier();
+      lds_barrier();
       write(1);
     }
-    dn_barrier();  // (the area's readers, before the next stretch's loads)
+    lds_barrier();  // (the area's readers, before the next stretch's loads)
     u += nch;
     c0 = 0;
     if (u < u1 && ++mt == tiles) {  // the next sequence with tokens
@@ -526,9 +506,9 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     const int x = b0 + t;
     const int n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, page_size)) : 0;
     int total;
-    dn_scan<DC_THREADS>(n, tot, total);
+    group_incl_scan<DC_THREADS>(n, tot, total);
     units += total;
-    dn_scan<DC_THREADS>(x < b ? n : 0, tot, total);
+    group_incl_scan<DC_THREADS>(x < b ? n : 0, tot, total);
     before += total;
   }
   units *= tiles;

@@ -1,0 +1,447 @@
+// Expanded latent attention for gfx950, the form of a prefill: the keys and values of every head from the cached latent rows
+// (expand_latent_kernel), and attention over them (expanded_attend_kernel). Per pair of tokens and head it costs 192 + 128
+// multiply-adds where the absorbed form's latent products cost 576 + 512.
+#include "dsa_async.h"
+#include "dsa_scan.h"
+
+namespace dsa {
+
+constexpr int EX_D = 128;   // a head's key width without rope, and its value width
+constexpr int EX_R = 64;    // the rope width, shared by the heads
+constexpr int EX_C = 512;   // the latent width
+
+// -- keys and values ------------------------------------------------------------------------------------------------
+// k[t, h, :] = sigma_t c_t[:512] . W[h, :128, :]^T, v[t, h, :] the same with W[h, 128:, :]: a product of P x 512 x 256 H
+// whose left side is e4m3 rows gathered through the page table (the scale is applied to the sums), and k_rope[t] =
+// sigma_t c_t[512:].
+// What bounds it: the matrix units (512 products a sum are few, so the output, half as many bytes as the sums in fp32,
+// takes a quarter of the time beside it). A workgroup has 256 tokens x one head's 128 keys or values, two of them run on a
+// CU so that one's stores are under the other's products; 64 of the 512 columns at a time come by asynchronous loads
+// straight into LDS, a step ahead. The rows stay e4m3 until they are operands (exact in bf16). The tiles of one XCD share
+// its heads' weights through its L2.
+constexpr int EL_THREADS = 256;
+constexpr int EL_TOK = 256;
+constexpr int EL_K = 64;
+
+struct ElShared {
+  alignas(1024) uint8_t a[2][EL_TOK * EL_K];    // rows: 64 bytes, 16-byte piece p at p ^ ((row >> 1) & 3)
+  alignas(1024) uint16_t b[2][EX_D * EL_K];     // weights: 128 bytes a row, piece p at p ^ (row & 7)
+  int slot[EL_TOK];
+  int seq;
+};
+
+__global__ __launch_bounds__(EL_THREADS, 2) void expand_latent_kernel(
+    const uint8_t* __restrict__ kv, const float* __restrict__ kvs, const int* __restrict__ table,
+    const int* __restrict__ cu, const uint16_t* __restrict__ wkv, uint16_t* __restrict__ k_out,
+    uint16_t* __restrict__ v_out, uint16_t* __restrict__ r_out, int B, int total, int H, int D, int max_pages,
+    int page_size, int num_pages) {
+  __shared__ ElShared sh;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int j = lane & 31, h = lane >> 5;
+  // parts: 2 H of 128 columns. An XCD (workgroup x runs on XCD x % 8) takes an eighth of them where they divide, all the
+  // parts of a token tile next to each other
+  const int parts = 2 * H;
+  int part, tile;
+  if ((parts & 7) == 0) {
+    const int per = parts >> 3, y = blockIdx.x >> 3;
+    part = (blockIdx.x & 7) * per + y % per;
+    tile = y / per;
+  } else {
+    part = blockIdx.x % parts;
+    tile = blockIdx.x / parts;
+  }
+  const int t0 = tile * EL_TOK, end = min(total, cu[B]);
+  if (t0 >= end) return;  // (rows past the last sequence are left as they were)
+  // the slots of the tile's tokens: the sequence of the first one by counting, the others' from there
+  if (tid == 0) sh.seq = 0;
+  __syncthreads();
+  int n = 0;
+  for (int b = tid; b < B; b += EL_THREADS) n += cu[b + 1] <= t0;
+  if (n) atomicAdd(&sh.seq, n);
+  __syncthreads();
+  {
+    const int t = min(t0 + tid, end - 1);
+    int b = min(sh.seq, B - 1);
+    while (b < B - 1 && cu[b + 1] <= t) ++b;
+    const int pos = max(t - cu[b], 0), pi = pos / page_size;
+    const int page = pi < max_pages ? safe_page(table[(size_t)b * max_pages + pi], num_pages) : 0;
+    sh.slot[tid] = page * page_size + (pos - pi * page_size);
+  }
+  __syncthreads();
+  // this lane's loads: rows 64 wave + 16 i + lane / 4 of the tokens, 32 wave + 8 i + lane / 8 of the weights
+  const uint8_t* ap[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    ap[i] = kv + (size_t)sh.slot[64 * wave + 16 * i + (lane >> 2)] * D + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
+  const uint16_t* bp =
+      wkv + ((size_t)part * EX_D + 32 * wave + (lane >> 3)) * EX_C + 8 * ((lane & 7) ^ (lane >> 3));
+  const uint32_t a_lds = lds_address(sh.a[0] + 4096 * wave), b_lds = lds_address(sh.b[0] + 2048 * wave);
+  auto issue = [&](int s, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      load_lds16(ap[i] + s * EL_K, a_lds + EL_TOK * EL_K * to + 1024 * i);
+      load_lds16(bp + s * EL_K + 8 * i * EX_C, b_lds + 2 * EX_D * EL_K * to + 1024 * i);
+    }
+  };
+  issue(0, 0);
+  // wave: tokens 128 wm .. + 127 x columns 64 wn .. + 63; the columns are the products' rows, so that a lane's sums are 4
+  // consecutive columns of one token
+  const int wm = wave >> 1, wn = wave & 1;
+  float sc[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) sc[x] = kvs ? kvs[sh.slot[128 * wm + 32 * x + j]] : 1.0f;
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) acc[x][y] = f32x16{};
+  arrive(sc);
+  const int arow = (128 * wm + j) * EL_K, asw = (j >> 1) & 3;
+  const int brow = (64 * wn + j) * EL_K, bsw = j & 7;
+#pragma unroll 1
+  for (int s = 0; s < EX_C / EL_K; ++s) {
+    wait_loads<0>();
+    lds_barrier();  // step s is in place, and nobody reads step s - 1 any more
+    if (s + 1 < EX_C / EL_K) issue(s + 1, (s + 1) & 1);
+    const uint8_t* a = sh.a[s & 1];
+    const uint16_t* b = sh.b[s & 1];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {  // 32 columns: lane half h takes 16, in two operands of 8
+      bf16x8 wf[2][2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          wf[y][e] = as_bf16x8(
+              *reinterpret_cast<const uint4*>(b + brow + 32 * EL_K * y + 8 * ((4 * g + 2 * h + e) ^ bsw)));
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const u32x4 c = *reinterpret_cast<const u32x4*>(a + arow + 32 * EL_K * x + 16 * ((2 * g + h) ^ asw));
+        const bf16x8 c0 = fp8x8_to_bf16x8(c[0], c[1]), c1 = fp8x8_to_bf16x8(c[2], c[3]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][0], c0, acc[x][y], 0, 0, 0);
+          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][1], c1, acc[x][y], 0, 0, 0);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // through LDS: 256 bytes a token, 16-byte piece p of row r at p ^ (r & 15), then whole rows
+  uint8_t* const st = sh.a[0];
+  static_assert(offsetof(ElShared, slot) >= EL_TOK * EX_D * 2, "the staged outputs");
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    const int r = 128 * wm + 32 * x + j;
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x16& v = acc[x][y];
+        *reinterpret_cast<uint2*>(st + 256 * r + 16 * ((8 * wn + 4 * y + g) ^ (r & 15)) + 8 * h) =
+            make_uint2(bf16_pack(v[4 * g] * sc[x], v[4 * g + 1] * sc[x]),
+                       bf16_pack(v[4 * g + 2] * sc[x], v[4 * g + 3] * sc[x]));
+      }
+  }
+  __syncthreads();
+  uint16_t* const out = (part & 1 ? v_out : k_out) + ((size_t)t0 * H + (part >> 1)) * EX_D;
+#pragma unroll
+  for (int i = 0; i < EL_TOK * 16 / EL_THREADS; ++i) {
+    const int x = tid + EL_THREADS * i, r = x >> 4, p = x & 15;
+    if (t0 + r < end)
+      *reinterpret_cast<u32x4*>(out + (size_t)r * H * EX_D + 8 * p) =
+          *reinterpret_cast<const u32x4*>(st + 256 * r + 16 * (p ^ (r & 15)));
+  }
+  if (part == 0 && r_out) {
+#pragma unroll
+    for (int i = 0; i < EL_TOK * 8 / EL_THREADS; ++i) {  // 8 rope columns of a token
+      const int x = tid + EL_THREADS * i, r = x >> 3, p = x & 7;
+      if (t0 + r < end) {
+        const int slot = sh.slot[r];
+        const uint2 c = *reinterpret_cast<const uint2*>(kv + (size_t)slot * D + EX_C + 8 * p);
+        const float f = kvs ? kvs[slot] : 1.0f;
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = (e & 2 ? c.y : c.x) >> (16 * (e & 1));
+          const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(two, false);
+          o[e] = bf16_pack(v[0] * f, v[1] * f);
+        }
+        *reinterpret_cast<uint4*>(r_out + (size_t)(t0 + r) * EX_R + 8 * p) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+  }
+}
+
+// -- attention ------------------------------------------------------------------------------------------------------
+// s = scale (q[:128] . k + q[128:] . k_rope), p = softmax(s), out = p . v, lse, for ragged batches of queries and keys,
+// causal (the last query sees every key) or full.
+// What bounds it: the matrix units, then the exponentials. One workgroup a CU has 256 queries of a head, 8 waves of 32,
+// two on each SIMD, the first of them with priority, so that one's softmax runs under the other's products. A tile of 64
+// keys and values comes by asynchronous loads straight into LDS two tiles ahead, with one barrier a tile. S^T = K . Q^T and
+// O^T += V^T . P on v_mfma_f32_32x32x16_bf16: a lane's scores are of one query, in the value product's operand layout as
+// they stand (the values are read transposed in the same order), so P never leaves the registers and the maxima and sums
+// stay in their lanes. The longest tiles of a causal batch go first.
+constexpr int XA_THREADS = 512;
+constexpr int XA_Q = 256;
+constexpr int XA_K = 64;
+constexpr int XA_STAGES = 3;
+constexpr float XA_SLACK = 11.5f;  // lazy rescaling (base 2): p = 2^(s - m) <= 2^11.5 between moves of m
+constexpr float XA_LOG2E = 1.44269504088896341f;
+
+typedef short xa_v4s __attribute__((ext_vector_type(4)));
+
+// A stage's keys and values lie in rows of 256 bytes, 16-byte piece p of key row r at p ^ (r & 7), of value row r at
+// p ^ 2 (r & 3) (its reads take two pieces of 4 rows), of rope row r (128 bytes) at p ^ (r & 7).
+template <int DQ>
+struct XaShared {
+  alignas(1024) uint8_t k[XA_STAGES][XA_K * 256];
+  alignas(1024) uint8_t v[XA_STAGES][XA_K * 256];
+  alignas(1024) uint8_t r[DQ > EX_D ? XA_STAGES : 1][DQ > EX_D ? XA_K * 128 : 16];
+  int tot[XA_THREADS / WAVE];
+  int found[2];
+};
+
+template <int DQ>
+__global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ kr,
+    const uint16_t* __restrict__ v, const int* __restrict__ cu_q, const int* __restrict__ cu_k,
+    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int Tq, int Tk, int H,
+    int q_tiles, int causal, float scale) {
+  constexpr int STEPS = DQ / 16;
+  constexpr int LOADS = DQ > EX_D ? 5 : 4;  // a tile's asynchronous loads per wave
+  __shared__ XaShared<DQ> sh;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int j = lane & 31, h = lane >> 5;
+  // heads of one XCD (workgroup x runs on XCD x % 8) next to each other, query tiles from the last to the first
+  int head, ti;
+  if ((H & 7) == 0) {
+    const int per = H >> 3, y = blockIdx.x >> 3;
+    head = (blockIdx.x & 7) * per + y % per;
+    ti = q_tiles - 1 - y / per;
+  } else {
+    head = blockIdx.x % H;
+    ti = q_tiles - 1 - blockIdx.x / H;
+  }
+  auto first_q = [&](int b) __attribute__((always_inline)) { return min(max(cu_q[b], 0), Tq); };
+  auto queries = [&](int b) __attribute__((always_inline)) { return max(min(cu_q[b + 1], Tq) - first_q(b), 0); };
+  {  // the sequence of tile ti
+    if (tid == 0) sh.found[0] = -1;
+    int before = 0;
+    for (int b0 = 0; b0 < B && before <= ti; b0 += XA_THREADS) {
+      const int b = b0 + tid;
+      const int n = b < B ? (queries(b) + XA_Q - 1) / XA_Q : 0;
+      int total;
+      const int incl = before + group_incl_scan<XA_THREADS>(n, sh.tot, total);
+      if (incl - n <= ti && ti < incl) {
+        sh.found[0] = b;
+        sh.found[1] = ti - (incl - n);
+      }
+      before += total;
+    }
+    __syncthreads();
+  }
+  const int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
+  if (b < 0) return;  // past the last tile
+  const int qt = __builtin_amdgcn_readfirstlane(sh.found[1]) * XA_Q;
+  const int nq = queries(b), qb = first_q(b);
+  const int kb = min(max(cu_k[b], 0), Tk), nk = max(min(cu_k[b + 1], Tk) - kb, 0);
+  // keys that query i sees
+  auto seen = [&](int i) __attribute__((always_inline)) { return causal ? min(nk - nq + i + 1, nk) : nk; };
+  const int nt = (max(seen(min(qt + XA_Q, nq) - 1), 0) + XA_K - 1) / XA_K;
+  const int w0 = qt + 32 * wave;  // the wave's first query
+  const int nt_w = w0 < nq ? (max(seen(min(w0 + 32, nq) - 1), 0) + XA_K - 1) / XA_K : 0;
+  const int seen0 = seen(w0);
+  const int qi = min(w0 + j, nq - 1), seen_j = seen(qi);
+
+  // this wave's loads of a tile: key and value rows 8 wave .. + 7, in two of 4 rows, rope rows 8 wave .. + 7
+  const size_t head_off = (size_t)kb * H * EX_D + (size_t)head * EX_D;
+  const uint16_t* const k_base = k + head_off;
+  const uint16_t* const v_base = v + head_off;
+  const int l4 = lane >> 4;
+  const int kcol[2] = {8 * ((lane & 15) ^ l4), 8 * ((lane & 15) ^ (4 | l4))};
+  const int vcol = 8 * ((lane & 15) ^ (2 * l4));
+  const int rcol = 8 * ((lane & 7) ^ (lane >> 3));
+  const uint32_t k_lds = lds_address(sh.k[0] + 2048 * wave), v_lds = lds_address(sh.v[0] + 2048 * wave);
+  const uint32_t r_lds = lds_address(sh.r[0] + 1024 * wave);
+  auto issue = [&](int i, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {  // (rows past the end: the last one, of weight 0)
+      const size_t t = (size_t)min(i * XA_K + 8 * wave + 4 * x + l4, nk - 1) * H * EX_D;
+      load_lds16(k_base + t + kcol[x], k_lds + XA_K * 256 * to + 1024 * x);
+      load_lds16(v_base + t + vcol, v_lds + XA_K * 256 * to + 1024 * x);
+    }
+    if (DQ > EX_D)
+      load_lds16(kr + (size_t)(kb + min(i * XA_K + 8 * wave + (lane >> 3), nk - 1)) * EX_R + rcol,
+                 r_lds + XA_K * 128 * to);
+  };
+  if (nt > 0) issue(0, 0);
+  if (nt > 1) issue(1, 1);
+  bf16x8 qf[STEPS];  // query qi: step s holds dims 16 s + 8 h .. + 7
+  {
+    const uint16_t* qr = q + ((size_t)(qb + qi) * H + head) * DQ + 8 * h;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * s));
+    arrive(qf);
+  }
+  int koff[4], roff[4], voff[2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 7));
+    roff[i] = 128 * j + 16 * ((2 * i | h) ^ (j & 7));
+  }
+  {  // the value operand: this lane's address is of row 4 h + (lane & 15) / 4, columns 16 (lane / 16 % 2) + 4 (lane % 4)
+    const int r = (lane & 15) >> 2, p = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) voff[i] = 256 * (4 * h + r) + 16 * ((4 * i | p) ^ (2 * r)) + 8 * (lane & 1);
+  }
+  const float sl2 = scale * XA_LOG2E;
+  float m_run = 0.0f, l_run = 0.0f;  // running maximum (base 2), this lane's share of the sum
+  f32x16 o[4];                       // dims 32 d + 8 (r / 4) + 4 h + r % 4
+#pragma unroll
+  for (int d = 0; d < 4; ++d) o[d] = f32x16{};
+  if (wave < 4) __builtin_amdgcn_s_setprio(1);
+  int stage = 0;
+#pragma unroll 1
+  for (int i = 0; i < nt; ++i) {
+    if (i + 1 < nt)
+      wait_loads<LOADS>();
+    else
+      wait_loads<0>();
+    lds_barrier();  // tile i is in place, and nobody reads tile i - 1 any more
+    if (i + 2 < nt) issue(i + 2, stage == 0 ? 2 : stage - 1);
+    if (i < nt_w) {
+      const uint8_t* const kt = sh.k[stage];
+      const uint8_t* const vt = sh.v[stage];
+      const uint8_t* const rt = sh.r[DQ > EX_D ? stage : 0];
+      f32x16 s2[2] = {f32x16{}, f32x16{}};  // scores: tokens 32 x + 8 (r / 4) + 4 h + r % 4
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint8_t* at = s < 8 ? kt + koff[s & 3] + 128 * (s >> 2) + 32 * 256 * x : rt + roff[s & 3] + 32 * 128 * x;
+          s2[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), qf[s], s2[x],
+                                                          0, 0, 0);
+        }
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s2[x][r] = fmaf(s2[x][r], sl2, -m_run);
+      if ((i + 1) * XA_K > seen0) {  // keys that a query does not see
+        const int lim = seen_j - i * XA_K - 4 * h;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[x][r] = 32 * x + 8 * (r >> 2) + (r & 3) < lim ? s2[x][r] : -INFINITY;
+      }
+      float cm = s2[0][0];
+#pragma unroll
+      for (int r = 1; r < 32; ++r) cm = max_nonan(cm, s2[r >> 4][r & 15]);
+      if (i == 0 || __ballot(cm > XA_SLACK) != 0) {
+        cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
+        // a query that sees none of tile 0 sees nothing: its maximum stays finite
+        const float up = i == 0 ? max_nonan(cm, -1e30f) : cm > XA_SLACK ? cm : 0.0f;
+        const float alpha = i == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+        m_run += up;
+        l_run *= alpha;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[x][r] -= up;
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+      }
+      // P in bf16 (each weight off by 2^-8 of it at most, as everywhere in this library; the sums take it unrounded)
+      uint32_t pk[16];
+#pragma unroll
+      for (int r = 0; r < 32; r += 4) {
+        float pv[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(s2[r >> 4][(r & 15) + e]);
+        l_run += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+        pk[r / 2] = bf16_pack(pv[0], pv[1]);
+        pk[r / 2 + 1] = bf16_pack(pv[2], pv[3]);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {  // tokens 16 t .. + 15
+        const bf16x8 pb = as_bf16x8(make_uint4(pk[4 * t], pk[4 * t + 1], pk[4 * t + 2], pk[4 * t + 3]));
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const uint8_t* at = vt + voff[d & 1] + 128 * (d >> 1) + 16 * 256 * t;
+          typedef __attribute__((address_space(3))) xa_v4s* lds4;
+          const xa_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
+          const xa_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * 256));
+          typedef short v8s __attribute__((ext_vector_type(8)));
+          const v8s both = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, both), pb, o[d], 0, 0, 0);
+        }
+      }
+    }
+    stage = stage == XA_STAGES - 1 ? 0 : stage + 1;
+  }
+  __syncthreads();  // the stages are free
+  const float l = l_run + __shfl_xor(l_run, 32, WAVE);
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a query that sees nothing: 0)
+  const int rows = min(32, nq - w0);
+  if (rows <= 0) return;
+  if (lse_out && h == 0 && j < rows)
+    lse_out[(size_t)(qb + w0 + j) * H + head] = l > 0.0f ? lse_base2(m_run, l) : NEG_INF;
+  const size_t at = ((size_t)(qb + w0) * H + head) * EX_D;
+  if (out) {  // through LDS (8 KiB a wave): 256 bytes a row, piece p of row r at p ^ (r & 15), then whole rows
+    uint8_t* const st = sh.k[0] + 8192 * wave;
+    static_assert(offsetof(XaShared<DQ>, r) >= 8 * 8192, "the staged outputs");
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<uint2*>(st + 256 * j + 16 * ((4 * d + g) ^ (j & 15)) + 8 * h) =
+            make_uint2(bf16_pack(o[d][4 * g] * inv, o[d][4 * g + 1] * inv),
+                       bf16_pack(o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv));
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int r = 4 * x + (lane >> 4), p = lane & 15;
+      if (r < rows)
+        *reinterpret_cast<u32x4*>(out + at + (size_t)r * H * EX_D + 8 * p) =
+            *reinterpret_cast<const u32x4*>(st + 256 * r + 16 * (p ^ (r & 15)));
+    }
+  }
+  if (out_f32 && j < rows) {
+    float* p = out_f32 + at + (size_t)j * H * EX_D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(p + 32 * d + 8 * g) = f32x4{o[d][4 * g] * inv, o[d][4 * g + 1] * inv,
+                                                              o[d][4 * g + 2] * inv, o[d][4 * g + 3] * inv};
+  }
+}
+
+hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* table, const int* cu,
+                                const uint16_t* w, uint16_t* k, uint16_t* v, uint16_t* r, int B, int total, int H,
+                                int D, int max_pages, int page_size, int num_pages, hipStream_t s) {
+  const unsigned grid = (unsigned)((total + EL_TOK - 1) / EL_TOK) * 2 * H;
+  return launch("expand_latent_kernel", expand_latent_kernel, dim3(grid), dim3(EL_THREADS), s, kv, kvs, table, cu, w,
+                k, v, r, B, total, H, D, max_pages, page_size, num_pages);
+}
+
+// Query tiles that a batch of Tq queries in B sequences may have.
+static int attend_tiles(int B, int Tq) { return Tq / XA_Q + B; }
+
+bool expanded_grid_ok(int B, int Tq, int H) {
+  return ((long)Tq / XA_Q + B) * H <= 0x7fffffL && (long)Tq + B <= 0x7fffffffL - XA_Q;
+}
+
+hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
+                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, int B,
+                                  int Tq, int Tk, int H, int causal, float scale, hipStream_t s) {
+  const int q_tiles = attend_tiles(B, Tq);
+  const auto kernel = kr ? expanded_attend_kernel<EX_D + EX_R> : expanded_attend_kernel<EX_D>;
+  return launch("expanded_attend_kernel", kernel, dim3((unsigned)q_tiles * H), dim3(XA_THREADS), s, q, k, kr, v, cu_q,
+                cu_k, out, out_f32, lse, B, Tq, Tk, H, q_tiles, causal, scale);
+}
+
+}  // namespace dsa

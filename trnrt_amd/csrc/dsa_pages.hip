@@ -8,8 +8,8 @@
 // fork of many sequences); a small fork is its two launches. Every cache of a model takes part in one launch (up to
 // PG_CACHES of them: latent rows, their scales, indexer keys, ... of every layer), a page of each cut into 16 KiB pieces,
 // one workgroup a piece, so that one page of one sequence already spreads over several CUs.
-#include "dsa_common.h"
 #include "dsa_pages.h"
+#include "dsa_scan.h"
 
 namespace dsa {
 
@@ -55,24 +55,6 @@ __global__ __launch_bounds__(PG_THREADS) void pages_copy_kernel(PageCaches set, 
   const int a = src[i], b = dst[i];
   if ((unsigned)a >= (unsigned)num_pages || (unsigned)b >= (unsigned)num_pages || b == 0 || a == b) return;
   copy_piece(set, piece, a, b);
-}
-
-// The workgroup's inclusive prefix sum of v, and its total; tot: PG_PLAN_THREADS / WAVE ints of LDS.
-__device__ __forceinline__ int block_incl_scan(int v, int* tot, int& total) {
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-  const int x = wave_incl_scan(v);
-  __syncthreads();  // (tot's earlier readers)
-  if (lane == WAVE - 1) tot[wave] = x;
-  __syncthreads();
-  int before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < PG_PLAN_THREADS / WAVE; ++w) {
-    const int s = tot[w];
-    before += w < wave ? s : 0;
-    total += s;
-  }
-  return before + x;
 }
 
 typedef int pg_v4i __attribute__((ext_vector_type(4), aligned(4)));  // (a count array may start at any int)
@@ -122,7 +104,7 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_fork_plan_kernel(
     int part = 0;
     if (i < n) part = fork_row(parents[i], ctx_len, B, max_pages, page_size).part;
     int total;
-    block_incl_scan(part, tot, total);
+    group_incl_scan<PG_PLAN_THREADS>(part, tot, total);
     need += total;
   }
   int found = 0;  // free pages so far
@@ -133,7 +115,7 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_fork_plan_kernel(
                       r.z <= 0 && p + 2 < num_pages, r.w <= 0 && p + 3 < num_pages};
     const int mine = f[0] + f[1] + f[2] + f[3];
     int total;
-    int at = found + block_incl_scan(mine, tot, total) - mine;
+    int at = found + group_incl_scan<PG_PLAN_THREADS>(mine, tot, total) - mine;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       if (f[e]) {
@@ -149,7 +131,7 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_fork_plan_kernel(
     ForkRow f{-1, 0, false};
     if (i < n) f = fork_row(parents[i], ctx_len, B, max_pages, page_size);
     int total;
-    const int rank = rank0 + block_incl_scan(f.part, tot, total) - (int)f.part;
+    const int rank = rank0 + group_incl_scan<PG_PLAN_THREADS>(f.part, tot, total) - (int)f.part;
     rank0 += total;
     if (i < n) pages[i] = f.parent < 0 ? -1 : !f.part ? 0 : rank < found ? free_list[rank] : -1;
   }
@@ -210,7 +192,7 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_count_kernel(const int*
   const int p = blockIdx.x * PG_BLOCK + 4 * threadIdx.x;
   const pg_v4i r = load_refs(ref, p, num_pages);
   int total;
-  block_incl_scan((int)(r.x > 0 && p > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), tot, total);
+  group_incl_scan<PG_PLAN_THREADS>((int)(r.x > 0 && p > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), tot, total);
   if (threadIdx.x == 0) counts[blockIdx.x] = total;
 }
 
@@ -226,22 +208,22 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* 
   int total, before = 0, live = 0;
   for (int b0 = 0; b0 < blocks; b0 += PG_PLAN_THREADS) {
     const int c = b0 + t < blocks ? counts[b0 + t] : 0;
-    block_incl_scan(c, tot, total);
+    group_incl_scan<PG_PLAN_THREADS>(c, tot, total);
     live += total;
-    block_incl_scan(b0 + t < blk ? c : 0, tot, total);
+    group_incl_scan<PG_PLAN_THREADS>(b0 + t < blk ? c : 0, tot, total);
     before += total;
   }
   // live pages up to page `live`: whole blocks before its own, and its own up to it
   const int lb = live / PG_BLOCK;
   int front = 0;
   for (int b0 = 0; b0 < lb; b0 += PG_PLAN_THREADS) {
-    block_incl_scan(b0 + t < lb ? counts[b0 + t] : 0, tot, total);
+    group_incl_scan<PG_PLAN_THREADS>(b0 + t < lb ? counts[b0 + t] : 0, tot, total);
     front += total;
   }
   {
     const int p = lb * PG_BLOCK + 4 * t;
     const pg_v4i r = load_refs(ref, p, num_pages);
-    block_incl_scan((int)(r.x > 0 && p > 0 && p <= live) + (r.y > 0 && p + 1 <= live) + (r.z > 0 && p + 2 <= live) +
+    group_incl_scan<PG_PLAN_THREADS>((int)(r.x > 0 && p > 0 && p <= live) + (r.y > 0 && p + 1 <= live) + (r.z > 0 && p + 2 <= live) +
                         (r.w > 0 && p + 3 <= live),
                     tot, total);
     front += total;
@@ -250,7 +232,7 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* 
   const pg_v4i r = load_refs(ref, p, num_pages);
   const int f[4] = {r.x > 0 && p > 0, r.y > 0, r.z > 0, r.w > 0};
   const int mine = f[0] + f[1] + f[2] + f[3];
-  int at = before + block_incl_scan(mine, tot, total) - mine;  // live pages before this thread's
+  int at = before + group_incl_scan<PG_PLAN_THREADS>(mine, tot, total) - mine;  // live pages before this thread's
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     const int x = p + e;
