@@ -114,6 +114,7 @@ hipError_t launch_value_order(const int64_t* pools, const int64_t* cnt, const fl
                               int64_t* out_pools, float* out_vals, hipStream_t s);
 
 size_t dense_workspace_bytes(int M, int num_cu);
+bool dense_list_ok(int B, int S, int H, int max_pages, int page_size);
 hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* kvs, const int* table,
                             const int* ctx_len, uint16_t* out, float* out_f32, float* lse, void* ws, int B, int S,
                             int H, int Dqk, int max_pages, int page_size, int num_pages, float scale, int num_cu,
@@ -1291,8 +1292,8 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
                   float scale, void* stream) {
   if (B < 0 || S < 1 || H < 1 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
   if (Dqk != 512 && Dqk != 576) return DSA_EUNSUPPORTED;
-  // a cache of less than 2^31 slots; rows within a launch's 2^32 threads
-  if ((long)num_pages * page_size > 0x7fffffffL || (long)B * S > 0x7fffffffL / H / 128) return DSA_EUNSUPPORTED;
+  if ((long)num_pages * page_size > 0x7fffffffL || !dsa::dense_list_ok(B, S, H, max_pages, page_size))
+    return DSA_EUNSUPPORTED;
   if (B == 0) return DSA_OK;
   if (!q_bf16 || !kv_fp8 || !page_table || !ctx_len || (!out_bf16 && !out_f32)) return DSA_EINVAL;
   if (!workspace || workspace_bytes < dsa::dense_workspace_bytes(S * H, num_cu())) return DSA_EWORKSPACE;

@@ -47,7 +47,7 @@ __device__ __forceinline__ int dn_swizzle(int r) { return r & 7; }
 // RB: blocks of 32 rows in a tile. Buffers: chunk c being scored, c - 1 whose values are multiplied, and the rest arriving.
 template <int DQK, int RB>
 struct DnShared {
-  static constexpr int BUFS = RB == 1 ? 4 : 3;  // (160 KiB of LDS)
+  static constexpr int BUFS = RB == 1 || DQK == 512 ? 4 : 3;  // (160 KiB of LDS)
   alignas(1024) uint8_t tile[BUFS][DN_CHUNK * DQK];
   alignas(16) uint16_t p[2][32 * RB * DN_PROW];  // P[row][token] of two chunks
   alignas(16) float ksc[BUFS][DN_CHUNK];         // the chunks' token scales
@@ -76,23 +76,25 @@ __device__ __forceinline__ int dn_len(int ctx_len, int max_pages, int page_size)
 }
 __device__ __forceinline__ int dn_chunks(int len) { return (len + DN_CHUNK - 1) / DN_CHUNK; }
 
-// The number of units (sequence, row tile, chunk of tokens). Every thread of the workgroup calls this.
-template <int THREADS>
-__device__ __forceinline__ long dn_total(const int* __restrict__ ctx_len, int B, int tiles, int max_pages,
-                                         int page_size, int* tot) {
-  long units = 0;
-  for (int b0 = 0; b0 < B; b0 += THREADS) {
-    const int b = b0 + (int)threadIdx.x;
-    int total;
-    group_incl_scan<THREADS>(b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, page_size)) : 0, tot, total);
-    units += (long)total * tiles;
-  }
-  return units;
+// The list of units (sequence, row tile, chunk of tokens), in equal shares (one unit more for the first `more`).
+struct DnList {
+  int groups;  // workgroups that have a share
+  int share;
+  int more;
+};
+__device__ __forceinline__ DnList dn_list(int units, int G) {
+  DnList x;
+  x.groups = min(G, units);
+  x.share = units > 0 ? units / x.groups : 0;
+  x.more = units - x.share * x.groups;
+  return x;
 }
-
-// The first unit of workgroup w of G, and the workgroup that has unit u.
-__device__ __forceinline__ long dn_start(long w, long units, int G) { return w * units / G; }
-__device__ __forceinline__ long dn_owner(long u, long units, int G) { return ((u + 1) * G - 1) / units; }
+// The first unit of workgroup w, and the workgroup that has unit u.
+__device__ __forceinline__ int dn_start(int w, const DnList& x) { return w * x.share + min(w, x.more); }
+__device__ __forceinline__ int dn_owner(int u, const DnList& x) {
+  const int big = x.more * (x.share + 1);
+  return u < big ? u / (x.share + 1) : x.more + (u - big) / x.share;
+}
 
 template <int DQK, int RB>
 __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
@@ -105,35 +107,46 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   constexpr int STEPS = DQK / 32;           // 32 dims: one 16-byte read of a key row per lane, two products
   constexpr int TAIL = DN_CHUNK * 512;      // where the rows' last 64 bytes lie
   constexpr int LOADS = DQK == 576 ? 9 : 8;  // a chunk's asynchronous loads per value wave
+  constexpr int AHEAD = BUFS - 2;            // chunks in flight
   __shared__ Sh sh;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int M = S * H, tiles = (M + ROWS - 1) / ROWS;
   const int G = gridDim.x;
-  const int wg = (blockIdx.x & 7) * (G >> 3) + (blockIdx.x >> 3);  // (workgroup x runs on XCD x % 8; G a multiple of 8)
 
-  const long units = dn_total<DN_THREADS>(ctx_len, B, tiles, max_pages, pg.size, sh.tot);
-  const long u0 = dn_start(wg, units, G), u1 = dn_start(wg + 1, units, G);
-  if (u0 >= u1) return;
-  {  // the sequence of unit u0
-    long before = 0;
-    for (int b0 = 0; b0 < B; b0 += DN_THREADS) {
-      const int b = b0 + tid;
-      const int n = b < B ? dn_chunks(dn_len(ctx_len[b], max_pages, pg.size)) : 0;
-      int total;
-      const int incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
-      const long lo = (before + incl - n) * tiles, hi = (before + incl) * tiles;
-      if (lo <= u0 && u0 < hi) {
-        sh.found[0] = b;
-        sh.found[1] = (int)((u0 - lo) / n);
-        sh.found[2] = (int)((u0 - lo) % n);
-      }
-      before += total;
-      if (u0 < before * tiles) break;
-    }
-    if (tid < 8) sh.flag[tid >> 2][tid & 3] = 0;
-    __syncthreads();
+  // the list, and the sequence of this workgroup's first unit
+  int chunks = 0, n = 0, incl = 0;
+  for (int b0 = 0; b0 < B; b0 += DN_THREADS) {
+    const int x = b0 + tid;
+    int total;
+    n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, pg.size)) : 0;
+    incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
+    chunks += total;
   }
+  const DnList list = dn_list(chunks * tiles, G);
+  // (workgroup x runs on XCD x % 8: neighbours in the list on one XCD, and all XCDs at work however few the groups)
+  const int per_xcd = (list.groups + 7) >> 3;
+  const int wg = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per_xcd || wg >= list.groups) return;
+  const int u0 = dn_start(wg, list), u1 = dn_start(wg + 1, list);
+  for (int b0 = 0, before = 0; b0 < B && before <= u0; b0 += DN_THREADS) {
+    const int x = b0 + tid;
+    int total = 0;
+    if (B > DN_THREADS) {  // (else they are still at hand)
+      n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, pg.size)) : 0;
+      incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
+    }
+    const int lo = before + (incl - n) * tiles;
+    if (lo <= u0 && u0 < lo + n * tiles) {
+      sh.found[0] = x;
+      sh.found[1] = (u0 - lo) / n;
+      sh.found[2] = (u0 - lo) % n;
+    }
+    before += total * tiles;
+  }
+  if (tid < 8) sh.flag[tid >> 2][tid & 3] = 0;
+  __syncthreads();
+
   // scale x log2 e to twice fp32's digits: rounded, its error would be the same for every score, and so the lse's
   auto uniform = [](float x) __attribute__((always_inline)) {
     return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(x)));
@@ -141,12 +154,13 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   const float sl2 = uniform(scale * DN_LOG2E);
   const float sl2_lo = uniform(fmaf(scale, DN_LOG2E, -sl2) + scale * DN_LOG2E_LO);
   // the stretch at hand: chunks c0 .. of row tile mt of sequence b
-  int b = __builtin_amdgcn_readfirstlane(sh.found[0]), mt = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
+  int mt = __builtin_amdgcn_readfirstlane(sh.found[1]);
   int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
 
-  for (long u = u0; u < u1;) {
+  for (int u = u0; u < u1;) {
     const int len = dn_len(ctx_len[b], max_pages, pg.size), all = dn_chunks(len);
-    const int nch = (int)min((long)(all - c0), u1 - u);  // this stretch's chunks
+    const int nch = min(all - c0, u1 - u);  // this stretch's chunks
     const bool whole = nch == all;
     const int t0 = c0 * DN_CHUNK, r0 = mt * ROWS;  // its first token and row
 
@@ -156,8 +170,10 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     auto write = [&](int half) __attribute__((always_inline)) {
       const size_t slot = 2 * (size_t)wg + (u > u0);
       const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
-#pragma unroll 1
-      for (int r = wave; r < ROWS && r0 + r < M; r += DN_THREADS / WAVE) {
+#pragma unroll 4
+      for (int i = 0; i < ROWS / 8; ++i) {
+        const int r = wave + 8 * i;
+        if (r0 + r >= M) break;
         f32x4 v = area[64 * lane + (r ^ (lane & 7))];
         const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
         if (whole) {
@@ -183,21 +199,49 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
       const int th = wave >> 1, hh = wave & 1;
       const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
-      const bool works = hh < RB;
-      const int row = min(r0 + 32 * (works ? hh : 0) + j, M - 1);
+      // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece p at
+      // p ^ (r & 7), so that one piece of 8 rows covers the banks once
+      {
+        constexpr int PIECES = DQK / 8, PER = ROWS * PIECES / (4 * WAVE);
+        const uint32_t q_lds = lds_address(sh.tile[AHEAD]) + 1024 * PER * wave;
+        const int r_max = M - 1 - r0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int x = WAVE * (PER * wave + i) + lane, r = x / PIECES, p = x - r * PIECES;
+          load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ (r & 7)), q_lds + 1024 * i);
+        }
+        wait_loads<0>();
+      }
+      lds_barrier();  // the queries and chunk 0 are in place
+      if (hh >= RB) {  // no rows for this wave
+        lds_barrier();
+        for (int c = 0; c <= nch; ++c) {
+          if (c > 0) {
+            const int4 fl = *reinterpret_cast<const int4*>(sh.flag[(c - 1) & 1]);
+            if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+              lds_barrier();
+              lds_barrier();
+            }
+          }
+          lds_barrier();
+        }
+        lds_barrier();
+        write(0);
+        lds_barrier();
+        lds_barrier();
+        write(1);
+      } else {
+      const int row = min(r0 + 32 * hh + j, M - 1);
       const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
       const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
       bf16x8 qb[2 * STEPS];  // row 32 hh + j: step s holds dims 32 s + 16 h .. + 15
-      if (works) {
-        const uint16_t* qr = q + ((size_t)b * M + row) * DQK + 16 * h;
+      {
+        const uint8_t* const qr = sh.tile[AHEAD] + (32 * hh + j) * 2 * DQK;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          qb[2 * s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s));
-          qb[2 * s + 1] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 32 * s + 8));
-        }
-        arrive(qb);
+        for (int s = 0; s < 2 * STEPS; ++s)
+          qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (j & 7))));
       }
-      lds_barrier();  // chunk 0 is in place
+      lds_barrier();  // the queries are read
       float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
                            // always up
       float l_run = 0.0f;  // this lane's share of its running sum
@@ -209,7 +253,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       for (int i = 0; i < 4; ++i) koff[i] = kr * 512 + 16 * ((2 * i | h) ^ dn_swizzle(kr));
 #pragma unroll
       for (int i = 0; i < 2; ++i) ktail[i] = TAIL + kr * 64 + 16 * ((2 * i | h) ^ ((kr >> 1) & 3));
-      uint16_t* const pw = &sh.p[0][(32 * (works ? hh : 0) + j) * DN_PROW + 32 * th + 4 * h];
+      uint16_t* const pw = &sh.p[0][(32 * hh + j) * DN_PROW + 32 * th + 4 * h];
       int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
       auto four = [&](const float* a, int g) __attribute__((always_inline)) {
         return *reinterpret_cast<const f32x4*>(a + 32 * th + 8 * g + 4 * h);
@@ -231,9 +275,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 #pragma unroll
           for (int r = 1; r < 16; ++r) cm = max_nonan(cm, sv[r]);
           cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
-          if (works && h == 0) sh.cmax[th][32 * hh + j] = cm;
+          if (h == 0) sh.cmax[th][32 * hh + j] = cm;
           lds_barrier();
-          cm = max_nonan(cm, sh.cmax[th ^ 1][32 * (works ? hh : 0) + j]);
+          cm = max_nonan(cm, sh.cmax[th ^ 1][32 * hh + j]);
           // a row that sees none of chunk 0 sees none of the stretch: its maximum stays finite
           const float up = c == 0 ? max_nonan(cm, -1e30f) : cm > DN_SLACK ? cm : 0.0f;
           // chunk 0 has nothing to rescale, and its factor would be infinite where every score is at or below -128
@@ -243,11 +287,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           psum = 0.0f;
 #pragma unroll
           for (int r = 0; r < 16; ++r) sv[r] -= up;
-          if (works) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
-            if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
-          }
+          for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
+          if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
           lds_barrier();
         }
         l_run += psum;
@@ -270,49 +312,47 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         for (int s = 0; s < DN_KAHEAD; ++s) kk[s] = k_read(s);
         __builtin_amdgcn_sched_barrier(0);
         settle(c - 1, fl);
-        if (works) {
-          ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
-          kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
+        ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
+        kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
 #pragma unroll
-          for (int s = 0; s < STEPS; ++s) {
-            if (s + DN_KAHEAD < STEPS) kk[(s + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(s + DN_KAHEAD);
-            sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[s & 1], qb[2 * s], sa, 0, 0, 0);
-            sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[s & 1], qb[2 * s + 1], sa, 0, 0, 0);
-            if (s + 1 < STEPS) {
-              const u32x4 k1 = kk[(s + 1) % (DN_KAHEAD + 1)];
-              ka[(s + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
-              kb[(s + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
-            }
-            if (s == STEPS - 2) {
-              ks[0] = four(sh.ksc[buf], 0);
-              kx[0] = four(sh.kfac[buf], 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        for (int s = 0; s < STEPS; ++s) {
+          if (s + DN_KAHEAD < STEPS) kk[(s + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(s + DN_KAHEAD);
+          sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[s & 1], qb[2 * s], sa, 0, 0, 0);
+          sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[s & 1], qb[2 * s + 1], sa, 0, 0, 0);
+          if (s + 1 < STEPS) {
+            const u32x4 k1 = kk[(s + 1) % (DN_KAHEAD + 1)];
+            ka[(s + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
+            kb[(s + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
           }
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (g < 3) kx[(g + 1) & 1] = four(sh.kfac[buf], g + 1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sv[4 * g + e] = fmaf(sa[4 * g + e], kx[g & 1][e], -m_run);
+          if (s == STEPS - 2) {
+            ks[0] = four(sh.ksc[buf], 0);
+            kx[0] = four(sh.kfac[buf], 0);
           }
-          if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
-            const int lim = seen - t0 - c * DN_CHUNK - 32 * th - 4 * h;
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sv[4 * g + e] = 8 * g + e < lim ? sv[4 * g + e] : -INFINITY;
-          }
-          float cm = -INFINITY;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (g < 3) ks[(g + 1) & 1] = four(sh.ksc[buf], g + 1);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) cm = max_nonan(cm, sv[4 * g + e]);
-            p_group(c, g, ks[g & 1]);
-          }
-          const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
-          if (lane == 0) sh.flag[c & 1][wave] = any;
+          __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (g < 3) kx[(g + 1) & 1] = four(sh.kfac[buf], g + 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sv[4 * g + e] = fmaf(sa[4 * g + e], kx[g & 1][e], -m_run);
+        }
+        if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
+          const int lim = seen - t0 - c * DN_CHUNK - 32 * th - 4 * h;
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sv[4 * g + e] = 8 * g + e < lim ? sv[4 * g + e] : -INFINITY;
+        }
+        float cm = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          if (g < 3) ks[(g + 1) & 1] = four(sh.ksc[buf], g + 1);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cm = max_nonan(cm, sv[4 * g + e]);
+          p_group(c, g, ks[g & 1]);
+        }
+        const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
+        if (lane == 0) sh.flag[c & 1][wave] = any;
         last = buf;
         buf = buf == BUFS - 1 ? 0 : buf + 1;
         lds_barrier();
@@ -320,22 +360,24 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       __builtin_amdgcn_s_setprio(0);
       settle(nch - 1, flags(nch - 1));
       const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
-      if (works && h == 0) sh.lsum[th][32 * hh + j] = lw;
-      if (works && th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
+      if (h == 0) sh.lsum[th][32 * hh + j] = lw;
+      if (th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
       lds_barrier();  // the tiles are free
       lds_barrier();  // the first 256 dims' outputs are in LDS
       write(0);
       lds_barrier();
       lds_barrier();  // and the others'
       write(1);
+      }
     } else {
       // -- the loads and the values: wave w brings rows 16 w .. + 15 of a chunk, takes dims 128 w .. + 127 of all rows --
       const int w = wave - 4;
       const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
       const int* trow = table + (size_t)b * max_pages;
-      // token `lane` of chunk c, the sequence's last one past its end (a slot behind it may never have been written, and
-      // its NaN x weight 0 is NaN)
-      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + lane, len - 1); };
+      // token `lane` of chunk c, the stretch's last one past its end (a slot behind the sequence may never have been
+      // written, and its NaN x weight 0 is NaN)
+      const int t_last = min(t0 + nch * DN_CHUNK, len) - 1;
+      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + lane, t_last); };
       auto page_of = [&](int t) __attribute__((always_inline)) { return (int)((uint64_t)t * pg.mul >> pg.shift); };
       const int mrow = 4 * (16 * w + h), trw = 4 * (16 * w + (lane >> 2));
       int mcol[4];  // load k < 8 brings rows 16 w + 2 k and + 1, load 8 the last pieces of all 16
@@ -346,31 +388,26 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       const uint32_t ksc_lds = lds_address(sh.ksc[0]), page_lds = lds_address(sh.page[0]);
       if (!kvs)
         for (int i = 0; i < BUFS; ++i) sh.ksc[i][lane] = 1.0f;
-      // chunk c's loads into buffer `to`, and its scales and the pages of chunk c + 2 (every value wave the same ones, so
-      // that each waits for its own); `page`: of this lane's token
-      auto issue = [&](int c, int to, int page) __attribute__((always_inline)) {
+      // chunk c's loads into buffer `to`: begin() its scales and the pages of chunk c + 2 (every value wave the same ones,
+      // so that each waits for its own; `page`: of this lane's token) and where its rows lie, then load() k < LOADS
+      unsigned src[LOADS];
+      auto begin = [&](int c, int to, int page) __attribute__((always_inline)) {
         const int t = token(c);
         const int slot = safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
         load_lds4(trow + page_of(token(c + 2)), page_lds + 4 * DN_CHUNK * ((c + 2) & 3));
         if (kvs) load_lds4(kvs + slot, ksc_lds + 4 * DN_CHUNK * to);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(mrow + 8 * k, slot);
-          load_lds16(kv + (size_t)s * DQK + mcol[k & 3], tile_lds + DN_CHUNK * DQK * to + 1024 * k);
-        }
-        if (DQK == 576) {
-          const unsigned s = (unsigned)__builtin_amdgcn_ds_bpermute(trw, slot);
-          load_lds16(kv + (size_t)s * DQK + tcol, tail_lds + DN_CHUNK * DQK * to);
-        }
+        for (int k = 0; k < LOADS; ++k)
+          src[k] = (unsigned)__builtin_amdgcn_ds_bpermute(k < 8 ? mrow + 8 * k : trw, slot);
       };
-      constexpr int AHEAD = BUFS - 2;  // chunks in flight
-      // chunk `to`'s loads have landed (`more`: with those of the AHEAD - 1 chunks after it out), and so the pages two
-      // chunks on; then the tokens' factors
-      auto landed = [&](int to, bool more) __attribute__((always_inline)) {
-        if (more)
-          wait_loads<(AHEAD - 1) * (LOADS + 1)>();
-        else
-          wait_loads<0>();
+      auto load = [&](int k, int to) __attribute__((always_inline)) {
+        load_lds16(kv + (size_t)src[k] * DQK + (k < 8 ? mcol[k & 3] : tcol),
+                   (k < 8 ? tile_lds + 1024 * k : tail_lds) + DN_CHUNK * DQK * to);
+      };
+      // chunk `to`'s loads have landed, with those of the AHEAD - 1 chunks after it out, and so the pages two chunks on; then
+      // the tokens' factors
+      auto landed = [&](int to) __attribute__((always_inline)) {
+        wait_loads<(AHEAD - 1) * (LOADS + 1)>();
         if (w == 0) {
           const float k = sh.ksc[to][lane];
           sh.kfac[to][lane] = fmaf(k, sl2, k * sl2_lo);
@@ -395,13 +432,21 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
         return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * ROWS * DN_PROW + 32 * i * DN_PROW + 16 * t));
       };
-      // chunk c's weights are final after this (and O on their maxima)
-      auto settle = [&](int c) __attribute__((always_inline)) {
-        const int4 fl = *reinterpret_cast<const int4*>(sh.flag[c & 1]);
+      // Interval c: chunk c - 1's weights are final (and O on their maxima) once its flags are seen; then its value product,
+      // 16 steps of RB products, the next steps' operands read and converted ahead, with chunk c + AHEAD's loads (into
+      // buffer `to`) spread over the steps: their issue waits on each other's.
+      auto interval = [&](int c, const uint8_t* kt, int to) __attribute__((always_inline)) {
+        const int pb = (c - 1) & 1;
+        const int4 fl = *reinterpret_cast<const int4*>(sh.flag[pb]);
+        const int page = sh.page[(c + AHEAD) & 3][lane];
+        dn_v2i vv[DN_VAHEAD + 1];
+        bf16x8 pa[2][RB], vb[2];
+#pragma unroll
+        for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
         if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
           lds_barrier();
           lds_barrier();
-          if (c > 0) {  // O is zero before
+          if (c > 1) {  // O is zero before
 #pragma unroll
             for (int i = 0; i < RB; ++i) {
               const float a = sh.al[32 * i + j];
@@ -412,16 +457,11 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             }
           }
         }
-      };
-      // a chunk's value product: 16 steps of RB products, the next steps' operands read and converted ahead
-      auto value = [&](const uint8_t* kt, int pb) __attribute__((always_inline)) {
-        dn_v2i vv[DN_VAHEAD + 1];
-        bf16x8 pa[2][RB], vb[2];
-#pragma unroll
-        for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
 #pragma unroll
         for (int i = 0; i < RB; ++i) pa[0][i] = p_read(pb, 0, i);
+        begin(c + AHEAD, to, page);
         vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = i >> 2, d = i & 3;
@@ -434,31 +474,41 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
             vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
           }
+#pragma unroll
+          for (int k = 0; k < LOADS; ++k)
+            if (k * 15 / LOADS + 1 == i) load(k, to);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      {
-        const int p0 = trow[page_of(token(0))], p1 = trow[page_of(token(1))];
-        if (AHEAD == 1) sh.page[1][lane] = p1;
-        issue(0, 0, p0);
-        if (AHEAD == 2 && nch > 1) issue(1, 1, p1);
+      sh.page[0][lane] = trow[page_of(token(0))];
+      sh.page[1][lane] = trow[page_of(token(1))];
+#pragma unroll
+      for (int c = 0; c < AHEAD; ++c) {
+        begin(c, c, sh.page[c][lane]);
+#pragma unroll
+        for (int k = 0; k < LOADS; ++k) load(k, c);
       }
-      landed(0, AHEAD == 2 && nch > 1);
-      lds_barrier();  // chunk 0 is in place
-      int buf = 0;   // chunk c's buffer
-      for (int c = 0; c < nch; ++c) {
+      landed(0);
+      lds_barrier();  // the queries and chunk 0 are in place
+      lds_barrier();  // the queries are read
+      // chunk c + AHEAD goes into the buffer that chunk c - 2 left, in the last intervals too (the stretch's last row then,
+      // into buffers that nobody reads: the loop stays one piece)
+      begin(AHEAD, AHEAD, sh.page[AHEAD][lane]);
+#pragma unroll
+      for (int k = 0; k < LOADS; ++k) load(k, AHEAD);
+      int buf = 1;  // chunk c's buffer
+      landed(1);
+      lds_barrier();
+#pragma unroll 1
+      for (int c = 1; c <= nch; ++c) {
         const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
-        if (c > 0) settle(c - 1);
-        // chunk c + AHEAD into the buffer that chunk c - 2 left
-        if (c + AHEAD < nch) issue(c + AHEAD, prev == 0 ? BUFS - 1 : prev - 1, sh.page[(c + AHEAD) & 3][lane]);
-        if (c > 0) value(sh.tile[prev], (c - 1) & 1);
-        if (c + 1 < nch) landed(next, c + AHEAD < nch);
+        const int to = prev == 0 ? BUFS - 1 : prev - 1;
+        interval(c, sh.tile[prev], to);
+        if (c == nch) wait_loads<0>();  // the tiles are free
+        landed(next);
         buf = next;
         lds_barrier();
       }
-      settle(nch - 1);
-      value(sh.tile[buf == 0 ? BUFS - 1 : buf - 1], (nch - 1) & 1);
-      lds_barrier();  // the tiles are free
       auto store = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < RB; ++i)
@@ -490,58 +540,115 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   }
 }
 
-constexpr int DC_THREADS = 128;  // a workgroup: one row's 512 outputs
+// Joins the partials of a row where its row tile was shared: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the
+// rows of sequences without tokens. Four partials are in flight in a wave, each lane has 8 of the dims. WPR waves a row: a
+// wave takes every WPR-th partial.
+constexpr int DC_WAVES = 8;
+constexpr int DC_THREADS = DC_WAVES * WAVE;
 
-// Joins the partials of row blockIdx.x where its row tile was shared: out = sum 2^(m - max) O / sum 2^(m - max) l; and
-// writes the rows of sequences without tokens.
+template <int WPR>
 __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ ctx_len,
     uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H, int rows,
     int G, int max_pages, int page_size) {
-  __shared__ int tot[DC_THREADS / WAVE];
-  const int M = S * H, tiles = (M + rows - 1) / rows, t = threadIdx.x;
-  const int b = blockIdx.x / M, row = blockIdx.x - b * M, mt = row / rows, j = row - mt * rows;
-  long units = 0, before = 0;
+  __shared__ int tot[DC_WAVES];
+  __shared__ int chunks_before[DC_WAVES];
+  __shared__ float wm[DC_WAVES], wl[DC_WAVES];
+  __shared__ alignas(16) float acc[WPR > 1 ? DC_WAVES : 1][DN_DV];
+  const int M = S * H, tiles = (M + rows - 1) / rows, tid = threadIdx.x;
+  const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  // this wave's row (the last one again past the end, not written)
+  const int at_row = blockIdx.x * (DC_WAVES / WPR) + wave / WPR, g = min(at_row, B * M - 1);
+  const int b = g / M, row = g - b * M, mt = row / rows, j = row - mt * rows;
+  const int first_b = __builtin_amdgcn_readfirstlane(min(blockIdx.x * (DC_WAVES / WPR), B * M - 1) / M);
+  int chunks = 0;
   for (int b0 = 0; b0 < B; b0 += DC_THREADS) {
-    const int x = b0 + t;
+    const int x = b0 + tid;
     const int n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, page_size)) : 0;
     int total;
-    group_incl_scan<DC_THREADS>(n, tot, total);
-    units += total;
-    group_incl_scan<DC_THREADS>(x < b ? n : 0, tot, total);
-    before += total;
+    const int incl = chunks + group_incl_scan<DC_THREADS>(n, tot, total);
+    if (x >= first_b && x < first_b + DC_WAVES) chunks_before[x - first_b] = incl - n;  // (rows of 8 sequences at most)
+    chunks += total;
   }
-  units *= tiles;
+  __syncthreads();
+  const DnList list = dn_list(chunks * tiles, G);
   const int nch = dn_chunks(dn_len(ctx_len[b], max_pages, page_size));
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  float lse = NEG_INF;
-  if (nch > 0) {
-    const long first = before * tiles + (long)mt * nch;  // the row tile's units: first .. first + nch - 1
-    const int w0 = (int)dn_owner(first, units, G), w1 = (int)dn_owner(first + nch - 1, units, G);
-    if (w0 == w1) return;  // written by its workgroup
+  const int first = chunks_before[b - first_b] * tiles + mt * nch;  // the row tile's units: first .. first + nch - 1
+  const int w0 = nch ? dn_owner(first, list) : 0, w1 = nch ? dn_owner(first + nch - 1, list) : -1;
+  const bool live = at_row < B * M && w0 != w1;  // (one workgroup's: it wrote them)
+  if (WPR > 1 && !live) return;                  // (the whole workgroup)
+  float m = -INFINITY, l = 0.0f;
+  f32x4 a[2] = {};
+  if (live && nch > 0) {
     // workgroup w0's stretch is its second one where it started before the tile, the others' is their first
-    const size_t slot0 = 2 * (size_t)w0 + (dn_start(w0, units, G) < first);
-    auto slot = [&](int w) __attribute__((always_inline)) { return (w == w0 ? slot0 : 2 * (size_t)w) * rows + j; };
-    float mm = -INFINITY, ll = 0.0f;
-    for (int w = w0; w <= w1; ++w)
-      if (dn_start(w, units, G) < dn_start(w + 1, units, G)) mm = max_nonan(mm, ws_ml[2 * slot(w)]);
-    for (int w = w0; w <= w1; ++w) {
-      if (dn_start(w, units, G) >= dn_start(w + 1, units, G)) continue;  // a workgroup without work
-      const float f = __builtin_amdgcn_exp2f(ws_ml[2 * slot(w)] - mm);
-      ll += f * ws_ml[2 * slot(w) + 1];
-      const f32x4 v = *reinterpret_cast<const f32x4*>(ws_o + slot(w) * DN_DV + 4 * t);
+    const int slot0 = 2 * w0 + (dn_start(w0, list) < first);
+    for (int w = w0 + wave % WPR; w <= w1; w += 4 * WPR) {
+      float pm[4], pl[4];
+      f32x4 v[4][2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+      for (int i = 0; i < 4; ++i) {
+        const int x = min(w + WPR * i, w1);
+        const size_t s = (size_t)(x == w0 ? slot0 : 2 * x) * rows + j;
+        pm[i] = ws_ml[2 * s];
+        pl[i] = ws_ml[2 * s + 1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[i][e] = *reinterpret_cast<const f32x4*>(ws_o + s * DN_DV + 256 * e + 4 * lane);
+      }
+      float mx = m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = max_nonan(mx, pm[i]);  // (past w1: the last one again, of weight 0 below)
+      const float f = __builtin_amdgcn_exp2f(m - mx);
+      m = mx;
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) a[e][x] *= f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float c = w + WPR * i <= w1 ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.0f;
+        l = fmaf(c, pl[i], l);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) a[e][x] = fmaf(c, v[i][e][x], a[e][x]);
+      }
     }
-    const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] *= inv;
-    if (ll > 0.0f) lse = lse_base2(mm, ll);
   }
-  const size_t at = (size_t)blockIdx.x * DN_DV + 4 * t;
-  if (out) *reinterpret_cast<uint2*>(out + at) = make_uint2(bf16_pack(acc[0], acc[1]), bf16_pack(acc[2], acc[3]));
-  if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at) = acc;
-  if (lse_out && t == 0) lse_out[blockIdx.x] = lse;
+  if (WPR == 1) {
+    if (!live) return;
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const size_t at = (size_t)g * DN_DV + 256 * e + 4 * lane;
+      const f32x4 v = {a[e][0] * inv, a[e][1] * inv, a[e][2] * inv, a[e][3] * inv};
+      if (out) *reinterpret_cast<uint2*>(out + at) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+      if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at) = v;
+    }
+    if (lse_out && lane == 0) lse_out[g] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+    return;
+  }
+  if (lane == 0) {
+    wm[wave] = m;
+    wl[wave] = l;
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) *reinterpret_cast<f32x4*>(&acc[wave % (WPR > 1 ? DC_WAVES : 1)][256 * e + 4 * lane]) = a[e];
+  __syncthreads();
+  float mm = wm[0], ll = 0.0f, o = 0.0f;
+#pragma unroll
+  for (int w = 1; w < DC_WAVES; ++w) mm = max_nonan(mm, wm[w]);
+#pragma unroll
+  for (int w = 0; w < DC_WAVES; ++w) {
+    const float f = mm > -INFINITY ? __builtin_amdgcn_exp2f(wm[w] - mm) : 0.0f;  // (0 for a wave without partials)
+    ll = fmaf(f, wl[w], ll);
+    o = fmaf(f, acc[WPR > 1 ? w : 0][tid], o);
+  }
+  const size_t at = (size_t)g * DN_DV + tid;
+  const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+  if (out) out[at] = f32_to_bf16_bits(o * inv);
+  if (out_f32) out_f32[at] = o * inv;
+  if (lse_out && tid == 0) lse_out[g] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
 }
 
 // Workgroups: one a CU, a multiple of the 8 XCDs.
@@ -568,8 +675,21 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
   const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
                               out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale);
   if (e != hipSuccess) return e;
-  return launch("dense_combine_kernel", dense_combine_kernel, dim3(B * S * H), dim3(DC_THREADS), s, ws_o, ws_ml,
-                ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+  // partials of a row tile: a share of the workgroups, and one more; a wave a row where its first four are most of them
+  // (512 rows of 33 partials: 8.7 us in 8 waves a row; 3,072 rows of 6: 19.0 in 8 waves a row)
+  const long row_tiles = (long)B * ((S * H + rows - 1) / rows), all = (long)B * S * H;
+  if (G >= 7 * row_tiles)
+    return launch("dense_combine_kernel", dense_combine_kernel<DC_WAVES>, dim3((unsigned)all), dim3(DC_THREADS), s,
+                  ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+  return launch("dense_combine_kernel", dense_combine_kernel<1>, dim3((unsigned)((all + DC_WAVES - 1) / DC_WAVES)),
+                dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+}
+
+// Whether the list of units fits 32 bits, whatever the lengths, and the rows a launch.
+bool dense_list_ok(int B, int S, int H, int max_pages, int page_size) {
+  const long M = (long)S * H, tiles = (M + 31) / 32, cap = (long)max_pages * page_size;
+  const long tokens = cap < 0x7fffffffL ? cap : 0x7fffffffL;
+  return M <= 0x7fffffffL && (long)B * M <= 0x7fffffL && (double)B * tiles * (tokens / DN_CHUNK + 1) < 2e9;
 }
 
 }  // namespace dsa
