@@ -131,6 +131,14 @@ def test_long_and_ragged(H):
     check(make([40000, 0, 3, 0, 0, 9000, 128, 20001], 1, H, 576, 64, seed=H), 64)
 
 
+@pytest.mark.parametrize("H,S,lens", [(64, 11, [700, 40, 0, 130]), (128, 20, [300, 90]), (128, 70, [200]), (16, 150, [1000, 149])])
+def test_many_row_tiles(H, S, lens):
+    """More row tiles than an XCD has CUs, and numbers of them that do not divide its CUs; appends longer than their
+    sequence's earlier tokens."""
+    say("dense row tiles", H, S, lens)
+    check(make(lens, S, H, 576 if S < 50 else 512, 64, seed=S), 64)
+
+
 def test_many_short_sequences():
     say("dense 1,100 sequences")
     g = torch.Generator().manual_seed(0)

@@ -76,20 +76,31 @@ __device__ __forceinline__ int dn_len(int ctx_len, int max_pages, int page_size)
 }
 __device__ __forceinline__ int dn_chunks(int len) { return (len + DN_CHUNK - 1) / DN_CHUNK; }
 
-// The list of units (sequence, row tile, chunk of tokens), in equal shares (one unit more for the first `more`).
+// How a sequence's row tiles go to workgroups: `span` neighbours on one XCD are a team, with the same stretch of chunks and
+// a tile each, so that they read the cache through one L2 at one time; more tiles than that are `sets` of span tiles, one
+// after another in the list. `teams` of them share the list.
+struct DnTeams {
+  int rows;   // of a tile
+  int tiles;
+  int span;
+  int sets;
+  int teams;
+};
+
+// The list of units (sequence, set of row tiles, chunk of tokens), in equal shares (one unit more for the first `more`).
 struct DnList {
-  int groups;  // workgroups that have a share
+  int teams;  // that have a share
   int share;
   int more;
 };
-__device__ __forceinline__ DnList dn_list(int units, int G) {
+__device__ __forceinline__ DnList dn_list(int units, int teams) {
   DnList x;
-  x.groups = min(G, units);
-  x.share = units > 0 ? units / x.groups : 0;
-  x.more = units - x.share * x.groups;
+  x.teams = min(teams, units);
+  x.share = units > 0 ? units / x.teams : 0;
+  x.more = units - x.share * x.teams;
   return x;
 }
-// The first unit of workgroup w, and the workgroup that has unit u.
+// The first unit of team w, and the team that has unit u.
 __device__ __forceinline__ int dn_start(int w, const DnList& x) { return w * x.share + min(w, x.more); }
 __device__ __forceinline__ int dn_owner(int u, const DnList& x) {
   const int big = x.more * (x.share + 1);
@@ -101,7 +112,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const uint16_t* __restrict__ q, const uint8_t* __restrict__ kv, const float* __restrict__ kvs,
     const int* __restrict__ table, const int* __restrict__ ctx_len, uint16_t* __restrict__ out,
     float* __restrict__ out_f32, float* __restrict__ lse_out, float* __restrict__ ws_o, float* __restrict__ ws_ml,
-    int B, int S, int H, int max_pages, DnPage pg, int num_pages, float scale) {
+    int B, int S, int H, int max_pages, DnPage pg, int num_pages, float scale, DnTeams tm) {
   typedef DnShared<DQK, RB> Sh;
   constexpr int ROWS = 32 * RB, BUFS = Sh::BUFS;
   constexpr int STEPS = DQK / 32;           // 32 dims: one 16-byte read of a key row per lane, two products
@@ -111,10 +122,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   __shared__ Sh sh;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int M = S * H, tiles = (M + ROWS - 1) / ROWS;
-  const int G = gridDim.x;
+  const int M = S * H;
 
-  // the list, and the sequence of this workgroup's first unit
+  // the list, and the sequence of this team's first unit
   int chunks = 0, n = 0, incl = 0;
   for (int b0 = 0; b0 < B; b0 += DN_THREADS) {
     const int x = b0 + tid;
@@ -123,12 +133,12 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
     chunks += total;
   }
-  const DnList list = dn_list(chunks * tiles, G);
-  // (workgroup x runs on XCD x % 8: neighbours in the list on one XCD, and all XCDs at work however few the groups)
-  const int per_xcd = (list.groups + 7) >> 3;
-  const int wg = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd || wg >= list.groups) return;
-  const int u0 = dn_start(wg, list), u1 = dn_start(wg + 1, list);
+  const DnList list = dn_list(chunks * tm.sets, tm.teams);
+  // (workgroup x runs on XCD x % 8: neighbours in the list on one XCD, and all XCDs at work however few the teams)
+  const int per_xcd = (list.teams + 7) >> 3, place = blockIdx.x >> 3;
+  const int team = (blockIdx.x & 7) * per_xcd + place / tm.span, member = place % tm.span;
+  if (place / tm.span >= per_xcd || team >= list.teams) return;
+  const int u0 = dn_start(team, list), u1 = dn_start(team + 1, list);
   for (int b0 = 0, before = 0; b0 < B && before <= u0; b0 += DN_THREADS) {
     const int x = b0 + tid;
     int total = 0;
@@ -136,13 +146,13 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, pg.size)) : 0;
       incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
     }
-    const int lo = before + (incl - n) * tiles;
-    if (lo <= u0 && u0 < lo + n * tiles) {
+    const int lo = before + (incl - n) * tm.sets;
+    if (lo <= u0 && u0 < lo + n * tm.sets) {
       sh.found[0] = x;
       sh.found[1] = (u0 - lo) / n;
       sh.found[2] = (u0 - lo) % n;
     }
-    before += total * tiles;
+    before += total * tm.sets;
   }
   if (tid < 8) sh.flag[tid >> 2][tid & 3] = 0;
   __syncthreads();
@@ -153,22 +163,23 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   };
   const float sl2 = uniform(scale * DN_LOG2E);
   const float sl2_lo = uniform(fmaf(scale, DN_LOG2E, -sl2) + scale * DN_LOG2E_LO);
-  // the stretch at hand: chunks c0 .. of row tile mt of sequence b
+  // the stretch at hand: chunks c0 .. of set `set` of sequence b
   int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
-  int mt = __builtin_amdgcn_readfirstlane(sh.found[1]);
+  int set = __builtin_amdgcn_readfirstlane(sh.found[1]);
   int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
 
   for (int u = u0; u < u1;) {
     const int len = dn_len(ctx_len[b], max_pages, pg.size), all = dn_chunks(len);
     const int nch = min(all - c0, u1 - u);  // this stretch's chunks
     const bool whole = nch == all;
-    const int t0 = c0 * DN_CHUNK, r0 = mt * ROWS;  // its first token and row
+    const int t0 = c0 * DN_CHUNK, r0 = (set * tm.span + member) * ROWS;  // its first token, and this workgroup's row
+    const int part = (2 * team + (u > u0)) * tm.span + member;            // where its partials go
+    if (r0 < M) {  // (else the last set has no tile for this member)
 
     // the outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x & 7)), so that a
     // row's pieces in order and a piece's rows in order both cover the banks once; a wave writes whole rows
     f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
     auto write = [&](int half) __attribute__((always_inline)) {
-      const size_t slot = 2 * (size_t)wg + (u > u0);
       const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
 #pragma unroll 4
       for (int i = 0; i < ROWS / 8; ++i) {
@@ -186,10 +197,10 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
           if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
         } else {
-          *reinterpret_cast<f32x4*>(ws_o + (slot * ROWS + r) * DN_DV + dim) = v;
+          *reinterpret_cast<f32x4*>(ws_o + ((size_t)part * ROWS + r) * DN_DV + dim) = v;
           if (half == 0 && lane == 0) {
-            ws_ml[2 * (slot * ROWS + r)] = m;
-            ws_ml[2 * (slot * ROWS + r) + 1] = l;
+            ws_ml[2 * ((size_t)part * ROWS + r)] = m;
+            ws_ml[2 * ((size_t)part * ROWS + r) + 1] = l;
           }
         }
       }
@@ -530,10 +541,11 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       write(1);
     }
     lds_barrier();  // (the area's readers, before the next stretch's loads)
+    }
     u += nch;
     c0 = 0;
-    if (u < u1 && ++mt == tiles) {  // the next sequence with tokens
-      mt = 0;
+    if (u < u1 && ++set == tm.sets) {  // the next sequence with tokens
+      set = 0;
       do ++b;
       while (ctx_len[b] <= 0);
     }
@@ -549,17 +561,17 @@ constexpr int DC_THREADS = DC_WAVES * WAVE;
 template <int WPR>
 __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ ctx_len,
-    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H, int rows,
-    int G, int max_pages, int page_size) {
+    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H,
+    int max_pages, int page_size, DnTeams tm) {
   __shared__ int tot[DC_WAVES];
   __shared__ int chunks_before[DC_WAVES];
   __shared__ float wm[DC_WAVES], wl[DC_WAVES];
   __shared__ alignas(16) float acc[WPR > 1 ? DC_WAVES : 1][DN_DV];
-  const int M = S * H, tiles = (M + rows - 1) / rows, tid = threadIdx.x;
+  const int M = S * H, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   // this wave's row (the last one again past the end, not written)
   const int at_row = blockIdx.x * (DC_WAVES / WPR) + wave / WPR, g = min(at_row, B * M - 1);
-  const int b = g / M, row = g - b * M, mt = row / rows, j = row - mt * rows;
+  const int b = g / M, row = g - b * M, mt = row / tm.rows, j = row - mt * tm.rows;
   const int first_b = __builtin_amdgcn_readfirstlane(min(blockIdx.x * (DC_WAVES / WPR), B * M - 1) / M);
   int chunks = 0;
   for (int b0 = 0; b0 < B; b0 += DC_THREADS) {
@@ -571,16 +583,17 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     chunks += total;
   }
   __syncthreads();
-  const DnList list = dn_list(chunks * tiles, G);
+  const DnList list = dn_list(chunks * tm.sets, tm.teams);
   const int nch = dn_chunks(dn_len(ctx_len[b], max_pages, page_size));
-  const int first = chunks_before[b - first_b] * tiles + mt * nch;  // the row tile's units: first .. first + nch - 1
+  // the row tile's units: first .. first + nch - 1
+  const int first = chunks_before[b - first_b] * tm.sets + mt / tm.span * nch;
   const int w0 = nch ? dn_owner(first, list) : 0, w1 = nch ? dn_owner(first + nch - 1, list) : -1;
-  const bool live = at_row < B * M && w0 != w1;  // (one workgroup's: it wrote them)
+  const bool live = at_row < B * M && w0 != w1;  // (one team's: its workgroup wrote them)
   if (WPR > 1 && !live) return;                  // (the whole workgroup)
   float m = -INFINITY, l = 0.0f;
   f32x4 a[2] = {};
   if (live && nch > 0) {
-    // workgroup w0's stretch is its second one where it started before the tile, the others' is their first
+    // team w0's stretch is not its first where it started before the tile, the others' is
     const int slot0 = 2 * w0 + (dn_start(w0, list) < first);
     for (int w = w0 + wave % WPR; w <= w1; w += 4 * WPR) {
       float pm[4], pl[4];
@@ -588,7 +601,7 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int x = min(w + WPR * i, w1);
-        const size_t s = (size_t)(x == w0 ? slot0 : 2 * x) * rows + j;
+        const size_t s = ((size_t)(x == w0 ? slot0 : 2 * x) * tm.span + mt % tm.span) * tm.rows + j;
         pm[i] = ws_ml[2 * s];
         pl[i] = ws_ml[2 * s + 1];
 #pragma unroll
@@ -656,33 +669,56 @@ static int dense_grid(int num_cu) { return num_cu < 8 ? 8 : num_cu / 8 * 8; }
 
 static int dense_rows(int M) { return M <= 32 ? 32 : 64; }
 
+// The teams of M rows: of the spans that divide the tiles and an XCD's CUs with the least left idle, the widest.
+static DnTeams dense_teams(int M, int num_cu) {
+  const int per_xcd = dense_grid(num_cu) / 8;
+  DnTeams t;
+  t.rows = dense_rows(M);
+  t.tiles = (int)(((long)M + t.rows - 1) / t.rows);
+  double best = 0.0;
+  for (int span = 1; span <= t.tiles && span <= per_xcd; ++span) {
+    if (span == 1 && t.tiles > 1 && per_xcd > 1) continue;  // (two tiles at least read the cache together)
+    const int sets = (t.tiles + span - 1) / span, teams = per_xcd / span;
+    const double used = (double)t.tiles / ((double)sets * span) * (teams * span) / per_xcd;
+    if (used >= best) {
+      best = used;
+      t.span = span;
+      t.sets = sets;
+      t.teams = 8 * teams;
+    }
+  }
+  return t;
+}
+
 size_t dense_workspace_bytes(int M, int num_cu) {
-  return (size_t)2 * dense_grid(num_cu) * dense_rows(M) * (DN_DV + 2) * sizeof(float);
+  const DnTeams t = dense_teams(M, num_cu);
+  return (size_t)2 * t.teams * t.span * t.rows * (DN_DV + 2) * sizeof(float);
 }
 
 hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* kvs, const int* table,
                             const int* ctx_len, uint16_t* out, float* out_f32, float* lse, void* ws, int B, int S,
                             int H, int Dqk, int max_pages, int page_size, int num_pages, float scale, int num_cu,
                             hipStream_t s) {
-  const int G = dense_grid(num_cu), rows = dense_rows(S * H);
+  const DnTeams tm = dense_teams(S * H, num_cu);
+  const int G = dense_grid(num_cu);
   int log2 = 0;
   while ((1L << log2) < page_size) ++log2;
   const DnPage pg = {(uint32_t)(((1ull << (31 + log2)) + page_size - 1) / page_size), 31 + log2, page_size};
   float* ws_o = static_cast<float*>(ws);
-  float* ws_ml = ws_o + (size_t)2 * G * rows * DN_DV;
-  const auto kernel = rows == 32 ? Dqk == 512 ? dense_mla_kernel<512, 1> : dense_mla_kernel<576, 1>
-                                 : Dqk == 512 ? dense_mla_kernel<512, 2> : dense_mla_kernel<576, 2>;
+  float* ws_ml = ws_o + (size_t)2 * tm.teams * tm.span * tm.rows * DN_DV;
+  const auto kernel = tm.rows == 32 ? Dqk == 512 ? dense_mla_kernel<512, 1> : dense_mla_kernel<576, 1>
+                                    : Dqk == 512 ? dense_mla_kernel<512, 2> : dense_mla_kernel<576, 2>;
   const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
-                              out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale);
+                              out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale, tm);
   if (e != hipSuccess) return e;
-  // partials of a row tile: a share of the workgroups, and one more; a wave a row where its first four are most of them
-  // (512 rows of 33 partials: 8.7 us in 8 waves a row; 3,072 rows of 6: 19.0 in 8 waves a row)
-  const long row_tiles = (long)B * ((S * H + rows - 1) / rows), all = (long)B * S * H;
-  if (G >= 7 * row_tiles)
+  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a row where its first four are
+  // most of them (512 rows of 33 partials: 8.4 us in 8 waves a row; 3,072 rows of 6: 11.1 in one, 19.0 in 8)
+  const long all = (long)B * S * H;
+  if (tm.teams >= 7L * B * tm.sets)
     return launch("dense_combine_kernel", dense_combine_kernel<DC_WAVES>, dim3((unsigned)all), dim3(DC_THREADS), s,
-                  ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+                  ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, max_pages, page_size, tm);
   return launch("dense_combine_kernel", dense_combine_kernel<1>, dim3((unsigned)((all + DC_WAVES - 1) / DC_WAVES)),
-                dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, rows, G, max_pages, page_size);
+                dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, max_pages, page_size, tm);
 }
 
 // Whether the list of units fits 32 bits, whatever the lengths, and the rows a launch.
