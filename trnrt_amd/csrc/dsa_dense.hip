@@ -36,28 +36,28 @@ constexpr float DN_LOG2E_LO = (float)(1.44269504088896341 - (double)DN_LOG2E);
 constexpr int DN_PROW = DN_CHUNK + 8;  // P row stride (bf16)
 constexpr int DN_KAHEAD = 3;           // score steps whose key reads are in flight
 constexpr int DN_VAHEAD = 3;           // value steps whose operand reads are in flight
+constexpr int DN_STORE = 5;            // the value step that begins storing the next chunk's rows
 
 typedef int dn_v2i __attribute__((ext_vector_type(2)));
 
-// A chunk's LDS layout: the rows' first 512 bytes at r x 512, 16-byte piece p of row r (token) at p ^ (r & 7); then, of
-// 576-byte rows, the last 64 at r x 64, piece p at p ^ ((r >> 1) & 3). With it the reads of one piece of 8 consecutive rows
-// (key operand, and value operand, read transposed) cover the 32 banks once.
-__device__ __forceinline__ int dn_swizzle(int r) { return r & 7; }
+// A chunk's LDS layout: row r (token) at r x DN_KROW, its 16-byte piece p at p ^ ((r >> 1) & 3). With it the stores of 8
+// lanes (2 rows x 4 pieces) and the reads of one piece of 8 consecutive rows (key operand, and value operand, read
+// transposed) cover the 32 banks once.
+constexpr int DN_KROW = 576;
+constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are multiplied, c + 1 being stored
 
-// RB: blocks of 32 rows in a tile. Buffers: chunk c being scored, c - 1 whose values are multiplied, and the rest arriving.
-template <int DQK, int RB>
+// RB: blocks of 32 rows in a tile.
+template <int RB>
 struct DnShared {
-  static constexpr int BUFS = RB == 1 || DQK == 512 ? 4 : 3;  // (160 KiB of LDS)
-  alignas(1024) uint8_t tile[BUFS][DN_CHUNK * DQK];
-  alignas(16) uint16_t p[2][32 * RB * DN_PROW];  // P[row][token] of two chunks
-  alignas(16) float ksc[BUFS][DN_CHUNK];         // the chunks' token scales
-  alignas(16) float kfac[BUFS][DN_CHUNK];        // x softmax scale x log2 e
-  int page[4][DN_CHUNK];                         // and the pages of their tokens, four chunks
-  float cmax[2][32 * RB];                        // [token half][row]: a chunk's maxima when one moves
-  float al[32 * RB];                             // and its rescale factors
-  alignas(16) int flag[2][4];                    // per chunk parity and wave: a score past the running maximum's slack
-  float lsum[2][32 * RB];                        // [token half][row]: a stretch's sums
-  float mfin[32 * RB];                           // and maxima (base 2)
+  alignas(1024) uint8_t tile[DN_BUFS][DN_CHUNK * DN_KROW];  // (the queries in the last two before)
+  alignas(16) uint16_t p[2][32 * RB * DN_PROW];   // P[row][token] of two chunks
+  alignas(16) float ksc[DN_BUFS][DN_CHUNK];       // the chunks' token scales
+  alignas(16) float kfac[DN_BUFS][DN_CHUNK];      // x softmax scale x log2 e
+  float cmax[2][32 * RB];                         // [token half][row]: a chunk's maxima when one moves
+  float al[32 * RB];                              // and its rescale factors
+  alignas(16) int flag[2][4];                     // per chunk parity and wave: a score past the running maximum's slack
+  float lsum[2][32 * RB];                         // [token half][row]: a stretch's sums
+  float mfin[32 * RB];                            // and maxima (base 2)
   int tot[DN_THREADS / WAVE];
   int found[3];
 };
@@ -113,13 +113,10 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const int* __restrict__ table, const int* __restrict__ ctx_len, uint16_t* __restrict__ out,
     float* __restrict__ out_f32, float* __restrict__ lse_out, float* __restrict__ ws_o, float* __restrict__ ws_ml,
     int B, int S, int H, int max_pages, DnPage pg, int num_pages, float scale, DnTeams tm) {
-  typedef DnShared<DQK, RB> Sh;
-  constexpr int ROWS = 32 * RB, BUFS = Sh::BUFS;
+  constexpr int ROWS = 32 * RB, BUFS = DN_BUFS;
   constexpr int STEPS = DQK / 32;           // 32 dims: one 16-byte read of a key row per lane, two products
-  constexpr int TAIL = DN_CHUNK * 512;      // where the rows' last 64 bytes lie
-  constexpr int LOADS = DQK == 576 ? 9 : 8;  // a chunk's asynchronous loads per value wave
-  constexpr int AHEAD = BUFS - 2;            // chunks in flight
-  __shared__ Sh sh;
+  constexpr int PIECES = DQK / 64;  // 16-byte pieces of a chunk per loading thread (4 threads a row)
+  __shared__ DnShared<RB> sh;
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int M = S * H;
@@ -213,12 +210,13 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece p at
       // p ^ (r & 7), so that one piece of 8 rows covers the banks once
       {
-        constexpr int PIECES = DQK / 8, PER = ROWS * PIECES / (4 * WAVE);
-        const uint32_t q_lds = lds_address(sh.tile[AHEAD]) + 1024 * PER * wave;
+        constexpr int QP = DQK / 8, PER = ROWS * QP / (4 * WAVE);
+        static_assert(ROWS * QP * 16 <= 2 * DN_CHUNK * DN_KROW, "the staged queries");
+        const uint32_t q_lds = lds_address(sh.tile[1]) + 1024 * PER * wave;
         const int r_max = M - 1 - r0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const int x = WAVE * (PER * wave + i) + lane, r = x / PIECES, p = x - r * PIECES;
+          const int x = WAVE * (PER * wave + i) + lane, r = x / QP, p = x - r * QP;
           load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ (r & 7)), q_lds + 1024 * i);
         }
         wait_loads<0>();
@@ -247,7 +245,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
       bf16x8 qb[2 * STEPS];  // row 32 hh + j: step s holds dims 32 s + 16 h .. + 15
       {
-        const uint8_t* const qr = sh.tile[AHEAD] + (32 * hh + j) * 2 * DQK;
+        const uint8_t* const qr = sh.tile[1] + (32 * hh + j) * 2 * DQK;
 #pragma unroll
         for (int s = 0; s < 2 * STEPS; ++s)
           qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (j & 7))));
@@ -259,11 +257,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       float psum = 0.0f;   // and of the last chunk's, not yet in l_run
       f32x16 sv = {};      // the last chunk's scores - m_run: row 32 hh + j, tokens 32 th + 8 (r / 4) + 4 h + r % 4
       const int kr = 32 * th + j;
-      int koff[4], ktail[2];  // byte offsets of a row's pieces in a chunk (they repeat after 4 steps of 32 dims)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) koff[i] = kr * 512 + 16 * ((2 * i | h) ^ dn_swizzle(kr));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) ktail[i] = TAIL + kr * 64 + 16 * ((2 * i | h) ^ ((kr >> 1) & 3));
+      const int kf = (kr >> 1) & 3;  // byte offsets of a row's pieces at even and odd steps of 32 dims
+      const int koff[2] = {kr * DN_KROW + 16 * (h ^ kf), kr * DN_KROW + 16 * ((2 | h) ^ kf)};
       uint16_t* const pw = &sh.p[0][(32 * hh + j) * DN_PROW + 32 * th + 4 * h];
       int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
       auto four = [&](const float* a, int g) __attribute__((always_inline)) {
@@ -311,7 +306,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       for (int c = 0; c < nch; ++c) {
         const uint8_t* tile = sh.tile[buf];
         auto k_read = [&](int s) __attribute__((always_inline)) {
-          return *reinterpret_cast<const u32x4*>(tile + (s < 16 ? koff[s & 3] + 128 * (s >> 2) : ktail[s & 1]));
+          return *reinterpret_cast<const u32x4*>(tile + koff[s & 1] + 64 * (s >> 1));
         };
         int4 fl = make_int4(0, 0, 0, 0);
         if (c > 0) fl = flags(c - 1);
@@ -381,47 +376,29 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       write(1);
       }
     } else {
-      // -- the loads and the values: wave w brings rows 16 w .. + 15 of a chunk, takes dims 128 w .. + 127 of all rows --
+      // -- the loads and the values: thread 4 r + e of the value waves brings row r of a chunk, pieces e + 4 i; wave w takes
+      // dims 128 w .. + 127 of all rows --
       const int w = wave - 4;
       const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
       const int* trow = table + (size_t)b * max_pages;
-      // token `lane` of chunk c, the stretch's last one past its end (a slot behind the sequence may never have been
-      // written, and its NaN x weight 0 is NaN)
+      const int gr = 16 * w + (lane >> 2);  // this thread's row
+      // its token in chunk c, the stretch's last one past its end (a slot behind the sequence may never have been written,
+      // and its NaN x weight 0 is NaN)
       const int t_last = min(t0 + nch * DN_CHUNK, len) - 1;
-      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + lane, t_last); };
+      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + gr, t_last); };
       auto page_of = [&](int t) __attribute__((always_inline)) { return (int)((uint64_t)t * pg.mul >> pg.shift); };
-      const int mrow = 4 * (16 * w + h), trw = 4 * (16 * w + (lane >> 2));
-      int mcol[4];  // load k < 8 brings rows 16 w + 2 k and + 1, load 8 the last pieces of all 16
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mcol[k] = 16 * (j ^ dn_swizzle(2 * k | h));
-      const int tcol = 512 + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
-      const uint32_t tile_lds = lds_address(sh.tile[0] + 16 * w * 512), tail_lds = lds_address(sh.tile[0] + TAIL + 1024 * w);
-      const uint32_t ksc_lds = lds_address(sh.ksc[0]), page_lds = lds_address(sh.page[0]);
-      if (!kvs)
-        for (int i = 0; i < BUFS; ++i) sh.ksc[i][lane] = 1.0f;
-      // chunk c's loads into buffer `to`: begin() its scales and the pages of chunk c + 2 (every value wave the same ones,
-      // so that each waits for its own; `page`: of this lane's token) and where its rows lie, then load() k < LOADS
-      unsigned src[LOADS];
-      auto begin = [&](int c, int to, int page) __attribute__((always_inline)) {
+      auto slot_of = [&](int c, int page) __attribute__((always_inline)) {
         const int t = token(c);
-        const int slot = safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
-        load_lds4(trow + page_of(token(c + 2)), page_lds + 4 * DN_CHUNK * ((c + 2) & 3));
-        if (kvs) load_lds4(kvs + slot, ksc_lds + 4 * DN_CHUNK * to);
-#pragma unroll
-        for (int k = 0; k < LOADS; ++k)
-          src[k] = (unsigned)__builtin_amdgcn_ds_bpermute(k < 8 ? mrow + 8 * k : trw, slot);
+        return safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
       };
-      auto load = [&](int k, int to) __attribute__((always_inline)) {
-        load_lds16(kv + (size_t)src[k] * DQK + (k < 8 ? mcol[k & 3] : tcol),
-                   (k < 8 ? tile_lds + 1024 * k : tail_lds) + DN_CHUNK * DQK * to);
-      };
-      // chunk `to`'s loads have landed, with those of the AHEAD - 1 chunks after it out, and so the pages two chunks on; then
-      // the tokens' factors
-      auto landed = [&](int to) __attribute__((always_inline)) {
-        wait_loads<(AHEAD - 1) * (LOADS + 1)>();
-        if (w == 0) {
-          const float k = sh.ksc[to][lane];
-          sh.kfac[to][lane] = fmaf(k, sl2, k * sl2_lo);
+      const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ ((gr >> 1) & 3));  // where its pieces go in a tile
+      u32x4 r0[PIECES];  // the pieces in flight, of the chunk after the one being stored
+      float sc;          // and its token's scale
+      auto row_of = [&](int slot) __attribute__((always_inline)) { return kv + (size_t)slot * DQK + 16 * (lane & 3); };
+      auto store_scale = [&](int to) __attribute__((always_inline)) {
+        if ((lane & 3) == 0) {
+          sh.ksc[to][gr] = sc;
+          sh.kfac[to][gr] = fmaf(sc, sl2, sc * sl2_lo);
         }
       };
       f32x16 o[4][RB];  // [dim block][row block]: row 32 i + j, dims 128 w + 32 d + 8 (r / 4) + 4 h + r % 4
@@ -429,27 +406,23 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
-      const int vr = 8 * h + ((lane & 15) >> 1);  // (value operand: this lane's address is of row vr + 16 t)
-      int voff[4];
-#pragma unroll
-      for (int d = 0; d < 4; ++d)
-        voff[d] = vr * 512 + 128 * w + 16 * ((2 * d | ((lane >> 4) & 1)) ^ dn_swizzle(vr)) + 8 * (lane & 1);
+      const int vf = (lane >> 2) & 3, vb0 = (lane >> 4) & 1;
+      const int vrow = (8 * h + ((lane & 15) >> 1)) * DN_KROW + 128 * w + 8 * (lane & 1);  // (of the value operand's reads)
+      const int voff[2] = {vrow + 16 * (vb0 ^ vf), vrow + 16 * ((2 | vb0) ^ vf)};
       const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
       // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed
       auto v_read = [&](const uint8_t* kt, int i) __attribute__((always_inline)) {
         return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 3] + 16 * (i >> 2) * 512));
+            (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW + 64 * ((i & 3) >> 1)));
       };
       auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
         return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * ROWS * DN_PROW + 32 * i * DN_PROW + 16 * t));
       };
       // Interval c: chunk c - 1's weights are final (and O on their maxima) once its flags are seen; then its value product,
-      // 16 steps of RB products, the next steps' operands read and converted ahead, with chunk c + AHEAD's loads (into
-      // buffer `to`) spread over the steps: their issue waits on each other's.
-      auto interval = [&](int c, const uint8_t* kt, int to) __attribute__((always_inline)) {
+      // 16 steps of RB products, the next steps' operands read and converted ahead, side(i) beside step i.
+      auto interval = [&](int c, const uint8_t* kt, auto side) __attribute__((always_inline)) {
         const int pb = (c - 1) & 1;
         const int4 fl = *reinterpret_cast<const int4*>(sh.flag[pb]);
-        const int page = sh.page[(c + AHEAD) & 3][lane];
         dn_v2i vv[DN_VAHEAD + 1];
         bf16x8 pa[2][RB], vb[2];
 #pragma unroll
@@ -470,7 +443,6 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         }
 #pragma unroll
         for (int i = 0; i < RB; ++i) pa[0][i] = p_read(pb, 0, i);
-        begin(c + AHEAD, to, page);
         vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -485,38 +457,61 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
             vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
           }
-#pragma unroll
-          for (int k = 0; k < LOADS; ++k)
-            if (k * 15 / LOADS + 1 == i) load(k, to);
+          side(i);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
-      sh.page[0][lane] = trow[page_of(token(0))];
-      sh.page[1][lane] = trow[page_of(token(1))];
+      int page = trow[page_of(token(2))];  // of this thread's token two chunks on
+      const int page0 = trow[page_of(token(0))], page1 = trow[page_of(token(1))];
+      {
+        const int slot = slot_of(0, page0);
+        const uint8_t* src = row_of(slot);
 #pragma unroll
-      for (int c = 0; c < AHEAD; ++c) {
-        begin(c, c, sh.page[c][lane]);
+        for (int i = 0; i < PIECES; ++i) r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
+        sc = kvs ? kvs[slot] : 1.0f;
 #pragma unroll
-        for (int k = 0; k < LOADS; ++k) load(k, c);
+        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<u32x4*>(sh.tile[0] + gs + 64 * i) = r0[i];
+        store_scale(0);
       }
-      landed(0);
+      {
+        const int slot = slot_of(1, page1);
+        const uint8_t* src = row_of(slot);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
+        sc = kvs ? kvs[slot] : 1.0f;
+      }
       lds_barrier();  // the queries and chunk 0 are in place
       lds_barrier();  // the queries are read
-      // chunk c + AHEAD goes into the buffer that chunk c - 2 left, in the last intervals too (the stretch's last row then,
-      // into buffers that nobody reads: the loop stays one piece)
-      begin(AHEAD, AHEAD, sh.page[AHEAD][lane]);
+      // Interval c stores chunk c + 1 into the buffer that chunk c - 2 left and loads chunk c + 2, piece by piece, in the
+      // last intervals too (the stretch's last row then, into buffers that nobody reads).
+      const uint8_t* src = nullptr;
+      float sc_next = 1.0f;
+      auto ahead = [&](int c) __attribute__((always_inline)) {
+        const int slot = slot_of(c + 2, page);
+        page = trow[page_of(token(c + 3))];
+        src = row_of(slot);
+        if (kvs) sc_next = kvs[slot];
+      };
+      auto piece = [&](int i, uint8_t* to) __attribute__((always_inline)) {
+        *reinterpret_cast<u32x4*>(to + gs + 64 * i) = r0[i];
+        r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
+      };
+      ahead(0);
 #pragma unroll
-      for (int k = 0; k < LOADS; ++k) load(k, AHEAD);
-      int buf = 1;  // chunk c's buffer
-      landed(1);
+      for (int i = 0; i < PIECES; ++i) piece(i, sh.tile[1]);
+      store_scale(1);
+      sc = sc_next;
       lds_barrier();
+      int buf = 1;  // chunk c's buffer
 #pragma unroll 1
       for (int c = 1; c <= nch; ++c) {
         const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
-        const int to = prev == 0 ? BUFS - 1 : prev - 1;
-        interval(c, sh.tile[prev], to);
-        if (c == nch) wait_loads<0>();  // the tiles are free
-        landed(next);
+        ahead(c);
+        interval(c, sh.tile[prev], [&](int i) __attribute__((always_inline)) {
+          if (i >= DN_STORE && i < DN_STORE + PIECES) piece(i - DN_STORE, sh.tile[next]);
+        });
+        store_scale(next);
+        sc = sc_next;
         buf = next;
         lds_barrier();
       }
