@@ -40,9 +40,10 @@ constexpr int DN_STORE = 5;            // the value step that begins storing the
 
 typedef int dn_v2i __attribute__((ext_vector_type(2)));
 
-// A chunk's LDS layout: row r (token) at r x DN_KROW, its 16-byte piece p at p ^ ((r >> 1) & 3). With it the stores of 8
-// lanes (2 rows x 4 pieces) and the reads of one piece of 8 consecutive rows (key operand, and value operand, read
-// transposed) cover the 32 banks once.
+// A chunk's LDS layout: row r (token) at r x DN_KROW, its 16-byte piece p at p ^ dn_swizzle(r). With it the stores of 16 lanes
+// (4 rows x 4 pieces), the key operand's reads (16 lanes: a piece of 16 rows) and the value operand's, transposed (32 lanes:
+// two pieces of 8 rows), cover the 64 banks once.
+__device__ __forceinline__ int dn_swizzle(int r) { return (r >> 2 & 1) << 1 | (r >> 3 & 1); }
 constexpr int DN_KROW = 576;
 constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are multiplied, c + 1 being stored
 
@@ -257,7 +258,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       float psum = 0.0f;   // and of the last chunk's, not yet in l_run
       f32x16 sv = {};      // the last chunk's scores - m_run: row 32 hh + j, tokens 32 th + 8 (r / 4) + 4 h + r % 4
       const int kr = 32 * th + j;
-      const int kf = (kr >> 1) & 3;  // byte offsets of a row's pieces at even and odd steps of 32 dims
+      const int kf = dn_swizzle(kr);  // byte offsets of a row's pieces at even and odd steps of 32 dims
       const int koff[2] = {kr * DN_KROW + 16 * (h ^ kf), kr * DN_KROW + 16 * ((2 | h) ^ kf)};
       uint16_t* const pw = &sh.p[0][(32 * hh + j) * DN_PROW + 32 * th + 4 * h];
       int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
@@ -391,7 +392,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         const int t = token(c);
         return safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
       };
-      const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ ((gr >> 1) & 3));  // where its pieces go in a tile
+      const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ dn_swizzle(gr));  // where its pieces go in a tile
       u32x4 r0[PIECES];  // the pieces in flight, of the chunk after the one being stored
       float sc;          // and its token's scale
       auto row_of = [&](int slot) __attribute__((always_inline)) { return kv + (size_t)slot * DQK + 16 * (lane & 3); };
@@ -406,8 +407,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
-      const int vf = (lane >> 2) & 3, vb0 = (lane >> 4) & 1;
-      const int vrow = (8 * h + ((lane & 15) >> 1)) * DN_KROW + 128 * w + 8 * (lane & 1);  // (of the value operand's reads)
+      const int vr = 8 * h + ((lane & 15) >> 1), vf = dn_swizzle(vr), vb0 = (lane >> 4) & 1;  // (the value operand's reads)
+      const int vrow = vr * DN_KROW + 128 * w + 8 * (lane & 1);
       const int voff[2] = {vrow + 16 * (vb0 ^ vf), vrow + 16 * ((2 | vb0) ^ vf)};
       const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
       // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed

@@ -24,8 +24,8 @@ constexpr int EL_TOK = 256;
 constexpr int EL_K = 64;
 
 struct ElShared {
-  alignas(1024) uint8_t a[2][EL_TOK * EL_K];    // rows: 64 bytes, 16-byte piece p at p ^ ((row >> 1) & 3)
-  alignas(1024) uint16_t b[2][EX_D * EL_K];     // weights: 128 bytes a row, piece p at p ^ (row & 7)
+  alignas(1024) uint8_t a[2][EL_TOK * EL_K];    // rows: 64 bytes, 16-byte piece p at p ^ ((row >> 2) & 3)
+  alignas(1024) uint16_t b[2][EX_D * EL_K];     // weights: 128 bytes a row, piece p at p ^ ((row >> 1) & 7)
   int slot[EL_TOK];
   int seq;
 };
@@ -72,15 +72,17 @@ __global__ __launch_bounds__(EL_THREADS, 2) void expand_latent_kernel(
   const uint8_t* ap[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    ap[i] = kv + (size_t)sh.slot[64 * wave + 16 * i + (lane >> 2)] * D + 16 * ((lane & 3) ^ ((lane >> 3) & 3));
-  const uint16_t* bp =
-      wkv + ((size_t)part * EX_D + 32 * wave + (lane >> 3)) * EX_C + 8 * ((lane & 7) ^ (lane >> 3));
+    ap[i] = kv + (size_t)sh.slot[64 * wave + 16 * i + (lane >> 2)] * D + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
+  const uint16_t* bp = wkv + ((size_t)part * EX_D + 32 * wave + (lane >> 3)) * EX_C;
+  int bcol[2];  // (of even and odd groups of 8 rows)
+#pragma unroll
+  for (int i = 0; i < 2; ++i) bcol[i] = 8 * ((lane & 7) ^ ((8 * i + (lane >> 3)) >> 1));
   const uint32_t a_lds = lds_address(sh.a[0] + 4096 * wave), b_lds = lds_address(sh.b[0] + 2048 * wave);
   auto issue = [&](int s, int to) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       load_lds16(ap[i] + s * EL_K, a_lds + EL_TOK * EL_K * to + 1024 * i);
-      load_lds16(bp + s * EL_K + 8 * i * EX_C, b_lds + 2 * EX_D * EL_K * to + 1024 * i);
+      load_lds16(bp + s * EL_K + 8 * i * EX_C + bcol[i & 1], b_lds + 2 * EX_D * EL_K * to + 1024 * i);
     }
   };
   issue(0, 0);
@@ -96,8 +98,8 @@ __global__ __launch_bounds__(EL_THREADS, 2) void expand_latent_kernel(
 #pragma unroll
     for (int y = 0; y < 2; ++y) acc[x][y] = f32x16{};
   arrive(sc);
-  const int arow = (128 * wm + j) * EL_K, asw = (j >> 1) & 3;
-  const int brow = (64 * wn + j) * EL_K, bsw = j & 7;
+  const int arow = (128 * wm + j) * EL_K, asw = (j >> 2) & 3;
+  const int brow = (64 * wn + j) * EL_K, bsw = (j >> 1) & 7;
 #pragma unroll 1
   for (int s = 0; s < EX_C / EL_K; ++s) {
     wait_loads<0>();
@@ -191,8 +193,8 @@ constexpr float XA_LOG2E = 1.44269504088896341f;
 
 typedef short xa_v4s __attribute__((ext_vector_type(4)));
 
-// A stage's keys and values lie in rows of 256 bytes, 16-byte piece p of key row r at p ^ (r & 7), of value row r at
-// p ^ 2 (r & 3) (its reads take two pieces of 4 rows), of rope row r (128 bytes) at p ^ (r & 7).
+// A stage's keys and values lie in rows of 256 bytes, 16-byte piece p of key row r at p ^ (r & 15), of value row r at
+// p ^ 4 (r & 3) (32 lanes read four pieces of 4 rows), of rope row r (128 bytes) at p ^ ((r >> 1) & 7).
 template <int DQ>
 struct XaShared {
   alignas(1024) uint8_t k[XA_STAGES][XA_K * 256];
@@ -259,9 +261,10 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   const uint16_t* const k_base = k + head_off;
   const uint16_t* const v_base = v + head_off;
   const int l4 = lane >> 4;
-  const int kcol[2] = {8 * ((lane & 15) ^ l4), 8 * ((lane & 15) ^ (4 | l4))};
-  const int vcol = 8 * ((lane & 15) ^ (2 * l4));
-  const int rcol = 8 * ((lane & 7) ^ (lane >> 3));
+  const int k8 = 8 * (wave & 1);  // (of the row's place in 16)
+  const int kcol[2] = {8 * ((lane & 15) ^ (k8 | l4)), 8 * ((lane & 15) ^ (k8 | 4 | l4))};
+  const int vcol = 8 * ((lane & 15) ^ (4 * l4));
+  const int rcol = 8 * ((lane & 7) ^ ((k8 + (lane >> 3)) >> 1));
   const uint32_t k_lds = lds_address(sh.k[0] + 2048 * wave), v_lds = lds_address(sh.v[0] + 2048 * wave);
   const uint32_t r_lds = lds_address(sh.r[0] + 1024 * wave);
   auto issue = [&](int i, int to) __attribute__((always_inline)) {
@@ -284,16 +287,15 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     for (int s = 0; s < STEPS; ++s) qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * s));
     arrive(qf);
   }
-  int koff[4], roff[4], voff[2];
+  int koff[8], roff[4], voff[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 7));
-    roff[i] = 128 * j + 16 * ((2 * i | h) ^ (j & 7));
-  }
+  for (int i = 0; i < 8; ++i) koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 15));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) roff[i] = 128 * j + 16 * ((2 * i | h) ^ ((j >> 1) & 7));
   {  // the value operand: this lane's address is of row 4 h + (lane & 15) / 4, columns 16 (lane / 16 % 2) + 4 (lane % 4)
     const int r = (lane & 15) >> 2, p = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) voff[i] = 256 * (4 * h + r) + 16 * ((4 * i | p) ^ (2 * r)) + 8 * (lane & 1);
+    for (int i = 0; i < 4; ++i) voff[i] = 256 * (4 * h + r) + 16 * ((4 * i | p) ^ (4 * r)) + 8 * (lane & 1);
   }
   const float sl2 = scale * XA_LOG2E;
   float m_run = 0.0f, l_run = 0.0f;  // running maximum (base 2), this lane's share of the sum
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
       for (int s = 0; s < STEPS; ++s)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint8_t* at = s < 8 ? kt + koff[s & 3] + 128 * (s >> 2) + 32 * 256 * x : rt + roff[s & 3] + 32 * 128 * x;
+          const uint8_t* at = s < 8 ? kt + koff[s] + 32 * 256 * x : rt + roff[s & 3] + 32 * 128 * x;
           s2[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), qf[s], s2[x],
                                                           0, 0, 0);
         }
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         const bf16x8 pb = as_bf16x8(make_uint4(pk[4 * t], pk[4 * t + 1], pk[4 * t + 2], pk[4 * t + 3]));
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-          const uint8_t* at = vt + voff[d & 1] + 128 * (d >> 1) + 16 * 256 * t;
+          const uint8_t* at = vt + voff[d] + 16 * 256 * t;
           typedef __attribute__((address_space(3))) xa_v4s* lds4;
           const xa_v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)at);
           const xa_v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at + 8 * 256));
