@@ -211,7 +211,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int Tq, int Tk, int H,
     int q_tiles, int causal, float scale) {
   constexpr int STEPS = DQ / 16;
-  constexpr int LOADS = DQ > EX_D ? 5 : 4;  // a tile's asynchronous loads per wave
+  constexpr int LOADS = DQ > EX_D ? 10 : 8;  // a tile's asynchronous loads per wave
   __shared__ XaShared<DQ> sh;
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int j = lane & 31, h = lane >> 5;
@@ -256,30 +256,33 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   const int seen0 = seen(w0);
   const int qi = min(w0 + j, nq - 1), seen_j = seen(qi);
 
-  // this wave's loads of a tile: key and value rows 8 wave .. + 7, in two of 4 rows, rope rows 8 wave .. + 7
+  // Waves 0 to 3, the ones with priority, bring the tiles, once they are through with theirs: the loads' issue would delay
+  // the others, for whom they wait anyway (8k tokens, 64 heads: 1,194 us; all waves before their tile 1,235, after it
+  // 1,207). Key and value rows 16 wave .. + 15 in fours, rope rows in eights.
+  const bool brings = wave < 4;
   const size_t head_off = (size_t)kb * H * EX_D + (size_t)head * EX_D;
   const uint16_t* const k_base = k + head_off;
   const uint16_t* const v_base = v + head_off;
-  const int l4 = lane >> 4;
-  const int k8 = 8 * (wave & 1);  // (of the row's place in 16)
-  const int kcol[2] = {8 * ((lane & 15) ^ (k8 | l4)), 8 * ((lane & 15) ^ (k8 | 4 | l4))};
+  const int l4 = lane >> 4, lw = wave & 3;
   const int vcol = 8 * ((lane & 15) ^ (4 * l4));
-  const int rcol = 8 * ((lane & 7) ^ ((k8 + (lane >> 3)) >> 1));
-  const uint32_t k_lds = lds_address(sh.k[0] + 2048 * wave), v_lds = lds_address(sh.v[0] + 2048 * wave);
-  const uint32_t r_lds = lds_address(sh.r[0] + 1024 * wave);
+  const uint32_t k_lds = lds_address(sh.k[0] + 4096 * lw), v_lds = lds_address(sh.v[0] + 4096 * lw);
+  const uint32_t r_lds = lds_address(sh.r[0] + 2048 * lw);
   auto issue = [&](int i, int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {  // (rows past the end: the last one, of weight 0)
-      const size_t t = (size_t)min(i * XA_K + 8 * wave + 4 * x + l4, nk - 1) * H * EX_D;
-      load_lds16(k_base + t + kcol[x], k_lds + XA_K * 256 * to + 1024 * x);
+    for (int x = 0; x < 4; ++x) {  // (rows past the end: the last one, of weight 0)
+      const size_t t = (size_t)min(i * XA_K + 16 * lw + 4 * x + l4, nk - 1) * H * EX_D;
+      load_lds16(k_base + t + 8 * ((lane & 15) ^ (4 * x | l4)), k_lds + XA_K * 256 * to + 1024 * x);
       load_lds16(v_base + t + vcol, v_lds + XA_K * 256 * to + 1024 * x);
     }
     if (DQ > EX_D)
-      load_lds16(kr + (size_t)(kb + min(i * XA_K + 8 * wave + (lane >> 3), nk - 1)) * EX_R + rcol,
-                 r_lds + XA_K * 128 * to);
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        load_lds16(kr + (size_t)(kb + min(i * XA_K + 16 * lw + 8 * x + (lane >> 3), nk - 1)) * EX_R +
+                       8 * ((lane & 7) ^ ((8 * x + (lane >> 3)) >> 1)),
+                   r_lds + XA_K * 128 * to + 1024 * x);
   };
-  if (nt > 0) issue(0, 0);
-  if (nt > 1) issue(1, 1);
+  if (brings && nt > 0) issue(0, 0);
+  if (brings && nt > 1) issue(1, 1);
   bf16x8 qf[STEPS];  // query qi: step s holds dims 16 s + 8 h .. + 7
   {
     const uint16_t* qr = q + ((size_t)(qb + qi) * H + head) * DQ + 8 * h;
@@ -306,12 +309,13 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   int stage = 0;
 #pragma unroll 1
   for (int i = 0; i < nt; ++i) {
-    if (i + 1 < nt)
-      wait_loads<LOADS>();
-    else
-      wait_loads<0>();
+    if (brings) {
+      if (i + 1 < nt)
+        wait_loads<LOADS>();
+      else
+        wait_loads<0>();
+    }
     lds_barrier();  // tile i is in place, and nobody reads tile i - 1 any more
-    if (i + 2 < nt) issue(i + 2, stage == 0 ? 2 : stage - 1);
     if (i < nt_w) {
       const uint8_t* const kt = sh.k[stage];
       const uint8_t* const vt = sh.v[stage];
@@ -381,6 +385,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         }
       }
     }
+    if (brings && i + 2 < nt) issue(i + 2, stage == 0 ? 2 : stage - 1);  // (where tile i - 1 was)
     stage = stage == XA_STAGES - 1 ? 0 : stage + 1;
   }
   __syncthreads();  // the stages are free
