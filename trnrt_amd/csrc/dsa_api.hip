@@ -121,7 +121,7 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
                             hipStream_t s);
 hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* table, const int* cu,
                                 const uint16_t* w, uint16_t* k, uint16_t* v, uint16_t* r, int B, int total, int H,
-                                int D, int max_pages, int page_size, int num_pages, hipStream_t s);
+                                int D, int max_pages, int page_size, int num_pages, int num_cu, hipStream_t s);
 bool expanded_grid_ok(int B, int Tq, int H);
 hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
                                   const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, int B,
@@ -1316,7 +1316,7 @@ int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_
   return status(dsa::launch_expand_latent(
       kv_fp8, kv_scale, page_table, cu_len, static_cast<const uint16_t*>(w_bf16), static_cast<uint16_t*>(k_bf16),
       static_cast<uint16_t*>(v_bf16), Dqk == 576 ? static_cast<uint16_t*>(rope_bf16) : nullptr, B, total, H, Dqk,
-      max_pages, page_size, num_pages, static_cast<hipStream_t>(stream)));
+      max_pages, page_size, num_pages, num_cu(), static_cast<hipStream_t>(stream)));
 }
 
 int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,

@@ -19,160 +19,204 @@ constexpr int EX_C = 512;   // the latent width
 // CU so that one's stores are under the other's products; 64 of the 512 columns at a time come by asynchronous loads
 // straight into LDS, a step ahead. The rows stay e4m3 until they are operands (exact in bf16). The tiles of one XCD share
 // its heads' weights through its L2.
-constexpr int EL_THREADS = 256;
-constexpr int EL_TOK = 256;
+constexpr int EL_THREADS = 512;
+constexpr int EL_TOK = 256;  // (or half of it)
 constexpr int EL_K = 64;
+constexpr int EL_STEPS = EX_C / EL_K;
+constexpr int EL_STAGES = 8;
 
 struct ElShared {
-  alignas(1024) uint8_t a[2][EL_TOK * EL_K];    // rows: 64 bytes, 16-byte piece p at p ^ ((row >> 2) & 3)
-  alignas(1024) uint16_t b[2][EX_D * EL_K];     // weights: 128 bytes a row, piece p at p ^ ((row >> 1) & 7)
+  // a step's weights: 128 bytes a row, 16-byte piece p at p ^ ((row >> 1) & 3 | (row >> 5 & 1) << 2). Before a token
+  // tile's first step the rows lie here, 512 bytes each, piece p at p ^ (row & 15).
+  alignas(1024) uint16_t b[EL_STAGES][EX_D * EL_K];
   int slot[EL_TOK];
   int seq;
 };
+static_assert(sizeof(ElShared::b) >= EL_TOK * EX_C, "the rows");
 
-__global__ __launch_bounds__(EL_THREADS, 2) void expand_latent_kernel(
+// Lane 4 t + c holds pieces i = 0 .. 3 of row 4 t + c; after this, piece c of rows 4 t + i.
+__device__ __forceinline__ void quad_transpose(uint32_t (&o)[4][4]) {
+  const int c = threadIdx.x & 3;
+#pragma unroll
+  for (int d = 1; d < 4; d *= 2)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & d) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {  // the lane whose bit d is clear gives its piece i + d for the other's i
+        const uint32_t lo = o[i][e], hi = o[i + d][e];
+        const uint32_t give = c & d ? lo : hi;
+        const uint32_t got = d == 1 ? __builtin_amdgcn_mov_dpp(give, 0xb1, 0xf, 0xf, true)
+                                    : __builtin_amdgcn_mov_dpp(give, 0x4e, 0xf, 0xf, true);
+        o[i][e] = c & d ? got : lo;
+        o[i + d][e] = c & d ? hi : got;
+      }
+    }
+}
+
+// X groups of 32 tokens a wave: tiles of 128 X tokens
+template <int X>
+__global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
     const uint8_t* __restrict__ kv, const float* __restrict__ kvs, const int* __restrict__ table,
     const int* __restrict__ cu, const uint16_t* __restrict__ wkv, uint16_t* __restrict__ k_out,
     uint16_t* __restrict__ v_out, uint16_t* __restrict__ r_out, int B, int total, int H, int D, int max_pages,
-    int page_size, int num_pages) {
+    int page_size, int num_pages, int units) {
+  constexpr int TOK = 128 * X, FIRST = EL_STAGES - TOK / 32;  // (stages that the rows do not take)
   __shared__ ElShared sh;
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int j = lane & 31, h = lane >> 5;
-  // parts: 2 H of 128 columns. An XCD (workgroup x runs on XCD x % 8) takes an eighth of them where they divide, all the
-  // parts of a token tile next to each other
-  const int parts = 2 * H;
-  int part, tile;
-  if ((parts & 7) == 0) {
-    const int per = parts >> 3, y = blockIdx.x >> 3;
-    part = (blockIdx.x & 7) * per + y % per;
-    tile = y / per;
-  } else {
-    part = blockIdx.x % parts;
-    tile = blockIdx.x / parts;
-  }
-  const int t0 = tile * EL_TOK, end = min(total, cu[B]);
-  if (t0 >= end) return;  // (rows past the last sequence are left as they were)
-  // the slots of the tile's tokens: the sequence of the first one by counting, the others' from there
-  if (tid == 0) sh.seq = 0;
-  __syncthreads();
-  int n = 0;
-  for (int b = tid; b < B; b += EL_THREADS) n += cu[b + 1] <= t0;
-  if (n) atomicAdd(&sh.seq, n);
-  __syncthreads();
-  {
-    const int t = min(t0 + tid, end - 1);
-    int b = min(sh.seq, B - 1);
-    while (b < B - 1 && cu[b + 1] <= t) ++b;
-    const int pos = max(t - cu[b], 0), pi = pos / page_size;
-    const int page = pi < max_pages ? safe_page(table[(size_t)b * max_pages + pi], num_pages) : 0;
-    sh.slot[tid] = page * page_size + (pos - pi * page_size);
-  }
-  __syncthreads();
-  // this lane's loads: rows 64 wave + 16 i + lane / 4 of the tokens, 32 wave + 8 i + lane / 8 of the weights
-  const uint8_t* ap[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    ap[i] = kv + (size_t)sh.slot[64 * wave + 16 * i + (lane >> 2)] * D + 16 * ((lane & 3) ^ ((lane >> 4) & 3));
-  const uint16_t* bp = wkv + ((size_t)part * EX_D + 32 * wave + (lane >> 3)) * EX_C;
-  int bcol[2];  // (of even and odd groups of 8 rows)
-#pragma unroll
-  for (int i = 0; i < 2; ++i) bcol[i] = 8 * ((lane & 7) ^ ((8 * i + (lane >> 3)) >> 1));
-  const uint32_t a_lds = lds_address(sh.a[0] + 4096 * wave), b_lds = lds_address(sh.b[0] + 2048 * wave);
-  auto issue = [&](int s, int to) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      load_lds16(ap[i] + s * EL_K, a_lds + EL_TOK * EL_K * to + 1024 * i);
-      load_lds16(bp + s * EL_K + 8 * i * EX_C + bcol[i & 1], b_lds + 2 * EX_D * EL_K * to + 1024 * i);
-    }
-  };
-  issue(0, 0);
-  // wave: tokens 128 wm .. + 127 x columns 64 wn .. + 63; the columns are the products' rows, so that a lane's sums are 4
-  // consecutive columns of one token
+  const int parts = 2 * H, end = min(total, cu[B]);
+  // this workgroup's share of the units (token tile, part), parts fastest; an XCD's (workgroup x runs on XCD x % 8) lie
+  // next to each other
+  const int xcd = blockIdx.x & 7, G = gridDim.x;
+  const int g = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
+  const int u0 = (int)((long)units * g / G), u1 = (int)((long)units * (g + 1) / G);
+  // wave: tokens 32 X wm .. + 63 x columns 64 wn .. + 63; the columns are the products' rows, taken in an order that leaves
+  // a lane 32 columns of one token in a row (32 h + 16 y + r)
   const int wm = wave >> 1, wn = wave & 1;
-  float sc[4];
-#pragma unroll
-  for (int x = 0; x < 4; ++x) sc[x] = kvs ? kvs[sh.slot[128 * wm + 32 * x + j]] : 1.0f;
-  f32x16 acc[4][2];
-#pragma unroll
-  for (int x = 0; x < 4; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) acc[x][y] = f32x16{};
-  arrive(sc);
-  const int arow = (128 * wm + j) * EL_K, asw = (j >> 2) & 3;
-  const int brow = (64 * wn + j) * EL_K, bsw = (j >> 1) & 7;
+  const uint32_t b_lds = lds_address(sh.b[0] + 1024 * wave);
+  const int bcol = 8 * ((lane & 7) ^ (((lane >> 4) & 3) | ((wave >> 1) & 1) << 2));
+  const int brow = 64 * wn + 32 * ((j >> 2) & 1) + 4 * (j >> 3) + (j & 3);  // (+ 16 y)
+  const int bsw = ((j >> 1) & 1) | ((j >> 3) & 1) << 1 | ((j >> 2) & 1) << 2;
+
 #pragma unroll 1
-  for (int s = 0; s < EX_C / EL_K; ++s) {
+  for (int u = u0; u < u1;) {
+    const int tile = u / parts, part0 = u - tile * parts, n = min(parts - part0, u1 - u), t0 = tile * TOK;
+    u += n;
     wait_loads<0>();
-    lds_barrier();  // step s is in place, and nobody reads step s - 1 any more
-    if (s + 1 < EX_C / EL_K) issue(s + 1, (s + 1) & 1);
-    const uint8_t* a = sh.a[s & 1];
-    const uint16_t* b = sh.b[s & 1];
+    if (t0 >= end) return;  // (rows past the last sequence are left as they were)
+    if (tid == 0) sh.seq = 0;
+    __syncthreads();  // (the last tile's stages are free)
+    // step s of part p0 + p: weights 64 s .. + 63 of the part's 128 rows, this wave's 16 in eights
+    const uint16_t* const bp = wkv + ((size_t)part0 * EX_D + 16 * wave + (lane >> 3)) * EX_C + bcol;
+    const int last = n * EL_STEPS - 1;
+    auto issue = [&](int st) __attribute__((always_inline)) {  // (past the end: the last step again, into a stage that is free)
+      const int f = min(st, last);
+      const uint16_t* from = bp + (size_t)(f / EL_STEPS) * EX_D * EX_C + (f % EL_STEPS) * EL_K;
+      const uint32_t to = b_lds + 2 * EX_D * EL_K * (st % EL_STAGES);
+      load_lds16(from, to);
+      load_lds16(from + 8 * EX_C, to + 1024);
+    };
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {  // 32 columns: lane half h takes 16, in two operands of 8
-      bf16x8 wf[2][2];
+    for (int i = 0; i < FIRST; ++i) issue(i);
+    // the slots of the tile's tokens: the sequence of the first one by counting, the others' from there
+    int c = 0;
+    for (int b = tid; b < B; b += EL_THREADS) c += cu[b + 1] <= t0;
+    if (c) atomicAdd(&sh.seq, c);
+    __syncthreads();
+    if (tid < TOK) {
+      const int t = min(t0 + tid, end - 1);
+      int b = min(sh.seq, B - 1);
+      while (b < B - 1 && cu[b + 1] <= t) ++b;
+      const int pos = max(t - cu[b], 0), pi = pos / page_size;
+      const int page = pi < max_pages ? safe_page(table[(size_t)b * max_pages + pi], num_pages) : 0;
+      sh.slot[tid] = page * page_size + (pos - pi * page_size);
+    }
+    __syncthreads();
+    {  // the rows into LDS: this wave's 16 X, two at a time
+      const uint32_t a_lds = lds_address(sh.b[FIRST]) + 16 * X * EX_C * wave;
+      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int i = 0; i < 8 * X; ++i) {
+        const int r = 16 * X * wave + 2 * i + h;
+        load_lds16(kv + (size_t)sh.slot[r] * D + 16 * (j ^ (r & 15)), a_lds + 2 * EX_C * i);
+      }
+    }
+    float sc[X];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          wf[y][e] = as_bf16x8(
-              *reinterpret_cast<const uint4*>(b + brow + 32 * EL_K * y + 8 * ((4 * g + 2 * h + e) ^ bsw)));
+    for (int x = 0; x < X; ++x) sc[x] = kvs ? kvs[sh.slot[32 * X * wm + 32 * x + j]] : 1.0f;
+    arrive(sc);
+    if (part0 == 0 && r_out) {
+      const int tid = WAVE * wave + fresh_lane();
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const u32x4 c = *reinterpret_cast<const u32x4*>(a + arow + 32 * EL_K * x + 16 * ((2 * g + h) ^ asw));
-        const bf16x8 c0 = fp8x8_to_bf16x8(c[0], c[1]), c1 = fp8x8_to_bf16x8(c[2], c[3]);
+      for (int i = 0; i < TOK * 8 / EL_THREADS; ++i) {  // 8 rope columns of a token
+        const int x = tid + EL_THREADS * i, r = x >> 3, p = x & 7;
+        if (t0 + r < end) {
+          const int slot = sh.slot[r];
+          const uint2 c8 = *reinterpret_cast<const uint2*>(kv + (size_t)slot * D + EX_C + 8 * p);
+          const float f = kvs ? kvs[slot] : 1.0f;
+          uint32_t o[4];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][0], c0, acc[x][y], 0, 0, 0);
-          acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][1], c1, acc[x][y], 0, 0, 0);
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t two = (e & 2 ? c8.y : c8.x) >> (16 * (e & 1));
+            const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(two, false);
+            o[e] = bf16_pack(v[0] * f, v[1] * f);
+          }
+          *reinterpret_cast<uint4*>(r_out + (size_t)(t0 + r) * EX_R + 8 * p) = make_uint4(o[0], o[1], o[2], o[3]);
         }
       }
     }
-  }
-  __syncthreads();
-  // through LDS: 256 bytes a token, 16-byte piece p of row r at p ^ (r & 15), then whole rows
-  uint8_t* const st = sh.a[0];
-  static_assert(offsetof(ElShared, slot) >= EL_TOK * EX_D * 2, "the staged outputs");
+    wait_loads<0>();
+    lds_barrier();
+    u32x4 a[X][2 * EL_STEPS];  // tokens 32 X wm + 32 x + j: columns 32 g + 16 h .. + 15
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    const int r = 128 * wm + 32 * x + j;
+    for (int x = 0; x < X; ++x) {
+      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(sh.b[FIRST]) + EX_C * (32 * X * wm + 32 * x + j);
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
+      for (int i = 0; i < 2 * EL_STEPS; ++i) a[x][i] = *reinterpret_cast<const u32x4*>(row + 16 * ((2 * i + h) ^ (j & 15)));
+    }
+    lds_barrier();  // the stages are free
+
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x16& v = acc[x][y];
-        *reinterpret_cast<uint2*>(st + 256 * r + 16 * ((8 * wn + 4 * y + g) ^ (r & 15)) + 8 * h) =
-            make_uint2(bf16_pack(v[4 * g] * sc[x], v[4 * g + 1] * sc[x]),
-                       bf16_pack(v[4 * g + 2] * sc[x], v[4 * g + 3] * sc[x]));
-      }
-  }
-  __syncthreads();
-  uint16_t* const out = (part & 1 ? v_out : k_out) + ((size_t)t0 * H + (part >> 1)) * EX_D;
+    for (int i = FIRST; i < EL_STAGES - 1; ++i) issue(i);
+#pragma unroll 1
+    for (int p = 0; p < n; ++p) {
+      f32x16 acc[X][2];
 #pragma unroll
-  for (int i = 0; i < EL_TOK * 16 / EL_THREADS; ++i) {
-    const int x = tid + EL_THREADS * i, r = x >> 4, p = x & 15;
-    if (t0 + r < end)
-      *reinterpret_cast<u32x4*>(out + (size_t)r * H * EX_D + 8 * p) =
-          *reinterpret_cast<const u32x4*>(st + 256 * r + 16 * (p ^ (r & 15)));
-  }
-  if (part == 0 && r_out) {
+      for (int x = 0; x < X; ++x)
 #pragma unroll
-    for (int i = 0; i < EL_TOK * 8 / EL_THREADS; ++i) {  // 8 rope columns of a token
-      const int x = tid + EL_THREADS * i, r = x >> 3, p = x & 7;
-      if (t0 + r < end) {
-        const int slot = sh.slot[r];
-        const uint2 c = *reinterpret_cast<const uint2*>(kv + (size_t)slot * D + EX_C + 8 * p);
-        const float f = kvs ? kvs[slot] : 1.0f;
-        uint32_t o[4];
+        for (int y = 0; y < 2; ++y) acc[x][y] = f32x16{};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t two = (e & 2 ? c.y : c.x) >> (16 * (e & 1));
-          const auto v = __builtin_amdgcn_cvt_pk_f32_fp8(two, false);
-          o[e] = bf16_pack(v[0] * f, v[1] * f);
+      for (int s = 0; s < EL_STEPS; ++s) {
+        wait_loads<2 * (EL_STAGES - 2)>();
+        lds_barrier();  // the step is in place, and nobody reads the one before it any more
+        issue(EL_STEPS * p + s + EL_STAGES - 1);
+        const uint16_t* b = sh.b[s % EL_STAGES] + brow * EL_K;
+#pragma unroll
+        for (int g2 = 0; g2 < 2; ++g2) {
+          bf16x8 wf[2][2];
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              wf[y][e] = as_bf16x8(*reinterpret_cast<const uint4*>(b + 16 * EL_K * y + 8 * ((4 * g2 + 2 * h + e) ^ bsw)));
+#pragma unroll
+          for (int x = 0; x < X; ++x) {
+            u32x4& c4 = a[x][2 * s + g2];
+            asm volatile("" : "+v"(c4));  // (else every operand would be made once, before the loop, in 256 registers)
+            const bf16x8 c0 = fp8x8_to_bf16x8(c4[0], c4[1]), c1 = fp8x8_to_bf16x8(c4[2], c4[3]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][0], c0, acc[x][y], 0, 0, 0);
+              acc[x][y] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wf[y][1], c1, acc[x][y], 0, 0, 0);
+            }
+          }
         }
-        *reinterpret_cast<uint4*>(r_out + (size_t)(t0 + r) * EX_R + 8 * p) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+      // a lane's 64 bytes of a token, 4 lanes' tokens: transposed among them, so that 4 lanes write one token's 64 bytes
+      const int part = part0 + p;
+      uint16_t* const out = (part & 1 ? v_out : k_out) +
+                            ((size_t)(t0 + 32 * X * wm + 4 * (j >> 2)) * H + (part >> 1)) * EX_D + 64 * wn + 32 * h + 8 * (j & 3);
+#pragma unroll
+      for (int x = 0; x < X; ++x) {
+        uint32_t o[4][4];  // piece, dword
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 8 * (i & 1) + 2 * e;
+            o[i][e] = bf16_pack(acc[x][i >> 1][r] * sc[x], acc[x][i >> 1][r + 1] * sc[x]);
+          }
+        quad_transpose(o);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t0 + 32 * X * wm + 32 * x + 4 * (j >> 2) + i < end)
+            *reinterpret_cast<u32x4*>(out + (size_t)(32 * x + i) * H * EX_D) = u32x4{o[i][0], o[i][1], o[i][2], o[i][3]};
       }
     }
   }
+  wait_loads<0>();
 }
 
 // -- attention ------------------------------------------------------------------------------------------------------
@@ -429,10 +473,14 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
 
 hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* table, const int* cu,
                                 const uint16_t* w, uint16_t* k, uint16_t* v, uint16_t* r, int B, int total, int H,
-                                int D, int max_pages, int page_size, int num_pages, hipStream_t s) {
-  const unsigned grid = (unsigned)((total + EL_TOK - 1) / EL_TOK) * 2 * H;
-  return launch("expand_latent_kernel", expand_latent_kernel, dim3(grid), dim3(EL_THREADS), s, kv, kvs, table, cu, w,
-                k, v, r, B, total, H, D, max_pages, page_size, num_pages);
+                                int D, int max_pages, int page_size, int num_pages, int num_cu, hipStream_t s) {
+  auto run = [&](auto kernel, int tok) {
+    const int units = (total + tok - 1) / tok * 2 * H;
+    return launch("expand_latent_kernel", kernel, dim3(min(units, num_cu)), dim3(EL_THREADS), s, kv, kvs, table, cu, w,
+                  k, v, r, B, total, H, D, max_pages, page_size, num_pages, units);
+  };
+  return (long)((total + EL_TOK - 1) / EL_TOK) * 2 * H < num_cu ? run(expand_latent_kernel<1>, EL_TOK / 2)
+                                                                : run(expand_latent_kernel<2>, EL_TOK);
 }
 
 // Query tiles that a batch of Tq queries in B sequences may have.
