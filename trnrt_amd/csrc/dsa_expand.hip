@@ -14,11 +14,13 @@ constexpr int EX_C = 512;   // the latent width
 // k[t, h, :] = sigma_t c_t[:512] . W[h, :128, :]^T, v[t, h, :] the same with W[h, 128:, :]: a product of P x 512 x 256 H
 // whose left side is e4m3 rows gathered through the page table (the scale is applied to the sums), and k_rope[t] =
 // sigma_t c_t[512:].
-// What bounds it: the matrix units (512 products a sum are few, so the output, half as many bytes as the sums in fp32,
-// takes a quarter of the time beside it). A workgroup has 256 tokens x one head's 128 keys or values, two of them run on a
-// CU so that one's stores are under the other's products; 64 of the 512 columns at a time come by asynchronous loads
-// straight into LDS, a step ahead. The rows stay e4m3 until they are operands (exact in bf16). The tiles of one XCD share
-// its heads' weights through its L2.
+// What bounds it: the matrix units, then the stores. A share is of units (tile of 256 tokens, one head's 128 keys or
+// values), a workgroup a CU. The rows of a tile stay in registers, e4m3 until they are operands (exact in bf16), while one
+// part's weights after another run through LDS, 64 of the 512 columns a step, by asynchronous loads 7 steps ahead that
+// cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights through LDS, and stores from registers
+// under the next unit's products (that form with two workgroups a CU: 336 us where this takes 256). The shares of one XCD
+// are 8 tiles' and run through the same weights together, out of its L2.
+// 16,384 tokens x 64 heads: 256 us, 1.07 PFLOP/s; 8,192 tokens, whose outputs the last-level cache holds: 112 us, 1.23.
 constexpr int EL_THREADS = 512;
 constexpr int EL_TOK = 256;  // (or half of it)
 constexpr int EL_K = 64;
@@ -479,8 +481,11 @@ hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* 
     return launch("expand_latent_kernel", kernel, dim3(min(units, num_cu)), dim3(EL_THREADS), s, kv, kvs, table, cu, w,
                   k, v, r, B, total, H, D, max_pages, page_size, num_pages, units);
   };
-  return (long)((total + EL_TOK - 1) / EL_TOK) * 2 * H < num_cu ? run(expand_latent_kernel<1>, EL_TOK / 2)
-                                                                : run(expand_latent_kernel<2>, EL_TOK);
+  // tiles of 128 tokens where all their units run at once (16 heads: 1 token 8.1 us with them, 11.0 with tiles of 256;
+  // 1,001 tokens 12.1 and 13.7), else of 256, which read the weights half as often (1,500 tokens 17.9 and 15.7; 64 heads,
+  // 8k tokens 136 and 112)
+  return (long)((total + EL_TOK / 2 - 1) / (EL_TOK / 2)) * 2 * H <= num_cu ? run(expand_latent_kernel<1>, EL_TOK / 2)
+                                                                           : run(expand_latent_kernel<2>, EL_TOK);
 }
 
 // Query tiles that a batch of Tq queries in B sequences may have.
