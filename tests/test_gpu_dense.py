@@ -212,7 +212,7 @@ def test_refusals():
     ok = dict(q=q, kv_cache=kv, kv_scale=sc, table=table, ctx_len=lens, page_size=64, scale=0.1)
     for bad in (dict(q=q[..., :500]), dict(q=q[0, 0]), dict(page_size=60), dict(page_size=0), dict(kv_scale=sc[:-1]),
                 dict(table=table[:1]), dict(table=table[0]), dict(ctx_len=lens[:1]), dict(kv_cache=kv.float()),
-                dict(kv_cache=kv.t()), dict(out=torch.empty(2, 1, 16, 500, device="cuda")),
+                dict(kv_cache=kv.t()), dict(kv_cache=kv.view(-1, 512), kv_scale=None), dict(out=torch.empty(2, 1, 16, 500, device="cuda")),
                 dict(out=torch.empty(2, 1, 16, 512, dtype=torch.float16, device="cuda")),
                 dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))):
         with pytest.raises(ValueError):

@@ -17,6 +17,7 @@ constexpr int PG_THREADS = 256;                       // a copying workgroup
 constexpr int PG_PIECE = PG_THREADS * 16 * 4;         // bytes: four 16-byte loads a thread, all in flight
 constexpr int PG_PLAN_THREADS = 1024;                 // a planning workgroup
 constexpr int PG_BLOCK = PG_PLAN_THREADS * 4;         // pages of a planning workgroup (one int4 of counts a thread)
+constexpr int PG_OWN = 4;                             // blocks up to which each planning workgroup counts all of them
 
 // One piece of page src of every cache it belongs to -> page dst (the whole workgroup).
 __device__ __forceinline__ void copy_piece(const PageCaches& set, int piece, int src, int dst) {
@@ -185,27 +186,41 @@ __global__ __launch_bounds__(PG_THREADS) void pages_release_kernel(int* __restri
 // L live pages go to pages 1 .. L: those already there stay; the k-th live page past L moves to the k-th hole up to L.
 // Moves read pages past L and write pages up to L, so they are independent of each other.
 
+// Of four pages from p on those in use.
+__device__ __forceinline__ int live_of(pg_v4i r, int p) {
+  return (int)(r.x > 0 && p > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0);
+}
+
 // Live pages of each block of PG_BLOCK.
 __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_count_kernel(const int* __restrict__ ref,
                                                                       int* __restrict__ counts, int num_pages) {
   __shared__ int tot[PG_PLAN_THREADS / WAVE];
   const int p = blockIdx.x * PG_BLOCK + 4 * threadIdx.x;
-  const pg_v4i r = load_refs(ref, p, num_pages);
   int total;
-  group_incl_scan<PG_PLAN_THREADS>((int)(r.x > 0 && p > 0) + (r.y > 0) + (r.z > 0) + (r.w > 0), tot, total);
+  group_incl_scan<PG_PLAN_THREADS>(live_of(load_refs(ref, p, num_pages), p), tot, total);
   if (threadIdx.x == 0) counts[blockIdx.x] = total;
 }
 
 // code[p]: p where it stays, -(k + 1) where it is the k-th to move, 0 where it is free; holes[k], movers[k]; moves: their
-// number.
+// number. counts: the live pages of each block, or null where the workgroup counts them itself (up to PG_OWN blocks).
 __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* __restrict__ ref,
-                                                                     const int* __restrict__ counts, int blocks,
+                                                                     const int* counts, int blocks,
                                                                      int* __restrict__ code, int* __restrict__ holes,
                                                                      int* __restrict__ movers, int* __restrict__ moves,
                                                                      int num_pages) {
   __shared__ int tot[PG_PLAN_THREADS / WAVE];
+  __shared__ int own[PG_OWN];
   const int t = threadIdx.x, blk = blockIdx.x;
   int total, before = 0, live = 0;
+  if (!counts) {
+    for (int b = 0; b < blocks; ++b) {
+      group_incl_scan<PG_PLAN_THREADS>(live_of(load_refs(ref, b * PG_BLOCK + 4 * t, num_pages), b * PG_BLOCK + 4 * t), tot,
+                                       total);
+      if (t == 0) own[b] = total;
+    }
+    __syncthreads();
+    counts = own;
+  }
   for (int b0 = 0; b0 < blocks; b0 += PG_PLAN_THREADS) {
     const int c = b0 + t < blocks ? counts[b0 + t] : 0;
     group_incl_scan<PG_PLAN_THREADS>(c, tot, total);
@@ -349,10 +364,13 @@ hipError_t launch_pages_compact(const int* ref, const int* table, int* new_ref, 
   const int blocks = compact_blocks(num_pages);
   int* counts = static_cast<int*>(ws);
   int *moves = counts + blocks, *code = moves + 1, *holes = code + num_pages, *movers = holes + num_pages;
-  hipError_t e = launch("pages_count_kernel", pages_count_kernel, dim3(blocks), dim3(PG_PLAN_THREADS), s, ref, counts,
-                        num_pages);
+  const bool counted = blocks > PG_OWN;
+  hipError_t e = hipSuccess;
+  if (counted)
+    e = launch("pages_count_kernel", pages_count_kernel, dim3(blocks), dim3(PG_PLAN_THREADS), s, ref, counts, num_pages);
   if (e == hipSuccess)
-    e = launch("pages_plan_kernel", pages_plan_kernel, dim3(blocks), dim3(PG_PLAN_THREADS), s, ref, counts, blocks,
+    e = launch("pages_plan_kernel", pages_plan_kernel, dim3(blocks), dim3(PG_PLAN_THREADS), s, ref,
+               counted ? counts : nullptr, blocks,
                code, holes, movers, moves, num_pages);
   for (int at = 0; e == hipSuccess && (at == 0 || at < n_caches); at += PG_CACHES) {
     const PageCaches set = page_caches(caches, page_bytes, n_caches, at);

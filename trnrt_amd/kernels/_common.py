@@ -29,7 +29,9 @@ def on_gpu(*ts: torch.Tensor | None) -> torch.device:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # (the handle alone: a torch.cuda.Stream around it costs more of the host's time than most of a wrapper's checks)
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 def call(device: torch.device, fn, *args) -> int:
@@ -47,8 +49,8 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def need(t: torch.Tensor, name: str, dtype: torch.dtype | tuple, shape: tuple | None = None) -> torch.Tensor:
     """t itself if it has the dtype (one of), shape (None entries free) and is contiguous; ValueError otherwise."""
-    dts = dtype if isinstance(dtype, tuple) else (dtype,)
-    if t.dtype not in dts:
+    if t.dtype is not dtype and (not isinstance(dtype, tuple) or t.dtype not in dtype):
+        dts = dtype if isinstance(dtype, tuple) else (dtype,)
         raise ValueError(f"{name}: dtype {t.dtype}, expected {' or '.join(map(str, dts))}")
     if shape is not None and t.shape != shape:  # (unequal also where an entry is free)
         if t.dim() != len(shape) or any(s is not None and s != d for s, d in zip(shape, t.shape)):
@@ -68,6 +70,15 @@ def as_i32(t: torch.Tensor) -> torch.Tensor:
 
 def as_f32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
+
+
+def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
+    """A contiguous tensor as rows [n, width] (itself where it is that already)."""
+    return t if t.dim() == 2 else t.reshape(-1, width)
+
+
+def flat(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dim() == 1 else t.reshape(-1)
 
 
 def fp8_bytes(t: torch.Tensor, name: str) -> torch.Tensor:

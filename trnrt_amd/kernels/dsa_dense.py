@@ -36,20 +36,22 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     B, H, dqk = q.shape[0], q.shape[-2], q.shape[-1]
     S = q.shape[1] if q.dim() == 4 else 1
     q = C.as_bf16(q)
-    kv = C.fp8_bytes(kv_cache, "kv cache").reshape(-1, dqk)
+    if kv_cache.shape[-1] != dqk:
+        raise ValueError(f"dsa_dense: cache rows of {kv_cache.shape[-1]} for q of {dqk}")
+    kv = C.rows_of(C.fp8_bytes(kv_cache, "kv cache"), dqk)
     slots = kv.shape[0]
     if page_size < 1 or slots < 1 or slots % page_size:
         raise ValueError(f"dsa_dense: {slots} cache slots are not whole pages of {page_size}")
     if kv_scale is not None:
-        kv_scale = C.need(C.as_f32(kv_scale).reshape(-1), "kv_scale", torch.float32, (slots,))
+        kv_scale = C.need(C.flat(C.as_f32(kv_scale)), "kv_scale", torch.float32, (slots,))
     tb, lens = C.as_i32(table), C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
     if tb.dim() != 2 or tb.shape[0] != B or tb.shape[1] < 1:
         raise ValueError(f"dsa_dense: page table {tuple(table.shape)} for {B} sequences")
     shape = q.shape[:-1] + (DV,)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype, device=dev)
+        out = q.new_empty(shape, dtype=out_dtype)
     C.need(out, "out", (torch.bfloat16, torch.float32), shape)
-    ls = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if lse else None
+    ls = q.new_empty(q.shape[:-1], dtype=torch.float32) if lse else None
     lib = _lib.lib()
     ws = workspace
     if ws is None:

@@ -37,12 +37,12 @@ def expand(kv_cache: torch.Tensor, kv_scale: torch.Tensor | None, table: torch.T
     D = kv_cache.shape[-1]
     if D not in DQK_WIDTHS:
         raise ValueError(f"dsa_expand: cache rows of {D}, expected 576 or 512")
-    kv = C.fp8_bytes(kv_cache, "kv cache").reshape(-1, D)
+    kv = C.rows_of(C.fp8_bytes(kv_cache, "kv cache"), D)
     slots = kv.shape[0]
     if page_size < 1 or slots < 1 or slots % page_size:
         raise ValueError(f"dsa_expand: {slots} cache slots are not whole pages of {page_size}")
     if kv_scale is not None:
-        kv_scale = C.need(C.as_f32(kv_scale).reshape(-1), "kv_scale", torch.float32, (slots,))
+        kv_scale = C.need(C.flat(C.as_f32(kv_scale)), "kv_scale", torch.float32, (slots,))
     if w.dim() != 3 or w.shape[0] < 1:
         raise ValueError(f"dsa_expand: w {tuple(w.shape)}, expected [H, {2 * DH}, {DV}]")
     H = w.shape[0]
@@ -55,8 +55,8 @@ def expand(kv_cache: torch.Tensor, kv_scale: torch.Tensor | None, table: torch.T
         raise ValueError(f"dsa_expand: {total} rows")
     cu = C.need(C.as_i32(cu_len), "cu_len", torch.int32, (B + 1,))
     if out is None:
-        k, v = (torch.empty(total, H, DH, dtype=torch.bfloat16, device=dev) for _ in range(2))
-        r = torch.empty(total, ROPE, dtype=torch.bfloat16, device=dev) if D > DV else None
+        k, v = w.new_empty((total, H, DH)), w.new_empty((total, H, DH))
+        r = w.new_empty((total, ROPE)) if D > DV else None
     else:
         k, r, v = out
         C.need(k, "k", torch.bfloat16, (total, H, DH))
@@ -96,9 +96,9 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
         raise ValueError(f"dsa_expand: cu_q {tuple(cu_q.shape)} and cu_k {tuple(cu_k.shape)}, expected [B + 1]")
     cq, ck = C.as_i32(cu_q), C.as_i32(cu_k)
     if out is None:
-        out = torch.empty(Tq, H, DH, dtype=out_dtype, device=dev)
+        out = q.new_empty((Tq, H, DH), dtype=out_dtype)
     C.need(out, "out", (torch.bfloat16, torch.float32), (Tq, H, DH))
-    ls = torch.empty(Tq, H, dtype=torch.float32, device=dev) if lse else None
+    ls = q.new_empty((Tq, H), dtype=torch.float32) if lse else None
     bf = out.dtype == torch.bfloat16
     st = C.call(dev, _lib.lib().dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),
                 C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), cu_q.numel() - 1, Tq, Tk, H,

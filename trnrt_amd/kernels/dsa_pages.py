@@ -82,8 +82,7 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     n = parents.numel()
     tb, par = C.as_i32(table), C.as_i32(parents)
     lens = C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
-    child = torch.empty(n, max_pages, dtype=torch.int32, device=dev)
-    pages = torch.empty(n, dtype=torch.int32, device=dev)
+    child, pages = tb.new_empty((n, max_pages)), tb.new_empty((n,))
     lib = _lib.lib()
     ws = workspace
     if ws is None:
@@ -124,7 +123,7 @@ def compact(ref: torch.Tensor, table: torch.Tensor, caches, page_size: int, *,
         raise ValueError(f"dsa_pages.compact: table {tuple(table.shape)}, expected [B, max_pages]")
     B, max_pages = table.shape
     tb = C.as_i32(table)
-    new_table = torch.empty(B, max_pages, dtype=torch.int32, device=dev)
+    new_table = tb.new_empty((B, max_pages))
     new_ref, remap = torch.empty_like(ref), torch.empty_like(ref)
     lib = _lib.lib()
     ws = workspace
