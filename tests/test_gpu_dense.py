@@ -124,6 +124,40 @@ def test_flat_and_steep_softmax(gain):
     check((-q.abs(), kv, sc, table, lens), 64)
 
 
+def test_scales_far_apart():
+    """Token scales from 2^-40 to 2^6 within a chunk, zeros among them; where every other score lies far below zero, the
+    tokens of scale 0 have the largest softmax weights and add nothing."""
+    say("dense scales far apart")
+    q, kv, sc, table, lens = make([900, 130, 64], 1, 24, 576, 64, seed=6, spread=0.0)
+    live = sc == sc
+    g = torch.Generator().manual_seed(7)
+    e = torch.randint(-40, 7, sc.shape, generator=g).float()
+    check((q, kv, torch.where(live, torch.exp2(e) / 448, sc), table, lens), 64)
+    check((q, kv, torch.where(live & (torch.arange(sc.numel()) % 3 > 0), torch.exp2(e) / 448, torch.where(live, 0.0, sc)), table, lens), 64)
+    low = torch.where(kv == 0x7F, kv, 0x38)  # every value 1
+    zero_late = torch.where(live, torch.where(torch.arange(sc.numel()) % 5 > 0, 1.0, 0.0), sc)
+    check((-q.abs() * 8, low, zero_late, table, lens), 64)  # scores near -2,500, and 0
+
+
+def test_one_token_outweighs_the_rest():
+    """A first token that only its rope columns score, with 2^22 times the weight of each other and no value: the outputs
+    are the others', to their own size."""
+    say("dense one token outweighs the rest")
+    q, kv, sc, table, lens = make([3000, 500], 1, 32, 576, 64, seed=8, spread=0.0)
+    scale = 192 ** -0.5
+    q[..., :512] *= 0.05
+    q[..., 512:] = 1.0
+    for b in range(2):
+        n = int(lens[b])
+        t = torch.arange(n)
+        slot = table[b][t // 64].long() * 64 + t % 64
+        kv[slot, 512:] = 0  # (+0)
+        first = table[b][0].long() * 64
+        kv[first, :512], kv[first, 512:], sc[first] = 0, 0x38, 22 * 0.6931471805599453 / (64 * scale)
+    check((q, kv, sc, table, lens), 64, scale=scale)
+    check((q, kv, sc, table, lens), 64, scale=scale, out_dtype=torch.float32)
+
+
 @pytest.mark.parametrize("H", [16, 64])
 def test_long_and_ragged(H):
     """Row tiles shared by many workgroups, several tiles in one workgroup, sequences without tokens between."""

@@ -234,7 +234,7 @@ constexpr int XA_THREADS = 512;
 constexpr int XA_Q = 256;
 constexpr int XA_K = 64;
 constexpr int XA_STAGES = 3;
-constexpr float XA_SLACK = 11.5f;  // lazy rescaling (base 2): p = 2^(s - m) <= 2^11.5 between moves of m
+constexpr float XA_SLACK = 60.0f;  // lazy rescaling (base 2): p = 2^(s - m) <= 2^60 between moves of m
 constexpr float XA_LOG2E = 1.44269504088896341f;
 
 typedef short xa_v4s __attribute__((ext_vector_type(4)));
