@@ -53,7 +53,7 @@ constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are mult
 template <int RB>
 struct DnShared {
   alignas(1024) uint8_t tile[DN_BUFS][DN_CHUNK * DN_KROW];  // (the queries in the last two before)
-  alignas(16) uint16_t p[2][32 * RB * DN_PROW];   // P[row][token] of two chunks
+  alignas(16) uint16_t p[2][64 * DN_PROW];        // P[row][token] of two chunks (32 rows: their second terms after them)
   alignas(16) float ksc[DN_BUFS][DN_CHUNK];       // the chunks' token scales
   alignas(16) float kfac[DN_BUFS][DN_CHUNK];      // x softmax scale x log2 e
   float cmax[2][32 * RB];                         // [token half][row]: a chunk's maxima when one moves
@@ -273,9 +273,19 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 #pragma unroll
         for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[4 * g + e]);
         psum += (pv[0] + pv[1]) + (pv[2] + pv[3]);
-        // (bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded)
-        *reinterpret_cast<uint2*>(pw + (c & 1) * ROWS * DN_PROW + 8 * g) =
-            make_uint2(bf16_pack(pv[0] * ks[0], pv[1] * ks[1]), bf16_pack(pv[2] * ks[2], pv[3] * ks[3]));
+        // bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded. A tile of
+        // 32 rows, whose bound is the cache's stream, takes what the rounding left as a second term (2^-16)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pv[e] *= ks[e];
+        uint32_t w[2] = {bf16_pack(pv[0], pv[1]), bf16_pack(pv[2], pv[3])};
+        uint16_t* const to = pw + (c & 1) * 64 * DN_PROW + 8 * g;
+        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        if (RB == 1) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            w[e] = bf16_pack(pv[2 * e] - __uint_as_float(w[e] << 16), pv[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+          *reinterpret_cast<uint2*>(to + 32 * DN_PROW) = make_uint2(w[0], w[1]);
+        }
       };
       // a chunk whose flags (fl) are up: its maxima over both token halves, the moved running maxima, P again
       auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
@@ -419,15 +429,15 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW + 64 * ((i & 3) >> 1)));
       };
       auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
-        return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * ROWS * DN_PROW + 32 * i * DN_PROW + 16 * t));
+        return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * 64 * DN_PROW + 32 * i * DN_PROW + 16 * t));
       };
       // Interval c: chunk c - 1's weights are final (and O on their maxima) once its flags are seen; then its value product,
-      // 16 steps of RB products, the next steps' operands read and converted ahead, side(i) beside step i.
+      // 16 steps of two products, the next steps' operands read and converted ahead, side(i) beside step i.
       auto interval = [&](int c, const uint8_t* kt, auto side) __attribute__((always_inline)) {
         const int pb = (c - 1) & 1;
         const int4 fl = *reinterpret_cast<const int4*>(sh.flag[pb]);
         dn_v2i vv[DN_VAHEAD + 1];
-        bf16x8 pa[2][RB], vb[2];
+        bf16x8 pa[2][2], vb[2];
 #pragma unroll
         for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
         if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
@@ -445,17 +455,19 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           }
         }
 #pragma unroll
-        for (int i = 0; i < RB; ++i) pa[0][i] = p_read(pb, 0, i);
+        for (int i = 0; i < 2; ++i) pa[0][i] = p_read(pb, 0, i);
         vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int t = i >> 2, d = i & 3;
           if (i + DN_VAHEAD < 16) vv[(i + DN_VAHEAD) % (DN_VAHEAD + 1)] = v_read(kt, i + DN_VAHEAD);
-          if (d < RB && t < 3) pa[(t + 1) & 1][d] = p_read(pb, t + 1, d);
+          if (d < 2 && t < 3) pa[(t + 1) & 1][d] = p_read(pb, t + 1, d);
 #pragma unroll
-          for (int x = 0; x < RB; ++x)
-            o[d][x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i & 1], pa[t & 1][x], o[d][x], 0, 0, 0);
+          for (int x = 0; x < 2; ++x) {
+            f32x16& sum = o[d][RB == 1 ? 0 : x];
+            sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i & 1], pa[t & 1][x], sum, 0, 0, 0);
+          }
           if (i < 15) {
             const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
             vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
