@@ -62,7 +62,7 @@ struct DnShared {
   float lsum[2][32 * RB];                         // [token half][row]: a stretch's sums
   float mfin[32 * RB];                            // and maxima (base 2)
   int tot[DN_THREADS / WAVE];
-  int found[3];
+  int found[4];
 };
 
 // t / page_size for 0 <= t < 2^31: t x mul >> shift (mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size)).
@@ -110,6 +110,12 @@ __device__ __forceinline__ int dn_owner(int u, const DnList& x) {
   return u < big ? u / (x.share + 1) : x.more + (u - big) / x.share;
 }
 
+// Where a partial's piece lies: dims 128 w + 32 d + 8 g + 4 h .. + 3 of row 32 i + j of a tile, at 4 (32 h + j) from there, as
+// the value waves' lanes hold it.
+__device__ __forceinline__ constexpr int dn_partial(int w, int i, int d, int g, int blocks) {
+  return (((w * blocks + i) * 4 + d) * 4 + g) * 4 * WAVE;
+}
+
 template <int DQK, int RB>
 __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const uint16_t* __restrict__ q, const uint8_t* __restrict__ kv, const float* __restrict__ kvs,
@@ -125,11 +131,12 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   const int M = S * H;
 
   // the list, and the sequence of this team's first unit
-  int chunks = 0, n = 0, incl = 0;
+  int chunks = 0, len = 0, n = 0, incl = 0;
   for (int b0 = 0; b0 < B; b0 += DN_THREADS) {
     const int x = b0 + tid;
     int total;
-    n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, pg.size)) : 0;
+    len = x < B ? dn_len(ctx_len[x], max_pages, pg.size) : 0;
+    n = dn_chunks(len);
     incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
     chunks += total;
   }
@@ -143,7 +150,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const int x = b0 + tid;
     int total = 0;
     if (B > DN_THREADS) {  // (else they are still at hand)
-      n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, pg.size)) : 0;
+      len = x < B ? dn_len(ctx_len[x], max_pages, pg.size) : 0;
+      n = dn_chunks(len);
       incl = group_incl_scan<DN_THREADS>(n, sh.tot, total);
     }
     const int lo = before + (incl - n) * tm.sets;
@@ -151,6 +159,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       sh.found[0] = x;
       sh.found[1] = (u0 - lo) / n;
       sh.found[2] = (u0 - lo) % n;
+      sh.found[3] = len;
     }
     before += total * tm.sets;
   }
@@ -167,17 +176,18 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
   int set = __builtin_amdgcn_readfirstlane(sh.found[1]);
   int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
+  len = __builtin_amdgcn_readfirstlane(sh.found[3]);
 
   for (int u = u0; u < u1;) {
-    const int len = dn_len(ctx_len[b], max_pages, pg.size), all = dn_chunks(len);
+    const int all = dn_chunks(len);
     const int nch = min(all - c0, u1 - u);  // this stretch's chunks
     const bool whole = nch == all;
     const int t0 = c0 * DN_CHUNK, r0 = (set * tm.span + member) * ROWS;  // its first token, and this workgroup's row
     const int part = (2 * team + (u > u0)) * tm.span + member;            // where its partials go
     if (r0 < M) {  // (else the last set has no tile for this member)
 
-    // the outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x & 7)), so that a
-    // row's pieces in order and a piece's rows in order both cover the banks once; a wave writes whole rows
+    // A whole row tile's outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x & 7)),
+    // so that a row's pieces in order and a piece's rows in order both cover the banks once; a wave writes whole rows.
     f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
     auto write = [&](int half) __attribute__((always_inline)) {
       const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
@@ -187,22 +197,30 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         if (r0 + r >= M) break;
         f32x4 v = area[64 * lane + (r ^ (lane & 7))];
         const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
-        if (whole) {
-          const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= inv;
-          const size_t at = (size_t)b * M + r0 + r;
-          if (out)
-            *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
-          if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
-          if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
-        } else {
-          *reinterpret_cast<f32x4*>(ws_o + ((size_t)part * ROWS + r) * DN_DV + dim) = v;
-          if (half == 0 && lane == 0) {
-            ws_ml[2 * ((size_t)part * ROWS + r)] = m;
-            ws_ml[2 * ((size_t)part * ROWS + r) + 1] = l;
-          }
-        }
+        for (int e = 0; e < 4; ++e) v[e] *= inv;
+        const size_t at = (size_t)b * M + r0 + r;
+        if (out)
+          *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+        if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
+        if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+      }
+    };
+    // The end of a stretch in every wave, after the barrier behind which the tiles are free and the sums in LDS; the value
+    // waves bring store(half).
+    auto finish = [&](auto store) __attribute__((always_inline)) {
+      if (whole) {
+        store(0);
+        lds_barrier();
+        write(0);
+        lds_barrier();
+        store(1);
+        lds_barrier();
+        write(1);
+      } else if (tid < ROWS && r0 + tid < M) {
+        float2* const ml = reinterpret_cast<float2*>(ws_ml) + (size_t)part * ROWS + tid;
+        *ml = make_float2(sh.mfin[tid], sh.lsum[0][tid] + sh.lsum[1][tid]);
       }
     };
 
@@ -237,11 +255,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           }
           lds_barrier();
         }
-        lds_barrier();
-        write(0);
-        lds_barrier();
-        lds_barrier();
-        write(1);
+        finish([](int) {});
       } else {
       const int row = min(r0 + 32 * hh + j, M - 1);
       const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
@@ -381,12 +395,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
       if (h == 0) sh.lsum[th][32 * hh + j] = lw;
       if (th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
-      lds_barrier();  // the tiles are free
-      lds_barrier();  // the first 256 dims' outputs are in LDS
-      write(0);
       lds_barrier();
-      lds_barrier();  // and the others'
-      write(1);
+      finish([](int) {});
       }
     } else {
       // -- the loads and the values: thread 4 r + e of the value waves brings row r of a chunk, pieces e + 4 i; wave w takes
@@ -405,7 +415,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         return safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
       };
       const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ dn_swizzle(gr));  // where its pieces go in a tile
-      u32x4 r0[PIECES];  // the pieces in flight, of the chunk after the one being stored
+      u32x4 held[PIECES];  // the pieces in flight, of the chunk after the one being stored
       float sc;          // and its token's scale
       auto row_of = [&](int slot) __attribute__((always_inline)) { return kv + (size_t)slot * DQK + 16 * (lane & 3); };
       auto store_scale = [&](int to) __attribute__((always_inline)) {
@@ -478,22 +488,22 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
       };
       int page = trow[page_of(token(2))];  // of this thread's token two chunks on
       const int page0 = trow[page_of(token(0))], page1 = trow[page_of(token(1))];
-      {
-        const int slot = slot_of(0, page0);
-        const uint8_t* src = row_of(slot);
+      {  // chunks 0 and 1 together: the first into LDS, the second stays in flight
+        const int slot0 = slot_of(0, page0), slot1 = slot_of(1, page1);
+        const uint8_t *src0 = row_of(slot0), *src1 = row_of(slot1);
+        u32x4 first[PIECES];
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
-        sc = kvs ? kvs[slot] : 1.0f;
+        for (int i = 0; i < PIECES; ++i) first[i] = *reinterpret_cast<const u32x4*>(src0 + 64 * i);
+        const float sc0 = kvs ? kvs[slot0] : 1.0f;
 #pragma unroll
-        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<u32x4*>(sh.tile[0] + gs + 64 * i) = r0[i];
+        for (int i = 0; i < PIECES; ++i) held[i] = *reinterpret_cast<const u32x4*>(src1 + 64 * i);
+        const float sc1 = kvs ? kvs[slot1] : 1.0f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<u32x4*>(sh.tile[0] + gs + 64 * i) = first[i];
+        sc = sc0;
         store_scale(0);
-      }
-      {
-        const int slot = slot_of(1, page1);
-        const uint8_t* src = row_of(slot);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
-        sc = kvs ? kvs[slot] : 1.0f;
+        sc = sc1;
       }
       lds_barrier();  // the queries and chunk 0 are in place
       lds_barrier();  // the queries are read
@@ -508,8 +518,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         if (kvs) sc_next = kvs[slot];
       };
       auto piece = [&](int i, uint8_t* to) __attribute__((always_inline)) {
-        *reinterpret_cast<u32x4*>(to + gs + 64 * i) = r0[i];
-        r0[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
+        *reinterpret_cast<u32x4*>(to + gs + 64 * i) = held[i];
+        held[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
       };
       ahead(0);
 #pragma unroll
@@ -530,7 +540,20 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         buf = next;
         lds_barrier();
       }
-      auto store = [&]() __attribute__((always_inline)) {
+      if (!whole) {  // as they lie in the registers: see dn_partial
+        float* const to = ws_o + (size_t)part * ROWS * DN_DV + dn_partial(w, 0, 0, 0, RB) + 4 * lane;
+#pragma unroll
+        for (int i = 0; i < RB; ++i)
+          if (32 * i + j < M - r0)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(to + dn_partial(0, i, d, g, RB)) =
+                    f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
+      }
+      finish([&](int half) __attribute__((always_inline)) {
+        if ((w >> 1) != half) return;
 #pragma unroll
         for (int i = 0; i < RB; ++i)
 #pragma unroll
@@ -541,14 +564,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
               area[64 * x + ((32 * i + j) ^ (x & 7))] =
                   f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
             }
-      };
-      if (w < 2) store();
-      lds_barrier();
-      write(0);
-      lds_barrier();
-      if (w >= 2) store();
-      lds_barrier();
-      write(1);
+      });
     }
     lds_barrier();  // (the area's readers, before the next stretch's loads)
     }
@@ -556,40 +572,43 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     c0 = 0;
     if (u < u1 && ++set == tm.sets) {  // the next sequence with tokens
       set = 0;
-      do ++b;
-      while (ctx_len[b] <= 0);
+      do len = dn_len(ctx_len[++b], max_pages, pg.size);
+      while (len == 0);
     }
   }
 }
 
-// Joins the partials of a row where its row tile was shared: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the
-// rows of sequences without tokens. Four partials are in flight in a wave, each lane has 8 of the dims. WPR waves a row: a
-// wave takes every WPR-th partial.
+// Joins the partials of a row tile where teams shared it: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the rows of
+// sequences without tokens. A wave has 32 rows x 32 dims, in the partials' own order, and four partials in flight; WPR waves
+// of a workgroup share them, each taking every WPR-th.
 constexpr int DC_WAVES = 8;
 constexpr int DC_THREADS = DC_WAVES * WAVE;
 
-template <int WPR>
+template <int RB, int WPR>
 __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ ctx_len,
     uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H,
     int max_pages, int page_size, DnTeams tm) {
+  constexpr int ROWS = 32 * RB, BLOCKS = 16 * RB;  // blocks of 32 x 32 in a tile
   __shared__ int tot[DC_WAVES];
-  __shared__ int chunks_before[DC_WAVES];
-  __shared__ float wm[DC_WAVES], wl[DC_WAVES];
-  __shared__ alignas(16) float acc[WPR > 1 ? DC_WAVES : 1][DN_DV];
+  __shared__ int chunks_before[2];
+  __shared__ float wm[DC_WAVES][32], wl[DC_WAVES][32];
+  __shared__ f32x4 acc[WPR > 1 ? DC_WAVES : 1][4][WAVE];
   const int M = S * H, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  // this wave's row (the last one again past the end, not written)
-  const int at_row = blockIdx.x * (DC_WAVES / WPR) + wave / WPR, g = min(at_row, B * M - 1);
-  const int b = g / M, row = g - b * M, mt = row / tm.rows, j = row - mt * tm.rows;
-  const int first_b = __builtin_amdgcn_readfirstlane(min(blockIdx.x * (DC_WAVES / WPR), B * M - 1) / M);
+  const int j = lane & 31, h = lane >> 5;
+  // this wave's block (the last one again past the end, not written)
+  const int blocks = B * tm.tiles * BLOCKS, first_at = blockIdx.x * (DC_WAVES / WPR), at = first_at + wave / WPR;
+  const int block = min(at, blocks - 1) % BLOCKS, tile = min(at, blocks - 1) / BLOCKS;
+  const int b = tile / tm.tiles, mt = tile - b * tm.tiles;
+  const int first_b = first_at / BLOCKS / tm.tiles;  // (8 blocks are of two tiles at most)
   int chunks = 0;
   for (int b0 = 0; b0 < B; b0 += DC_THREADS) {
     const int x = b0 + tid;
     const int n = x < B ? dn_chunks(dn_len(ctx_len[x], max_pages, page_size)) : 0;
     int total;
     const int incl = chunks + group_incl_scan<DC_THREADS>(n, tot, total);
-    if (x >= first_b && x < first_b + DC_WAVES) chunks_before[x - first_b] = incl - n;  // (rows of 8 sequences at most)
+    if (x >= first_b && x < first_b + 2) chunks_before[x - first_b] = incl - n;
     chunks += total;
   }
   __syncthreads();
@@ -598,80 +617,102 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
   // the row tile's units: first .. first + nch - 1
   const int first = chunks_before[b - first_b] * tm.sets + mt / tm.span * nch;
   const int w0 = nch ? dn_owner(first, list) : 0, w1 = nch ? dn_owner(first + nch - 1, list) : -1;
-  const bool live = at_row < B * M && w0 != w1;  // (one team's: its workgroup wrote them)
-  if (WPR > 1 && !live) return;                  // (the whole workgroup)
+  if (at >= blocks || w0 == w1) return;  // (one team's: its workgroup wrote them; the same for all of a block's waves)
+  const int w = block / (4 * RB), i = block / 4 % RB, d = block & 3;
+  const int r = 32 * i + j, row = mt * ROWS + r;  // this lane's row of the tile, and of the sequence
   float m = -INFINITY, l = 0.0f;
-  f32x4 a[2] = {};
-  if (live && nch > 0) {
+  f32x4 a[4] = {};
+  if (nch > 0) {
+    const float* const from = ws_o + dn_partial(w, i, d, 0, RB) + 4 * lane;
     // team w0's stretch is not its first where it started before the tile, the others' is
     const int slot0 = 2 * w0 + (dn_start(w0, list) < first);
-    for (int w = w0 + wave % WPR; w <= w1; w += 4 * WPR) {
-      float pm[4], pl[4];
-      f32x4 v[4][2];
+    for (int t = w0 + wave % WPR; t <= w1; t += 4 * WPR) {
+      float2 ml[4];
+      f32x4 v[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = min(w + WPR * i, w1);
-        const size_t s = ((size_t)(x == w0 ? slot0 : 2 * x) * tm.span + mt % tm.span) * tm.rows + j;
-        pm[i] = ws_ml[2 * s];
-        pl[i] = ws_ml[2 * s + 1];
+      for (int x = 0; x < 4; ++x) {
+        const int u = min(t + WPR * x, w1);
+        const size_t part = ((size_t)(u == w0 ? slot0 : 2 * u) * tm.span + mt % tm.span) * ROWS;
+        ml[x] = reinterpret_cast<const float2*>(ws_ml)[part + r];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) v[i][e] = *reinterpret_cast<const f32x4*>(ws_o + s * DN_DV + 256 * e + 4 * lane);
+        for (int g = 0; g < 4; ++g) v[x][g] = *reinterpret_cast<const f32x4*>(from + part * DN_DV + 4 * WAVE * g);
       }
       float mx = m;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mx = max_nonan(mx, pm[i]);  // (past w1: the last one again, of weight 0 below)
+      for (int x = 0; x < 4; ++x) mx = max_nonan(mx, ml[x].x);  // (past w1: the last one again, of weight 0 below)
       const float f = __builtin_amdgcn_exp2f(m - mx);
       m = mx;
       l *= f;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int g = 0; g < 4; ++g)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) a[e][x] *= f;
+        for (int e = 0; e < 4; ++e) a[g][e] *= f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float c = w + WPR * i <= w1 ? __builtin_amdgcn_exp2f(pm[i] - m) : 0.0f;
-        l = fmaf(c, pl[i], l);
+      for (int x = 0; x < 4; ++x) {
+        const float c = t + WPR * x <= w1 ? __builtin_amdgcn_exp2f(ml[x].x - m) : 0.0f;
+        l = fmaf(c, ml[x].y, l);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) a[e][x] = fmaf(c, v[i][e][x], a[e][x]);
+          for (int e = 0; e < 4; ++e) a[g][e] = fmaf(c, v[x][g][e], a[g][e]);
       }
     }
   }
+  const size_t out_row = (size_t)b * M + row;
   if (WPR == 1) {
-    if (!live) return;
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    uint2 pk[4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const size_t at = (size_t)g * DN_DV + 256 * e + 4 * lane;
-      const f32x4 v = {a[e][0] * inv, a[e][1] * inv, a[e][2] * inv, a[e][3] * inv};
-      if (out) *reinterpret_cast<uint2*>(out + at) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
-      if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at) = v;
+    for (int g = 0; g < 4; ++g) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[g][e] *= inv;
+      pk[g] = make_uint2(bf16_pack(a[g][0], a[g][1]), bf16_pack(a[g][2], a[g][3]));
     }
-    if (lse_out && lane == 0) lse_out[g] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+    // lanes j and 32 + j have a row's 64 bytes by eights in turn: each takes a half of them
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const uint2 give = h ? pk[g] : pk[g + 2];
+      const uint2 got = make_uint2(__shfl_xor((int)give.x, 32, WAVE), __shfl_xor((int)give.y, 32, WAVE));
+      const uint2 own = h ? pk[g + 2] : pk[g];
+      if (out && row < M)
+        *reinterpret_cast<uint4*>(out + out_row * DN_DV + 128 * w + 32 * d + 16 * h + 8 * g) =
+            h ? make_uint4(got.x, got.y, own.x, own.y) : make_uint4(own.x, own.y, got.x, got.y);
+    }
+    if (row >= M) return;
+    if (out_f32)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(out_f32 + out_row * DN_DV + 128 * w + 32 * d + 8 * g + 4 * h) = a[g];
+    if (lse_out && w == 0 && d == 0 && h == 0) lse_out[out_row] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
     return;
   }
-  if (lane == 0) {
-    wm[wave] = m;
-    wl[wave] = l;
+  if (h == 0) {
+    wm[wave][j] = m;
+    wl[wave][j] = l;
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e) *reinterpret_cast<f32x4*>(&acc[wave % (WPR > 1 ? DC_WAVES : 1)][256 * e + 4 * lane]) = a[e];
+  for (int g = 0; g < 4; ++g) acc[WPR > 1 ? wave : 0][g][lane] = a[g];
   __syncthreads();
-  float mm = wm[0], ll = 0.0f, o = 0.0f;
+  if (wave >= 4 || row >= M) return;  // wave g joins the pieces g
+  float mm = wm[0][j], ll = 0.0f;
+  f32x4 o = {};
 #pragma unroll
-  for (int w = 1; w < DC_WAVES; ++w) mm = max_nonan(mm, wm[w]);
+  for (int x = 1; x < DC_WAVES; ++x) mm = max_nonan(mm, wm[x][j]);
 #pragma unroll
-  for (int w = 0; w < DC_WAVES; ++w) {
-    const float f = mm > -INFINITY ? __builtin_amdgcn_exp2f(wm[w] - mm) : 0.0f;  // (0 for a wave without partials)
-    ll = fmaf(f, wl[w], ll);
-    o = fmaf(f, acc[WPR > 1 ? w : 0][tid], o);
+  for (int x = 0; x < DC_WAVES; ++x) {
+    const float f = mm > -INFINITY ? __builtin_amdgcn_exp2f(wm[x][j] - mm) : 0.0f;  // (0 for a wave without partials)
+    ll = fmaf(f, wl[x][j], ll);
+    const f32x4 v = acc[WPR > 1 ? x : 0][wave][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(f, v[e], o[e]);
   }
-  const size_t at = (size_t)g * DN_DV + tid;
+  const size_t to = out_row * DN_DV + 128 * w + 32 * d + 8 * wave + 4 * h;
   const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
-  if (out) out[at] = f32_to_bf16_bits(o * inv);
-  if (out_f32) out_f32[at] = o * inv;
-  if (lse_out && tid == 0) lse_out[g] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  if (out) *reinterpret_cast<uint2*>(out + to) = make_uint2(bf16_pack(o[0], o[1]), bf16_pack(o[2], o[3]));
+  if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + to) = o;
+  if (lse_out && block == 4 * i && wave == 0 && h == 0) lse_out[out_row] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
 }
 
 // Workgroups: one a CU, a multiple of the 8 XCDs.
@@ -721,21 +762,21 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
   const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
                               out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale, tm);
   if (e != hipSuccess) return e;
-  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a row where its first four are
-  // most of them (512 rows of 33 partials: 8.4 us in 8 waves a row; 3,072 rows of 6: 11.1 in one, 19.0 in 8)
-  const long all = (long)B * S * H;
-  if (tm.teams >= 7L * B * tm.sets)
-    return launch("dense_combine_kernel", dense_combine_kernel<DC_WAVES>, dim3((unsigned)all), dim3(DC_THREADS), s,
-                  ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, max_pages, page_size, tm);
-  return launch("dense_combine_kernel", dense_combine_kernel<1>, dim3((unsigned)((all + DC_WAVES - 1) / DC_WAVES)),
-                dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out, out_f32, lse, B, S, H, max_pages, page_size, tm);
+  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a block where its first four are
+  // most of them
+  const bool many = tm.teams >= 7L * B * tm.sets;
+  const long blocks = (long)B * tm.tiles * (tm.rows / 2), groups = many ? blocks : (blocks + DC_WAVES - 1) / DC_WAVES;
+  const auto combine = tm.rows == 32 ? many ? dense_combine_kernel<1, DC_WAVES> : dense_combine_kernel<1, 1>
+                                     : many ? dense_combine_kernel<2, DC_WAVES> : dense_combine_kernel<2, 1>;
+  return launch("dense_combine_kernel", combine, dim3((unsigned)groups), dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out,
+                out_f32, lse, B, S, H, max_pages, page_size, tm);
 }
 
 // Whether the list of units fits 32 bits, whatever the lengths, and the rows a launch.
 bool dense_list_ok(int B, int S, int H, int max_pages, int page_size) {
   const long M = (long)S * H, tiles = (M + 31) / 32, cap = (long)max_pages * page_size;
   const long tokens = cap < 0x7fffffffL ? cap : 0x7fffffffL;
-  return M <= 0x7fffffffL && (long)B * M <= 0x7fffffL && (double)B * tiles * (tokens / DN_CHUNK + 1) < 2e9;
+  return M <= 0x7fffffffL && (long)B * tiles <= 0x3fffffL && (double)B * tiles * (tokens / DN_CHUNK + 1) < 2e9;
 }
 
 }  // namespace dsa
