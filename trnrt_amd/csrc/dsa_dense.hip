@@ -579,21 +579,21 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 }
 
 // Joins the partials of a row tile where teams shared it: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the rows of
-// sequences without tokens. A wave has 32 rows x 32 dims, in the partials' own order, and four partials in flight; WPR waves
-// of a workgroup share them, each taking every WPR-th.
+// sequences without tokens. A wave has a block of 32 rows x 8 G dims, in the partials' own order; WPR waves of a workgroup
+// share a block's partials, each taking every WPR-th, DEEP of them in flight.
 constexpr int DC_WAVES = 8;
 constexpr int DC_THREADS = DC_WAVES * WAVE;
 
-template <int RB, int WPR>
+template <int RB, int WPR, int G>
 __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     const float* __restrict__ ws_o, const float* __restrict__ ws_ml, const int* __restrict__ ctx_len,
     uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int S, int H,
     int max_pages, int page_size, DnTeams tm) {
-  constexpr int ROWS = 32 * RB, BLOCKS = 16 * RB;  // blocks of 32 x 32 in a tile
+  constexpr int ROWS = 32 * RB, BLOCKS = 64 / G * RB, DEEP = G == 1 ? 8 : 4;
   __shared__ int tot[DC_WAVES];
   __shared__ int chunks_before[2];
   __shared__ float wm[DC_WAVES][32], wl[DC_WAVES][32];
-  __shared__ f32x4 acc[WPR > 1 ? DC_WAVES : 1][4][WAVE];
+  __shared__ f32x4 acc[WPR > 1 ? DC_WAVES : 1][G][WAVE];
   const int M = S * H, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int j = lane & 31, h = lane >> 5;
@@ -618,48 +618,55 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
   const int first = chunks_before[b - first_b] * tm.sets + mt / tm.span * nch;
   const int w0 = nch ? dn_owner(first, list) : 0, w1 = nch ? dn_owner(first + nch - 1, list) : -1;
   if (at >= blocks || w0 == w1) return;  // (one team's: its workgroup wrote them; the same for all of a block's waves)
-  const int w = block / (4 * RB), i = block / 4 % RB, d = block & 3;
+  const int block32 = block * G / 4, w = block32 / (4 * RB), i = block32 / 4 % RB, d = block32 & 3;
+  const int g0 = G == 1 ? block & 3 : 0;
   const int r = 32 * i + j, row = mt * ROWS + r;  // this lane's row of the tile, and of the sequence
   float m = -INFINITY, l = 0.0f;
-  f32x4 a[4] = {};
-  if (nch > 0) {
-    const float* const from = ws_o + dn_partial(w, i, d, 0, RB) + 4 * lane;
+  f32x4 a[G] = {};
+  if (nch > 0 && row < M) {
+    const float* const from = ws_o + dn_partial(w, i, d, g0, RB) + 4 * lane;
     // team w0's stretch is not its first where it started before the tile, the others' is
     const int slot0 = 2 * w0 + (dn_start(w0, list) < first);
-    for (int t = w0 + wave % WPR; t <= w1; t += 4 * WPR) {
-      float2 ml[4];
-      f32x4 v[4][4];
+    for (int t = w0 + wave % WPR; t <= w1; t += DEEP * WPR) {
+      const int n = (w1 - t) / WPR + 1;  // this round's, up to DEEP
+      float2 ml[DEEP];
+      f32x4 v[DEEP][G];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int u = min(t + WPR * x, w1);
-        const size_t part = ((size_t)(u == w0 ? slot0 : 2 * u) * tm.span + mt % tm.span) * ROWS;
-        ml[x] = reinterpret_cast<const float2*>(ws_ml)[part + r];
+      for (int x = 0; x < DEEP; ++x) {
+        ml[x] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) v[x][g] = *reinterpret_cast<const f32x4*>(from + part * DN_DV + 4 * WAVE * g);
+        for (int g = 0; g < G; ++g) v[x][g] = f32x4{};
+        if (x < n) {
+          const int u = t + WPR * x;
+          const size_t part = ((size_t)(u == w0 ? slot0 : 2 * u) * tm.span + mt % tm.span) * ROWS;
+          ml[x] = reinterpret_cast<const float2*>(ws_ml)[part + r];
+#pragma unroll
+          for (int g = 0; g < G; ++g) v[x][g] = *reinterpret_cast<const f32x4*>(from + part * DN_DV + 4 * WAVE * g);
+        }
       }
       float mx = m;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) mx = max_nonan(mx, ml[x].x);  // (past w1: the last one again, of weight 0 below)
+      for (int x = 0; x < DEEP; ++x) mx = max_nonan(mx, ml[x].x);
       const float f = __builtin_amdgcn_exp2f(m - mx);
       m = mx;
       l *= f;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
+      for (int g = 0; g < G; ++g)
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[g][e] *= f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const float c = t + WPR * x <= w1 ? __builtin_amdgcn_exp2f(ml[x].x - m) : 0.0f;
+      for (int x = 0; x < DEEP; ++x) {
+        const float c = __builtin_amdgcn_exp2f(ml[x].x - m);
         l = fmaf(c, ml[x].y, l);
 #pragma unroll
-        for (int g = 0; g < 4; ++g)
+        for (int g = 0; g < G; ++g)
 #pragma unroll
           for (int e = 0; e < 4; ++e) a[g][e] = fmaf(c, v[x][g][e], a[g][e]);
       }
     }
   }
   const size_t out_row = (size_t)b * M + row;
-  if (WPR == 1) {
+  if constexpr (WPR == 1) {
     const float inv = l > 0.0f ? 1.0f / l : 0.0f;
     uint2 pk[4];
 #pragma unroll
@@ -691,9 +698,9 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     wl[wave][j] = l;
   }
 #pragma unroll
-  for (int g = 0; g < 4; ++g) acc[WPR > 1 ? wave : 0][g][lane] = a[g];
+  for (int g = 0; g < G; ++g) acc[WPR > 1 ? wave : 0][g][lane] = a[g];
   __syncthreads();
-  if (wave >= 4 || row >= M) return;  // wave g joins the pieces g
+  if (wave >= G || row >= M) return;  // wave g joins group g
   float mm = wm[0][j], ll = 0.0f;
   f32x4 o = {};
 #pragma unroll
@@ -706,13 +713,13 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(f, v[e], o[e]);
   }
-  const size_t to = out_row * DN_DV + 128 * w + 32 * d + 8 * wave + 4 * h;
+  const size_t to = out_row * DN_DV + 128 * w + 32 * d + 8 * (g0 + wave) + 4 * h;
   const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
   if (out) *reinterpret_cast<uint2*>(out + to) = make_uint2(bf16_pack(o[0], o[1]), bf16_pack(o[2], o[3]));
   if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + to) = o;
-  if (lse_out && block == 4 * i && wave == 0 && h == 0) lse_out[out_row] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
+  if (lse_out && w == 0 && d == 0 && g0 + wave == 0 && h == 0) lse_out[out_row] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
 }
 
 // Workgroups: one a CU, a multiple of the 8 XCDs.
@@ -764,12 +771,22 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
   if (e != hipSuccess) return e;
   // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a block where its first four are
   // most of them
-  const bool many = tm.teams >= 7L * B * tm.sets;
-  const long blocks = (long)B * tm.tiles * (tm.rows / 2), groups = many ? blocks : (blocks + DC_WAVES - 1) / DC_WAVES;
-  const auto combine = tm.rows == 32 ? many ? dense_combine_kernel<1, DC_WAVES> : dense_combine_kernel<1, 1>
-                                     : many ? dense_combine_kernel<2, DC_WAVES> : dense_combine_kernel<2, 1>;
-  return launch("dense_combine_kernel", combine, dim3((unsigned)groups), dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out,
-                out_f32, lse, B, S, H, max_pages, page_size, tm);
+  // Waves of 32 rows x 32 dims with a partial after another where there are 3 such blocks a CU; workgroups whose 8 waves share
+  // a block's partials where there are fewer, of a quarter of the dims where they would fill only a quarter of the CUs.
+  // Measured, us in turn with quarters, shared, one wave: 1 x 4k tokens, 16 heads (16 blocks) 4.0, 5.5, 21; 1 x 128k, 128
+  // heads (64) 8.0, 9.5, 45; 8 x 32k, 64 heads (256) 9.6, 8.1, 14.6; 16 x 32k (512) 14.7, 8.7, 10.0; 30 x 4k (960) 27, 12.2,
+  // 9.3; 4 x 4 new tokens after 1k, 128 heads (1,024) 22, 10.4, 7.8.
+  const long blocks = (long)B * tm.tiles * (tm.rows / 2);
+  const bool one = tm.rows == 32;
+  auto join = [&](auto kernel, long groups) {
+    return launch("dense_combine_kernel", kernel, dim3((unsigned)groups), dim3(DC_THREADS), s, ws_o, ws_ml, ctx_len, out,
+                  out_f32, lse, B, S, H, max_pages, page_size, tm);
+  };
+  if (blocks >= 3L * num_cu)
+    return join(one ? dense_combine_kernel<1, 1, 4> : dense_combine_kernel<2, 1, 4>, (blocks + DC_WAVES - 1) / DC_WAVES);
+  if (4 * blocks > num_cu)
+    return join(one ? dense_combine_kernel<1, DC_WAVES, 4> : dense_combine_kernel<2, DC_WAVES, 4>, blocks);
+  return join(one ? dense_combine_kernel<1, DC_WAVES, 1> : dense_combine_kernel<2, DC_WAVES, 1>, 4 * blocks);
 }
 
 // Whether the list of units fits 32 bits, whatever the lengths, and the rows a launch.
