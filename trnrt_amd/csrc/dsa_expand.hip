@@ -246,6 +246,7 @@ struct XaShared {
   alignas(1024) uint8_t k[XA_STAGES][XA_K * 256];
   alignas(1024) uint8_t v[XA_STAGES][XA_K * 256];
   alignas(1024) uint8_t r[DQ > EX_D ? XA_STAGES : 1][DQ > EX_D ? XA_K * 128 : 16];
+  alignas(16) uint8_t q[DQ > EX_D ? 16384 : 16];  // (the queries' last 64 columns lie over r[1], r[2] and this)
   int tot[XA_THREADS / WAVE];
   int found[2];
 };
@@ -328,14 +329,28 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                    r_lds + XA_K * 128 * to + 1024 * x);
   };
   if (brings && nt > 0) issue(0, 0);
-  if (brings && nt > 1) issue(1, 1);
+  // the queries through LDS, over the stages that tiles 1 and 2 take: columns 64 p .. + 63 of the wave's 32 rows are 4 KiB
+  // of k, v or r, laid out as rope rows. (Read straight into the operands' layout, 32 bytes of 32 rows at a time, they took
+  // 5,000 cycles more.)
   bf16x8 qf[STEPS];  // query qi: step s holds dims 16 s + 8 h .. + 7
   {
-    const uint16_t* qr = q + ((size_t)(qb + qi) * H + head) * DQ + 8 * h;
+    uint8_t* const at[3] = {sh.k[1], sh.v[1], sh.r[DQ > EX_D ? 1 : 0]};
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * s));
-    arrive(qf);
+    for (int p = 0; p < DQ / 64; ++p)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = 8 * x + (lane >> 3);
+        load_lds16(q + ((size_t)(qb + min(w0 + r, nq - 1)) * H + head) * DQ + 64 * p + 8 * ((lane & 7) ^ ((r >> 1) & 7)),
+                   lds_address(at[p] + 4096 * wave) + 1024 * x);
+      }
+    wait_loads<0>();
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s)
+      qf[s] = as_bf16x8(*reinterpret_cast<const uint4*>(at[s >> 2] + 4096 * wave + 128 * j +
+                                                        16 * ((2 * (s & 3) + h) ^ ((j >> 1) & 7))));
   }
+  lds_barrier();  // the queries are read
+  if (brings && nt > 1) issue(1, 1);
   int koff[8], roff[4], voff[4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 15));
