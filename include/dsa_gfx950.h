@@ -462,13 +462,17 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
  *   v[t, h, :], lse = log sum_t exp(s[t]); a query that sees no key: out 0, lse NEG_INF (-1e30).
  *   q bf16 [Tq, H, 192] with rope bf16 [Tk, 64], or [Tq, H, 128] with rope null; k, v bf16 [Tk, H, 128]; out_bf16 and / or
  *   out_f32 [Tq, H, 128], lse fp32 [Tq, H] or null. Rows of q outside every sequence have no output written.
+ *   workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes on the same device, for the partials of few queries over
+ *   many keys, which several workgroups share (0, and null, where none do; no zero fill needed).
  */
+size_t dsa_expanded_workspace_bytes(int B, int Tq, int Tk, int H);
 int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table, const int32_t* cu_len,
                       const void* w_bf16, void* k_bf16, void* v_bf16, void* rope_bf16, int B, int total, int H,
                       int Dqk, int max_pages, int page_size, int num_pages, void* stream);
 int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
-                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse, int B,
-                     int Tq, int Tk, int H, int causal, float scale, void* stream);
+                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse,
+                     void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal, float scale,
+                     void* stream);
 
 /*
  * Pages of the paged caches (no counterpart among the reference's kernels: its page pool and prefix caches are host

@@ -25,13 +25,18 @@ def test_expand_refusals():
 
 
 def test_attend_refusals():
-    def call(q=P, k=P, v=P, out=P, B=2, Tq=10, Tk=10, H=16):
-        return _lib.lib().dsa_expanded_mla(q, k, None, v, P, P, out, None, P, B, Tq, Tk, H, 1, 0.1, None)
+    def call(q=P, k=P, v=P, out=P, ws=None, size=0, B=2, Tq=10, Tk=10, H=16):
+        return _lib.lib().dsa_expanded_mla(q, k, None, v, P, P, out, None, P, ws, size, B, Tq, Tk, H, 1, 0.1, None)
 
     for kw in (dict(B=-1), dict(Tq=-1), dict(Tk=-1), dict(H=0), dict(q=None), dict(k=None), dict(v=None), dict(out=None)):
         assert call(**kw) == _lib.DSA_EINVAL, kw
     assert call(Tq=1 << 30, H=1 << 10) == _lib.DSA_EUNSUPPORTED
     assert call(B=0) == _lib.DSA_OK and call(Tq=0, q=None) == _lib.DSA_OK
+    need = _lib.lib().dsa_expanded_workspace_bytes
+    assert need(2, 10, 10, 16) == 0 and need(0, 10, 10, 16) == 0 and need(2, 10, -1, 16) == 0
+    size = need(1, 10, 100000, 16)  # one query tile a head, the keys in splits
+    assert size >= 2 * 16 * 256 * 130 * 4
+    assert call(B=1, Tk=100000) == _lib.DSA_EWORKSPACE and call(B=1, Tk=100000, ws=P, size=size - 1) == _lib.DSA_EWORKSPACE
 
 
 def test_host_tensors_raise():

@@ -124,6 +124,44 @@ def test_attend(lq, lk, H, rope, causal):
     check_attend(lq, lk, H, rope, causal, seed=H)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lq,lk,H,rope", [
+    ([100], [5000], 16, True), ([1], [1500], 1, False), ([300, 1, 0], [9001, 4000, 70], 3, True),
+    ([256, 257], [3000, 2900], 8, False), ([40, 3], [20000, 2], 16, True), ([600], [700], 5, True), ([2, 2], [0, 9000], 24, True)])
+def test_attend_splits(lq, lk, H, rope, causal):
+    """Few queries over many keys: the keys of a query tile shared by several workgroups, some of them without any."""
+    say("attend splits", lq, lk, H, rope, causal)
+    check_attend(lq, lk, H, rope, causal)
+
+
+def test_attend_graph_has_its_own_workspace():
+    """Graphs captured without a workspace keep their results while eager calls and another graph use the stream's."""
+    say("attend, two graphs and eager calls")
+    g = torch.Generator().manual_seed(3)
+    ins = []
+    for nq, nk, H in ((70, 4000, 4), (130, 9000, 8)):
+        t = [torch.randn(n, H, d, generator=g).bfloat16().cuda() for n, d in ((nq, 128), (nk, 128), (nk, 128))]
+        ins.append((t[0], t[1], None, t[2], cu_of([nq]).cuda(), cu_of([nk]).cuda(), 0.1))
+    want = [tuple(x.clone() for x in dsa_expand.attend(*a)) for a in ins]
+    graphs = []
+    for a in ins:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = dsa_expand.attend(*a)
+        graphs.append((graph, got))
+    for _ in range(3):
+        for graph, got in graphs:
+            for x in got:
+                x.zero_()
+        for i in (0, 1, 0):
+            graphs[i][0].replay()
+        for i in (1, 0):
+            assert all(torch.equal(x, y) for x, y in zip(dsa_expand.attend(*ins[i]), want[i]))
+        torch.cuda.synchronize()
+        for (_, got), w in zip(graphs, want):
+            assert all(torch.equal(x, y) for x, y in zip(got, w))
+
+
 def test_attend_more_sequences_than_threads():
     say("expanded attend, 1,300 sequences")
     g = torch.Generator().manual_seed(1)

@@ -113,7 +113,8 @@ SIGNATURES: dict[str, tuple] = {
     "dsa_dense_mla": (c_int, [P, P, P, P, P, P, P, P, P, c_size_t, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                               c_float, P]),
     "dsa_expand_latent": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),
-    "dsa_expanded_mla": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_float, P]),
+    "dsa_expanded_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "dsa_expanded_mla": (c_int, [P, P, P, P, P, P, P, P, P, P, c_size_t, c_int, c_int, c_int, c_int, c_int, c_float, P]),
     "dsa_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
     "dsa_pages_copy": (c_int, [P, P, c_int, P, P, c_int, c_int, P]),
     "dsa_pages_fork": (c_int, [P, P, P, P, P, P, P, P, c_int, P, c_size_t, c_int, c_int, c_int, c_int, c_int, P]),

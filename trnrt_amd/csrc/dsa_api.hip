@@ -124,8 +124,9 @@ hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* 
                                 int D, int max_pages, int page_size, int num_pages, int num_cu, hipStream_t s);
 bool expanded_grid_ok(int B, int Tq, int H);
 hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
-                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, int B,
-                                  int Tq, int Tk, int H, int causal, float scale, hipStream_t s);
+                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, void* ws,
+                                  int B, int Tq, int Tk, int H, int causal, float scale, int num_cu, hipStream_t s);
+size_t expanded_workspace_bytes(int B, int Tq, int Tk, int H, int num_cu);
 size_t pages_fork_bytes(int n);
 size_t pages_compact_bytes(int num_pages);
 bool pages_units_ok(const long long* page_bytes, int n_caches, long n);
@@ -1319,18 +1320,26 @@ int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_
       max_pages, page_size, num_pages, num_cu(), static_cast<hipStream_t>(stream)));
 }
 
+size_t dsa_expanded_workspace_bytes(int B, int Tq, int Tk, int H) {
+  if (B < 1 || Tq < 1 || Tk < 0 || H < 1 || !dsa::expanded_grid_ok(B, Tq, H)) return 0;
+  return align256(dsa::expanded_workspace_bytes(B, Tq, Tk, H, num_cu()));
+}
+
 int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
-                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse, int B,
-                     int Tq, int Tk, int H, int causal, float scale, void* stream) {
+                     const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse,
+                     void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal, float scale,
+                     void* stream) {
   if (B < 0 || Tq < 0 || Tk < 0 || H < 1) return DSA_EINVAL;
   if (!dsa::expanded_grid_ok(B, Tq, H)) return DSA_EUNSUPPORTED;
   if (B == 0 || Tq == 0) return DSA_OK;
   // (no keys: k, v and rope_bf16 may be null, and every query sees nothing)
   if (!q_bf16 || !cu_q || !cu_k || (!out_bf16 && !out_f32) || (Tk > 0 && (!k_bf16 || !v_bf16))) return DSA_EINVAL;
+  const size_t need = dsa::expanded_workspace_bytes(B, Tq, Tk, H, num_cu());
+  if (need > 0 && (!workspace || workspace_bytes < need)) return DSA_EWORKSPACE;
   return status(dsa::launch_expanded_attend(
       static_cast<const uint16_t*>(q_bf16), static_cast<const uint16_t*>(k_bf16),
       static_cast<const uint16_t*>(rope_bf16), static_cast<const uint16_t*>(v_bf16), cu_q, cu_k,
-      static_cast<uint16_t*>(out_bf16), out_f32, lse, B, Tq, Tk, H, causal != 0, scale,
+      static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, Tq, Tk, H, causal != 0, scale, num_cu(),
       static_cast<hipStream_t>(stream)));
 }
 

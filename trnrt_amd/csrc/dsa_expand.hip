@@ -234,6 +234,7 @@ constexpr int XA_THREADS = 512;
 constexpr int XA_Q = 256;
 constexpr int XA_K = 64;
 constexpr int XA_STAGES = 3;
+constexpr int XA_SPLITS = 16;
 constexpr float XA_SLACK = 60.0f;  // lazy rescaling (base 2): p = 2^(s - m) <= 2^60 between moves of m
 constexpr float XA_LOG2E = 1.44269504088896341f;
 
@@ -251,53 +252,64 @@ struct XaShared {
   int found[2];
 };
 
+// A sequence's first query and their number (the offsets clamped to the queries there are).
+__device__ __forceinline__ int xa_first(int b, const int* __restrict__ cu_q, int Tq) {
+  return min(max(cu_q[b], 0), Tq);
+}
+__device__ __forceinline__ int xa_queries(int b, const int* __restrict__ cu_q, int Tq) {
+  return max(min(cu_q[b + 1], Tq) - xa_first(b, cu_q, Tq), 0);
+}
+// The sequence of query tile ti and the tile's place in it, into found (-1: past the last one); the whole workgroup.
+__device__ __forceinline__ void xa_find(int ti, const int* __restrict__ cu_q, int B, int Tq, int* tot, int* found) {
+  if (threadIdx.x == 0) found[0] = -1;
+  int before = 0;
+  for (int b0 = 0; b0 < B && before <= ti; b0 += XA_THREADS) {
+    const int b = b0 + threadIdx.x;
+    const int n = b < B ? (xa_queries(b, cu_q, Tq) + XA_Q - 1) / XA_Q : 0;
+    int total;
+    const int incl = before + group_incl_scan<XA_THREADS>(n, tot, total);
+    if (incl - n <= ti && ti < incl) {
+      found[0] = b;
+      found[1] = ti - (incl - n);
+    }
+    before += total;
+  }
+  __syncthreads();
+}
+
 template <int DQ>
 __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ kr,
     const uint16_t* __restrict__ v, const int* __restrict__ cu_q, const int* __restrict__ cu_k,
-    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, int B, int Tq, int Tk, int H,
-    int q_tiles, int causal, float scale) {
+    uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, float* __restrict__ ws, int B,
+    int Tq, int Tk, int H, int q_tiles, int splits, int causal, float scale) {
   constexpr int STEPS = DQ / 16;
   constexpr int LOADS = DQ > EX_D ? 10 : 8;  // a tile's asynchronous loads per wave
   __shared__ XaShared<DQ> sh;
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int j = lane & 31, h = lane >> 5;
   // heads of one XCD (workgroup x runs on XCD x % 8) next to each other, query tiles from the last to the first
+  const int grid = q_tiles * H, split = blockIdx.x / grid, at_tile = blockIdx.x - split * grid;
   int head, ti;
   if ((H & 7) == 0) {
-    const int per = H >> 3, y = blockIdx.x >> 3;
-    head = (blockIdx.x & 7) * per + y % per;
+    const int per = H >> 3, y = at_tile >> 3;
+    head = (at_tile & 7) * per + y % per;
     ti = q_tiles - 1 - y / per;
   } else {
-    head = blockIdx.x % H;
-    ti = q_tiles - 1 - blockIdx.x / H;
+    head = at_tile % H;
+    ti = q_tiles - 1 - at_tile / H;
   }
-  auto first_q = [&](int b) __attribute__((always_inline)) { return min(max(cu_q[b], 0), Tq); };
-  auto queries = [&](int b) __attribute__((always_inline)) { return max(min(cu_q[b + 1], Tq) - first_q(b), 0); };
-  {  // the sequence of tile ti
-    if (tid == 0) sh.found[0] = -1;
-    int before = 0;
-    for (int b0 = 0; b0 < B && before <= ti; b0 += XA_THREADS) {
-      const int b = b0 + tid;
-      const int n = b < B ? (queries(b) + XA_Q - 1) / XA_Q : 0;
-      int total;
-      const int incl = before + group_incl_scan<XA_THREADS>(n, sh.tot, total);
-      if (incl - n <= ti && ti < incl) {
-        sh.found[0] = b;
-        sh.found[1] = ti - (incl - n);
-      }
-      before += total;
-    }
-    __syncthreads();
-  }
+  xa_find(ti, cu_q, B, Tq, sh.tot, sh.found);
   const int b = __builtin_amdgcn_readfirstlane(sh.found[0]);
   if (b < 0) return;  // past the last tile
   const int qt = __builtin_amdgcn_readfirstlane(sh.found[1]) * XA_Q;
-  const int nq = queries(b), qb = first_q(b);
+  const int nq = xa_queries(b, cu_q, Tq), qb = xa_first(b, cu_q, Tq);
   const int kb = min(max(cu_k[b], 0), Tk), nk = max(min(cu_k[b + 1], Tk) - kb, 0);
   // keys that query i sees
   auto seen = [&](int i) __attribute__((always_inline)) { return causal ? min(nk - nq + i + 1, nk) : nk; };
-  const int nt = (max(seen(min(qt + XA_Q, nq) - 1), 0) + XA_K - 1) / XA_K;
+  // the tiles of keys, i0 .. nt - 1 of this split's
+  const int all = (max(seen(min(qt + XA_Q, nq) - 1), 0) + XA_K - 1) / XA_K;
+  const int i0 = (int)((long)all * split / splits), nt = (int)((long)all * (split + 1) / splits);
   const int w0 = qt + 32 * wave;  // the wave's first query
   const int nt_w = w0 < nq ? (max(seen(min(w0 + 32, nq) - 1), 0) + XA_K - 1) / XA_K : 0;
   const int seen0 = seen(w0);
@@ -328,7 +340,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                        8 * ((lane & 7) ^ ((8 * x + (lane >> 3)) >> 1)),
                    r_lds + XA_K * 128 * to + 1024 * x);
   };
-  if (brings && nt > 0) issue(0, 0);
+  if (brings && nt > i0) issue(i0, 0);
   // the queries through LDS, over the stages that tiles 1 and 2 take: columns 64 p .. + 63 of the wave's 32 rows are 4 KiB
   // of k, v or r, laid out as rope rows. (Read straight into the operands' layout, 32 bytes of 32 rows at a time, they took
   // 5,000 cycles more.)
@@ -350,7 +362,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                                                         16 * ((2 * (s & 3) + h) ^ ((j >> 1) & 7))));
   }
   lds_barrier();  // the queries are read
-  if (brings && nt > 1) issue(1, 1);
+  if (brings && nt > i0 + 1) issue(i0 + 1, 1);
   int koff[8], roff[4], voff[4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 15));
@@ -369,7 +381,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   if (wave < 4) __builtin_amdgcn_s_setprio(1);
   int stage = 0;
 #pragma unroll 1
-  for (int i = 0; i < nt; ++i) {
+  for (int i = i0; i < nt; ++i) {
     if (brings) {
       if (i + 1 < nt)
         wait_loads<LOADS>();
@@ -404,11 +416,11 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
       float cm = s2[0][0];
 #pragma unroll
       for (int r = 1; r < 32; ++r) cm = max_nonan(cm, s2[r >> 4][r & 15]);
-      if (i == 0 || __ballot(cm > XA_SLACK) != 0) {
+      if (i == i0 || __ballot(cm > XA_SLACK) != 0) {
         cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
-        // a query that sees none of tile 0 sees nothing: its maximum stays finite
-        const float up = i == 0 ? max_nonan(cm, -1e30f) : cm > XA_SLACK ? cm : 0.0f;
-        const float alpha = i == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+        // a query that sees none of the first tile sees nothing: its maximum stays finite
+        const float up = i == i0 ? max_nonan(cm, -1e30f) : cm > XA_SLACK ? cm : 0.0f;
+        const float alpha = i == i0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
         m_run += up;
         l_run *= alpha;
 #pragma unroll
@@ -451,6 +463,19 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   }
   __syncthreads();  // the stages are free
   const float l = l_run + __shfl_xor(l_run, 32, WAVE);
+  if (splits > 1) {  // a partial, as the registers hold it (expanded_combine_kernel reads it so)
+    const size_t part = ((size_t)ti * H + head) * splits + split;
+    float* const to = ws + part * XA_Q * EX_D + 32 * EX_D * wave + 4 * lane;
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(to + 4 * WAVE * (4 * d + g)) =
+            f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+    float2* const ml = reinterpret_cast<float2*>(ws + (size_t)grid * splits * XA_Q * EX_D) + part * XA_Q + 32 * wave;
+    if (h == 0) ml[j] = make_float2(l > 0.0f ? m_run : -1e30f, l);
+    return;
+  }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a query that sees nothing: 0)
   const int rows = min(32, nq - w0);
   if (rows <= 0) return;
@@ -504,19 +529,104 @@ hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* 
 }
 
 // Query tiles that a batch of Tq queries in B sequences may have.
-static int attend_tiles(int B, int Tq) { return Tq / XA_Q + B; }
+static int attend_tiles(int B, int Tq) { return (int)((Tq + (XA_Q - 1L) * B) / XA_Q); }
 
 bool expanded_grid_ok(int B, int Tq, int H) {
   return ((long)Tq / XA_Q + B) * H <= 0x7fffffL && (long)Tq + B <= 0x7fffffffL - XA_Q;
 }
 
+// Joins a query tile's splits: out = sum 2^(m - max) O / sum 2^(m - max) l. A workgroup has a tile of a head, a wave its 32
+// queries, the lanes as the partials hold them.
+__global__ __launch_bounds__(XA_THREADS) void expanded_combine_kernel(
+    const float* __restrict__ ws, const int* __restrict__ cu_q, uint16_t* __restrict__ out, float* __restrict__ out_f32,
+    float* __restrict__ lse_out, int B, int Tq, int H, int q_tiles, int splits) {
+  __shared__ int tot[XA_THREADS / WAVE];
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int j = lane & 31, h = lane >> 5;
+  const int unit = blockIdx.x >> 2, d = blockIdx.x & 3, ti = unit / H, head = unit - ti * H;  // (d: 32 of the 128 dims)
+  xa_find(ti, cu_q, B, Tq, tot, found);
+  const int b = __builtin_amdgcn_readfirstlane(found[0]);
+  if (b < 0) return;
+  const int i = __builtin_amdgcn_readfirstlane(found[1]) * XA_Q + 32 * wave + j;  // this lane's query
+  const size_t part0 = (size_t)unit * splits;
+  const float2* const ml = reinterpret_cast<const float2*>(ws + (size_t)q_tiles * H * splits * XA_Q * EX_D) +
+                           part0 * XA_Q + 32 * wave + j;
+  const float* const from = ws + part0 * XA_Q * EX_D + 32 * EX_D * wave + 4 * WAVE * 4 * d + 4 * lane;
+  float m = -INFINITY, l = 0.0f;
+  f32x4 a[4] = {};
+  for (int s0 = 0; s0 < splits; s0 += 4) {
+    float2 x[4];
+    f32x4 v[4][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      x[s] = make_float2(-INFINITY, 0.0f);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) v[s][g] = f32x4{};
+      if (s0 + s < splits) {
+        x[s] = ml[(size_t)(s0 + s) * XA_Q];
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          v[s][g] = *reinterpret_cast<const f32x4*>(from + (size_t)(s0 + s) * XA_Q * EX_D + 4 * WAVE * g);
+      }
+    }
+    float mx = m;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) mx = max_nonan(mx, x[s].x);
+    const float f = __builtin_amdgcn_exp2f(m - mx);
+    m = mx;
+    l *= f;
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) a[g][e] *= f;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const float c = __builtin_amdgcn_exp2f(x[s].x - m);
+      l = fmaf(c, x[s].y, l);
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[g][e] = fmaf(c, v[s][g][e], a[g][e]);
+    }
+  }
+  if (i >= xa_queries(b, cu_q, Tq)) return;
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a query that sees nothing: 0)
+  const size_t row = (size_t)(xa_first(b, cu_q, Tq) + i) * H + head;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const f32x4 v = {a[g][0] * inv, a[g][1] * inv, a[g][2] * inv, a[g][3] * inv};
+    const size_t to = row * EX_D + 32 * d + 8 * g + 4 * h;
+    if (out) *reinterpret_cast<uint2*>(out + to) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+    if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + to) = v;
+  }
+  if (lse_out && d == 0 && h == 0) lse_out[row] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+}
+
+// In how many splits a tile's keys are taken: as many as leave the CUs a workgroup each where every sequence has queries (the
+// fewest tiles that they can be), none of fewer than 4 tiles of keys on average.
+static int attend_splits(int B, int Tq, int Tk, int H, int num_cu) {
+  const long tiles = ((long)Tq + XA_Q - 1) / XA_Q, least = (tiles > B ? tiles : B) * H;
+  const long by_cu = num_cu / least, by_keys = (long)Tk / B / (4 * XA_K), n = by_cu < by_keys ? by_cu : by_keys;
+  return n < 1 ? 1 : n > XA_SPLITS ? XA_SPLITS : (int)n;
+}
+
+size_t expanded_workspace_bytes(int B, int Tq, int Tk, int H, int num_cu) {
+  const int splits = attend_splits(B, Tq, Tk, H, num_cu);
+  return splits > 1 ? (size_t)attend_tiles(B, Tq) * H * splits * XA_Q * (EX_D + 2) * sizeof(float) : 0;
+}
+
 hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
-                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, int B,
-                                  int Tq, int Tk, int H, int causal, float scale, hipStream_t s) {
-  const int q_tiles = attend_tiles(B, Tq);
+                                  const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, void* ws,
+                                  int B, int Tq, int Tk, int H, int causal, float scale, int num_cu, hipStream_t s) {
+  const int q_tiles = attend_tiles(B, Tq), splits = attend_splits(B, Tq, Tk, H, num_cu);
   const auto kernel = kr ? expanded_attend_kernel<EX_D + EX_R> : expanded_attend_kernel<EX_D>;
-  return launch("expanded_attend_kernel", kernel, dim3((unsigned)q_tiles * H), dim3(XA_THREADS), s, q, k, kr, v, cu_q,
-                cu_k, out, out_f32, lse, B, Tq, Tk, H, q_tiles, causal, scale);
+  const hipError_t e = launch("expanded_attend_kernel", kernel, dim3((unsigned)q_tiles * H * splits), dim3(XA_THREADS), s,
+                              q, k, kr, v, cu_q, cu_k, out, out_f32, lse, static_cast<float*>(ws), B, Tq, Tk, H, q_tiles,
+                              splits, causal, scale);
+  if (e != hipSuccess || splits == 1) return e;
+  return launch("expanded_combine_kernel", expanded_combine_kernel, dim3((unsigned)q_tiles * H * 4), dim3(XA_THREADS), s,
+                static_cast<const float*>(ws), cu_q, out, out_f32, lse, B, Tq, H, q_tiles, splits);
 }
 
 }  // namespace dsa

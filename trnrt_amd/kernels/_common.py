@@ -107,6 +107,15 @@ def cached_workspace(device: torch.device, nbytes: int, use: str) -> torch.Tenso
     return ws
 
 
+def scratch(device: torch.device, nbytes: int, use: str) -> torch.Tensor:
+    """A uint8 device buffer of at least nbytes that a call writes before it reads: the one kept for `use` on the current
+    stream, and in a graph capture one of the graph's own memory (a graph that kept the stream's would replay into it after a
+    later call had let it go for a larger one, or beside another graph's replay)."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+    return cached_workspace(device, nbytes, use)
+
+
 def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:
     """A new uint8 device buffer of nbytes (a multiple of 256) zero-filled by the library's dsa_workspace_clear on the
     current stream, which also records it as zero, so its first call does not fill it again."""

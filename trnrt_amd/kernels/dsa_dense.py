@@ -29,7 +29,7 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     512] bf16; q [B, H, D] is one new token a sequence, its outputs [B, H, 512] and [B, H]. kv_cache [slots, D] e4m3fn (or
     its bits) with kv_scale [slots] fp32, or None for the unscaled cache; table [B, max_pages] int32, ctx_len [B] int32.
     Any number of heads, any page size. workspace: dsa_dense_workspace_bytes(S, H) bytes, or None for one kept per
-    stream."""
+    stream (a captured graph has its own)."""
     dev = C.on_gpu(q, kv_cache, kv_scale, table, ctx_len, out, workspace)
     if q.dim() not in (3, 4) or q.shape[-1] not in DQK_WIDTHS or q.shape[-2] < 1 or (q.dim() == 4 and q.shape[1] < 1):
         raise ValueError(f"dsa_dense: q {tuple(q.shape)}, expected [B, H, 576 or 512] or [B, S, H, 576 or 512]")
@@ -54,9 +54,8 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     ls = q.new_empty(q.shape[:-1], dtype=torch.float32) if lse else None
     lib = _lib.lib()
     ws = workspace
-    if ws is None:
-        # the partials of the row tiles that workgroups share (written before they are read), kept per stream
-        ws = C.cached_workspace(dev, int(lib.dsa_dense_workspace_bytes(S, H)), "dense")
+    if ws is None:  # the partials of the row tiles that workgroups share
+        ws = C.scratch(dev, int(lib.dsa_dense_workspace_bytes(S, H)), "dense")
     bf = out.dtype == torch.bfloat16
     st = C.call(dev, lib.dsa_dense_mla, C.ptr(q), C.ptr(kv), C.ptr(kv_scale), C.ptr(tb), C.ptr(lens),
                 C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), C.ptr(ws),

@@ -74,13 +74,15 @@ def expand(kv_cache: torch.Tensor, kv_scale: torch.Tensor | None, table: torch.T
 
 def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: torch.Tensor, cu_q: torch.Tensor,
            cu_k: torch.Tensor, scale: float, *, causal: bool = True, lse: bool = True, out_dtype=torch.bfloat16,
-           out: torch.Tensor | None = None):
+           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """o [Tq, H, 128] in out_dtype (bf16 or fp32) and lse [Tq, H] fp32 (o alone without lse) of ragged sequences: q
     [Tq, H, 192] bf16 with k_rope [Tk, 64] bf16 shared by the heads, or [Tq, H, 128] without (k_rope None); k, v
     [Tk, H, 128] bf16; cu_q, cu_k [B + 1] int32 on the device: sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1,
     its keys rows cu_k[b] .. . causal: query i of nq sees the first nk - nq + i + 1 of the nk keys (the last sees all);
-    otherwise every key. A query that sees no key has o = 0 and lse NEG_INF; rows of q in no sequence are not written."""
-    dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out)
+    otherwise every key. A query that sees no key has o = 0 and lse NEG_INF; rows of q in no sequence are not written.
+    workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream (a captured graph
+    has its own)."""
+    dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
     dq = DH if k_rope is None else DH + ROPE
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[2] != dq:
         raise ValueError(f"dsa_expand: q {tuple(q.shape)}, expected [Tq, H, {dq}]")
@@ -100,8 +102,13 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     C.need(out, "out", (torch.bfloat16, torch.float32), (Tq, H, DH))
     ls = q.new_empty((Tq, H), dtype=torch.float32) if lse else None
     bf = out.dtype == torch.bfloat16
-    st = C.call(dev, _lib.lib().dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),
-                C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), cu_q.numel() - 1, Tq, Tk, H,
+    lib, B, ws = _lib.lib(), cu_q.numel() - 1, workspace
+    if ws is None:
+        need = int(lib.dsa_expanded_workspace_bytes(B, Tq, Tk, H))
+        ws = C.scratch(dev, need, "expanded") if need else None
+    st = C.call(dev, lib.dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),
+                C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), C.ptr(ws),
+                0 if ws is None else ws.numel() * ws.element_size(), B, Tq, Tk, H,
                 int(bool(causal)), float(scale))
     _lib.check(st, "dsa_expand.attend")
     return (out, ls) if lse else out

@@ -69,7 +69,8 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     [n, max_pages] int32, pages [n] int32). The parent's full pages are shared (ref, in place, rises by one), a partial
     last page is copied into the lowest free page of every cache; pages[i] is that page, 0 where there is no partial page,
     -1 where the pool had none left or parents[i] is no row (the child's table row is then 0 and counts nothing).
-    workspace: dsa_pages_workspace_bytes(num_pages, n) bytes, or None for one kept per stream."""
+    workspace: dsa_pages_workspace_bytes(num_pages, n) bytes, or None for one kept per stream
+    (a captured graph has its own)."""
     caches = list(caches)
     dev = C.on_gpu(ref, table, ctx_len, parents, workspace, *caches)
     _ref(ref, "dsa_pages.fork")
@@ -86,7 +87,7 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     lib = _lib.lib()
     ws = workspace
     if ws is None:
-        ws = C.cached_workspace(dev, int(lib.dsa_pages_workspace_bytes(num_pages, n)), "pages")
+        ws = C.scratch(dev, int(lib.dsa_pages_workspace_bytes(num_pages, n)), "pages")
     st = C.call(dev, lib.dsa_pages_fork, C.ptr(ref), C.ptr(tb), C.ptr(lens), C.ptr(par), C.ptr(child), C.ptr(pages),
                 ptrs, size, n_caches, C.ptr(ws), ws.numel() * ws.element_size(), B, n, max_pages, int(page_size),
                 num_pages)
@@ -114,7 +115,8 @@ def compact(ref: torch.Tensor, table: torch.Tensor, caches, page_size: int, *,
     counts in the new places and each page's new place [num_pages] (0: a free page), all int32. Pages already up to L
     stay; the k-th one past L goes to the k-th free page. ref and table are not changed, the caches are, in place (pages
     past L keep their bytes). Table entries of free pages become 0. workspace: dsa_pages_workspace_bytes(num_pages, 0)
-    bytes, or None for one kept per stream."""
+    bytes, or None for one kept per stream
+    (a captured graph has its own)."""
     caches = list(caches)
     dev = C.on_gpu(ref, table, workspace, *caches)
     _ref(ref, "dsa_pages.compact")
@@ -128,7 +130,7 @@ def compact(ref: torch.Tensor, table: torch.Tensor, caches, page_size: int, *,
     lib = _lib.lib()
     ws = workspace
     if ws is None:
-        ws = C.cached_workspace(dev, int(lib.dsa_pages_workspace_bytes(num_pages, 0)), "pages")
+        ws = C.scratch(dev, int(lib.dsa_pages_workspace_bytes(num_pages, 0)), "pages")
     st = C.call(dev, lib.dsa_pages_compact, C.ptr(ref), C.ptr(tb), C.ptr(new_ref), C.ptr(new_table), C.ptr(remap), ptrs,
                 size, n_caches, C.ptr(ws), ws.numel() * ws.element_size(), B, max_pages, num_pages)
     _lib.check(st, "dsa_pages.compact")
