@@ -1,5 +1,5 @@
-// Asynchronous loads straight into LDS whose waits are the kernel's own. (The builtin's are counted by the compiler, which
-// then waits for every one of them before any LDS read that follows, whichever tile it is of.)
+// Asynchronous loads straight into LDS whose waits are the kernel's own. (The builtin's are counted by the compiler,
+// which then waits for every one of them before any LDS read that follows, whichever tile it is of.)
 #pragma once
 
 #include "dsa_common.h"
@@ -12,14 +12,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
       (int)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
 }
 
-// (The compiler sets m0 anew before any use of its own, so these need not save it.)
-// 16 (4) bytes from each lane's address into LDS at lds + 16 (4) x lane. Nothing waits for it: s_waitcnt vmcnt before the
-// barrier that hands the data on (the loads of a wave end in order, and count with its other global accesses).
+// 16 bytes from each lane's address into LDS at lds + 16 x lane. Nothing waits for it: s_waitcnt vmcnt before the barrier
+// that hands the data on (the loads of a wave end in order, and count with its other global accesses). (The compiler
+// sets m0 anew before any use of its own, so this need not save it.)
 __device__ __forceinline__ void load_lds16(const void* p, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
-}
-__device__ __forceinline__ void load_lds4(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(lds) : "memory");
 }
 
 // At most N of the wave's global accesses are still out (loads end in order).
@@ -33,8 +30,8 @@ __device__ __forceinline__ void lds_barrier() {
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The lane, as a value that the compiler knows nothing about: what is computed from it stays where it is used instead of
-// being carried in registers around a loop.
+// The lane, as a value that the compiler knows nothing about: what is computed from it stays where it is used instead
+// of being carried in registers around a loop.
 __device__ __forceinline__ int fresh_lane() {
   int x = threadIdx.x & (WAVE - 1);
   asm volatile("" : "+v"(x));

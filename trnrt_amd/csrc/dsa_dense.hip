@@ -5,23 +5,30 @@
 //
 // for the M = S x H rows r (query, head) of a sequence over its tokens t: e4m3 rows c_t with a scale sigma_t.
 //
-// What bounds it: a token is 580 bytes for 2 x M x 1,088 FLOP, so up to about 64 rows the cache's stream through HBM is the
-// bound, above it the matrix units. One workgroup a CU has a tile of 32 or 64 rows of one sequence and a range of its
-// chunks of 64 tokens; its 8 waves have two kinds of work, one of each on every SIMD, a chunk apart, with one barrier a
-// chunk (products of one kind run under the other's conversions and exponentials):
-//   - scoring waves 0-3, interval c: chunk c's scores S^T = K . Q^T, 32 tokens x 32 rows a wave, the queries in registers,
-//     then P = 2^(s - m) x the tokens' scales in bf16 into LDS;
-//   - value waves 4-7, interval c: chunk c - 1's O^T += V^T . P, 128 dims of all rows a wave, in registers, and the loads
-//     of a later chunk: asynchronous 16-byte loads straight into LDS, which wait for nothing until their chunk's turn.
+// What bounds it: a token is 580 bytes for 2 x M x 1,088 FLOP, so up to about 64 rows the cache's stream is the bound,
+// above it the matrix units and the conversions beside them. One workgroup a CU has a tile of 32 or 64 rows of one
+// sequence and a range of its chunks of 64 tokens; its 8 waves have two kinds of work, one of each on every SIMD, a
+// chunk apart, with one barrier a chunk (products of one kind run under the other's conversions and exponentials):
+//   - scoring waves 0-3, interval c: chunk c's scores S^T = K . Q^T, 32 tokens x 32 rows a wave, the queries in
+//     registers, then P = 2^(s - m) x the tokens' scales in bf16 into LDS;
+//   - value waves 4-7, interval c: chunk c - 1's O^T += V^T . P, 128 dims of all rows a wave, in registers; and the
+//     rows of chunk c + 1 from their registers into LDS and chunk c + 2's loads into the same registers, piece by piece
+//     between the products. (Loads straight into LDS cost their wave 150 to 200 cycles each beside the other waves' LDS
+//     reads.)
 // Both products are v_mfma_f32_32x32x16_bf16 with the e4m3 operand converted on the way (exact). The chunks of all
-// sequences and row tiles form one list that the workgroups share evenly, whatever the lengths: each takes a stretch of it
-// and writes a row tile's outputs where it holds all its chunks, else a partial (the rows x 512 in fp32, their maxima and
-// sums) that dense_combine_kernel joins. Neighbouring stretches lie on one XCD, so that the row tiles of a sequence read its
-// cache through the same L2.
-// The online softmax rescales lazily without waiting for the chunk's maximum: P is taken against the running maximum as it
-// stands; a wave that meets a score past its slack raises a flag, and before the chunk's values are multiplied every wave
-// sees the flags and, when one is up, the maxima are exchanged, P is taken again and O rescaled (a stretch's chunk 0 always
-// does, with O still zero).
+// sequences and row tiles form one list that the workgroups share evenly, whatever the lengths: each takes a stretch of
+// it and writes a row tile's outputs where it holds all its chunks, else a partial (the rows x 512 in fp32, their
+// maxima and sums) that dense_combine_kernel joins. Neighbouring stretches lie on one XCD, so that the row tiles of a
+// sequence read its cache through the same L2.
+//
+// Measured (the attention alone, the joining beside it): 8 x 32k tokens, 64 heads 44 + 8 us, of which the loop is 27 at
+// 5.6 TB/s of cache rows, the rest the list's search, the first loads and the partials; 13 x 4 new tokens of 128 heads
+// (2k to 12k tokens, 512 wide) 108 + 11, 920 TFLOP/s over the call; 1 x 4k tokens, 16 heads 9.7 + 4.2, latency.
+//
+// The online softmax rescales lazily without waiting for the chunk's maximum: P is taken against the running maximum as
+// it stands; a wave that meets a score past its slack raises a flag, and before the chunk's values are multiplied every
+// wave sees the flags and, when one is up, the maxima are exchanged, P is taken again and O rescaled (a stretch's chunk
+// 0 always does, with O still zero).
 #include "dsa_async.h"
 #include "dsa_scan.h"
 
@@ -30,8 +37,9 @@ namespace dsa {
 constexpr int DN_DV = 512;
 constexpr int DN_CHUNK = 64;
 constexpr int DN_THREADS = 512;
-// Lazy rescaling (base 2): p = 2^(s - m) <= 2^60 between moves of m. (bf16 and fp32 keep their precision at that size, and
-// 2^31 such weights sum to less than fp32's end. With 2^11.5 m moved so often that 8 x 32k tokens took 50.0 us for 45.5.)
+// Lazy rescaling (base 2): p = 2^(s - m) <= 2^60 between moves of m. (bf16 and fp32 keep their precision at that size,
+// and 2^31 such weights sum to less than fp32's end. With 2^11.5 m moved so often that 8 x 32k tokens took 50.0 us for
+// 45.5.)
 constexpr float DN_SLACK = 60.0f;
 constexpr float DN_LOG2E = 1.44269504088896341f;
 constexpr float DN_LOG2E_LO = (float)(1.44269504088896341 - (double)DN_LOG2E);
@@ -42,9 +50,9 @@ constexpr int DN_STORE = 5;            // the value step that begins storing the
 
 typedef int dn_v2i __attribute__((ext_vector_type(2)));
 
-// A chunk's LDS layout: row r (token) at r x DN_KROW, its 16-byte piece p at p ^ dn_swizzle(r). With it the stores of 16 lanes
-// (4 rows x 4 pieces), the key operand's reads (16 lanes: a piece of 16 rows) and the value operand's, transposed (32 lanes:
-// two pieces of 8 rows), cover the 64 banks once.
+// A chunk's LDS layout: row r (token) at r x DN_KROW, its 16-byte piece p at p ^ dn_swizzle(r). With it the stores of
+// 16 lanes (4 rows x 4 pieces), the key operand's reads (16 lanes: a piece of 16 rows) and the value operand's,
+// transposed (32 lanes: two pieces of 8 rows), cover the 64 banks once.
 __device__ __forceinline__ int dn_swizzle(int r) { return (r >> 2 & 1) << 1 | (r >> 3 & 1); }
 constexpr int DN_KROW = 576;
 constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are multiplied, c + 1 being stored
@@ -53,7 +61,7 @@ constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are mult
 template <int RB>
 struct DnShared {
   alignas(1024) uint8_t tile[DN_BUFS][DN_CHUNK * DN_KROW];  // (the queries in the last two before)
-  alignas(16) uint16_t p[2][64 * DN_PROW];        // P[row][token] of two chunks (32 rows: their second terms after them)
+  alignas(16) uint16_t p[2][64 * DN_PROW];  // P[row][token] of two chunks (32 rows: their second terms after them)
   alignas(16) float ksc[DN_BUFS][DN_CHUNK];       // the chunks' token scales
   alignas(16) float kfac[DN_BUFS][DN_CHUNK];      // x softmax scale x log2 e
   float cmax[2][32 * RB];                         // [token half][row]: a chunk's maxima when one moves
@@ -65,7 +73,8 @@ struct DnShared {
   int found[4];
 };
 
-// t / page_size for 0 <= t < 2^31: t x mul >> shift (mul = ceil(2^shift / page_size), shift = 31 + ceil(log2 page_size)).
+// t / page_size for 0 <= t < 2^31: t x mul >> shift (mul = ceil(2^shift / page_size), shift = 31 + ceil(log2
+// page_size)).
 struct DnPage {
   uint32_t mul;
   int shift;
@@ -79,9 +88,9 @@ __device__ __forceinline__ int dn_len(int ctx_len, int max_pages, int page_size)
 }
 __device__ __forceinline__ int dn_chunks(int len) { return (len + DN_CHUNK - 1) / DN_CHUNK; }
 
-// How a sequence's row tiles go to workgroups: `span` neighbours on one XCD are a team, with the same stretch of chunks and
-// a tile each, so that they read the cache through one L2 at one time; more tiles than that are `sets` of span tiles, one
-// after another in the list. `teams` of them share the list.
+// How a sequence's row tiles go to workgroups: `span` neighbours on one XCD are a team, with the same stretch of chunks
+// and a tile each, so that they read the cache through one L2 at one time; more tiles than that are `sets` of span
+// tiles, one after another in the list. `teams` of them share the list.
 struct DnTeams {
   int rows;   // of a tile
   int tiles;
@@ -90,7 +99,8 @@ struct DnTeams {
   int teams;
 };
 
-// The list of units (sequence, set of row tiles, chunk of tokens), in equal shares (one unit more for the first `more`).
+// The list of units (sequence, set of row tiles, chunk of tokens), in equal shares (one unit more for the first
+// `more`).
 struct DnList {
   int teams;  // that have a share
   int share;
@@ -110,8 +120,8 @@ __device__ __forceinline__ int dn_owner(int u, const DnList& x) {
   return u < big ? u / (x.share + 1) : x.more + (u - big) / x.share;
 }
 
-// Where a partial's piece lies: dims 128 w + 32 d + 8 g + 4 h .. + 3 of row 32 i + j of a tile, at 4 (32 h + j) from there, as
-// the value waves' lanes hold it.
+// Where a partial's piece lies: dims 128 w + 32 d + 8 g + 4 h .. + 3 of row 32 i + j of a tile, at 4 (32 h + j) from
+// there, as the value waves' lanes hold it.
 __device__ __forceinline__ constexpr int dn_partial(int w, int i, int d, int g, int blocks) {
   return (((w * blocks + i) * 4 + d) * 4 + g) * 4 * WAVE;
 }
@@ -185,388 +195,389 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const int t0 = c0 * DN_CHUNK, r0 = (set * tm.span + member) * ROWS;  // its first token, and this workgroup's row
     const int part = (2 * team + (u > u0)) * tm.span + member;            // where its partials go
     if (r0 < M) {  // (else the last set has no tile for this member)
-
-    // A whole row tile's outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x & 7)),
-    // so that a row's pieces in order and a piece's rows in order both cover the banks once; a wave writes whole rows.
-    f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
-    auto write = [&](int half) __attribute__((always_inline)) {
-      const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
+      // A whole row tile's outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x
+      // & 7)), so that a row's pieces in order and a piece's rows in order both cover the banks once; a wave writes
+      // whole rows.
+      f32x4* const area = reinterpret_cast<f32x4*>(&sh.tile[0][0]);
+      auto write = [&](int half) __attribute__((always_inline)) {
+        const int lane = fresh_lane(), dim = 256 * half + 4 * lane;
 #pragma unroll 4
-      for (int i = 0; i < ROWS / 8; ++i) {
-        const int r = wave + 8 * i;
-        if (r0 + r >= M) break;
-        f32x4 v = area[64 * lane + (r ^ (lane & 7))];
-        const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
-        const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
+        for (int i = 0; i < ROWS / 8; ++i) {
+          const int r = wave + 8 * i;
+          if (r0 + r >= M) break;
+          f32x4 v = area[64 * lane + (r ^ (lane & 7))];
+          const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
+          const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= inv;
-        const size_t at = (size_t)b * M + r0 + r;
-        if (out)
-          *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
-        if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
-        if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
-      }
-    };
-    // The end of a stretch in every wave, after the barrier behind which the tiles are free and the sums in LDS; the value
-    // waves bring store(half).
-    auto finish = [&](auto store) __attribute__((always_inline)) {
-      if (whole) {
-        store(0);
-        lds_barrier();
-        write(0);
-        lds_barrier();
-        store(1);
-        lds_barrier();
-        write(1);
-      } else if (tid < ROWS && r0 + tid < M) {
-        float2* const ml = reinterpret_cast<float2*>(ws_ml) + (size_t)part * ROWS + tid;
-        *ml = make_float2(sh.mfin[tid], sh.lsum[0][tid] + sh.lsum[1][tid]);
-      }
-    };
-
-    if (wave < 4) {
-      // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
-      const int th = wave >> 1, hh = wave & 1;
-      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
-      // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece p at
-      // p ^ (r & 7), so that one piece of 8 rows covers the banks once
-      {
-        constexpr int QP = DQK / 8, PER = ROWS * QP / (4 * WAVE);
-        static_assert(ROWS * QP * 16 <= 2 * DN_CHUNK * DN_KROW, "the staged queries");
-        const uint32_t q_lds = lds_address(sh.tile[1]) + 1024 * PER * wave;
-        const int r_max = M - 1 - r0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const int x = WAVE * (PER * wave + i) + lane, r = x / QP, p = x - r * QP;
-          load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ (r & 7)), q_lds + 1024 * i);
+          for (int e = 0; e < 4; ++e) v[e] *= inv;
+          const size_t at = (size_t)b * M + r0 + r;
+          if (out)
+            *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
+          if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
+          if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
         }
-        wait_loads<0>();
-      }
-      lds_barrier();  // the queries and chunk 0 are in place
-      if (hh >= RB) {  // no rows for this wave
-        lds_barrier();
-        for (int c = 0; c <= nch; ++c) {
-          if (c > 0) {
-            const int4 fl = *reinterpret_cast<const int4*>(sh.flag[(c - 1) & 1]);
+      };
+      // The end of a stretch in every wave, after the barrier behind which the tiles are free and the sums in LDS; the
+      // value waves bring store(half).
+      auto finish = [&](auto store) __attribute__((always_inline)) {
+        if (whole) {
+          store(0);
+          lds_barrier();
+          write(0);
+          lds_barrier();
+          store(1);
+          lds_barrier();
+          write(1);
+        } else if (tid < ROWS && r0 + tid < M) {
+          float2* const ml = reinterpret_cast<float2*>(ws_ml) + (size_t)part * ROWS + tid;
+          *ml = make_float2(sh.mfin[tid], sh.lsum[0][tid] + sh.lsum[1][tid]);
+        }
+      };
+
+      if (wave < 4) {
+        // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
+        const int th = wave >> 1, hh = wave & 1;
+        const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
+        // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece
+        // p at p ^ (r & 7), so that one piece of 8 rows covers the banks once
+        {
+          constexpr int QP = DQK / 8, PER = ROWS * QP / (4 * WAVE);
+          static_assert(ROWS * QP * 16 <= 2 * DN_CHUNK * DN_KROW, "the staged queries");
+          const uint32_t q_lds = lds_address(sh.tile[1]) + 1024 * PER * wave;
+          const int r_max = M - 1 - r0;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            const int x = WAVE * (PER * wave + i) + lane, r = x / QP, p = x - r * QP;
+            load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ (r & 7)), q_lds + 1024 * i);
+          }
+          wait_loads<0>();
+        }
+        lds_barrier();  // the queries and chunk 0 are in place
+        if (hh >= RB) {  // no rows for this wave
+          lds_barrier();
+          for (int c = 0; c <= nch; ++c) {
+            if (c > 0) {
+              const int4 fl = *reinterpret_cast<const int4*>(sh.flag[(c - 1) & 1]);
+              if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+                lds_barrier();
+                lds_barrier();
+              }
+            }
+            lds_barrier();
+          }
+          finish([](int) {});
+        } else {
+          const int row = min(r0 + 32 * hh + j, M - 1);
+          const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
+          const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
+          bf16x8 qb[2 * STEPS];  // row 32 hh + j: step s holds dims 32 s + 16 h .. + 15
+          {
+            const uint8_t* const qr = sh.tile[1] + (32 * hh + j) * 2 * DQK;
+#pragma unroll
+            for (int s = 0; s < 2 * STEPS; ++s)
+              qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (j & 7))));
+          }
+          lds_barrier();  // the queries are read
+          float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
+                               // always up
+          float l_run = 0.0f;  // this lane's share of its running sum
+          float psum = 0.0f;   // and of the last chunk's, not yet in l_run
+          f32x16 sv = {};      // the last chunk's scores - m_run: row 32 hh + j, tokens 32 th + 8 (r / 4) + 4 h + r % 4
+          const int kr = 32 * th + j;
+          const int kf = dn_swizzle(kr);  // byte offsets of a row's pieces at even and odd steps of 32 dims
+          const int koff[2] = {kr * DN_KROW + 16 * (h ^ kf), kr * DN_KROW + 16 * ((2 | h) ^ kf)};
+          uint16_t* const pw = &sh.p[0][(32 * hh + j) * DN_PROW + 32 * th + 4 * h];
+          int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
+          auto four = [&](const float* a, int g) __attribute__((always_inline)) {
+            return *reinterpret_cast<const f32x4*>(a + 32 * th + 8 * g + 4 * h);
+          };
+          // four tokens (group g of the lane's 16) of P from their scores and scales
+          auto p_group = [&](int c, int g, const f32x4& ks) __attribute__((always_inline)) {
+            float pv[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[4 * g + e]);
+            psum += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+            // bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded. A
+            // tile of 32 rows, whose bound is the cache's stream, takes what the rounding left as a second term (2^-16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pv[e] *= ks[e];
+            uint32_t w[2] = {bf16_pack(pv[0], pv[1]), bf16_pack(pv[2], pv[3])};
+            uint16_t* const to = pw + (c & 1) * 64 * DN_PROW + 8 * g;
+            *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            if (RB == 1) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                w[e] = bf16_pack(pv[2 * e] - __uint_as_float(w[e] << 16),
+                                 pv[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+              *reinterpret_cast<uint2*>(to + 32 * DN_PROW) = make_uint2(w[0], w[1]);
+            }
+          };
+          // a chunk whose flags (fl) are up: its maxima over both token halves, the moved running maxima, P again
+          auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
             if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+              float cm = sv[0];
+#pragma unroll
+              for (int r = 1; r < 16; ++r) cm = max_nonan(cm, sv[r]);
+              cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
+              if (h == 0) sh.cmax[th][32 * hh + j] = cm;
               lds_barrier();
+              cm = max_nonan(cm, sh.cmax[th ^ 1][32 * hh + j]);
+              // a row that sees none of chunk 0 sees none of the stretch: its maximum stays finite
+              const float up = c == 0 ? max_nonan(cm, -1e30f) : cm > DN_SLACK ? cm : 0.0f;
+              // chunk 0 has nothing to rescale, and its factor would be infinite where every score is at or below -128
+              const float alpha = c == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+              m_run += up;
+              l_run *= alpha;
+              psum = 0.0f;
+#pragma unroll
+              for (int r = 0; r < 16; ++r) sv[r] -= up;
+#pragma unroll
+              for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
+              if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
               lds_barrier();
             }
+            l_run += psum;
+            psum = 0.0f;
+          };
+          auto flags = [&](int c) __attribute__((always_inline)) { return *reinterpret_cast<const int4*>(sh.flag[c & 1]); };
+          __builtin_amdgcn_s_setprio(1);  // these waves bound the interval: their products go before the value products
+          for (int c = 0; c < nch; ++c) {
+            const uint8_t* tile = sh.tile[buf];
+            auto k_read = [&](int s) __attribute__((always_inline)) {
+              return *reinterpret_cast<const u32x4*>(tile + koff[s & 1] + 64 * (s >> 1));
+            };
+            int4 fl = make_int4(0, 0, 0, 0);
+            if (c > 0) fl = flags(c - 1);
+            f32x16 sa = {};
+            u32x4 kk[DN_KAHEAD + 1];
+            bf16x8 ka[2], kb[2];
+            f32x4 ks[2], kx[2];
+#pragma unroll
+            for (int s = 0; s < DN_KAHEAD; ++s) kk[s] = k_read(s);
+            __builtin_amdgcn_sched_barrier(0);
+            settle(c - 1, fl);
+            ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
+            kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
+#pragma unroll
+            for (int s = 0; s < STEPS; ++s) {
+              if (s + DN_KAHEAD < STEPS) kk[(s + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(s + DN_KAHEAD);
+              sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[s & 1], qb[2 * s], sa, 0, 0, 0);
+              sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[s & 1], qb[2 * s + 1], sa, 0, 0, 0);
+              if (s + 1 < STEPS) {
+                const u32x4 k1 = kk[(s + 1) % (DN_KAHEAD + 1)];
+                ka[(s + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
+                kb[(s + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
+              }
+              if (s == STEPS - 2) {
+                ks[0] = four(sh.ksc[buf], 0);
+                kx[0] = four(sh.kfac[buf], 0);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              if (g < 3) kx[(g + 1) & 1] = four(sh.kfac[buf], g + 1);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sv[4 * g + e] = fmaf(sa[4 * g + e], kx[g & 1][e], -m_run);
+            }
+            if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
+              const int lim = seen - t0 - c * DN_CHUNK - 32 * th - 4 * h;
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sv[4 * g + e] = 8 * g + e < lim ? sv[4 * g + e] : -INFINITY;
+            }
+            float cm = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              if (g < 3) ks[(g + 1) & 1] = four(sh.ksc[buf], g + 1);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) cm = max_nonan(cm, sv[4 * g + e]);
+              p_group(c, g, ks[g & 1]);
+            }
+            const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
+            if (lane == 0) sh.flag[c & 1][wave] = any;
+            last = buf;
+            buf = buf == BUFS - 1 ? 0 : buf + 1;
+            lds_barrier();
           }
+          __builtin_amdgcn_s_setprio(0);
+          settle(nch - 1, flags(nch - 1));
+          const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
+          if (h == 0) sh.lsum[th][32 * hh + j] = lw;
+          if (th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
           lds_barrier();
+          finish([](int) {});
         }
-        finish([](int) {});
       } else {
-      const int row = min(r0 + 32 * hh + j, M - 1);
-      const int seen = len - S + row / H + 1;  // tokens that this lane's row sees
-      const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
-      bf16x8 qb[2 * STEPS];  // row 32 hh + j: step s holds dims 32 s + 16 h .. + 15
-      {
-        const uint8_t* const qr = sh.tile[1] + (32 * hh + j) * 2 * DQK;
-#pragma unroll
-        for (int s = 0; s < 2 * STEPS; ++s)
-          qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (j & 7))));
-      }
-      lds_barrier();  // the queries are read
-      float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
-                           // always up
-      float l_run = 0.0f;  // this lane's share of its running sum
-      float psum = 0.0f;   // and of the last chunk's, not yet in l_run
-      f32x16 sv = {};      // the last chunk's scores - m_run: row 32 hh + j, tokens 32 th + 8 (r / 4) + 4 h + r % 4
-      const int kr = 32 * th + j;
-      const int kf = dn_swizzle(kr);  // byte offsets of a row's pieces at even and odd steps of 32 dims
-      const int koff[2] = {kr * DN_KROW + 16 * (h ^ kf), kr * DN_KROW + 16 * ((2 | h) ^ kf)};
-      uint16_t* const pw = &sh.p[0][(32 * hh + j) * DN_PROW + 32 * th + 4 * h];
-      int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
-      auto four = [&](const float* a, int g) __attribute__((always_inline)) {
-        return *reinterpret_cast<const f32x4*>(a + 32 * th + 8 * g + 4 * h);
-      };
-      // four tokens (group g of the lane's 16) of P from their scores and scales
-      auto p_group = [&](int c, int g, const f32x4& ks) __attribute__((always_inline)) {
-        float pv[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[4 * g + e]);
-        psum += (pv[0] + pv[1]) + (pv[2] + pv[3]);
-        // bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded. A tile of
-        // 32 rows, whose bound is the cache's stream, takes what the rounding left as a second term (2^-16)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) pv[e] *= ks[e];
-        uint32_t w[2] = {bf16_pack(pv[0], pv[1]), bf16_pack(pv[2], pv[3])};
-        uint16_t* const to = pw + (c & 1) * 64 * DN_PROW + 8 * g;
-        *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-        if (RB == 1) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            w[e] = bf16_pack(pv[2 * e] - __uint_as_float(w[e] << 16), pv[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
-          *reinterpret_cast<uint2*>(to + 32 * DN_PROW) = make_uint2(w[0], w[1]);
-        }
-      };
-      // a chunk whose flags (fl) are up: its maxima over both token halves, the moved running maxima, P again
-      auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
-        if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
-          float cm = sv[0];
-#pragma unroll
-          for (int r = 1; r < 16; ++r) cm = max_nonan(cm, sv[r]);
-          cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
-          if (h == 0) sh.cmax[th][32 * hh + j] = cm;
-          lds_barrier();
-          cm = max_nonan(cm, sh.cmax[th ^ 1][32 * hh + j]);
-          // a row that sees none of chunk 0 sees none of the stretch: its maximum stays finite
-          const float up = c == 0 ? max_nonan(cm, -1e30f) : cm > DN_SLACK ? cm : 0.0f;
-          // chunk 0 has nothing to rescale, and its factor would be infinite where every score is at or below -128
-          const float alpha = c == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
-          m_run += up;
-          l_run *= alpha;
-          psum = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) sv[r] -= up;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) p_group(c, g, four(sh.ksc[last], g));
-          if (th == 0 && h == 0) sh.al[32 * hh + j] = alpha;
-          lds_barrier();
-        }
-        l_run += psum;
-        psum = 0.0f;
-      };
-      auto flags = [&](int c) __attribute__((always_inline)) { return *reinterpret_cast<const int4*>(sh.flag[c & 1]); };
-      __builtin_amdgcn_s_setprio(1);  // these waves bound the interval: their products go before the value products
-      for (int c = 0; c < nch; ++c) {
-        const uint8_t* tile = sh.tile[buf];
-        auto k_read = [&](int s) __attribute__((always_inline)) {
-          return *reinterpret_cast<const u32x4*>(tile + koff[s & 1] + 64 * (s >> 1));
+        // -- the loads and the values: thread 4 r + e of the value waves brings row r of a chunk, pieces e + 4 i; wave w
+        // takes dims 128 w .. + 127 of all rows --
+        const int w = wave - 4;
+        const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
+        const int* trow = table + (size_t)b * max_pages;
+        const int gr = 16 * w + (lane >> 2);  // this thread's row
+        // its token in chunk c, the stretch's last one past its end (a slot behind the sequence may never have been
+        // written, and its NaN x weight 0 is NaN)
+        const int t_last = min(t0 + nch * DN_CHUNK, len) - 1;
+        auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + gr, t_last); };
+        auto page_of = [&](int t) __attribute__((always_inline)) { return (int)((uint64_t)t * pg.mul >> pg.shift); };
+        auto slot_of = [&](int c, int page) __attribute__((always_inline)) {
+          const int t = token(c);
+          return safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
         };
-        int4 fl = make_int4(0, 0, 0, 0);
-        if (c > 0) fl = flags(c - 1);
-        f32x16 sa = {};
-        u32x4 kk[DN_KAHEAD + 1];
-        bf16x8 ka[2], kb[2];
-        f32x4 ks[2], kx[2];
-#pragma unroll
-        for (int s = 0; s < DN_KAHEAD; ++s) kk[s] = k_read(s);
-        __builtin_amdgcn_sched_barrier(0);
-        settle(c - 1, fl);
-        ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
-        kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          if (s + DN_KAHEAD < STEPS) kk[(s + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(s + DN_KAHEAD);
-          sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[s & 1], qb[2 * s], sa, 0, 0, 0);
-          sa = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kb[s & 1], qb[2 * s + 1], sa, 0, 0, 0);
-          if (s + 1 < STEPS) {
-            const u32x4 k1 = kk[(s + 1) % (DN_KAHEAD + 1)];
-            ka[(s + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
-            kb[(s + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
+        const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ dn_swizzle(gr));  // where its pieces go in a tile
+        u32x4 held[PIECES];  // the pieces in flight, of the chunk after the one being stored
+        float sc;          // and its token's scale
+        auto row_of = [&](int slot) __attribute__((always_inline)) { return kv + (size_t)slot * DQK + 16 * (lane & 3); };
+        auto store_scale = [&](int to) __attribute__((always_inline)) {
+          if ((lane & 3) == 0) {
+            sh.ksc[to][gr] = sc;
+            sh.kfac[to][gr] = fmaf(sc, sl2, sc * sl2_lo);
           }
-          if (s == STEPS - 2) {
-            ks[0] = four(sh.ksc[buf], 0);
-            kx[0] = four(sh.kfac[buf], 0);
+        };
+        f32x16 o[4][RB];  // [dim block][row block]: row 32 i + j, dims 128 w + 32 d + 8 (r / 4) + 4 h + r % 4
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+          for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
+        const int vr = 8 * h + ((lane & 15) >> 1), vf = dn_swizzle(vr), vb0 = (lane >> 4) & 1;  // (the value operand's reads)
+        const int vrow = vr * DN_KROW + 128 * w + 8 * (lane & 1);
+        const int voff[2] = {vrow + 16 * (vb0 ^ vf), vrow + 16 * ((2 | vb0) ^ vf)};
+        const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
+        // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed
+        auto v_read = [&](const uint8_t* kt, int i) __attribute__((always_inline)) {
+          return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW + 64 * ((i & 3) >> 1)));
+        };
+        auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
+          return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * 64 * DN_PROW + 32 * i * DN_PROW + 16 * t));
+        };
+        // Interval c: chunk c - 1's weights are final (and O on their maxima) once its flags are seen; then its value
+        // product, 16 steps of two products, the next steps' operands read and converted ahead, side(i) beside step i.
+        auto interval = [&](int c, const uint8_t* kt, auto side) __attribute__((always_inline)) {
+          const int pb = (c - 1) & 1;
+          const int4 fl = *reinterpret_cast<const int4*>(sh.flag[pb]);
+          dn_v2i vv[DN_VAHEAD + 1];
+          bf16x8 pa[2][2], vb[2];
+#pragma unroll
+          for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
+          if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+            lds_barrier();
+            lds_barrier();
+            if (c > 1) {  // O is zero before
+#pragma unroll
+              for (int i = 0; i < RB; ++i) {
+                const float a = sh.al[32 * i + j];
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+#pragma unroll
+                  for (int r = 0; r < 16; ++r) o[d][i][r] *= a;
+              }
+            }
           }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) pa[0][i] = p_read(pb, 0, i);
+          vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
           __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int t = i >> 2, d = i & 3;
+            if (i + DN_VAHEAD < 16) vv[(i + DN_VAHEAD) % (DN_VAHEAD + 1)] = v_read(kt, i + DN_VAHEAD);
+            if (d < 2 && t < 3) pa[(t + 1) & 1][d] = p_read(pb, t + 1, d);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              f32x16& sum = o[d][RB == 1 ? 0 : x];
+              sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i & 1], pa[t & 1][x], sum, 0, 0, 0);
+            }
+            if (i < 15) {
+              const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
+              vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
+            }
+            side(i);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        };
+        int page = trow[page_of(token(2))];  // of this thread's token two chunks on
+        const int page0 = trow[page_of(token(0))], page1 = trow[page_of(token(1))];
+        {  // chunks 0 and 1 together: the first into LDS, the second stays in flight
+          const int slot0 = slot_of(0, page0), slot1 = slot_of(1, page1);
+          const uint8_t *src0 = row_of(slot0), *src1 = row_of(slot1);
+          u32x4 first[PIECES];
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) first[i] = *reinterpret_cast<const u32x4*>(src0 + 64 * i);
+          const float sc0 = kvs ? kvs[slot0] : 1.0f;
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) held[i] = *reinterpret_cast<const u32x4*>(src1 + 64 * i);
+          const float sc1 = kvs ? kvs[slot1] : 1.0f;
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int i = 0; i < PIECES; ++i) *reinterpret_cast<u32x4*>(sh.tile[0] + gs + 64 * i) = first[i];
+          sc = sc0;
+          store_scale(0);
+          sc = sc1;
         }
+        lds_barrier();  // the queries and chunk 0 are in place
+        lds_barrier();  // the queries are read
+        // Interval c stores chunk c + 1 into the buffer that chunk c - 2 left and loads chunk c + 2, piece by piece, in
+        // the last intervals too (the stretch's last row then, into buffers that nobody reads).
+        const uint8_t* src = nullptr;
+        float sc_next = 1.0f;
+        auto ahead = [&](int c) __attribute__((always_inline)) {
+          const int slot = slot_of(c + 2, page);
+          page = trow[page_of(token(c + 3))];
+          src = row_of(slot);
+          if (kvs) sc_next = kvs[slot];
+        };
+        auto piece = [&](int i, uint8_t* to) __attribute__((always_inline)) {
+          *reinterpret_cast<u32x4*>(to + gs + 64 * i) = held[i];
+          held[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
+        };
+        ahead(0);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (g < 3) kx[(g + 1) & 1] = four(sh.kfac[buf], g + 1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sv[4 * g + e] = fmaf(sa[4 * g + e], kx[g & 1][e], -m_run);
-        }
-        if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
-          const int lim = seen - t0 - c * DN_CHUNK - 32 * th - 4 * h;
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sv[4 * g + e] = 8 * g + e < lim ? sv[4 * g + e] : -INFINITY;
-        }
-        float cm = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          if (g < 3) ks[(g + 1) & 1] = four(sh.ksc[buf], g + 1);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) cm = max_nonan(cm, sv[4 * g + e]);
-          p_group(c, g, ks[g & 1]);
-        }
-        const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
-        if (lane == 0) sh.flag[c & 1][wave] = any;
-        last = buf;
-        buf = buf == BUFS - 1 ? 0 : buf + 1;
+        for (int i = 0; i < PIECES; ++i) piece(i, sh.tile[1]);
+        store_scale(1);
+        sc = sc_next;
         lds_barrier();
-      }
-      __builtin_amdgcn_s_setprio(0);
-      settle(nch - 1, flags(nch - 1));
-      const float lw = l_run + __shfl_xor(l_run, 32, WAVE);
-      if (h == 0) sh.lsum[th][32 * hh + j] = lw;
-      if (th == 0 && h == 0) sh.mfin[32 * hh + j] = m_run;
-      lds_barrier();
-      finish([](int) {});
-      }
-    } else {
-      // -- the loads and the values: thread 4 r + e of the value waves brings row r of a chunk, pieces e + 4 i; wave w takes
-      // dims 128 w .. + 127 of all rows --
-      const int w = wave - 4;
-      const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
-      const int* trow = table + (size_t)b * max_pages;
-      const int gr = 16 * w + (lane >> 2);  // this thread's row
-      // its token in chunk c, the stretch's last one past its end (a slot behind the sequence may never have been written,
-      // and its NaN x weight 0 is NaN)
-      const int t_last = min(t0 + nch * DN_CHUNK, len) - 1;
-      auto token = [&](int c) __attribute__((always_inline)) { return min(t0 + c * DN_CHUNK + gr, t_last); };
-      auto page_of = [&](int t) __attribute__((always_inline)) { return (int)((uint64_t)t * pg.mul >> pg.shift); };
-      auto slot_of = [&](int c, int page) __attribute__((always_inline)) {
-        const int t = token(c);
-        return safe_page(page, num_pages) * pg.size + (t - page_of(t) * pg.size);
-      };
-      const int gs = gr * DN_KROW + 16 * ((lane & 3) ^ dn_swizzle(gr));  // where its pieces go in a tile
-      u32x4 held[PIECES];  // the pieces in flight, of the chunk after the one being stored
-      float sc;          // and its token's scale
-      auto row_of = [&](int slot) __attribute__((always_inline)) { return kv + (size_t)slot * DQK + 16 * (lane & 3); };
-      auto store_scale = [&](int to) __attribute__((always_inline)) {
-        if ((lane & 3) == 0) {
-          sh.ksc[to][gr] = sc;
-          sh.kfac[to][gr] = fmaf(sc, sl2, sc * sl2_lo);
+        int buf = 1;  // chunk c's buffer
+#pragma unroll 1
+        for (int c = 1; c <= nch; ++c) {
+          const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
+          ahead(c);
+          interval(c, sh.tile[prev], [&](int i) __attribute__((always_inline)) {
+            if (i >= DN_STORE && i < DN_STORE + PIECES) piece(i - DN_STORE, sh.tile[next]);
+          });
+          store_scale(next);
+          sc = sc_next;
+          buf = next;
+          lds_barrier();
         }
-      };
-      f32x16 o[4][RB];  // [dim block][row block]: row 32 i + j, dims 128 w + 32 d + 8 (r / 4) + 4 h + r % 4
+        if (!whole) {  // as they lie in the registers: see dn_partial
+          float* const to = ws_o + (size_t)part * ROWS * DN_DV + dn_partial(w, 0, 0, 0, RB) + 4 * lane;
 #pragma unroll
-      for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
-      const int vr = 8 * h + ((lane & 15) >> 1), vf = dn_swizzle(vr), vb0 = (lane >> 4) & 1;  // (the value operand's reads)
-      const int vrow = vr * DN_KROW + 128 * w + 8 * (lane & 1);
-      const int voff[2] = {vrow + 16 * (vb0 ^ vf), vrow + 16 * ((2 | vb0) ^ vf)};
-      const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
-      // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed
-      auto v_read = [&](const uint8_t* kt, int i) __attribute__((always_inline)) {
-        return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-            (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW + 64 * ((i & 3) >> 1)));
-      };
-      auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
-        return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * 64 * DN_PROW + 32 * i * DN_PROW + 16 * t));
-      };
-      // Interval c: chunk c - 1's weights are final (and O on their maxima) once its flags are seen; then its value product,
-      // 16 steps of two products, the next steps' operands read and converted ahead, side(i) beside step i.
-      auto interval = [&](int c, const uint8_t* kt, auto side) __attribute__((always_inline)) {
-        const int pb = (c - 1) & 1;
-        const int4 fl = *reinterpret_cast<const int4*>(sh.flag[pb]);
-        dn_v2i vv[DN_VAHEAD + 1];
-        bf16x8 pa[2][2], vb[2];
-#pragma unroll
-        for (int i = 0; i < DN_VAHEAD; ++i) vv[i] = v_read(kt, i);
-        if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
-          lds_barrier();
-          lds_barrier();
-          if (c > 1) {  // O is zero before
-#pragma unroll
-            for (int i = 0; i < RB; ++i) {
-              const float a = sh.al[32 * i + j];
+          for (int i = 0; i < RB; ++i)
+            if (32 * i + j < M - r0)
 #pragma unroll
               for (int d = 0; d < 4; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) o[d][i][r] *= a;
-            }
-          }
+                for (int g = 0; g < 4; ++g)
+                  *reinterpret_cast<f32x4*>(to + dn_partial(0, i, d, g, RB)) =
+                      f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
         }
+        finish([&](int half) __attribute__((always_inline)) {
+          if ((w >> 1) != half) return;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) pa[0][i] = p_read(pb, 0, i);
-        vb[0] = fp8x8_to_bf16x8((uint32_t)vv[0].x, (uint32_t)vv[0].y);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = i >> 2, d = i & 3;
-          if (i + DN_VAHEAD < 16) vv[(i + DN_VAHEAD) % (DN_VAHEAD + 1)] = v_read(kt, i + DN_VAHEAD);
-          if (d < 2 && t < 3) pa[(t + 1) & 1][d] = p_read(pb, t + 1, d);
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            f32x16& sum = o[d][RB == 1 ? 0 : x];
-            sum = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vb[i & 1], pa[t & 1][x], sum, 0, 0, 0);
-          }
-          if (i < 15) {
-            const dn_v2i r = vv[(i + 1) % (DN_VAHEAD + 1)];
-            vb[(i + 1) & 1] = fp8x8_to_bf16x8((uint32_t)r.x, (uint32_t)r.y);
-          }
-          side(i);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      };
-      int page = trow[page_of(token(2))];  // of this thread's token two chunks on
-      const int page0 = trow[page_of(token(0))], page1 = trow[page_of(token(1))];
-      {  // chunks 0 and 1 together: the first into LDS, the second stays in flight
-        const int slot0 = slot_of(0, page0), slot1 = slot_of(1, page1);
-        const uint8_t *src0 = row_of(slot0), *src1 = row_of(slot1);
-        u32x4 first[PIECES];
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) first[i] = *reinterpret_cast<const u32x4*>(src0 + 64 * i);
-        const float sc0 = kvs ? kvs[slot0] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) held[i] = *reinterpret_cast<const u32x4*>(src1 + 64 * i);
-        const float sc1 = kvs ? kvs[slot1] : 1.0f;
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) *reinterpret_cast<u32x4*>(sh.tile[0] + gs + 64 * i) = first[i];
-        sc = sc0;
-        store_scale(0);
-        sc = sc1;
-      }
-      lds_barrier();  // the queries and chunk 0 are in place
-      lds_barrier();  // the queries are read
-      // Interval c stores chunk c + 1 into the buffer that chunk c - 2 left and loads chunk c + 2, piece by piece, in the
-      // last intervals too (the stretch's last row then, into buffers that nobody reads).
-      const uint8_t* src = nullptr;
-      float sc_next = 1.0f;
-      auto ahead = [&](int c) __attribute__((always_inline)) {
-        const int slot = slot_of(c + 2, page);
-        page = trow[page_of(token(c + 3))];
-        src = row_of(slot);
-        if (kvs) sc_next = kvs[slot];
-      };
-      auto piece = [&](int i, uint8_t* to) __attribute__((always_inline)) {
-        *reinterpret_cast<u32x4*>(to + gs + 64 * i) = held[i];
-        held[i] = *reinterpret_cast<const u32x4*>(src + 64 * i);
-      };
-      ahead(0);
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) piece(i, sh.tile[1]);
-      store_scale(1);
-      sc = sc_next;
-      lds_barrier();
-      int buf = 1;  // chunk c's buffer
-#pragma unroll 1
-      for (int c = 1; c <= nch; ++c) {
-        const int prev = buf == 0 ? BUFS - 1 : buf - 1, next = buf == BUFS - 1 ? 0 : buf + 1;
-        ahead(c);
-        interval(c, sh.tile[prev], [&](int i) __attribute__((always_inline)) {
-          if (i >= DN_STORE && i < DN_STORE + PIECES) piece(i - DN_STORE, sh.tile[next]);
-        });
-        store_scale(next);
-        sc = sc_next;
-        buf = next;
-        lds_barrier();
-      }
-      if (!whole) {  // as they lie in the registers: see dn_partial
-        float* const to = ws_o + (size_t)part * ROWS * DN_DV + dn_partial(w, 0, 0, 0, RB) + 4 * lane;
-#pragma unroll
-        for (int i = 0; i < RB; ++i)
-          if (32 * i + j < M - r0)
+          for (int i = 0; i < RB; ++i)
 #pragma unroll
             for (int d = 0; d < 4; ++d)
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-                *reinterpret_cast<f32x4*>(to + dn_partial(0, i, d, g, RB)) =
+              for (int g = 0; g < 4; ++g) {
+                const int x = 32 * (w & 1) + 8 * d + 2 * g + h;
+                area[64 * x + ((32 * i + j) ^ (x & 7))] =
                     f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
+              }
+        });
       }
-      finish([&](int half) __attribute__((always_inline)) {
-        if ((w >> 1) != half) return;
-#pragma unroll
-        for (int i = 0; i < RB; ++i)
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const int x = 32 * (w & 1) + 8 * d + 2 * g + h;
-              area[64 * x + ((32 * i + j) ^ (x & 7))] =
-                  f32x4{o[d][i][4 * g], o[d][i][4 * g + 1], o[d][i][4 * g + 2], o[d][i][4 * g + 3]};
-            }
-      });
-    }
-    lds_barrier();  // (the area's readers, before the next stretch's loads)
+      lds_barrier();  // (the area's readers, before the next stretch's loads)
     }
     u += nch;
     c0 = 0;
@@ -578,9 +589,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   }
 }
 
-// Joins the partials of a row tile where teams shared it: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the rows of
-// sequences without tokens. A wave has a block of 32 rows x 8 G dims, in the partials' own order; WPR waves of a workgroup
-// share a block's partials, each taking every WPR-th, DEEP of them in flight.
+// Joins the partials of a row tile where teams shared it: out = sum 2^(m - max) O / sum 2^(m - max) l; and writes the
+// rows of sequences without tokens. A wave has a block of 32 rows x 8 G dims, in the partials' own order; WPR waves of
+// a workgroup share a block's partials, each taking every WPR-th, DEEP of them in flight.
 constexpr int DC_WAVES = 8;
 constexpr int DC_THREADS = DC_WAVES * WAVE;
 
@@ -769,13 +780,12 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
   const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
                               out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale, tm);
   if (e != hipSuccess) return e;
-  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a block where its first four are
-  // most of them
-  // Waves of 32 rows x 32 dims with a partial after another where there are 3 such blocks a CU; workgroups whose 8 waves share
-  // a block's partials where there are fewer, of a quarter of the dims where they would fill only a quarter of the CUs.
-  // Measured, us in turn with quarters, shared, one wave: 1 x 4k tokens, 16 heads (16 blocks) 4.0, 5.5, 21; 1 x 128k, 128
-  // heads (64) 8.0, 9.5, 45; 8 x 32k, 64 heads (256) 9.6, 8.1, 14.6; 16 x 32k (512) 14.7, 8.7, 10.0; 30 x 4k (960) 27, 12.2,
-  // 9.3; 4 x 4 new tokens after 1k, 128 heads (1,024) 22, 10.4, 7.8.
+  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a block where its first
+  // four are most of them Waves of 32 rows x 32 dims with a partial after another where there are 3 such blocks a CU;
+  // workgroups whose 8 waves share a block's partials where there are fewer, of a quarter of the dims where they would
+  // fill only a quarter of the CUs. Measured, us in turn with quarters, shared, one wave: 1 x 4k tokens, 16 heads (16
+  // blocks) 4.0, 5.5, 21; 1 x 128k, 128 heads (64) 8.0, 9.5, 45; 8 x 32k, 64 heads (256) 9.6, 8.1, 14.6; 16 x 32k (512)
+  // 14.7, 8.7, 10.0; 30 x 4k (960) 27, 12.2, 9.3; 4 x 4 new tokens after 1k, 128 heads (1,024) 22, 10.4, 7.8.
   const long blocks = (long)B * tm.tiles * (tm.rows / 2);
   const bool one = tm.rows == 32;
   auto join = [&](auto kernel, long groups) {

@@ -1,6 +1,6 @@
-// Expanded latent attention for gfx950, the form of a prefill: the keys and values of every head from the cached latent rows
-// (expand_latent_kernel), and attention over them (expanded_attend_kernel). Per pair of tokens and head it costs 192 + 128
-// multiply-adds where the absorbed form's latent products cost 576 + 512.
+// Expanded latent attention for gfx950, the form of a prefill: the keys and values of every head from the cached latent
+// rows (expand_latent_kernel), and attention over them (expanded_attend_kernel). Per pair of tokens and head it costs
+// 192 + 128 multiply-adds where the absorbed form's latent products cost 576 + 512.
 #include "dsa_async.h"
 #include "dsa_scan.h"
 
@@ -11,15 +11,16 @@ constexpr int EX_R = 64;    // the rope width, shared by the heads
 constexpr int EX_C = 512;   // the latent width
 
 // -- keys and values ------------------------------------------------------------------------------------------------
-// k[t, h, :] = sigma_t c_t[:512] . W[h, :128, :]^T, v[t, h, :] the same with W[h, 128:, :]: a product of P x 512 x 256 H
-// whose left side is e4m3 rows gathered through the page table (the scale is applied to the sums), and k_rope[t] =
+// k[t, h, :] = sigma_t c_t[:512] . W[h, :128, :]^T, v[t, h, :] the same with W[h, 128:, :]: a product of P x 512 x 256
+// H whose left side is e4m3 rows gathered through the page table (the scale is applied to the sums), and k_rope[t] =
 // sigma_t c_t[512:].
-// What bounds it: the matrix units, then the stores. A share is of units (tile of 256 tokens, one head's 128 keys or
-// values), a workgroup a CU. The rows of a tile stay in registers, e4m3 until they are operands (exact in bf16), while one
-// part's weights after another run through LDS, 64 of the 512 columns a step, by asynchronous loads 7 steps ahead that
-// cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights through LDS, and stores from registers
-// under the next unit's products (that form with two workgroups a CU: 336 us where this takes 256). The shares of one XCD
-// are 8 tiles' and run through the same weights together, out of its L2.
+//
+// What bounds it: the matrix units, then the stores. A share is of units (tile of 256 tokens, one
+// head's 128 keys or values), a workgroup a CU. The rows of a tile stay in registers, e4m3 until they are operands
+// (exact in bf16), while one part's weights after another run through LDS, 64 of the 512 columns a step, by
+// asynchronous loads 7 steps ahead that cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights
+// through LDS, and stores from registers under the next unit's products (that form with two workgroups a CU: 336 us
+// where this takes 256). The shares of one XCD are 8 tiles' and run through the same weights together, out of its L2.
 // 16,384 tokens x 64 heads: 256 us, 1.07 PFLOP/s; 8,192 tokens, whose outputs the last-level cache holds: 112 us, 1.23.
 constexpr int EL_THREADS = 512;
 constexpr int EL_TOK = 256;  // (or half of it)
@@ -73,8 +74,8 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
   const int xcd = blockIdx.x & 7, G = gridDim.x;
   const int g = xcd * (G >> 3) + min(xcd, G & 7) + (blockIdx.x >> 3);
   const int u0 = (int)((long)units * g / G), u1 = (int)((long)units * (g + 1) / G);
-  // wave: tokens 32 X wm .. + 63 x columns 64 wn .. + 63; the columns are the products' rows, taken in an order that leaves
-  // a lane 32 columns of one token in a row (32 h + 16 y + r)
+  // wave: tokens 32 X wm .. + 63 x columns 64 wn .. + 63; the columns are the products' rows, taken in an order that
+  // leaves a lane 32 columns of one token in a row (32 h + 16 y + r)
   const int wm = wave >> 1, wn = wave & 1;
   const uint32_t b_lds = lds_address(sh.b[0] + 1024 * wave);
   const int bcol = 8 * ((lane & 7) ^ (((lane >> 4) & 3) | ((wave >> 1) & 1) << 2));
@@ -92,7 +93,7 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
     // step s of part p0 + p: weights 64 s .. + 63 of the part's 128 rows, this wave's 16 in eights
     const uint16_t* const bp = wkv + ((size_t)part0 * EX_D + 16 * wave + (lane >> 3)) * EX_C + bcol;
     const int last = n * EL_STEPS - 1;
-    auto issue = [&](int st) __attribute__((always_inline)) {  // (past the end: the last step again, into a stage that is free)
+    auto issue = [&](int st) __attribute__((always_inline)) {  // (past the end: the last step again, into a free stage)
       const int f = min(st, last);
       const uint16_t* from = bp + (size_t)(f / EL_STEPS) * EX_D * EX_C + (f % EL_STEPS) * EL_K;
       const uint32_t to = b_lds + 2 * EX_D * EL_K * (st % EL_STAGES);
@@ -156,7 +157,8 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
       const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
       const uint8_t* row = reinterpret_cast<const uint8_t*>(sh.b[FIRST]) + EX_C * (32 * X * wm + 32 * x + j);
 #pragma unroll
-      for (int i = 0; i < 2 * EL_STEPS; ++i) a[x][i] = *reinterpret_cast<const u32x4*>(row + 16 * ((2 * i + h) ^ (j & 15)));
+      for (int i = 0; i < 2 * EL_STEPS; ++i)
+        a[x][i] = *reinterpret_cast<const u32x4*>(row + 16 * ((2 * i + h) ^ (j & 15)));
     }
     lds_barrier();  // the stages are free
 
@@ -196,10 +198,11 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
           }
         }
       }
-      // a lane's 64 bytes of a token, 4 lanes' tokens: transposed among them, so that 4 lanes write one token's 64 bytes
+      // a lane's 64 bytes of a token, 4 lanes' tokens: transposed among them, so that 4 lanes write one token's 64
+      // bytes
       const int part = part0 + p;
-      uint16_t* const out = (part & 1 ? v_out : k_out) +
-                            ((size_t)(t0 + 32 * X * wm + 4 * (j >> 2)) * H + (part >> 1)) * EX_D + 64 * wn + 32 * h + 8 * (j & 3);
+      const size_t row0 = (size_t)(t0 + 32 * X * wm + 4 * (j >> 2));
+      uint16_t* const out = (part & 1 ? v_out : k_out) + (row0 * H + (part >> 1)) * EX_D + 64 * wn + 32 * h + 8 * (j & 3);
 #pragma unroll
       for (int x = 0; x < X; ++x) {
         uint32_t o[4][4];  // piece, dword
@@ -224,12 +227,16 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
 // -- attention ------------------------------------------------------------------------------------------------------
 // s = scale (q[:128] . k + q[128:] . k_rope), p = softmax(s), out = p . v, lse, for ragged batches of queries and keys,
 // causal (the last query sees every key) or full.
-// What bounds it: the matrix units, then the exponentials. One workgroup a CU has 256 queries of a head, 8 waves of 32,
-// two on each SIMD, the first of them with priority, so that one's softmax runs under the other's products. A tile of 64
-// keys and values comes by asynchronous loads straight into LDS two tiles ahead, with one barrier a tile. S^T = K . Q^T and
-// O^T += V^T . P on v_mfma_f32_32x32x16_bf16: a lane's scores are of one query, in the value product's operand layout as
-// they stand (the values are read transposed in the same order), so P never leaves the registers and the maxima and sums
-// stay in their lanes. The longest tiles of a causal batch go first.
+//
+// What bounds it: the matrix units, then the LDS reads that feed them and the exponentials. One workgroup a CU has 256 queries of a head, 8 waves of 32, two on each SIMD, the first of
+// them with priority, so that one's softmax runs under the other's products. A tile of 64 keys and values comes by
+// asynchronous loads straight into LDS two tiles ahead, with one barrier a tile. S^T = K . Q^T and O^T += V^T . P on
+// v_mfma_f32_32x32x16_bf16: a lane's scores are of one query, in the value product's operand layout as they stand (the
+// values are read transposed in the same order), so P never leaves the registers and the maxima and sums stay in their
+// lanes. The longest tiles of a causal batch go first. Where there are few query tiles, their keys are taken in splits
+// that expanded_combine_kernel joins.
+//
+// 8,192 tokens, 64 heads, causal: 1,255 us, 1.10 PFLOP/s (a large library product: 1.29).
 constexpr int XA_THREADS = 512;
 constexpr int XA_Q = 256;
 constexpr int XA_K = 64;
@@ -315,9 +322,9 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   const int seen0 = seen(w0);
   const int qi = min(w0 + j, nq - 1), seen_j = seen(qi);
 
-  // Waves 0 to 3, the ones with priority, bring the tiles, once they are through with theirs: the loads' issue would delay
-  // the others, for whom they wait anyway (8k tokens, 64 heads: 1,194 us; all waves before their tile 1,235, after it
-  // 1,207). Key and value rows 16 wave .. + 15 in fours, rope rows in eights.
+  // Waves 0 to 3, the ones with priority, bring the tiles, once they are through with theirs: the loads' issue would
+  // delay the others, for whom they wait anyway (8k tokens, 64 heads: 1,194 us; all waves before their tile 1,235,
+  // after it 1,207). Key and value rows 16 wave .. + 15 in fours, rope rows in eights.
   const bool brings = wave < 4;
   const size_t head_off = (size_t)kb * H * EX_D + (size_t)head * EX_D;
   const uint16_t* const k_base = k + head_off;
@@ -341,9 +348,9 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                    r_lds + XA_K * 128 * to + 1024 * x);
   };
   if (brings && nt > i0) issue(i0, 0);
-  // the queries through LDS, over the stages that tiles 1 and 2 take: columns 64 p .. + 63 of the wave's 32 rows are 4 KiB
-  // of k, v or r, laid out as rope rows. (Read straight into the operands' layout, 32 bytes of 32 rows at a time, they took
-  // 5,000 cycles more.)
+  // the queries through LDS, over the stages that tiles 1 and 2 take: columns 64 p .. + 63 of the wave's 32 rows are 4
+  // KiB of k, v or r, laid out as rope rows. (Read straight into the operands' layout, 32 bytes of 32 rows at a time,
+  // they took 5,000 cycles more.)
   bf16x8 qf[STEPS];  // query qi: step s holds dims 16 s + 8 h .. + 7
   {
     uint8_t* const at[3] = {sh.k[1], sh.v[1], sh.r[DQ > EX_D ? 1 : 0]};
@@ -523,8 +530,8 @@ hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* 
                   k, v, r, B, total, H, D, max_pages, page_size, num_pages, units);
   };
   // tiles of 128 tokens where all their units run at once (16 heads: 1 token 8.1 us with them, 11.0 with tiles of 256;
-  // 1,001 tokens 12.1 and 13.7), else of 256, which read the weights half as often (1,500 tokens 17.9 and 15.7; 64 heads,
-  // 8k tokens 136 and 112)
+  // 1,001 tokens 12.1 and 13.7), else of 256, which read the weights half as often (1,500 tokens 17.9 and 15.7; 64
+  // heads, 8k tokens 136 and 112)
   return (long)((total + EL_TOK / 2 - 1) / (EL_TOK / 2)) * 2 * H <= num_cu ? run(expand_latent_kernel<1>, EL_TOK / 2)
                                                                            : run(expand_latent_kernel<2>, EL_TOK);
 }
@@ -536,8 +543,8 @@ bool expanded_grid_ok(int B, int Tq, int H) {
   return ((long)Tq / XA_Q + B) * H <= 0x7fffffL && (long)Tq + B <= 0x7fffffffL - XA_Q;
 }
 
-// Joins a query tile's splits: out = sum 2^(m - max) O / sum 2^(m - max) l. A workgroup has a tile of a head, a wave its 32
-// queries, the lanes as the partials hold them.
+// Joins a query tile's splits: out = sum 2^(m - max) O / sum 2^(m - max) l. A workgroup has a tile of a head, a wave
+// its 32 queries, the lanes as the partials hold them.
 __global__ __launch_bounds__(XA_THREADS) void expanded_combine_kernel(
     const float* __restrict__ ws, const int* __restrict__ cu_q, uint16_t* __restrict__ out, float* __restrict__ out_f32,
     float* __restrict__ lse_out, int B, int Tq, int H, int q_tiles, int splits) {
@@ -604,9 +611,9 @@ __global__ __launch_bounds__(XA_THREADS) void expanded_combine_kernel(
   if (lse_out && d == 0 && h == 0) lse_out[row] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
 }
 
-// In how many splits a tile's keys are taken: as many as leave the CUs a workgroup each where every sequence has queries (the
-// fewest tiles that they can be), none of fewer than 4 tiles of keys on average. (16 heads: 256 queries of 32k keys 839 us
-// unsplit, 103 in 16; 1,000 of 1,000 33 and 29 in 3.)
+// In how many splits a tile's keys are taken: as many as leave the CUs a workgroup each where every sequence has
+// queries (the fewest tiles that they can be), none of fewer than 4 tiles of keys on average. (16 heads: 256 queries of
+// 32k keys 839 us unsplit, 103 in 16; 1,000 of 1,000 33 and 29 in 3.)
 static int attend_splits(int B, int Tq, int Tk, int H, int num_cu) {
   const long tiles = ((long)Tq + XA_Q - 1) / XA_Q, least = (tiles > B ? tiles : B) * H;
   const long by_cu = num_cu / least, by_keys = (long)Tk / B / (4 * XA_K), n = by_cu < by_keys ? by_cu : by_keys;

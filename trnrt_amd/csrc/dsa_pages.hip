@@ -4,10 +4,12 @@
 // moved. Integers only and every choice in ascending order (the lowest free pages, the k-th live page past the front to
 // the k-th hole), so the results do not depend on the order in which workgroups run.
 //
-// What bounds them: the copies move bytes at a large copy's rate once there are enough pages (compaction of 12,345 pages,
-// fork of many sequences); a small fork is its two launches. Every cache of a model takes part in one launch (up to
-// PG_CACHES of them: latent rows, their scales, indexer keys, ... of every layer), a page of each cut into 16 KiB pieces,
-// one workgroup a piece, so that one page of one sequence already spreads over several CUs.
+// What bounds them: the copies move bytes at a large copy's rate once there are enough pages (compaction of 12,345
+// pages, fork of many sequences); a small fork is its two launches. Every cache of a model takes part in one launch (up
+// to PG_CACHES of them: latent rows, their scales, indexer keys, ... of every layer), a page of each cut into 16 KiB
+// pieces, one workgroup a piece, so that one page of one sequence already spreads over several CUs. Measured:
+// compaction of 12,345 pages of five caches, 320 MB read and written, 7.7 us of planning and 72 of moves at 4.4 TB/s (a
+// large copy: 4.8); fork of 8 or 128 sequences 3.5 + 4 to 6 us, their release 3 to 4.
 #include "dsa_pages.h"
 #include "dsa_scan.h"
 
@@ -17,7 +19,9 @@ constexpr int PG_THREADS = 256;                       // a copying workgroup
 constexpr int PG_PIECE = PG_THREADS * 16 * 4;         // bytes: four 16-byte loads a thread, all in flight
 constexpr int PG_PLAN_THREADS = 1024;                 // a planning workgroup
 constexpr int PG_BLOCK = PG_PLAN_THREADS * 4;         // pages of a planning workgroup (one int4 of counts a thread)
-constexpr int PG_OWN = 4;                             // blocks up to which each planning workgroup counts all of them
+// Blocks up to which each planning workgroup counts all of them, a launch less (300 pages: 3.7 us for 1.6 + 3.3 in two
+// launches, 12k pages, 4 blocks, 7.7 for 2.6 + 5.0).
+constexpr int PG_OWN = 4;
 
 // One piece of page src of every cache it belongs to -> page dst (the whole workgroup).
 __device__ __forceinline__ void copy_piece(const PageCaches& set, int piece, int src, int dst) {
@@ -138,7 +142,8 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_fork_plan_kernel(
   }
 }
 
-// Workgroup 0 of a child writes its table row and counts its pages (with_table), the others copy its last page's pieces.
+// Workgroup 0 of a child writes its table row and counts its pages (with_table), the others copy its last page's
+// pieces.
 __global__ __launch_bounds__(PG_THREADS) void pages_fork_kernel(
     PageCaches set, int with_table, int* __restrict__ ref, const int* __restrict__ table,
     const int* __restrict__ ctx_len, const int* __restrict__ parents, const int* __restrict__ pages,
@@ -201,8 +206,9 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_count_kernel(const int*
   if (threadIdx.x == 0) counts[blockIdx.x] = total;
 }
 
-// code[p]: p where it stays, -(k + 1) where it is the k-th to move, 0 where it is free; holes[k], movers[k]; moves: their
-// number. counts: the live pages of each block, or null where the workgroup counts them itself (up to PG_OWN blocks).
+// code[p]: p where it stays, -(k + 1) where it is the k-th to move, 0 where it is free; holes[k], movers[k]; moves:
+// their number. counts: the live pages of each block, or null where the workgroup counts them itself (up to PG_OWN
+// blocks).
 __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* __restrict__ ref,
                                                                      const int* counts, int blocks,
                                                                      int* __restrict__ code, int* __restrict__ holes,
@@ -214,8 +220,8 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* 
   int total, before = 0, live = 0;
   if (!counts) {
     for (int b = 0; b < blocks; ++b) {
-      group_incl_scan<PG_PLAN_THREADS>(live_of(load_refs(ref, b * PG_BLOCK + 4 * t, num_pages), b * PG_BLOCK + 4 * t), tot,
-                                       total);
+      const int p = b * PG_BLOCK + 4 * t;
+      group_incl_scan<PG_PLAN_THREADS>(live_of(load_refs(ref, p, num_pages), p), tot, total);
       if (t == 0) own[b] = total;
     }
     __syncthreads();
@@ -238,9 +244,9 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* 
   {
     const int p = lb * PG_BLOCK + 4 * t;
     const pg_v4i r = load_refs(ref, p, num_pages);
-    group_incl_scan<PG_PLAN_THREADS>((int)(r.x > 0 && p > 0 && p <= live) + (r.y > 0 && p + 1 <= live) + (r.z > 0 && p + 2 <= live) +
-                        (r.w > 0 && p + 3 <= live),
-                    tot, total);
+    const int up_to = (int)(r.x > 0 && p > 0 && p <= live) + (r.y > 0 && p + 1 <= live) + (r.z > 0 && p + 2 <= live) +
+                      (r.w > 0 && p + 3 <= live);
+    group_incl_scan<PG_PLAN_THREADS>(up_to, tot, total);
     front += total;
   }
   const int p = blk * PG_BLOCK + 4 * t;
