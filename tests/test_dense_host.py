@@ -28,6 +28,9 @@ def test_refusals():
     assert call(wsp=None) == _lib.DSA_EWORKSPACE
     assert call(size=2 * 256 * 64 * 514 * 4 - 1) == _lib.DSA_EWORKSPACE
     assert call(B=0, q=None) == _lib.DSA_OK
+    odd = ctypes.c_void_p(264)  # not a multiple of 16
+    assert call(q=odd) == _lib.DSA_EINVAL and call(out=odd) == _lib.DSA_EINVAL
+    assert call(wsp=odd) == _lib.DSA_EWORKSPACE
 
 
 def test_host_tensors_raise():

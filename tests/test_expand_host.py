@@ -22,6 +22,9 @@ def test_expand_refusals():
     assert call(pages=1 << 26) == _lib.DSA_EUNSUPPORTED  # 2^32 slots
     assert call(total=1 << 30, H=1 << 10) == _lib.DSA_EUNSUPPORTED  # more workgroups than a launch takes
     assert call(total=0, kv=None) == _lib.DSA_OK and call(B=0) == _lib.DSA_OK
+    odd = ctypes.c_void_p(264)  # not a multiple of 16
+    for kw in (dict(kv=odd), dict(w=odd), dict(k=odd), dict(rope=odd)):
+        assert call(**kw) == _lib.DSA_EINVAL, kw
 
 
 def test_attend_refusals():
@@ -33,10 +36,14 @@ def test_attend_refusals():
     assert call(Tq=1 << 30, H=1 << 10) == _lib.DSA_EUNSUPPORTED
     assert call(B=0) == _lib.DSA_OK and call(Tq=0, q=None) == _lib.DSA_OK
     need = _lib.lib().dsa_expanded_workspace_bytes
+    odd = ctypes.c_void_p(264)  # not a multiple of 16
+    for kw in (dict(q=odd), dict(k=odd), dict(v=odd), dict(out=odd)):
+        assert call(**kw) == _lib.DSA_EINVAL, kw
     assert need(2, 10, 10, 16) == 0 and need(0, 10, 10, 16) == 0 and need(2, 10, -1, 16) == 0
     size = need(1, 10, 100000, 16)  # one query tile a head, the keys in splits
     assert size >= 2 * 16 * 256 * 130 * 4
     assert call(B=1, Tk=100000) == _lib.DSA_EWORKSPACE and call(B=1, Tk=100000, ws=P, size=size - 1) == _lib.DSA_EWORKSPACE
+    assert call(B=1, Tk=100000, ws=odd, size=size) == _lib.DSA_EWORKSPACE
 
 
 def test_host_tensors_raise():

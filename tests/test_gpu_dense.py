@@ -241,6 +241,22 @@ def test_graph_replays_and_another_stream():
             assert torch.equal(out, eager[0])
 
 
+def test_views_at_odd_places():
+    """Queries that start at an odd element are copied; a cache that does is refused."""
+    say("dense odd places")
+    q, kv, sc, table, lens = (x.cuda() for x in make([100, 5], 1, 16, 576, 64, seed=12))
+    want = dsa_dense.attend(q, kv, sc, table, lens, 64, 0.1)
+    flat = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")
+    odd = flat[1:].view(q.shape)
+    odd.copy_(q)
+    got = dsa_dense.attend(odd, kv, sc, table, lens, 64, 0.1)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    cache = torch.empty(kv.numel() + 8, dtype=torch.uint8, device="cuda")[8:].view(kv.shape)
+    cache.copy_(kv)
+    with pytest.raises(ValueError):
+        dsa_dense.attend(q, cache, sc, table, lens, 64, 0.1)
+
+
 def test_refusals():
     q, kv, sc, table, lens = (x.cuda() for x in make([100, 5], 1, 16, 576, 64, seed=0))
     ok = dict(q=q, kv_cache=kv, kv_scale=sc, table=table, ctx_len=lens, page_size=64, scale=0.1)
@@ -248,7 +264,8 @@ def test_refusals():
                 dict(table=table[:1]), dict(table=table[0]), dict(ctx_len=lens[:1]), dict(kv_cache=kv.float()),
                 dict(kv_cache=kv.t()), dict(kv_cache=kv.view(-1, 512), kv_scale=None), dict(out=torch.empty(2, 1, 16, 500, device="cuda")),
                 dict(out=torch.empty(2, 1, 16, 512, dtype=torch.float16, device="cuda")),
-                dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))):
+                dict(workspace=torch.empty(64, dtype=torch.uint8, device="cuda")),
+                dict(workspace=torch.empty(1, dtype=torch.uint8, device="cuda").expand(1 << 30))):
         with pytest.raises(ValueError):
             dsa_dense.attend(**{**ok, **bad})
     with pytest.raises(RuntimeError, match="GPU only"):

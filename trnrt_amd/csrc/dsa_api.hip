@@ -1282,6 +1282,16 @@ static int pooled_layer(const void* q_idx_bf16, const float* w, const void* pool
 
 extern "C" {
 
+}  // extern "C"
+
+// Whether every pointer may be accessed 16 bytes at a time (null ones too).
+template <typename... P>
+static bool aligned16(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & 15) == 0;
+}
+
+extern "C" {
+
 size_t dsa_dense_workspace_bytes(int S, int H) {
   if (S < 1 || H < 1 || (long)S * H > 0x7fffffffL) return 0;
   return align256(dsa::dense_workspace_bytes(S * H, num_cu()));
@@ -1297,7 +1307,9 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
     return DSA_EUNSUPPORTED;
   if (B == 0) return DSA_OK;
   if (!q_bf16 || !kv_fp8 || !page_table || !ctx_len || (!out_bf16 && !out_f32)) return DSA_EINVAL;
-  if (!workspace || workspace_bytes < dsa::dense_workspace_bytes(S * H, num_cu())) return DSA_EWORKSPACE;
+  if (!aligned16(q_bf16, kv_fp8, out_bf16, out_f32)) return DSA_EINVAL;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::dense_workspace_bytes(S * H, num_cu()))
+    return DSA_EWORKSPACE;
   return status(dsa::launch_dense_mla(static_cast<const uint16_t*>(q_bf16), kv_fp8, kv_scale, page_table, ctx_len,
                                       static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, S, H, Dqk,
                                       max_pages, page_size, num_pages, scale, num_cu(),
@@ -1314,6 +1326,7 @@ int dsa_expand_latent(const uint8_t* kv_fp8, const float* kv_scale, const int32_
   if (B == 0 || total == 0) return DSA_OK;
   if (!kv_fp8 || !page_table || !cu_len || !w_bf16 || !k_bf16 || !v_bf16 || (Dqk == 576 && !rope_bf16))
     return DSA_EINVAL;
+  if (!aligned16(kv_fp8, w_bf16, k_bf16, v_bf16, rope_bf16)) return DSA_EINVAL;
   return status(dsa::launch_expand_latent(
       kv_fp8, kv_scale, page_table, cu_len, static_cast<const uint16_t*>(w_bf16), static_cast<uint16_t*>(k_bf16),
       static_cast<uint16_t*>(v_bf16), Dqk == 576 ? static_cast<uint16_t*>(rope_bf16) : nullptr, B, total, H, Dqk,
@@ -1334,8 +1347,9 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
   if (B == 0 || Tq == 0) return DSA_OK;
   // (no keys: k, v and rope_bf16 may be null, and every query sees nothing)
   if (!q_bf16 || !cu_q || !cu_k || (!out_bf16 && !out_f32) || (Tk > 0 && (!k_bf16 || !v_bf16))) return DSA_EINVAL;
+  if (!aligned16(q_bf16, k_bf16, rope_bf16, v_bf16, out_bf16, out_f32)) return DSA_EINVAL;
   const size_t need = dsa::expanded_workspace_bytes(B, Tq, Tk, H, num_cu());
-  if (need > 0 && (!workspace || workspace_bytes < need)) return DSA_EWORKSPACE;
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return DSA_EWORKSPACE;
   return status(dsa::launch_expanded_attend(
       static_cast<const uint16_t*>(q_bf16), static_cast<const uint16_t*>(k_bf16),
       static_cast<const uint16_t*>(rope_bf16), static_cast<const uint16_t*>(v_bf16), cu_q, cu_k,
@@ -1381,7 +1395,7 @@ int dsa_pages_fork(int32_t* ref, const int32_t* page_table, const int32_t* ctx_l
   const int st = page_caches_status(caches, page_bytes, n_caches, n);
   if (st != DSA_OK || n == 0) return st;
   if (!ref || !page_table || !ctx_len || !parents || !child_table || !pages) return DSA_EINVAL;
-  if (!workspace || workspace_bytes < dsa::pages_fork_bytes(n)) return DSA_EWORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::pages_fork_bytes(n)) return DSA_EWORKSPACE;
   return status(dsa::launch_pages_fork(ref, page_table, ctx_len, parents, child_table, pages, caches, page_bytes,
                                        n_caches, workspace, B, n, max_pages, page_size, num_pages,
                                        static_cast<hipStream_t>(stream)));
@@ -1406,7 +1420,8 @@ int dsa_pages_compact(const int32_t* ref, const int32_t* page_table, int32_t* ne
   if (!ref || !new_ref || !remap || (B > 0 && (!page_table || !new_table))) return DSA_EINVAL;
   if (ref == new_ref || (B > 0 && page_table == new_table)) return DSA_EINVAL;  // read after the first are written
   if (num_pages > 0x1fffffff) return DSA_EUNSUPPORTED;
-  if (!workspace || workspace_bytes < dsa::pages_compact_bytes(num_pages)) return DSA_EWORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::pages_compact_bytes(num_pages))
+    return DSA_EWORKSPACE;
   return status(dsa::launch_pages_compact(ref, page_table, new_ref, new_table, remap, caches, page_bytes, n_caches,
                                           workspace, (long)B * max_pages, num_pages, num_cu(),
                                           static_cast<hipStream_t>(stream)));

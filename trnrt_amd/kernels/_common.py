@@ -72,6 +72,18 @@ def as_f32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """t itself if it starts at a multiple of 16 bytes (a view may not), else a copy that does."""
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def given(workspace: torch.Tensor, what: str) -> torch.Tensor:
+    """A caller's workspace; ValueError where its bytes are not one range."""
+    if not workspace.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous")
+    return workspace
+
+
 def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
     """A contiguous tensor as rows [n, width] (itself where it is that already)."""
     return t if t.dim() == 2 else t.reshape(-1, width)
@@ -107,13 +119,21 @@ def cached_workspace(device: torch.device, nbytes: int, use: str) -> torch.Tenso
     return ws
 
 
+_SCRATCH: dict = {}
+
+
 def scratch(device: torch.device, nbytes: int, use: str) -> torch.Tensor:
     """A uint8 device buffer of at least nbytes that a call writes before it reads: the one kept for `use` on the current
     stream, and in a graph capture one of the graph's own memory (a graph that kept the stream's would replay into it after a
     later call had let it go for a larger one, or beside another graph's replay)."""
+    n = max(int(nbytes), 256)
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
-    return cached_workspace(device, nbytes, use)
+        return torch.empty(n, dtype=torch.uint8, device=device)
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device), use)
+    ws = _SCRATCH.get(key)
+    if ws is None or ws.numel() < n:
+        ws = _SCRATCH[key] = torch.empty(n, dtype=torch.uint8, device=device)
+    return ws
 
 
 def zeroed_workspace(nbytes: int, device: torch.device) -> torch.Tensor:

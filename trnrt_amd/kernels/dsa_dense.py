@@ -35,7 +35,7 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
         raise ValueError(f"dsa_dense: q {tuple(q.shape)}, expected [B, H, 576 or 512] or [B, S, H, 576 or 512]")
     B, H, dqk = q.shape[0], q.shape[-2], q.shape[-1]
     S = q.shape[1] if q.dim() == 4 else 1
-    q = C.as_bf16(q)
+    q = C.aligned(C.as_bf16(q))
     if kv_cache.shape[-1] != dqk:
         raise ValueError(f"dsa_dense: cache rows of {kv_cache.shape[-1]} for q of {dqk}")
     kv = C.rows_of(C.fp8_bytes(kv_cache, "kv cache"), dqk)
@@ -53,8 +53,9 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     C.need(out, "out", (torch.bfloat16, torch.float32), shape)
     ls = q.new_empty(q.shape[:-1], dtype=torch.float32) if lse else None
     lib = _lib.lib()
-    ws = workspace
-    if ws is None:  # the partials of the row tiles that workgroups share
+    if workspace is not None:
+        ws = C.given(workspace, "dsa_dense")
+    else:  # the partials of the row tiles that workgroups share
         ws = C.scratch(dev, int(lib.dsa_dense_workspace_bytes(S, H)), "dense")
     bf = out.dtype == torch.bfloat16
     st = C.call(dev, lib.dsa_dense_mla, C.ptr(q), C.ptr(kv), C.ptr(kv_scale), C.ptr(tb), C.ptr(lens),

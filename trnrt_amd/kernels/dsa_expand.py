@@ -46,7 +46,7 @@ def expand(kv_cache: torch.Tensor, kv_scale: torch.Tensor | None, table: torch.T
     if w.dim() != 3 or w.shape[0] < 1:
         raise ValueError(f"dsa_expand: w {tuple(w.shape)}, expected [H, {2 * DH}, {DV}]")
     H = w.shape[0]
-    w = C.need(w, "w", torch.bfloat16, (H, 2 * DH, DV))
+    w = C.aligned(C.need(w, "w", torch.bfloat16, (H, 2 * DH, DV)))
     tb = C.as_i32(table)
     if tb.dim() != 2 or tb.shape[1] < 1:
         raise ValueError(f"dsa_expand: page table {tuple(table.shape)}, expected [B, max_pages]")
@@ -87,13 +87,13 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[2] != dq:
         raise ValueError(f"dsa_expand: q {tuple(q.shape)}, expected [Tq, H, {dq}]")
     Tq, H = q.shape[:2]
-    q = C.as_bf16(q)
+    q = C.aligned(C.as_bf16(q))
     if k.dim() != 3:
         raise ValueError(f"dsa_expand: k {tuple(k.shape)}, expected [Tk, {H}, {DH}]")
     Tk = k.shape[0]
-    k = C.need(C.as_bf16(k), "k", torch.bfloat16, (Tk, H, DH))
-    v = C.need(C.as_bf16(v), "v", torch.bfloat16, (Tk, H, DH))
-    r = None if k_rope is None else C.need(C.as_bf16(k_rope), "k_rope", torch.bfloat16, (Tk, ROPE))
+    k = C.aligned(C.need(C.as_bf16(k), "k", torch.bfloat16, (Tk, H, DH)))
+    v = C.aligned(C.need(C.as_bf16(v), "v", torch.bfloat16, (Tk, H, DH)))
+    r = None if k_rope is None else C.aligned(C.need(C.as_bf16(k_rope), "k_rope", torch.bfloat16, (Tk, ROPE)))
     if cu_q.dim() != 1 or cu_q.shape != cu_k.shape or cu_q.numel() < 1:
         raise ValueError(f"dsa_expand: cu_q {tuple(cu_q.shape)} and cu_k {tuple(cu_k.shape)}, expected [B + 1]")
     cq, ck = C.as_i32(cu_q), C.as_i32(cu_k)
@@ -102,8 +102,10 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     C.need(out, "out", (torch.bfloat16, torch.float32), (Tq, H, DH))
     ls = q.new_empty((Tq, H), dtype=torch.float32) if lse else None
     bf = out.dtype == torch.bfloat16
-    lib, B, ws = _lib.lib(), cu_q.numel() - 1, workspace
-    if ws is None:
+    lib, B = _lib.lib(), cu_q.numel() - 1
+    if workspace is not None:
+        ws = C.given(workspace, "dsa_expand")
+    else:
         need = int(lib.dsa_expanded_workspace_bytes(B, Tq, Tk, H))
         ws = C.scratch(dev, need, "expanded") if need else None
     st = C.call(dev, lib.dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),

@@ -85,8 +85,9 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     lens = C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
     child, pages = tb.new_empty((n, max_pages)), tb.new_empty((n,))
     lib = _lib.lib()
-    ws = workspace
-    if ws is None:
+    if workspace is not None:
+        ws = C.given(workspace, "dsa_pages")
+    else:
         ws = C.scratch(dev, int(lib.dsa_pages_workspace_bytes(num_pages, n)), "pages")
     st = C.call(dev, lib.dsa_pages_fork, C.ptr(ref), C.ptr(tb), C.ptr(lens), C.ptr(par), C.ptr(child), C.ptr(pages),
                 ptrs, size, n_caches, C.ptr(ws), ws.numel() * ws.element_size(), B, n, max_pages, int(page_size),
@@ -128,8 +129,9 @@ def compact(ref: torch.Tensor, table: torch.Tensor, caches, page_size: int, *,
     new_table = tb.new_empty((B, max_pages))
     new_ref, remap = torch.empty_like(ref), torch.empty_like(ref)
     lib = _lib.lib()
-    ws = workspace
-    if ws is None:
+    if workspace is not None:
+        ws = C.given(workspace, "dsa_pages")
+    else:
         ws = C.scratch(dev, int(lib.dsa_pages_workspace_bytes(num_pages, 0)), "pages")
     st = C.call(dev, lib.dsa_pages_compact, C.ptr(ref), C.ptr(tb), C.ptr(new_ref), C.ptr(new_table), C.ptr(remap), ptrs,
                 size, n_caches, C.ptr(ws), ws.numel() * ws.element_size(), B, max_pages, num_pages)
