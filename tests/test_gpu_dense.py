@@ -180,6 +180,13 @@ def test_many_short_sequences():
     check(make(lens, 1, 16, 512, 16, seed=2), 16)
 
 
+def test_padded_batch():
+    """Thousands of sequences without tokens around the few that have some."""
+    say("dense padded batch")
+    lens = [700] + [0] * 1500 + [65, 0, 900] + [0] * 511 + [3] + [0] * 512 + [64, 1000] + [0] * 300
+    check(make(lens, 1, 16, 576, 64, seed=13), 64)
+
+
 def test_all_empty_and_no_sequence():
     say("dense empty")
     out, lse = check(make([0, 0, 0], 2, 16, 576, 64, seed=2), 64)

@@ -63,6 +63,12 @@ def test_expand(lens, H, D, ps, scaled):
         assert r is None
 
 
+def test_expand_padded_batch():
+    """Thousands of sequences without tokens around the few that have some."""
+    say("expand padded batch")
+    test_expand([5] + [0] * 3000 + [300, 0, 1] + [0] * 700 + [40], 2, 576, 64, True)
+
+
 def attend_ref(q, k, r, v, lq, lk, scale, causal):
     Tq, H, _ = q.shape
     out = torch.zeros(Tq, H, 128, dtype=torch.float64, device="cuda")

@@ -583,8 +583,20 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     c0 = 0;
     if (u < u1 && ++set == tm.sets) {  // the next sequence with tokens
       set = 0;
-      do len = dn_len(ctx_len[++b], max_pages, pg.size);
-      while (len == 0);
+      if (++b >= B) return;
+      len = dn_len(ctx_len[b], max_pages, pg.size);
+      while (len == 0) {  // (a padded batch may have many without: the next of them looked for side by side)
+        if (tid == 0) sh.found[0] = B;
+        __syncthreads();
+        const int x = b + 1 + tid;
+        if (x < B && ctx_len[x] > 0) atomicMin(&sh.found[0], x);
+        __syncthreads();
+        const int next = __builtin_amdgcn_readfirstlane(sh.found[0]);
+        __syncthreads();
+        if (next >= B && b + DN_THREADS >= B - 1) return;
+        b = min(next, b + DN_THREADS);
+        len = dn_len(ctx_len[b], max_pages, pg.size);
+      }
     }
   }
 }

@@ -109,8 +109,10 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
     __syncthreads();
     if (tid < TOK) {
       const int t = min(t0 + tid, end - 1);
-      int b = min(sh.seq, B - 1);
-      while (b < B - 1 && cu[b + 1] <= t) ++b;
+      int b = min(sh.seq, B - 1), step = 1;  // the last sequence that starts by t, in doubling steps and halving ones
+      for (; b + step < B && cu[b + step] <= t; step *= 2) b += step;
+      for (step /= 2; step > 0; step /= 2)
+        if (b + step < B && cu[b + step] <= t) b += step;
       const int pos = max(t - cu[b], 0), pi = pos / page_size;
       const int page = pi < max_pages ? safe_page(table[(size_t)b * max_pages + pi], num_pages) : 0;
       sh.slot[tid] = page * page_size + (pos - pi * page_size);
