@@ -55,6 +55,12 @@ typedef int dn_v2i __attribute__((ext_vector_type(2)));
 // transposed (32 lanes: two pieces of 8 rows), cover the 64 banks once.
 __device__ __forceinline__ int dn_swizzle(int r) { return (r >> 2 & 1) << 1 | (r >> 3 & 1); }
 constexpr int DN_KROW = 576;
+
+// The same of the staged queries, rows of 2 DQK bytes: one piece of 16 rows covers the 64 banks once.
+template <int DQK>
+__device__ __forceinline__ int dn_q_swizzle(int r) {
+  return DQK == 576 ? r >> 1 & 7 : r & 15;
+}
 constexpr int DN_BUFS = 3;  // chunk c being scored, c - 1 whose values are multiplied, c + 1 being stored
 
 // RB: blocks of 32 rows in a tile.
@@ -239,7 +245,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         const int th = wave >> 1, hh = wave & 1;
         const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
         // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece
-        // p at p ^ (r & 7), so that one piece of 8 rows covers the banks once
+        // p at p ^ dn_q_swizzle(r)
         {
           constexpr int QP = DQK / 8, PER = ROWS * QP / (4 * WAVE);
           static_assert(ROWS * QP * 16 <= 2 * DN_CHUNK * DN_KROW, "the staged queries");
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 #pragma unroll
           for (int i = 0; i < PER; ++i) {
             const int x = WAVE * (PER * wave + i) + lane, r = x / QP, p = x - r * QP;
-            load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ (r & 7)), q_lds + 1024 * i);
+            load_lds16(q + ((size_t)b * M + r0 + min(r, r_max)) * DQK + 8 * (p ^ dn_q_swizzle<DQK>(r)), q_lds + 1024 * i);
           }
           wait_loads<0>();
         }
@@ -275,7 +281,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             const uint8_t* const qr = sh.tile[1] + (32 * hh + j) * 2 * DQK;
 #pragma unroll
             for (int s = 0; s < 2 * STEPS; ++s)
-              qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ (j & 7))));
+              qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ dn_q_swizzle<DQK>(j))));
           }
           lds_barrier();  // the queries are read
           float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
