@@ -8,7 +8,7 @@
 // pages, fork of many sequences); a small fork is its two launches. Every cache of a model takes part in one launch (up
 // to PG_CACHES of them: latent rows, their scales, indexer keys, ... of every layer), a page of each cut into 16 KiB
 // pieces, one workgroup a piece, so that one page of one sequence already spreads over several CUs. Measured:
-// compaction of 12,345 pages of five caches, 320 MB read and written, 7.7 us of planning and 72 of moves at 4.4 TB/s (a
+// compaction of 12,345 pages of five caches, 320 MB read and written, 6.2 us of planning and 61 of moves at 5.2 TB/s (a
 // large copy: 4.8); fork of 8 or 128 sequences 3.5 + 4 to 6 us, their release 3 to 4.
 #include "dsa_pages.h"
 #include "dsa_scan.h"
@@ -20,7 +20,7 @@ constexpr int PG_PIECE = PG_THREADS * 16 * 4;         // bytes: four 16-byte loa
 constexpr int PG_PLAN_THREADS = 1024;                 // a planning workgroup
 constexpr int PG_BLOCK = PG_PLAN_THREADS * 4;         // pages of a planning workgroup (one int4 of counts a thread)
 // Blocks up to which each planning workgroup counts all of them, a launch less (300 pages: 3.7 us for 1.6 + 3.3 in two
-// launches, 12k pages, 4 blocks, 7.7 for 2.6 + 5.0).
+// launches, 12k pages, 4 blocks, 6.2 for 2.6 + 5.0).
 constexpr int PG_OWN = 4;
 
 // One piece of page src of every cache it belongs to -> page dst (the whole workgroup).
@@ -210,39 +210,48 @@ __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_count_kernel(const int*
 // their number. counts: the live pages of each block, or null where the workgroup counts them itself (up to PG_OWN
 // blocks).
 __global__ __launch_bounds__(PG_PLAN_THREADS) void pages_plan_kernel(const int* __restrict__ ref,
-                                                                     const int* counts, int blocks,
+                                                                     const int* __restrict__ counts, int blocks,
                                                                      int* __restrict__ code, int* __restrict__ holes,
                                                                      int* __restrict__ movers, int* __restrict__ moves,
                                                                      int num_pages) {
   __shared__ int tot[PG_PLAN_THREADS / WAVE];
   __shared__ int own[PG_OWN];
   const int t = threadIdx.x, blk = blockIdx.x;
-  int total, before = 0, live = 0;
+  int total, before = 0, live = 0, front = 0;
   if (!counts) {
-    for (int b = 0; b < blocks; ++b) {
-      const int p = b * PG_BLOCK + 4 * t;
-      group_incl_scan<PG_PLAN_THREADS>(live_of(load_refs(ref, p, num_pages), p), tot, total);
-      if (t == 0) own[b] = total;
+    if (t < PG_OWN) own[t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < PG_OWN; ++b) {  // (past the pool: none)
+      const pg_v4i r = load_refs(ref, b * PG_BLOCK + 4 * t, num_pages);
+      const int n = __popcll(__ballot(r.x > 0 && b + t > 0)) + __popcll(__ballot(r.y > 0)) + __popcll(__ballot(r.z > 0)) +
+                    __popcll(__ballot(r.w > 0));
+      if ((t & (WAVE - 1)) == 0) atomicAdd(&own[b], n);
     }
     __syncthreads();
-    counts = own;
+#pragma unroll
+    for (int b = 0; b < PG_OWN; ++b) {
+      live += own[b];
+      before += b < blk ? own[b] : 0;
+    }
+#pragma unroll
+    for (int b = 0; b < PG_OWN; ++b) front += b < live / PG_BLOCK ? own[b] : 0;
+  } else {
+    for (int b0 = 0; b0 < blocks; b0 += PG_PLAN_THREADS) {
+      const int c = b0 + t < blocks ? counts[b0 + t] : 0;
+      group_incl_scan<PG_PLAN_THREADS>(c, tot, total);
+      live += total;
+      group_incl_scan<PG_PLAN_THREADS>(b0 + t < blk ? c : 0, tot, total);
+      before += total;
+    }
+    for (int b0 = 0; b0 < live / PG_BLOCK; b0 += PG_PLAN_THREADS) {
+      group_incl_scan<PG_PLAN_THREADS>(b0 + t < live / PG_BLOCK ? counts[b0 + t] : 0, tot, total);
+      front += total;
+    }
   }
-  for (int b0 = 0; b0 < blocks; b0 += PG_PLAN_THREADS) {
-    const int c = b0 + t < blocks ? counts[b0 + t] : 0;
-    group_incl_scan<PG_PLAN_THREADS>(c, tot, total);
-    live += total;
-    group_incl_scan<PG_PLAN_THREADS>(b0 + t < blk ? c : 0, tot, total);
-    before += total;
-  }
-  // live pages up to page `live`: whole blocks before its own, and its own up to it
-  const int lb = live / PG_BLOCK;
-  int front = 0;
-  for (int b0 = 0; b0 < lb; b0 += PG_PLAN_THREADS) {
-    group_incl_scan<PG_PLAN_THREADS>(b0 + t < lb ? counts[b0 + t] : 0, tot, total);
-    front += total;
-  }
+  // live pages up to page `live`: whole blocks before its own, so far, and its own up to it
   {
-    const int p = lb * PG_BLOCK + 4 * t;
+    const int p = live / PG_BLOCK * PG_BLOCK + 4 * t;
     const pg_v4i r = load_refs(ref, p, num_pages);
     const int up_to = (int)(r.x > 0 && p > 0 && p <= live) + (r.y > 0 && p + 1 <= live) + (r.z > 0 && p + 2 <= live) +
                       (r.w > 0 && p + 3 <= live);
@@ -380,7 +389,13 @@ hipError_t launch_pages_compact(const int* ref, const int* table, int* new_ref, 
                code, holes, movers, moves, num_pages);
   for (int at = 0; e == hipSuccess && (at == 0 || at < n_caches); at += PG_CACHES) {
     const PageCaches set = page_caches(caches, page_bytes, n_caches, at);
-    e = launch("pages_compact_kernel", pages_compact_kernel, dim3(8 * num_cu), dim3(PG_THREADS), s, set,
+    // Up to 64 workgroups a CU, 8 of them at a time: as they come, what is being copied stays close together (12,345
+    // pages: 8 a CU 73.5 us, 32 62.6, 64 60.8). No more than there can be moves, half the pages' (300 pages: 64 a CU
+    // would take 6.3 us for 4.7).
+    const long moved = (long)(num_pages / 2) * set.pieces;
+    const long rows = (max(table_size, (long)num_pages) + PG_THREADS - 1) / PG_THREADS;
+    const unsigned groups = (unsigned)min(max(moved, rows), 64L * num_cu);
+    e = launch("pages_compact_kernel", pages_compact_kernel, dim3(groups), dim3(PG_THREADS), s, set,
                (int)(at == 0), ref, table, code, holes, movers, moves, new_ref, new_table, remap, table_size,
                num_pages);
   }
