@@ -281,7 +281,8 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
             const uint8_t* const qr = sh.tile[1] + (32 * hh + j) * 2 * DQK;
 #pragma unroll
             for (int s = 0; s < 2 * STEPS; ++s)
-              qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ dn_q_swizzle<DQK>(j))));
+              qb[s] = as_bf16x8(*reinterpret_cast<const uint4*>(
+                  qr + 16 * ((4 * (s >> 1) + 2 * h + (s & 1)) ^ dn_q_swizzle<DQK>(j))));
           }
           lds_barrier();  // the queries are read
           float m_run = 0.0f;  // running max (base 2) of row 32 hh + j; chunk 0's scores are taken against 0, its flags are
@@ -446,14 +447,16 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
         for (int d = 0; d < 4; ++d)
 #pragma unroll
           for (int i = 0; i < RB; ++i) o[d][i] = f32x16{};
-        const int vr = 8 * h + ((lane & 15) >> 1), vf = dn_swizzle(vr), vb0 = (lane >> 4) & 1;  // (the value operand's reads)
+        // (the value operand's reads)
+        const int vr = 8 * h + ((lane & 15) >> 1), vf = dn_swizzle(vr), vb0 = (lane >> 4) & 1;
         const int vrow = vr * DN_KROW + 128 * w + 8 * (lane & 1);
         const int voff[2] = {vrow + 16 * (vb0 ^ vf), vrow + 16 * ((2 | vb0) ^ vf)};
         const uint16_t* const pr = &sh.p[0][j * DN_PROW + 8 * h];
         // the value operand of step i (tokens 16 (i / 4) .. + 15, dims 128 w + 32 (i % 4) .. + 31), read transposed
         auto v_read = [&](const uint8_t* kt, int i) __attribute__((always_inline)) {
           return __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW + 64 * ((i & 3) >> 1)));
+              (__attribute__((address_space(3))) dn_v2i*)(kt + voff[i & 1] + 16 * (i >> 2) * DN_KROW +
+                                                          64 * ((i & 3) >> 1)));
         };
         auto p_read = [&](int pb, int t, int i) __attribute__((always_inline)) {
           return as_bf16x8(*reinterpret_cast<const uint4*>(pr + pb * 64 * DN_PROW + 32 * i * DN_PROW + 16 * t));

@@ -15,8 +15,8 @@ constexpr int EX_C = 512;   // the latent width
 // H whose left side is e4m3 rows gathered through the page table (the scale is applied to the sums), and k_rope[t] =
 // sigma_t c_t[512:].
 //
-// What bounds it: the matrix units, then the stores. A share is of units (tile of 256 tokens, one
-// head's 128 keys or values), a workgroup a CU. The rows of a tile stay in registers, e4m3 until they are operands
+// What bounds it: the matrix units, then the stores. A share is of units (tile of 256 tokens, one head's 128 keys or
+// values), a workgroup a CU. The rows of a tile stay in registers, e4m3 until they are operands
 // (exact in bf16), while one part's weights after another run through LDS, 64 of the 512 columns a step, by
 // asynchronous loads 7 steps ahead that cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights
 // through LDS, and stores from registers under the next unit's products (that form with two workgroups a CU: 336 us
@@ -230,8 +230,9 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
 // s = scale (q[:128] . k + q[128:] . k_rope), p = softmax(s), out = p . v, lse, for ragged batches of queries and keys,
 // causal (the last query sees every key) or full.
 //
-// What bounds it: the matrix units, then the LDS reads that feed them and the exponentials. One workgroup a CU has 256 queries of a head, 8 waves of 32, two on each SIMD, the first of
-// them with priority, so that one's softmax runs under the other's products. A tile of 64 keys and values comes by
+// What bounds it: the matrix units, then the LDS reads that feed them and the exponentials. One workgroup a CU has 256
+// queries of a head, 8 waves of 32, two on each SIMD, the first of them with priority, so that one's softmax runs under
+// the other's products. A tile of 64 keys and values comes by
 // asynchronous loads straight into LDS two tiles ahead, with one barrier a tile. S^T = K . Q^T and O^T += V^T . P on
 // v_mfma_f32_32x32x16_bf16: a lane's scores are of one query, in the value product's operand layout as they stand (the
 // values are read transposed in the same order), so P never leaves the registers and the maxima and sums stay in their

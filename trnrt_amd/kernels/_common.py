@@ -124,8 +124,8 @@ _SCRATCH: dict = {}
 
 def scratch(device: torch.device, nbytes: int, use: str) -> torch.Tensor:
     """A uint8 device buffer of at least nbytes that a call writes before it reads: the one kept for `use` on the current
-    stream, and in a graph capture one of the graph's own memory (a graph that kept the stream's would replay into it after a
-    later call had let it go for a larger one, or beside another graph's replay)."""
+    stream, and in a graph capture one of the graph's own memory (a graph that kept the stream's would replay into it
+    after a later call had let it go for a larger one, or beside another graph's replay)."""
     n = max(int(nbytes), 256)
     if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(n, dtype=torch.uint8, device=device)
