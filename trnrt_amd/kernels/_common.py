@@ -37,8 +37,9 @@ def stream_ptr(device: torch.device) -> int:
 def call(device: torch.device, fn, *args) -> int:
     """fn(*args, stream): a C entry point on device's current stream, with device the current one (a launch goes to the
     current device, whichever the tensors are on)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return fn(*args, stream_ptr(device))
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(device):
         return fn(*args, stream_ptr(device))
 

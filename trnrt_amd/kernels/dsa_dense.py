@@ -31,10 +31,11 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     Any number of heads, any page size. workspace: dsa_dense_workspace_bytes(S, H) bytes, or None for one kept per
     stream (a captured graph has its own)."""
     dev = C.on_gpu(q, kv_cache, kv_scale, table, ctx_len, out, workspace)
-    if q.dim() not in (3, 4) or q.shape[-1] not in DQK_WIDTHS or q.shape[-2] < 1 or (q.dim() == 4 and q.shape[1] < 1):
+    rows = q.shape[:-1]  # B, (S,) H
+    if len(rows) not in (2, 3) or q.shape[-1] not in DQK_WIDTHS or min(rows[1:]) < 1:
         raise ValueError(f"dsa_dense: q {tuple(q.shape)}, expected [B, H, 576 or 512] or [B, S, H, 576 or 512]")
-    B, H, dqk = q.shape[0], q.shape[-2], q.shape[-1]
-    S = q.shape[1] if q.dim() == 4 else 1
+    B, H, dqk = rows[0], rows[-1], q.shape[-1]
+    S = rows[1] if len(rows) == 3 else 1
     q = C.aligned(C.as_bf16(q))
     if kv_cache.shape[-1] != dqk:
         raise ValueError(f"dsa_dense: cache rows of {kv_cache.shape[-1]} for q of {dqk}")
@@ -47,17 +48,15 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     tb, lens = C.as_i32(table), C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
     if tb.dim() != 2 or tb.shape[0] != B or tb.shape[1] < 1:
         raise ValueError(f"dsa_dense: page table {tuple(table.shape)} for {B} sequences")
-    shape = q.shape[:-1] + (DV,)
     if out is None:
-        out = q.new_empty(shape, dtype=out_dtype)
-    C.need(out, "out", (torch.bfloat16, torch.float32), shape)
-    ls = q.new_empty(q.shape[:-1], dtype=torch.float32) if lse else None
+        out = q.new_empty((*rows, DV), dtype=out_dtype)
+    bf = C.need(out, "out", (torch.bfloat16, torch.float32), (*rows, DV)).dtype is torch.bfloat16
+    ls = q.new_empty(rows, dtype=torch.float32) if lse else None
     lib = _lib.lib()
     if workspace is not None:
         ws = C.given(workspace, "dsa_dense")
     else:  # the partials of the row tiles that workgroups share
         ws = C.scratch(dev, int(lib.dsa_dense_workspace_bytes(S, H)), "dense")
-    bf = out.dtype == torch.bfloat16
     st = C.call(dev, lib.dsa_dense_mla, C.ptr(q), C.ptr(kv), C.ptr(kv_scale), C.ptr(tb), C.ptr(lens),
                 C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), C.ptr(ws),
                 ws.numel() * ws.element_size(), B, S, H, dqk, tb.shape[1], int(page_size), slots // page_size,
