@@ -9,13 +9,14 @@
 // above it the matrix units and the conversions beside them. One workgroup a CU has a tile of 32 or 64 rows of one
 // sequence and a range of its chunks of 64 tokens; its 8 waves have two kinds of work, one of each on every SIMD, a
 // chunk apart, with one barrier a chunk (products of one kind run under the other's conversions and exponentials):
-//   - scoring waves 0-3, interval c: chunk c's scores S^T = K . Q^T, 32 tokens x 32 rows a wave, the queries in
-//     registers, then P = 2^(s - m) x the tokens' scales in bf16 into LDS;
+//   - scoring waves 0-3, interval c: chunk c's scores S^T = K . Q^T, 32 tokens x 32 rows a wave (16 x 32 where there are
+//     32 rows), the queries in registers, then P = 2^(s - m) x the tokens' scales in bf16 into LDS;
 //   - value waves 4-7, interval c: chunk c - 1's O^T += V^T . P, 128 dims of all rows a wave, in registers; and the
 //     rows of chunk c + 1 from their registers into LDS and chunk c + 2's loads into the same registers, piece by piece
 //     between the products. (Loads straight into LDS cost their wave 150 to 200 cycles each beside the other waves' LDS
 //     reads.)
-// Both products are v_mfma_f32_32x32x16_bf16 with the e4m3 operand converted on the way (exact). The chunks of all
+// Both products are v_mfma_f32_32x32x16_bf16 (16x16x32 in the scores of 32 rows) with the e4m3 operand converted on the
+// way (exact). The chunks of all
 // sequences and row tiles form one list that the workgroups share evenly, whatever the lengths: each takes a stretch of
 // it and writes a row tile's outputs where it holds all its chunks, else a partial (the rows x 512 in fp32, their
 // maxima and sums) that dense_combine_kernel joins. Neighbouring stretches lie on one XCD, so that the row tiles of a
@@ -23,7 +24,8 @@
 //
 // Measured (the attention alone, the joining beside it): 8 x 32k tokens, 64 heads 44 + 8 us, of which the loop is 27 at
 // 5.6 TB/s of cache rows, the rest the list's search, the first loads and the partials; 13 x 4 new tokens of 128 heads
-// (2k to 12k tokens, 512 wide) 108 + 11, 920 TFLOP/s over the call; 1 x 4k tokens, 16 heads 9.7 + 4.2, latency.
+// (2k to 12k tokens, 512 wide) 106 + 11, 920 TFLOP/s over the call; 16 heads: 8 x 32k tokens 34 + 5, 1 x 4k 9.2 + 4.2,
+// latency.
 //
 // The online softmax rescales lazily without waiting for the chunk's maximum: P is taken against the running maximum as
 // it stands; a wave that meets a score past its slack raises a flag, and before the chunk's values are multiplied every
@@ -70,11 +72,13 @@ struct DnShared {
   alignas(16) uint16_t p[2][64 * DN_PROW];  // P[row][token] of two chunks (32 rows: their second terms after them)
   alignas(16) float ksc[DN_BUFS][DN_CHUNK];       // the chunks' token scales
   alignas(16) float kfac[DN_BUFS][DN_CHUNK];      // x softmax scale x log2 e
-  float cmax[2][32 * RB];                         // [token half][row]: a chunk's maxima when one moves
+  // [part][row], of the halves of a chunk's tokens (with 32 rows its quarters): a chunk's maxima when one moves, and a
+  // stretch's sums
+  float cmax[4 / RB][32 * RB];
+  float lsum[4 / RB][32 * RB];
   float al[32 * RB];                              // and its rescale factors
   alignas(16) int flag[2][4];                     // per chunk parity and wave: a score past the running maximum's slack
-  float lsum[2][32 * RB];                         // [token half][row]: a stretch's sums
-  float mfin[32 * RB];                            // and maxima (base 2)
+  float mfin[32 * RB];                            // and its maxima (base 2)
   int tot[DN_THREADS / WAVE];
   int found[4];
 };
@@ -130,6 +134,21 @@ __device__ __forceinline__ int dn_owner(int u, const DnList& x) {
 // there, as the value waves' lanes hold it.
 __device__ __forceinline__ constexpr int dn_partial(int w, int i, int d, int g, int blocks) {
   return (((w * blocks + i) * 4 + d) * 4 + g) * 4 * WAVE;
+}
+
+// Four weights into P: bf16, off by 2^-8 of each at most, as everywhere in this library (the sums take them unrounded).
+// With two TERMS what that left follows 32 rows on, bf16 again (2^-16): for a tile of 32 rows, whose bound is the cache's
+// stream.
+template <int TERMS>
+__device__ __forceinline__ void dn_store_weights(uint16_t* to, const float (&p)[4]) {
+  uint32_t w[2] = {bf16_pack(p[0], p[1]), bf16_pack(p[2], p[3])};
+  *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+  if (TERMS == 2) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      w[e] = bf16_pack(p[2 * e] - __uint_as_float(w[e] << 16), p[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
+    *reinterpret_cast<uint2*>(to + 32 * DN_PROW) = make_uint2(w[0], w[1]);
+  }
 }
 
 template <int DQK, int RB>
@@ -201,6 +220,11 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
     const int t0 = c0 * DN_CHUNK, r0 = (set * tm.span + member) * ROWS;  // its first token, and this workgroup's row
     const int part = (2 * team + (u > u0)) * tm.span + member;            // where its partials go
     if (r0 < M) {  // (else the last set has no tile for this member)
+      auto row_sum = [&](int r) __attribute__((always_inline)) {
+        float l = sh.lsum[0][r] + sh.lsum[1][r];
+        if constexpr (RB == 1) l += sh.lsum[2][r] + sh.lsum[3][r];
+        return l;
+      };
       // A whole row tile's outputs go through LDS, 256 dims at a time: dims 4 x .. + 3 of row r at place 64 x + (r ^ (x
       // & 7)), so that a row's pieces in order and a piece's rows in order both cover the banks once; a wave writes
       // whole rows.
@@ -212,7 +236,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           const int r = wave + 8 * i;
           if (r0 + r >= M) break;
           f32x4 v = area[64 * lane + (r ^ (lane & 7))];
-          const float m = sh.mfin[r], l = sh.lsum[0][r] + sh.lsum[1][r];
+          const float m = sh.mfin[r], l = row_sum(r);
           const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= inv;
@@ -236,12 +260,12 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           write(1);
         } else if (tid < ROWS && r0 + tid < M) {
           float2* const ml = reinterpret_cast<float2*>(ws_ml) + (size_t)part * ROWS + tid;
-          *ml = make_float2(sh.mfin[tid], sh.lsum[0][tid] + sh.lsum[1][tid]);
+          *ml = make_float2(sh.mfin[tid], row_sum(tid));
         }
       };
 
       if (wave < 4) {
-        // -- the scores: wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
+        // -- the scores: of 64 rows wave (th, hh) takes tokens 32 th .. + 31 of a chunk for rows 32 hh .. + 31 --
         const int th = wave >> 1, hh = wave & 1;
         const int lane = fresh_lane(), j = lane & 31, h = lane >> 5;
         // the queries through LDS, into the buffers that the first chunks leave: row r at r x 2 DQK, its 16-byte piece
@@ -259,18 +283,144 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           wait_loads<0>();
         }
         lds_barrier();  // the queries and chunk 0 are in place
-        if (hh >= RB) {  // no rows for this wave
-          lds_barrier();
-          for (int c = 0; c <= nch; ++c) {
-            if (c > 0) {
-              const int4 fl = *reinterpret_cast<const int4*>(sh.flag[(c - 1) & 1]);
-              if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
-                lds_barrier();
-                lds_barrier();
-              }
+        if constexpr (RB == 1) {
+          // of 32 rows wave w takes tokens 16 w .. + 15 of a chunk, by products of 16 x 16, so that no SIMD has more of
+          // them (8 x 32k tokens, 16 heads: 33.9 us, where two waves of 32 tokens took 38.2)
+          const int j = lane & 15, kq = lane >> 4;
+          int seen[2];  // tokens that this lane's rows 16 x + j see
+#pragma unroll
+          for (int x = 0; x < 2; ++x) seen[x] = len - S + min(r0 + 16 * x + j, M - 1) / H + 1;
+          const int seen0 = len - S + r0 / H + 1;  // and the tile's first row, the fewest
+          bf16x8 qb[2][2 * PIECES];  // rows 16 x + j: step s holds dims 64 (s / 2) + 16 kq + 8 (s % 2) .. + 7
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int s = 0; s < 2 * PIECES; ++s)
+              qb[x][s] = as_bf16x8(*reinterpret_cast<const uint4*>(
+                  sh.tile[1] + (16 * x + j) * 2 * DQK +
+                  16 * ((8 * (s >> 1) + 2 * kq + (s & 1)) ^ dn_q_swizzle<DQK>(16 * x + j))));
+          lds_barrier();  // the queries are read
+          float m_run[2] = {}, l_run[2] = {}, psum[2] = {};  // as in the other form, of each of its two rows
+          f32x4 sv[2] = {};  // the last chunk's scores - m_run: rows 16 x + j, tokens 16 w + 4 kq + r
+          const int koff = (16 * wave + j) * DN_KROW + 16 * (kq ^ dn_swizzle(16 * wave + j));
+          uint16_t* const pw = &sh.p[0][j * DN_PROW + 16 * wave + 4 * kq];
+          int buf = 0, last = 0;  // chunk c's buffer and chunk c - 1's
+          auto four = [&](const float* a) __attribute__((always_inline)) {
+            return *reinterpret_cast<const f32x4*>(a + 16 * wave + 4 * kq);
+          };
+          auto weights = [&](int c, const f32x4& ks) __attribute__((always_inline)) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              float pv[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[x][e]);
+              psum[x] += (pv[0] + pv[1]) + (pv[2] + pv[3]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) pv[e] *= ks[e];
+              dn_store_weights<2>(pw + (c & 1) * 64 * DN_PROW + 16 * x * DN_PROW, pv);
             }
+          };
+          auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
+            if (__builtin_amdgcn_readfirstlane(fl.x | fl.y | fl.z | fl.w)) {
+              float cm[2];
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+                cm[x] = max_nonan(max_nonan(sv[x][0], sv[x][1]), max_nonan(sv[x][2], sv[x][3]));
+                cm[x] = max_nonan(cm[x], __shfl_xor(cm[x], 16, WAVE));
+                cm[x] = max_nonan(cm[x], __shfl_xor(cm[x], 32, WAVE));
+                if (kq == 0) sh.cmax[wave][16 * x + j] = cm[x];
+              }
+              lds_barrier();
+#pragma unroll
+              for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) cm[x] = max_nonan(cm[x], sh.cmax[w][16 * x + j]);
+                const float up = c == 0 ? max_nonan(cm[x], -1e30f) : cm[x] > DN_SLACK ? cm[x] : 0.0f;
+                const float alpha = c == 0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+                m_run[x] += up;
+                l_run[x] *= alpha;
+                psum[x] = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sv[x][e] -= up;
+                if (wave == 0 && kq == 0) sh.al[16 * x + j] = alpha;
+              }
+              weights(c, four(sh.ksc[last]));
+              lds_barrier();
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              l_run[x] += psum[x];
+              psum[x] = 0.0f;
+            }
+          };
+          auto flags = [&](int c) __attribute__((always_inline)) {
+            return *reinterpret_cast<const int4*>(sh.flag[c & 1]);
+          };
+          __builtin_amdgcn_s_setprio(1);
+          for (int c = 0; c < nch; ++c) {
+            const uint8_t* tile = sh.tile[buf];
+            auto k_read = [&](int m) __attribute__((always_inline)) {
+              return *reinterpret_cast<const u32x4*>(tile + koff + 64 * m);
+            };
+            int4 fl = make_int4(0, 0, 0, 0);
+            if (c > 0) fl = flags(c - 1);
+            f32x4 sa[2] = {};
+            u32x4 kk[DN_KAHEAD + 1];
+            bf16x8 ka[2], kb[2];
+#pragma unroll
+            for (int m = 0; m < DN_KAHEAD; ++m) kk[m] = k_read(m);
+            __builtin_amdgcn_sched_barrier(0);
+            settle(c - 1, fl);
+            ka[0] = fp8x8_to_bf16x8(kk[0][0], kk[0][1]);
+            kb[0] = fp8x8_to_bf16x8(kk[0][2], kk[0][3]);
+#pragma unroll
+            for (int m = 0; m < PIECES; ++m) {
+              if (m + DN_KAHEAD < PIECES) kk[(m + DN_KAHEAD) % (DN_KAHEAD + 1)] = k_read(m + DN_KAHEAD);
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                sa[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka[m & 1], qb[x][2 * m], sa[x], 0, 0, 0);
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+                sa[x] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kb[m & 1], qb[x][2 * m + 1], sa[x], 0, 0, 0);
+              if (m + 1 < PIECES) {
+                const u32x4 k1 = kk[(m + 1) % (DN_KAHEAD + 1)];
+                ka[(m + 1) & 1] = fp8x8_to_bf16x8(k1[0], k1[1]);
+                kb[(m + 1) & 1] = fp8x8_to_bf16x8(k1[2], k1[3]);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+            const f32x4 kx = four(sh.kfac[buf]), ks = four(sh.ksc[buf]);
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sv[x][e] = fmaf(sa[x][e], kx[e], -m_run[x]);
+            if (t0 + (c + 1) * DN_CHUNK > seen0) {  // tokens that a row does not see
+              const int at = t0 + c * DN_CHUNK + 16 * wave + 4 * kq;
+#pragma unroll
+              for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sv[x][e] = at + e < seen[x] ? sv[x][e] : -INFINITY;
+            }
+            float cm = sv[0][0];
+#pragma unroll
+            for (int e = 1; e < 8; ++e) cm = max_nonan(cm, sv[e >> 2][e & 3]);
+            weights(c, ks);
+            const bool any = c == 0 || __ballot(cm > DN_SLACK) != 0;
+            if (lane == 0) sh.flag[c & 1][wave] = any;
+            last = buf;
+            buf = buf == BUFS - 1 ? 0 : buf + 1;
             lds_barrier();
           }
+          __builtin_amdgcn_s_setprio(0);
+          settle(nch - 1, flags(nch - 1));
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            float lw = l_run[x] + __shfl_xor(l_run[x], 16, WAVE);
+            lw += __shfl_xor(lw, 32, WAVE);
+            if (kq == 0) sh.lsum[wave][16 * x + j] = lw;
+            if (wave == 0 && kq == 0) sh.mfin[16 * x + j] = m_run[x];
+          }
+          lds_barrier();
           finish([](int) {});
         } else {
           const int row = min(r0 + 32 * hh + j, M - 1);
@@ -304,20 +454,9 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
 #pragma unroll
             for (int e = 0; e < 4; ++e) pv[e] = __builtin_amdgcn_exp2f(sv[4 * g + e]);
             psum += (pv[0] + pv[1]) + (pv[2] + pv[3]);
-            // bf16 weights, off by 2^-8 of each at most, as everywhere in this library; the sums take them unrounded. A
-            // tile of 32 rows, whose bound is the cache's stream, takes what the rounding left as a second term (2^-16)
 #pragma unroll
             for (int e = 0; e < 4; ++e) pv[e] *= ks[e];
-            uint32_t w[2] = {bf16_pack(pv[0], pv[1]), bf16_pack(pv[2], pv[3])};
-            uint16_t* const to = pw + (c & 1) * 64 * DN_PROW + 8 * g;
-            *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
-            if (RB == 1) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e)
-                w[e] = bf16_pack(pv[2 * e] - __uint_as_float(w[e] << 16),
-                                 pv[2 * e + 1] - __uint_as_float(w[e] & 0xffff0000u));
-              *reinterpret_cast<uint2*>(to + 32 * DN_PROW) = make_uint2(w[0], w[1]);
-            }
+            dn_store_weights<1>(pw + (c & 1) * 64 * DN_PROW + 8 * g, pv);
           };
           // a chunk whose flags (fl) are up: its maxima over both token halves, the moved running maxima, P again
           auto settle = [&](int c, const int4& fl) __attribute__((always_inline)) {
