@@ -16,11 +16,10 @@
 //     between the products. (Loads straight into LDS cost their wave 150 to 200 cycles each beside the other waves' LDS
 //     reads.)
 // Both products are v_mfma_f32_32x32x16_bf16 (16x16x32 in the scores of 32 rows) with the e4m3 operand converted on the
-// way (exact). The chunks of all
-// sequences and row tiles form one list that the workgroups share evenly, whatever the lengths: each takes a stretch of
-// it and writes a row tile's outputs where it holds all its chunks, else a partial (the rows x 512 in fp32, their
-// maxima and sums) that dense_combine_kernel joins. Neighbouring stretches lie on one XCD, so that the row tiles of a
-// sequence read its cache through the same L2.
+// way (exact). The chunks of all sequences and row tiles form one list that the workgroups share evenly, whatever the
+// lengths: each takes a stretch of it and writes a row tile's outputs where it holds all its chunks, else a partial
+// (the rows x 512 in fp32, their maxima and sums) that dense_combine_kernel joins. Neighbouring stretches lie on one
+// XCD, so that the row tiles of a sequence read its cache through the same L2.
 //
 // Measured (the attention alone, the joining beside it): 8 x 32k tokens, 64 heads 44 + 8 us, of which the loop is 27 at
 // 5.6 TB/s of cache rows, the rest the list's search, the first loads and the partials; 13 x 4 new tokens of 128 heads
