@@ -13,10 +13,11 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 }
 
 // 16 bytes from each lane's address into LDS at lds + 16 x lane. Nothing waits for it: s_waitcnt vmcnt before the barrier
-// that hands the data on (the loads of a wave end in order, and count with its other global accesses). (The compiler
-// sets m0 anew before any use of its own, so this need not save it.)
+// that hands the data on (the loads of a wave end in order, and count with its other global accesses). m0, the LDS
+// address, is an operand, so that the compiler knows of its value; a scalar write of it needs one wait state before the
+// load, which the compiler does not see in here and may leave no other instruction for.
 __device__ __forceinline__ void load_lds16(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
 }
 
 // At most N of the wave's global accesses are still out (loads end in order).
