@@ -277,3 +277,11 @@ def test_refusals():
             dsa_dense.attend(**{**ok, **bad})
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_dense.attend(**{**ok, "q": q.cpu()})
+
+
+@pytest.mark.parametrize("H,S,D", [(64, 11, 576), (64, 13, 512), (48, 14, 576), (96, 7, 512)])
+def test_workgroups_without_a_tile(H, S, D):
+    """Row tiles that are no multiple of a team's, shares of several units that begin in a sequence's last set and go on
+    behind sequences without tokens: some workgroups' first step is the search for the next sequence."""
+    say("dense workgroups without a tile", H, S, D)
+    check(make([130, 0, 0, 70, 0, 200] * 14, S, H, D, 64, seed=H + S), 64)

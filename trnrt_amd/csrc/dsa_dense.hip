@@ -211,6 +211,7 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
   int set = __builtin_amdgcn_readfirstlane(sh.found[1]);
   int c0 = __builtin_amdgcn_readfirstlane(sh.found[2]);
   len = __builtin_amdgcn_readfirstlane(sh.found[3]);
+  __syncthreads();  // every wave has them: a workgroup without a tile in this set goes straight to the next search
 
   for (int u = u0; u < u1;) {
     const int all = dn_chunks(len);
