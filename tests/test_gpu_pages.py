@@ -252,3 +252,25 @@ def test_captured_and_replayed():
             assert torch.equal(a.cpu(), b)
         for a, b in zip(gc, cs):
             assert torch.equal(a.cpu(), b)
+
+
+def test_fork_free_counts_below_zero():
+    """A count of 0 or less is free: the page that a child gets from it is counted once, and not given out again."""
+    say("fork, counts below zero")
+    ps = 8
+    ref = torch.tensor([0, 1, 1, -2, 0, -1, 1, -7, -(2 ** 31)], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[1, 2, 0], [6, 0, 0]], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([11, 8], dtype=torch.int32, device="cuda")  # a whole page and a part, a whole page
+    parents = torch.tensor([0, 1, 0, 0], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(2)
+    cache = torch.randint(0, 256, (9 * ps, 16), dtype=torch.uint8, generator=g)
+    got = cache.cuda()
+    child, pages = dsa_pages.fork(ref, table, lens, parents, [got], ps)
+    assert pages.tolist() == [3, 0, 4, 5] and child.tolist() == [[1, 3, 0], [6, 0, 0], [1, 4, 0], [1, 5, 0]]
+    assert ref.tolist() == [0, 4, 1, 1, 1, 1, 2, -7, -(2 ** 31)]
+    child, pages = dsa_pages.fork(ref, table, lens, parents, [got], ps)  # two free pages are left for three
+    assert pages.tolist() == [7, 0, 8, -1] and child.tolist() == [[1, 7, 0], [6, 0, 0], [1, 8, 0], [0, 0, 0]]
+    assert ref.tolist() == [0, 6, 1, 1, 1, 1, 3, 1, 1]
+    for p in (3, 4, 5, 7, 8):
+        cache[p * ps:(p + 1) * ps] = cache[2 * ps:3 * ps]
+    assert torch.equal(got.cpu(), cache)

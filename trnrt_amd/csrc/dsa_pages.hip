@@ -165,7 +165,8 @@ __global__ __launch_bounds__(PG_THREADS) void pages_fork_kernel(
       else if (c == f.full && f.part) p = page;
     }
     out[c] = p;
-    if (p) atomicAdd(ref + p, 1);
+    if (p && c == f.full) ref[p] = 1;  // (the new page is this child's alone, whatever its count was: 0 or less is free)
+    else if (p) atomicAdd(ref + p, 1);
   }
 }
 
