@@ -437,7 +437,7 @@ int dsa_pool_keys_write(const void* rows, int rows_fp8, const float* rows_scale,
  *   workspace: dsa_dense_workspace_bytes(S, H) bytes whatever B (no zero fill needed).
  * q_bf16, kv_fp8, the outputs and the workspace start at multiples of 16 bytes, as the tensors of dsa_expand_latent and
  * dsa_expanded_mla do. A token's NaN or infinity reaches every query of its sequence in the call, as 0 x NaN those too
- * that do not see the token (here and in dsa_expanded_mla).
+ * that do not see the token (here and in dsa_expanded_mla); the lse is NaN where a score that the query sees is.
  */
 size_t dsa_dense_workspace_bytes(int S, int H);
 int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_scale, const int32_t* page_table,

@@ -285,3 +285,22 @@ def test_workgroups_without_a_tile(H, S, D):
     behind sequences without tokens: some workgroups' first step is the search for the next sequence."""
     say("dense workgroups without a tile", H, S, D)
     check(make([130, 0, 0, 70, 0, 200] * 14, S, H, D, 64, seed=H + S), 64)
+
+
+@pytest.mark.parametrize("H", [8, 16, 64])
+@pytest.mark.parametrize("n", [200, 60000])
+def test_nan_reaches_the_lse(H, n):
+    """A token's NaN (in its row or its scale) shows in the lse of the queries that see it, not as the value of a query that
+    sees nothing, whether a row tile is one workgroup's or joined; the other sequences and queries have theirs."""
+    say("dense NaN", H, n)
+    q, kv, sc, table, lens = make([n, 3, 130, 0], 3, H, 576, 64, seed=H)
+    ref, lref, _, E = reference(q, kv, sc, table, lens, 64, 0.05)
+    kv[table[0, 1].long() * 64 + 5, 7] = 0x7F  # token 69 of the first sequence, which every query sees
+    sc[table[2, 2].long() * 64 + 1] = float("nan")  # the last token of the third, which only its last query sees
+    out, lse = dsa_dense.attend(*(x.cuda() for x in (q, kv, sc, table, lens)), 64, 0.05)
+    out, lse = out.double().cpu(), lse.double().cpu()
+    assert out[0].isnan().all() and lse[0].isnan().all()
+    assert out[2].isnan().all() and lse[2, 2].isnan().all()
+    for b, i in ((1, 0), (1, 1), (1, 2), (2, 0), (2, 1), (3, 0), (3, 2)):
+        assert ((lse[b, i] - lref[b, i]).abs() <= E[b, i] + 2.0 ** -21 + 2.0 ** -22 * lref[b, i].abs()).all()
+    assert not out[3].any() and (lse[3].float() == -1e30).all()

@@ -282,3 +282,27 @@ def test_store_fork_attend_compact():
     want = torch.cat([rows[1], rows[0], added[:1], rows[0], added[1:2], rows[1], added[2:]])[:, 512:]
     assert (r.float() - want).abs().max() <= 2.0 ** -4 * want.abs().max()  # e4m3's half step
     assert not torch.isnan(k).any() and not torch.isnan(v).any()
+
+
+@pytest.mark.parametrize("lq,lk,H", [([70, 3], [70, 3], 8), ([3, 2], [9000, 40], 4)])
+def test_attend_nan_reaches_the_lse(lq, lk, H):
+    """A key's NaN shows in the lse of the queries that see it, with the keys in splits or not; a value's only in the
+    outputs."""
+    say("expanded attend NaN", lq, lk, H)
+    g = torch.Generator().manual_seed(H)
+    q = torch.randn(sum(lq), H, 128, generator=g).bfloat16().cuda()
+    k, v = (torch.randn(sum(lk), H, 128, generator=g).bfloat16().cuda() for _ in range(2))
+    cu_q, cu_k = cu_of(lq).cuda(), cu_of(lk).cuda()
+    k2, v2 = k.clone(), v.clone()
+    k2[lk[0] - 2, 1, 5] = float("nan")  # the first sequence's last key but one: its last two queries see it
+    v2[lk[0] + 1, 0, 9] = float("nan")  # a value of the second sequence
+    want, lwant = dsa_expand.attend(q, k, None, v, cu_q, cu_k, 0.1)
+    out, lse = dsa_expand.attend(q, k2, None, v2, cu_q, cu_k, 0.1)
+    n = lq[0]
+    assert lse[n - 2:n, 1].isnan().all() and out[n - 2:n, 1].isnan().all()
+    rest = torch.ones_like(lse, dtype=torch.bool)
+    rest[n - 2:n, 1] = False
+    assert torch.equal(lse[rest], lwant[rest])
+    heads = [h for h in range(H) if h != 1]
+    assert torch.equal(out[:n, heads], want[:n, heads])
+    assert out[-1, 0, 9].isnan() and torch.equal(out[n:, 1:], want[n:, 1:])

@@ -73,6 +73,10 @@ __device__ __forceinline__ float lse_base2(float m, float l) {
   return m > NEG_INF ? fmaf(m, 0.69314718055994531f, __logf(l)) : NEG_INF + __logf(l);
 }
 
+// The same and the outputs' factor 1 / l where the sum may be of nothing (0): NEG_INF and 0. (A sum that is NaN stays NaN.)
+__device__ __forceinline__ float lse_or_none(float m, float l) { return l == 0.0f ? NEG_INF : lse_base2(m, l); }
+__device__ __forceinline__ float inverse_or_0(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 // The pooled decode step's pool-key write, folded into the pooled layer's launch (dsa_pooled_decode_step): the
 // indexer rows cache [slots][rows_width] (e4m3 with a per-slot fp32 scale, or bf16: rows_fp8 0), the pool-position
 // bias [kpool][128] fp32 and each row's written token's cache slot.

@@ -237,14 +237,14 @@ __global__ __launch_bounds__(DN_THREADS, 1) void dense_mla_kernel(
           if (r0 + r >= M) break;
           f32x4 v = area[64 * lane + (r ^ (lane & 7))];
           const float m = sh.mfin[r], l = row_sum(r);
-          const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a row that sees nothing: 0)
+          const float inv = inverse_or_0(l);  // (a row that sees nothing: 0)
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[e] *= inv;
           const size_t at = (size_t)b * M + r0 + r;
           if (out)
             *reinterpret_cast<uint2*>(out + at * DN_DV + dim) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
           if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + at * DN_DV + dim) = v;
-          if (lse_out && half == 0 && lane == 0) lse_out[at] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+          if (lse_out && half == 0 && lane == 0) lse_out[at] = lse_or_none(m, l);
         }
       };
       // The end of a stretch in every wave, after the barrier behind which the tiles are free and the sums in LDS; the
@@ -838,7 +838,7 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
   }
   const size_t out_row = (size_t)b * M + row;
   if constexpr (WPR == 1) {
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float inv = inverse_or_0(l);
     uint2 pk[4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -861,7 +861,7 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
 #pragma unroll
       for (int g = 0; g < 4; ++g)
         *reinterpret_cast<f32x4*>(out_f32 + out_row * DN_DV + 128 * w + 32 * d + 8 * g + 4 * h) = a[g];
-    if (lse_out && w == 0 && d == 0 && h == 0) lse_out[out_row] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+    if (lse_out && w == 0 && d == 0 && h == 0) lse_out[out_row] = lse_or_none(m, l);
     return;
   }
   if (h == 0) {
@@ -885,12 +885,12 @@ __global__ __launch_bounds__(DC_THREADS) void dense_combine_kernel(
     for (int e = 0; e < 4; ++e) o[e] = fmaf(f, v[e], o[e]);
   }
   const size_t to = out_row * DN_DV + 128 * w + 32 * d + 8 * (g0 + wave) + 4 * h;
-  const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+  const float inv = inverse_or_0(ll);
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
   if (out) *reinterpret_cast<uint2*>(out + to) = make_uint2(bf16_pack(o[0], o[1]), bf16_pack(o[2], o[3]));
   if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + to) = o;
-  if (lse_out && w == 0 && d == 0 && g0 + wave == 0 && h == 0) lse_out[out_row] = ll > 0.0f ? lse_base2(mm, ll) : NEG_INF;
+  if (lse_out && w == 0 && d == 0 && g0 + wave == 0 && h == 0) lse_out[out_row] = lse_or_none(mm, ll);
 }
 
 // Workgroups: one a CU, a multiple of the 8 XCDs.

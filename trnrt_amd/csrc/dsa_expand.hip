@@ -487,11 +487,11 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     if (h == 0) ml[j] = make_float2(l > 0.0f ? m_run : -1e30f, l);
     return;
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a query that sees nothing: 0)
+  const float inv = inverse_or_0(l);  // (a query that sees nothing: 0)
   const int rows = min(32, nq - w0);
   if (rows <= 0) return;
   if (lse_out && h == 0 && j < rows)
-    lse_out[(size_t)(qb + w0 + j) * H + head] = l > 0.0f ? lse_base2(m_run, l) : NEG_INF;
+    lse_out[(size_t)(qb + w0 + j) * H + head] = lse_or_none(m_run, l);
   const size_t at = ((size_t)(qb + w0) * H + head) * EX_D;
   if (out) {  // through LDS (8 KiB a wave): 256 bytes a row, piece p of row r at p ^ (r & 15), then whole rows
     uint8_t* const st = sh.k[0] + 8192 * wave;
@@ -602,7 +602,7 @@ __global__ __launch_bounds__(XA_THREADS) void expanded_combine_kernel(
         for (int e = 0; e < 4; ++e) a[g][e] = fmaf(c, v[s][g][e], a[g][e]);
     }
   }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;  // (a query that sees nothing: 0)
+  const float inv = inverse_or_0(l);  // (a query that sees nothing: 0)
   const size_t row = (size_t)(xa_first(b, cu_q, Tq) + i) * H + head;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
@@ -611,7 +611,7 @@ __global__ __launch_bounds__(XA_THREADS) void expanded_combine_kernel(
     if (out) *reinterpret_cast<uint2*>(out + to) = make_uint2(bf16_pack(v[0], v[1]), bf16_pack(v[2], v[3]));
     if (out_f32) *reinterpret_cast<f32x4*>(out_f32 + to) = v;
   }
-  if (lse_out && d == 0 && h == 0) lse_out[row] = l > 0.0f ? lse_base2(m, l) : NEG_INF;
+  if (lse_out && d == 0 && h == 0) lse_out[row] = lse_or_none(m, l);
 }
 
 // In how many splits a tile's keys are taken: as many as leave the CUs a workgroup each where every sequence has
