@@ -304,3 +304,27 @@ def test_nan_reaches_the_lse(H, n):
     for b, i in ((1, 0), (1, 1), (1, 2), (2, 0), (2, 1), (3, 0), (3, 2)):
         assert ((lse[b, i] - lref[b, i]).abs() <= E[b, i] + 2.0 ** -21 + 2.0 ** -22 * lref[b, i].abs()).all()
     assert not out[3].any() and (lse[3].float() == -1e30).all()
+
+
+def test_two_threads_on_one_stream():
+    """Calls of two host threads on one stream, whose launches come between each other's: each joins its own partials."""
+    say("dense, two threads")
+    import threading
+
+    ins = [tuple(x.cuda() for x in make([5000 + 900 * i, 400], 1, 16, 576, 64, seed=40 + i)) for i in range(2)]
+    want = [dsa_dense.attend(*x, 64, 0.05) for x in ins]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        for _ in range(200):
+            got[i].append(dsa_dense.attend(*ins[i], 64, 0.05))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 200 and all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i])

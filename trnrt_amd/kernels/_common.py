@@ -3,6 +3,8 @@ dtypes and layouts the C ABI expects, and the current HIP stream."""
 
 from __future__ import annotations
 
+import threading
+
 import torch
 
 FP8 = torch.float8_e4m3fn  # OCP e4m3fn: gfx950's FP8 and the reference's CPU cache dtype (model_runner.py:54-70)
@@ -103,16 +105,20 @@ def fp8_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
     return t
 
 
-# Zero-filled workspaces kept per (device, stream, use) and reused by the functional surfaces when the caller passes
-# none: every call leaves the regions that must start at zero at zero again, so one zero fill serves every later call
-# on the same stream (calls on one stream never overlap; each stream has its own). A call needing more grows it: a
-# new zero-filled buffer on the same stream (the old one returns to torch's stream-ordered allocator).
+# Zero-filled workspaces kept per (device, stream, use, host thread) and reused by the functional surfaces when the caller
+# passes none: every call leaves the regions that must start at zero at zero again, so one zero fill serves every later
+# call of the thread on the same stream (its calls on one stream never overlap; each stream has its own, and each thread,
+# since a call of several launches lets another thread's in between). A call needing more grows it: a new zero-filled
+# buffer on the same stream (the old one returns to torch's stream-ordered allocator). They outlive their threads, as a
+# graph may have recorded one.
 _WORKSPACES: dict = {}
 
 
 def cached_workspace(device: torch.device, nbytes: int, use: str) -> torch.Tensor:
-    """A zero-filled uint8 device buffer of at least nbytes for `use` on the current stream of `device`."""
-    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device), use)
+    """A zero-filled uint8 device buffer of at least nbytes for `use` on the current stream of `device`, this host
+    thread's."""
+    key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device), use,
+           threading.get_ident())
     ws = _WORKSPACES.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = zeroed_workspace(max(int(nbytes), 256), device)
@@ -120,20 +126,26 @@ def cached_workspace(device: torch.device, nbytes: int, use: str) -> torch.Tenso
     return ws
 
 
-_SCRATCH: dict = {}
+class _Scratch(threading.local):  # (a thread's own buffers, let go with it)
+    def __init__(self):
+        self.kept: dict = {}
+
+
+_SCRATCH = _Scratch()
 
 
 def scratch(device: torch.device, nbytes: int, use: str) -> torch.Tensor:
-    """A uint8 device buffer of at least nbytes that a call writes before it reads: the one kept for `use` on the current
-    stream, and in a graph capture one of the graph's own memory (a graph that kept the stream's would replay into it
-    after a later call had let it go for a larger one, or beside another graph's replay)."""
+    """A uint8 device buffer of at least nbytes that a call writes before it reads: the one that this host thread keeps for
+    `use` on the current stream (another thread's launches may come between those of a call), and in a graph capture one
+    of the graph's own memory (a graph that kept the stream's would replay into it after a later call had let it go for a
+    larger one, or beside another graph's replay)."""
     n = max(int(nbytes), 256)
     if torch._C._cuda_isCurrentStreamCapturing():
         return torch.empty(n, dtype=torch.uint8, device=device)
     key = (device.index if device.index is not None else torch.cuda.current_device(), stream_ptr(device), use)
-    ws = _SCRATCH.get(key)
+    ws = _SCRATCH.kept.get(key)
     if ws is None or ws.numel() < n:
-        ws = _SCRATCH[key] = torch.empty(n, dtype=torch.uint8, device=device)
+        ws = _SCRATCH.kept[key] = torch.empty(n, dtype=torch.uint8, device=device)
     return ws
 
 

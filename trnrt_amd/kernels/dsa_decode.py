@@ -68,7 +68,8 @@ def _run(q: torch.Tensor, kv: torch.Tensor, kv_scale: torch.Tensor | None, scale
     ls = (torch.zeros if n_live is not None else torch.empty)(B, H, dtype=torch.float32, device=dev) if lse else None
     wsb = _lib.workspace_bytes(_lib.DSA_WS_ATTENTION, B, H, keep, 0, splits)
     if workspace is None and wsb:
-        # the split partials (written before they are read: no zero fill), kept per stream
+        # the split partials (written before they are read: no zero fill), kept per stream and
+        # host thread
         workspace = C.cached_workspace(dev, wsb, "attention")
     ws_len = 0 if workspace is None else workspace.numel() * workspace.element_size()
     o_bf = out if out.dtype == torch.bfloat16 else None
@@ -111,7 +112,8 @@ def attend(q_lat: torch.Tensor, kc: torch.Tensor, rows: torch.Tensor, bias: torc
     for kp > 1 it may be the reference's pool view [N / kp, kp D]), kc_scale [N] fp32 its per-token scales or None
     for the reference's unscaled cache (scale 1), rows [B, NS] int each slot's row, bias [B, NS] or [B, NS, kp] fp32
     (0 / NEG_INF): with kp > 1 a slot is a pool of kp consecutive tokens. With lse also lse [B, H] fp32. workspace:
-    the split partials (dsa_workspace_bytes(DSA_WS_ATTENTION, ...)), or None for one kept per stream."""
+    the split partials (dsa_workspace_bytes(DSA_WS_ATTENTION, ...)), or None for one kept per stream
+    and host thread."""
     rows, bias = pool_token_rows(rows, bias)
     return _run(q_lat, kc, kc_scale, scale, rows=rows, bias=bias, lse=lse, splits=splits, workspace=workspace)
 

@@ -29,7 +29,7 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, kv_scale: torch.Tensor | Non
     512] bf16; q [B, H, D] is one new token a sequence, its outputs [B, H, 512] and [B, H]. kv_cache [slots, D] e4m3fn (or
     its bits) with kv_scale [slots] fp32, or None for the unscaled cache; table [B, max_pages] int32, ctx_len [B] int32.
     Any number of heads, any page size. workspace: dsa_dense_workspace_bytes(S, H) bytes, or None for one kept per
-    stream (a captured graph has its own)."""
+    stream and host thread (a captured graph has its own)."""
     dev = C.on_gpu(q, kv_cache, kv_scale, table, ctx_len, out, workspace)
     rows = q.shape[:-1]  # B, (S,) H
     if len(rows) not in (2, 3) or q.shape[-1] not in DQK_WIDTHS or min(rows[1:]) < 1:

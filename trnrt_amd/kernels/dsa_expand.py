@@ -80,8 +80,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     [Tk, H, 128] bf16; cu_q, cu_k [B + 1] int32 on the device: sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1,
     its keys rows cu_k[b] .. . causal: query i of nq sees the first nk - nq + i + 1 of the nk keys (the last sees all);
     otherwise every key. A query that sees no key has o = 0 and lse NEG_INF; rows of q in no sequence are not written.
-    workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream (a captured graph
-    has its own)."""
+    workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
+    captured graph has its own)."""
     dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
     dq = DH if k_rope is None else DH + ROPE
     if q.dim() != 3 or q.shape[1] < 1 or q.shape[2] != dq:

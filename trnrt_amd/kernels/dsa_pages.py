@@ -69,8 +69,8 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     [n, max_pages] int32, pages [n] int32). The parent's full pages are shared (ref, in place, rises by one), a partial
     last page is copied into the lowest free page of every cache; pages[i] is that page, 0 where there is no partial page,
     -1 where the pool had none left or parents[i] is no row (the child's table row is then 0 and counts nothing).
-    workspace: dsa_pages_workspace_bytes(num_pages, n) bytes, or None for one kept per stream
-    (a captured graph has its own)."""
+    workspace: dsa_pages_workspace_bytes(num_pages, n) bytes, or None for one kept per stream and host
+    thread (a captured graph has its own)."""
     caches = list(caches)
     dev = C.on_gpu(ref, table, ctx_len, parents, workspace, *caches)
     _ref(ref, "dsa_pages.fork")
@@ -116,8 +116,7 @@ def compact(ref: torch.Tensor, table: torch.Tensor, caches, page_size: int, *,
     counts in the new places and each page's new place [num_pages] (0: a free page), all int32. Pages already up to L
     stay; the k-th one past L goes to the k-th free page. ref and table are not changed, the caches are, in place (pages
     past L keep their bytes). Table entries of free pages become 0. workspace: dsa_pages_workspace_bytes(num_pages, 0)
-    bytes, or None for one kept per stream
-    (a captured graph has its own)."""
+    bytes, or None for one kept per stream and host thread (a captured graph has its own)."""
     caches = list(caches)
     dev = C.on_gpu(ref, table, workspace, *caches)
     _ref(ref, "dsa_pages.compact")

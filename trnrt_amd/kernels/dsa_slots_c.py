@@ -38,7 +38,7 @@ def attend(q_lat: torch.Tensor, kc: torch.Tensor, rows: torch.Tensor, bias: torc
     with kc_scale [slots] fp32 its per-token scales, or None for the reference's unscaled cache) with bias
     [N, NS, kp] or [N, NS] fp32 (0 / NEG_INF). workspace: dsa_slots_compact_workspace_bytes(N, H, NS, kp, splits)
     bytes (no zero fill needed; with less the attention takes fewer splits, down to the split form's need), or None for
-    one kept per stream."""
+    one kept per stream and host thread."""
     dev = C.on_gpu(q_lat, kc, rows, bias, kc_scale, workspace)
     if q_lat.dim() != 3 or q_lat.shape[2] not in DQK_WIDTHS:
         raise ValueError(f"dsa_slots_c: q_lat {tuple(q_lat.shape)}, expected [N, H, 576 or 512]")

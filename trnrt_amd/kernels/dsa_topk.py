@@ -34,7 +34,8 @@ def select_indices(scores: torch.Tensor, keep: int, lengths: torch.Tensor | None
     """(idx int32 [R, keep] ascending selected positions, 0 past the count; cnt int32 [R]) of scores [R, P] fp32.
     lengths [R] int32: positions at or past a row's length are not selectable (None: all P); max_len an upper bound
     of the lengths (default P). workspace: the caller's (dsa_workspace_bytes(DSA_WS_TOPK, R, 0, keep, max_len),
-    zero-filled before its first use; calls leave it so), or None for one kept per stream."""
+    zero-filled before its first use; calls leave it so), or None for one kept per stream and host
+    thread."""
     dev = C.on_gpu(scores, lengths, idx, cnt, workspace)
     if scores.dim() != 2:
         raise ValueError(f"dsa_topk: scores {tuple(scores.shape)}, expected [rows, P]")

@@ -61,7 +61,8 @@ def select_device(sc: torch.Tensor, keep: int, lengths: torch.Tensor | None = No
                   workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The exact selection of scores [N, P] (non-candidates at or below VISIBLE) as (indices [N, keep] int64
     ascending, 0 past the count; count [N] int64). lengths [N] int32 optionally bounds each row's candidates.
-    workspace: the caller's top-k workspace (dsa_topk.select_indices), or None for one kept per stream."""
+    workspace: the caller's top-k workspace (dsa_topk.select_indices), or None for one kept per stream
+    and host thread."""
     idx, cnt = dsa_topk.select_indices(sc, keep, lengths=lengths, vis_only=True, workspace=workspace)
     return idx.to(torch.int64), cnt.to(torch.int64)
 
