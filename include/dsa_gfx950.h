@@ -506,6 +506,7 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
  * page_table in the new places (an entry of a free page becomes 0), remap int32 [num_pages] each page's new place (0: a
  * free page), for whatever else holds page ids. The outputs must not be the inputs; pages past L keep their bytes.
  *
+ * A fork's pool has up to 0x7fff0000 pages, a compaction's up to 0x1fffffff (DSA_EUNSUPPORTED past them).
  * workspace: dsa_pages_workspace_bytes(num_pages, n) (n: the children of a fork; no zero fill needed).
  */
 size_t dsa_pages_workspace_bytes(int num_pages, int n);

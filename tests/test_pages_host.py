@@ -81,3 +81,11 @@ def test_host_tensors_and_shapes_raise():
         dsa_pages._caches([torch.zeros(64, 8)], 0, 4, "x")
     with pytest.raises(ValueError, match="ref"):
         dsa_pages._ref(torch.zeros(2, 2, dtype=torch.int32), "x")
+
+
+def test_fork_refuses_pools_at_the_end_of_32_bits():
+    """The search for free pages goes in steps of 4,096: past 2^31 - 4,096 pages its index would turn negative."""
+    lib = _lib.lib()
+    c, s, k = _set()
+    for pages in (0x7fff0001, 0x7fffffff):
+        assert lib.dsa_pages_fork(P, P, P, P, P, P, c, s, k, P, 1 << 20, 2, 7, 4, 64, pages, None) == _lib.DSA_EUNSUPPORTED
