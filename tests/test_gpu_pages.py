@@ -274,3 +274,18 @@ def test_fork_free_counts_below_zero():
     for p in (3, 4, 5, 7, 8):
         cache[p * ps:(p + 1) * ps] = cache[2 * ps:3 * ps]
     assert torch.equal(got.cpu(), cache)
+
+
+def test_fork_of_an_empty_table():
+    """No rows: no children, or children whose parents are no rows."""
+    say("fork of an empty table")
+    ref = torch.tensor([0, 1, 0, 2], dtype=torch.int32, device="cuda")
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    table, cache = torch.zeros(0, 3, dtype=torch.int32, device="cuda"), torch.ones(32, 4, device="cuda")
+    child, pages = dsa_pages.fork(ref, table, none, none, [cache], 8)
+    assert child.shape == (0, 3) and pages.shape == (0,)
+    child, pages = dsa_pages.fork(ref, table, none, torch.tensor([0, -1], dtype=torch.int32, device="cuda"), [cache], 8)
+    assert pages.tolist() == [-1, -1] and child.tolist() == [[0, 0, 0]] * 2
+    assert ref.tolist() == [0, 1, 0, 2] and (cache == 1).all()
+    with pytest.raises(ValueError):
+        dsa_pages.fork(ref, table[:, :0], none, none, [cache], 8)

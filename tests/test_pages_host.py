@@ -89,3 +89,12 @@ def test_fork_refuses_pools_at_the_end_of_32_bits():
     c, s, k = _set()
     for pages in (0x7fff0001, 0x7fffffff):
         assert lib.dsa_pages_fork(P, P, P, P, P, P, c, s, k, P, 1 << 20, 2, 7, 4, 64, pages, None) == _lib.DSA_EUNSUPPORTED
+
+
+def test_fork_of_an_empty_table():
+    """A table without rows has no parent: nothing of it is read, so it may be null."""
+    lib = _lib.lib()
+    c, s, k = _set()
+    assert lib.dsa_pages_fork(P, P, P, P, P, P, c, s, k, None, 0, 0, 7, 4, 64, 100, None) == _lib.DSA_EWORKSPACE
+    assert lib.dsa_pages_fork(P, None, None, P, P, P, c, s, k, None, 0, 0, 7, 4, 64, 100, None) == _lib.DSA_EWORKSPACE
+    assert lib.dsa_pages_fork(P, None, None, P, P, P, c, s, k, P, 1 << 20, 1, 7, 4, 64, 100, None) == _lib.DSA_EINVAL

@@ -1394,7 +1394,7 @@ int dsa_pages_fork(int32_t* ref, const int32_t* page_table, const int32_t* ctx_l
   if (B < 0 || n < 0 || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
   const int st = page_caches_status(caches, page_bytes, n_caches, n);
   if (st != DSA_OK || n == 0) return st;
-  if (!ref || !page_table || !ctx_len || !parents || !child_table || !pages) return DSA_EINVAL;
+  if (!ref || (B > 0 && (!page_table || !ctx_len)) || !parents || !child_table || !pages) return DSA_EINVAL;
   if (num_pages > 0x7fff0000) return DSA_EUNSUPPORTED;  // (the search for free pages steps past the pool's end)
   if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::pages_fork_bytes(n)) return DSA_EWORKSPACE;
   return status(dsa::launch_pages_fork(ref, page_table, ctx_len, parents, child_table, pages, caches, page_bytes,

@@ -75,7 +75,7 @@ def fork(ref: torch.Tensor, table: torch.Tensor, ctx_len: torch.Tensor, parents:
     dev = C.on_gpu(ref, table, ctx_len, parents, workspace, *caches)
     _ref(ref, "dsa_pages.fork")
     ptrs, size, n_caches, num_pages = _caches(caches, page_size, ref.numel(), "dsa_pages.fork")
-    if table.dim() != 2 or table.numel() == 0:
+    if table.dim() != 2 or table.shape[1] < 1:
         raise ValueError(f"dsa_pages.fork: table {tuple(table.shape)}, expected [B, max_pages]")
     B, max_pages = table.shape
     if parents.dim() != 1:
