@@ -289,3 +289,16 @@ def test_fork_of_an_empty_table():
     assert ref.tolist() == [0, 1, 0, 2] and (cache == 1).all()
     with pytest.raises(ValueError):
         dsa_pages.fork(ref, table[:, :0], none, none, [cache], 8)
+
+
+@pytest.mark.parametrize("pages,live", [(16384, 8200), (16385, 8192), (16385, 16384), (20481, 4095), (20481, 4096), (20481, 4097),
+                                        (20481, 12288), (40000, 3), (40000, 20000), (40000, 24576), (40000, 39998)])
+def test_compact_large_pools(pages, live):
+    """Pools up to and past the 16,384 pages for which each planning workgroup counts all of them, with the live pages' number
+    on and beside multiples of a workgroup's 4,096."""
+    say("compact a large pool", pages, live)
+    g = torch.Generator().manual_seed(pages + live)
+    ref = torch.zeros(pages, dtype=torch.int32)
+    ref[torch.randperm(pages - 1, generator=g)[:live] + 1] = torch.randint(1, 5, (live,), generator=g).to(torch.int32)
+    table = torch.randint(0, pages, (5, 300), generator=g).to(torch.int32)
+    check_compact(ref, table, make_caches(pages * 2, [8, 4], g), 2)
