@@ -306,3 +306,28 @@ def test_attend_nan_reaches_the_lse(lq, lk, H):
     heads = [h for h in range(H) if h != 1]
     assert torch.equal(out[:n, heads], want[:n, heads])
     assert out[-1, 0, 9].isnan() and torch.equal(out[n:, 1:], want[n:, 1:])
+
+
+@pytest.mark.parametrize("lens,H,D", [
+    ([1021], 16, 576), ([1022], 16, 576),  # the last batch whose 128-token tiles run at once, and one row past it
+    ([700, 1, 0, 1500, 797], 16, 576), ([4095], 16, 512), ([4097 - 3], 16, 576), ([4097], 16, 512),
+    ([12000], 3, 576), ([9000, 0, 20000, 1, 999], 5, 512), ([257] * 40, 7, 576), ([2], 160, 576)])
+def test_expand_shares(lens, H, D):
+    """Tiles of 256 tokens, and workgroups with several units: weights that run on from part to part, stores under the next
+    unit's products, shares that begin and end inside a tile and go on into the next, tiles that end early."""
+    say("expand shares", len(lens), sum(lens), H, D)
+    test_expand(lens, H, D, 64, True)
+
+
+def test_expand_shares_plan():
+    """Which form and how many units a workgroup those take (as launch_expand_latent has it, 256 CUs): both forms, shares of
+    one unit and of several, some of them beginning inside a tile."""
+    seen = set()
+    for lens, H in (([1021], 16), ([1022], 16), ([12000], 3), ([9000, 0, 20000, 1, 999], 5), ([2], 160)):
+        total = sum(lens) + 3
+        tok = 128 if -(-total // 128) * 2 * H <= 256 else 256
+        units = -(-total // tok) * 2 * H
+        grid = min(units, 256)
+        starts = [units * g // grid for g in range(grid + 1)]
+        seen.add((tok, units > grid, any(u % (2 * H) and u // (2 * H) != (v - 1) // (2 * H) for u, v in zip(starts, starts[1:]))))
+    assert {(128, False, False), (256, False, False), (256, True, True)} <= seen
