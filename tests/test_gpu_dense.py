@@ -328,3 +328,59 @@ def test_two_threads_on_one_stream():
     torch.cuda.synchronize()
     for i in range(2):
         assert len(got[i]) == 200 and all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i])
+
+
+def exact_scores(lens, S, H, D, seed, step):
+    """Inputs whose scores are exact in fp32 in any order (values in halves and scales in powers of two), and with `step` higher
+    by 69 of base 2 from token 128 on, past what the running maximum lets pass."""
+    q, kv, sc, table, lens = make(lens, S, H, D, 64, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    live = sc == sc
+    x = torch.tensor([-1.0, -0.5, 0.0, 0.5, 1.0, 1.5])[torch.randint(0, 6, kv.shape, generator=g)]
+    for b, n in enumerate(lens.tolist()):
+        t = torch.arange(n)
+        slot = table[b][t // 64].long() * 64 + t % 64
+        x[slot, 0] = torch.where(t >= 128, 96.0, 0.0) if step else 0.0
+    kv = torch.where(live[:, None], x.to(FP8).view(torch.uint8), kv)
+    sc = torch.where(live, torch.exp2(torch.randint(-1, 2, sc.shape, generator=g).float()) if not step else torch.ones_like(sc), sc)
+    q = (torch.randint(-8, 9, q.shape, generator=g) / 8).to(torch.bfloat16)
+    q[..., 0] = 8.0
+    return q, kv, sc, table, lens
+
+
+@pytest.mark.parametrize("step", [False, True])
+@pytest.mark.parametrize("H,S,D,lens", [(16, 1, 576, [200, 1, 64, 300]), (32, 1, 512, [130, 300]), (8, 3, 576, [65, 280]),
+                                        (16, 2, 512, [300] * 200), (16, 1, 576, [300, 290, 0] * 80)])
+def test_two_terms_of_the_weights(H, S, D, lens, step):
+    """Up to 32 rows a softmax weight is two bf16 terms, off by 2^-8 of 2^-8 of it. With exact scores s (base 2, at most M in size)
+    the exponent's error is that of the factor's, the difference's and the maximum's roundings, 4 M 2^-24 at most, the
+    exponential's 2^-23 of its value; the sums of n tokens in two terms are off by less than 3 n 2^-24 of A. One term alone
+    would not pass."""
+    say("dense two terms", H, S, D, len(lens), step)
+    scale = 1 / 16
+    q, kv, sc, table, lens = exact_scores(lens, S, H, D, 3, step)
+    out = dsa_dense.attend(q.cuda(), kv.cuda(), sc.cuda(), table.cuda(), lens.cuda(), 64, scale, lse=False,
+                           out_dtype=torch.float32).double()
+    one_term = 0
+    for b, n in enumerate(lens.tolist()):
+        t = torch.arange(n)
+        slot = table[b][t // 64].long() * 64 + t % 64
+        K = (kv[slot].view(FP8).double() * sc[slot].double()[:, None]).cuda()
+        sigma = sc[slot].double().cuda()
+        for i in range(S):
+            m = n - S + i + 1
+            if m <= 0:
+                assert not out[b, i].any()
+                continue
+            s = q[b, i].double().cuda() @ K[:m].T.contiguous() * scale
+            p = torch.softmax(s, -1)
+            V = K[:m, :512].contiguous()
+            ref, A = p @ V, p @ V.abs()
+            M = float(s.abs().max()) * 1.4426950408889634
+            tol = A * (2.0 ** -16 + 2 * (4 * M * 2.0 ** -24 * 0.6931471805599453 + 2.0 ** -23) + 3 * n * 2.0 ** -24) + 1e-30
+            err = (out[b, i] - ref).abs()
+            assert (err <= tol).all(), f"sequence {b}: the worst {float((err / tol).max())} of the tolerance"
+            w = torch.exp(s - s.amax(-1, keepdim=True)) * sigma[:m]  # the oracle with one bf16 term
+            planted = (w.float().bfloat16().double() / sigma[:m] / torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)) @ V
+            one_term += int(((planted - ref).abs() > tol).sum())
+    assert one_term > 0
