@@ -435,6 +435,9 @@ int dsa_pool_keys_write(const void* rows, int rows_fp8, const float* rows_scale,
  *   ctx_len int32 [B] (clamped to [0, max_pages * page_size]); out_bf16 [B, S, H, 512] and / or out_f32 (either may be
  *   null), lse fp32 [B, S, H] or null. Only slots of tokens t < ctx_len[b] are read.
  *   workspace: dsa_dense_workspace_bytes(S, H) bytes whatever B (no zero fill needed).
+ * Products are of bf16 operands with fp32 sums. p[t], times its token's scale, is one of them, whatever the outputs' type:
+ * rounded to bf16 (off by 2^-8 of it at most, so an output by 2^-8 of sum_t p[t] |V[t]|) where S * H > 32, in two bf16 terms
+ * (2^-16) where S * H <= 32. The sum that the weights are divided by and the lse take them unrounded.
  * q_bf16, kv_fp8, the outputs and the workspace start at multiples of 16 bytes, as the tensors of dsa_expand_latent and
  * dsa_expanded_mla do. A token's NaN or infinity reaches every query of its sequence in the call, as 0 x NaN those too
  * that do not see the token (here and in dsa_expanded_mla); the lse is NaN where a score that the query sees is.
@@ -459,10 +462,11 @@ int dsa_dense_mla(const void* q_bf16, const uint8_t* kv_fp8, const float* kv_sca
  *   nor any from `total` on.
  *
  * dsa_expanded_mla: ragged attention over them. Sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1 of q, its keys
- * and values rows cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1] each, clamped to [0, Tq] and [0, Tk]); query i of nq sees keys
- * t < nk (causal = 0) or t < nk - nq + i + 1 (causal):
+ * and values rows cu_k[b] .. cu_k[b + 1] - 1 (int32 [B + 1] each, ascending, clamped to [0, Tq] and [0, Tk]); query i of nq
+ * sees keys t < nk (causal = 0) or t < nk - nq + i + 1 (causal):
  *   s[t] = scale * (q[i, h, :128] . k[t, h, :] + q[i, h, 128:] . rope[t, :]), p = softmax_t(s), out[i, h, :] = sum_t p[t]
- *   v[t, h, :], lse = log sum_t exp(s[t]); a query that sees no key: out 0, lse NEG_INF (-1e30).
+ *   v[t, h, :], lse = log sum_t exp(s[t]); a query that sees no key: out 0, lse NEG_INF (-1e30). p[t] is rounded to bf16
+ *   for its product, whatever the outputs' type (off by 2^-8 of it at most); its sum and the lse take it unrounded.
  *   q bf16 [Tq, H, 192] with rope bf16 [Tk, 64], or [Tq, H, 128] with rope null; k, v bf16 [Tk, H, 128]; out_bf16 and / or
  *   out_f32 [Tq, H, 128], lse fp32 [Tq, H] or null. Rows of q outside every sequence have no output written.
  *   workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes on the same device, for the partials of few queries over

@@ -5,7 +5,10 @@ What it computes, per sequence b, new token i < S and head h, over the tokens t 
 the S new tokens, whose rows are in the cache):
     s[t] = scale q[b, i, h] . K[t],  p = softmax(s),  o[b, i, h] = sum_t p[t] V[t],  lse = log sum_t exp(s[t])
 with K[t] the cached FP8 latent row times its per-token scale, 576 wide (512 latent + 64 rope) or 512 (NoPE), and V[t] its
-first 512 columns: dsa_decode.attend_tokens with every token selected. A query that sees no token has o = 0 and lse NEG_INF.
+first 512 columns: dsa_decode.attend_tokens with every token selected. A query that sees no token has o = 0 and lse NEG_INF;
+one that sees a NaN score has lse NaN. The weights p times the tokens' scales are bf16 in their product with the rows,
+whatever out_dtype: off by 2^-8 of each at most where S * H > 32, and by 2^-16, in two bf16 terms, where S * H <= 32. Sums,
+maxima and the lse are fp32.
 
 The HIP kernel (csrc/dsa_dense.hip) shares the chunks of all sequences evenly among the GPU's workgroups, whatever the
 lengths, so nothing about them is needed on the host.

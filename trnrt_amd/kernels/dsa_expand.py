@@ -7,7 +7,9 @@ from the cached latent rows, and ragged causal attention over them.
 Per pair of tokens and head this costs 192 + 128 multiply-adds where the absorbed form (dsa_dense.attend) costs 576 + 512,
 so it is the form for many queries a sequence; for one or a few, whose time is the cache's stream, it is dsa_dense.attend.
 The two are the same attention: with w = [W_UK; W_UV] of each head, attend(q) equals dsa_dense.attend of the absorbed
-queries (q_nope W_UK, q_rope) times W_UV^T, to rounding. The HIP kernels are in csrc/dsa_expand.hip.
+queries (q_nope W_UK, q_rope) times W_UV^T, to rounding. The softmax weights are bf16 in their product with the values,
+whatever out_dtype (off by 2^-8 of each at most); sums, maxima and the lse are fp32. A query that sees a NaN score has lse
+NaN. The HIP kernels are in csrc/dsa_expand.hip.
 """
 
 from __future__ import annotations
