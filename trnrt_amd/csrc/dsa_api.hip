@@ -1280,10 +1280,6 @@ static int pooled_layer(const void* q_idx_bf16, const float* w, const void* pool
 
 // -- latent attention without a selection ---------------------------------------------------------------------------
 
-extern "C" {
-
-}  // extern "C"
-
 // Whether every pointer may be accessed 16 bytes at a time (null ones too).
 template <typename... P>
 static bool aligned16(const P*... p) {

@@ -940,12 +940,12 @@ hipError_t launch_dense_mla(const uint16_t* q, const uint8_t* kv, const float* k
   const hipError_t e = launch("dense_mla_kernel", kernel, dim3(G), dim3(DN_THREADS), s, q, kv, kvs, table, ctx_len,
                               out, out_f32, lse, ws_o, ws_ml, B, S, H, max_pages, pg, num_pages, scale, tm);
   if (e != hipSuccess) return e;
-  // partials of a row tile: about the teams to each of the sequences' sets, and one; a wave a block where its first
-  // four are most of them Waves of 32 rows x 32 dims with a partial after another where there are 3 such blocks a CU;
-  // workgroups whose 8 waves share a block's partials where there are fewer, of a quarter of the dims where they would
-  // fill only a quarter of the CUs. Measured, us in turn with quarters, shared, one wave: 1 x 4k tokens, 16 heads (16
-  // blocks) 4.0, 5.5, 21; 1 x 128k, 128 heads (64) 8.0, 9.5, 45; 8 x 32k, 64 heads (256) 9.6, 8.1, 14.6; 16 x 32k (512)
-  // 14.7, 8.7, 10.0; 30 x 4k (960) 27, 12.2, 9.3; 4 x 4 new tokens after 1k, 128 heads (1,024) 22, 10.4, 7.8.
+  // How a block of 32 rows x 32 dims is joined, by how many there are: from 3 blocks a CU on by one wave, a partial after
+  // another (4 in flight); fewer by a workgroup, whose 8 waves share its partials; and where there are no more than a
+  // quarter of the CUs, each quarter of its dims by a workgroup. Measured, us in turn with quarters, shared, one wave:
+  // 1 x 4k tokens, 16 heads (16 blocks) 4.0, 5.5, 21; 1 x 128k, 128 heads (64) 8.0, 9.5, 45; 8 x 32k, 64 heads (256) 9.6,
+  // 8.1, 14.6; 16 x 32k (512) 14.7, 8.7, 10.0; 30 x 4k (960) 27, 12.2, 9.3; 4 x 4 new tokens after 1k, 128 heads (1,024)
+  // 22, 10.4, 7.8.
   const long blocks = (long)B * tm.tiles * (tm.rows / 2);
   const bool one = tm.rows == 32;
   auto join = [&](auto kernel, long groups) {
