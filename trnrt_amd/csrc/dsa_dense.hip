@@ -23,7 +23,7 @@
 //
 // Measured (the attention alone, the joining beside it): 8 x 32k tokens, 64 heads 44 + 8 us, of which the loop is 27 at
 // 5.6 TB/s of cache rows, the rest the list's search, the first loads and the partials; 13 x 4 new tokens of 128 heads
-// (2k to 12k tokens, 512 wide) 106 + 11, 920 TFLOP/s over the call; 16 heads: 8 x 32k tokens 34 + 5, 1 x 4k 9.2 + 4.2,
+// (2k to 12k tokens, 512 wide) 106 + 11, 920 TFLOP/s over the call; 16 heads: 8 x 32k tokens 34 + 5, 1 x 4k 9.6 + 4.8,
 // latency.
 //
 // The online softmax rescales lazily without waiting for the chunk's maximum: P is taken against the running maximum as

@@ -20,8 +20,9 @@ constexpr int EX_C = 512;   // the latent width
 // (exact in bf16), while one part's weights after another run through LDS, 64 of the 512 columns a step, by
 // asynchronous loads 7 steps ahead that cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights
 // through LDS, and stores from registers under the next unit's products (that form with two workgroups a CU: 336 us
-// where this takes 256). The shares of one XCD are 8 tiles' and run through the same weights together, out of its L2.
-// 16,384 tokens x 64 heads: 256 us, 1.07 PFLOP/s; 8,192 tokens, whose outputs the last-level cache holds: 112 us, 1.23.
+// where this took 256 on the same card). The shares of one XCD are 8 tiles' and run through the same weights together, out of its L2.
+// 16,384 tokens x 64 heads: 257 to 273 us from card to card, 1.01 to 1.07 PFLOP/s; 8,192 tokens, whose outputs the
+// last-level cache holds: 112 us, 1.23.
 constexpr int EL_THREADS = 512;
 constexpr int EL_TOK = 256;  // (or half of it)
 constexpr int EL_K = 64;
@@ -239,7 +240,9 @@ __global__ __launch_bounds__(EL_THREADS, 1) void expand_latent_kernel(
 // lanes. The longest tiles of a causal batch go first. Where there are few query tiles, their keys are taken in splits
 // that expanded_combine_kernel joins.
 //
-// 8,192 tokens, 64 heads, causal: 1,255 us, 1.10 PFLOP/s (a large library product: 1.29).
+// 8,192 tokens, 64 heads, causal: 1,208 to 1,250 us from card to card, 1.10 to 1.14 PFLOP/s (a large library product:
+// 1.29). A grid of one round lasts as long as its longest tile: 4,096 causal tokens of 16 heads, a workgroup a CU, 119 us
+// where an even share of the tiles' keys would be half of that.
 constexpr int XA_THREADS = 512;
 constexpr int XA_Q = 256;
 constexpr int XA_K = 64;
@@ -326,8 +329,8 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   const int qi = min(w0 + j, nq - 1), seen_j = seen(qi);
 
   // Waves 0 to 3, the ones with priority, bring the tiles, once they are through with theirs: the loads' issue would
-  // delay the others, for whom they wait anyway (8k tokens, 64 heads: 1,194 us; all waves before their tile 1,235,
-  // after it 1,207). Key and value rows 16 wave .. + 15 in fours, rope rows in eights.
+  // delay the others, for whom they wait anyway (8k tokens, 64 heads, on one card: 1,194 us; all waves before
+  // their tile 1,235, after it 1,207). Key and value rows 16 wave .. + 15 in fours, rope rows in eights.
   const bool brings = wave < 4;
   const size_t head_off = (size_t)kb * H * EX_D + (size_t)head * EX_D;
   const uint16_t* const k_base = k + head_off;
