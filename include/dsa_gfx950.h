@@ -499,8 +499,9 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
  * ctx_len int32 [B] tokens, clamped to the table): the parent's floor(len / page_size) full pages are shared (their
  * counts rise by one), a partial last page is copied into the lowest free page (whose count becomes one), and
  * child_table [n, max_pages] gets the row (0 past its pages). pages int32 [n]: the child's new page, 0 where it needs
- * none, -1 where there was none left, or parents[i] is no row: such a child's row is 0 and counts nothing. The pages of
- * the parents' rows must be counted in ref, and no output may overlap an input.
+ * none, -1 where there was none left, or parents[i] is no row: such a child's row is 0 and counts nothing (B = 0: every
+ * one's, and page_table and ctx_len may be null). The pages of the parents' rows must be counted in ref, and no output may
+ * overlap an input.
  *
  * dsa_pages_release: every row i < n of page_table gives up its ceil(ctx_len[i] / page_size) pages: their counts fall by
  * one, never below 0 (a row given twice is released twice).

@@ -20,9 +20,9 @@ constexpr int EX_C = 512;   // the latent width
 // (exact in bf16), while one part's weights after another run through LDS, 64 of the 512 columns a step, by
 // asynchronous loads 7 steps ahead that cross the parts: a unit reads 128 KiB instead of the 256 of rows and weights
 // through LDS, and stores from registers under the next unit's products (that form with two workgroups a CU: 336 us
-// where this took 256 on the same card). The shares of one XCD are 8 tiles' and run through the same weights together, out of its L2.
-// 16,384 tokens x 64 heads: 257 to 273 us from card to card, 1.01 to 1.07 PFLOP/s; 8,192 tokens, whose outputs the
-// last-level cache holds: 112 us, 1.23.
+// where this took 256 on the same card). The shares of one XCD are 8 tiles' and run through the same weights together,
+// out of its L2. 16,384 tokens x 64 heads: 257 to 273 us from card to card, 1.01 to 1.07 PFLOP/s; 8,192 tokens, whose
+// outputs the last-level cache holds: 112 us, 1.23.
 constexpr int EL_THREADS = 512;
 constexpr int EL_TOK = 256;  // (or half of it)
 constexpr int EL_K = 64;
