@@ -384,3 +384,44 @@ def test_two_terms_of_the_weights(H, S, D, lens, step):
             planted = (w.float().bfloat16().double() / sigma[:m] / torch.exp(s - s.amax(-1, keepdim=True)).sum(-1, keepdim=True)) @ V
             one_term += int(((planted - ref).abs() > tol).sum())
     assert one_term > 0
+
+
+@pytest.mark.parametrize("H,S,D,lens", [(64, 1, 576, [1, 2, 0, 5, 64, 33] * 4), (128, 1, 512, [3, 1, 17]), (40, 2, 576, [64, 1, 9]),
+                                        (128, 4, 576, [1, 6, 50]), (64, 1, 576, [300, 64, 1000, 129])])
+@pytest.mark.parametrize("gain", [0.25, 1.0])
+def test_the_heaviest_weight_is_exact(H, S, D, lens, gain):
+    """Past 32 rows a softmax weight times its token's scale is one bf16 term, off by 2^-8 of it; in a stretch of one chunk the
+    token with the largest score plus its scale's log2 without the whole part has a power of two there, which is off by
+    nothing. With exact products in the scores s (base 2, at most M in size; values in halves, any scales), the exponent's error
+    is 4 M 2^-24 at most, with the logarithm's 2^-21, the exponential's 2^-23; sums of n tokens are off by n 2^-24 of A."""
+    say("dense heaviest weight", H, S, D, lens, gain)
+    q, kv, sc, table, lens_t = exact_scores(lens, S, H, D, 5, False)
+    g = torch.Generator().manual_seed(6)
+    sc = torch.where(sc == sc, torch.exp2(torch.rand(sc.shape, generator=g) - 7), sc)
+    q = (q.float() * gain * 64).to(torch.bfloat16)  # (an exact factor)
+    scale = 1 / 32
+    out = dsa_dense.attend(q.cuda(), kv.cuda(), sc.cuda(), table.cuda(), lens_t.cuda(), 64, scale, lse=False,
+                           out_dtype=torch.float32).double()
+    for b, n in enumerate(lens):
+        t = torch.arange(n)
+        slot = table[b][t // 64].long() * 64 + t % 64
+        sigma = sc[slot].double().cuda()
+        K = kv[slot].view(FP8).double().cuda() * sigma[:, None]
+        frac = torch.log2(sigma) - torch.log2(sigma).round()
+        for i in range(S):
+            m = n - S + i + 1
+            if m <= 0:
+                assert not out[b, i].any()
+                continue
+            s = q[b, i].double().cuda() @ K[:m].T.contiguous() * scale
+            p = torch.softmax(s, -1)
+            V = K[:m, :512].contiguous()
+            ref, A = p @ V, p @ V.abs()
+            rest = p.clone()
+            key = s * 1.4426950408889634 + frac[:m]
+            for c0 in range(0, m, 64):
+                rest[:, c0:c0 + 64].scatter_(1, key[:, c0:c0 + 64].argmax(-1, keepdim=True), 0.0)
+            M = float(s.abs().max()) * 1.4426950408889634
+            tol = 2.0 ** -8 * (rest @ V.abs()) + A * (2 * (4 * M * 2.0 ** -24 + 2.0 ** -21) + (n + 8) * 2.0 ** -24) + 1e-30
+            err = (out[b, i] - ref).abs()
+            assert (err <= tol).all(), f"sequence {b}: the worst {float((err / tol).max())} of the tolerance"
