@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define DSA_ABI_VERSION 11
+#define DSA_ABI_VERSION 12
 
 #define DSA_OK 0
 #define DSA_EINVAL (-1)      /* a null pointer or a size out of range */
@@ -480,6 +480,88 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
                      const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse,
                      void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal, float scale,
                      void* stream);
+
+/*
+ * dsa_expanded_mla with more asked of the scores (the rest, the workspace among it, as there). Query i of a sequence stands
+ * at place p = nk - nq + i among its nk keys; first, last int32 [Tq] (either may be null: 0 and nk), slopes fp32 [H] or
+ * null, softcap >= 0 (0: none):
+ *   z[t] = scale * (q . k[t]),  z = softcap * tanh(z / softcap),  z -= slopes[h] * |p - t|,
+ *   over the keys first[i] <= t < last[i] of the query's sequence, and t <= p where causal != 0.
+ * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
+ * document's start; a window: first = p - window + 1. Only the tiles of 64 keys that some query of a workgroup's 256 sees
+ * are read. DSA_EINVAL for a softcap that is negative, infinite or NaN.
+ */
+int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
+                           const int32_t* cu_q, const int32_t* cu_k, const int32_t* first, const int32_t* last,
+                           const float* slopes, float softcap, void* out_bf16, float* out_f32, float* lse,
+                           void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal,
+                           float scale, void* stream);
+
+/*
+ * Rotary positions of one or several axes (time, height, width; the reference's rope is host-built tables of one). Pair i
+ * < R of each row turns by the angle positions[axes[i]][t] * inv_freq[i], taken in 64 bits:
+ *   (y0, y1) = factor * (x0 cos - x1 sin, x1 cos + x0 sin)   (inverse != 0: by the negative angle)
+ * with (x0, x1) columns (2i, 2i + 1) (interleaved != 0) or (i, i + R).
+ *   x, out [T, H, 2R] bf16 (x_fp32 = 0) or fp32, rows x_row and heads x_head values apart (out likewise; out may be x);
+ *   positions int32 [n_axes, T]; inv_freq fp32 [R]; axes: a host array of R axes < n_axes, or null with one axis.
+ *   R <= 256, n_axes <= 4, H <= 65,536, T <= 4,194,304 (DSA_EUNSUPPORTED past them).
+ */
+int dsa_rope_rotate(const void* x, int x_fp32, long long x_row, long long x_head, const int32_t* positions,
+                    const float* inv_freq, const uint8_t* axes, void* out, long long out_row, long long out_head, int T,
+                    int H, int R, int n_axes, int interleaved, float factor, int inverse, void* stream);
+
+/*
+ * Appends to the paged caches: T new tokens of B sequences, each token's n_kinds <= 4 rows (its latent row, its indexer
+ * key) normed, rotated, quantised and written in one launch, all in fp32 and rounded once. Sequence b's new tokens are rows
+ * cu_new[b] .. cu_new[b + 1] - 1 of every x (int32 [B + 1], ascending; null: T / B each), the last of its ctx_len[b] tokens
+ * (int32 [B], the new ones counted): token j of n has place ctx_len[b] - n + j, slot page_table[b][place / page_size] *
+ * page_size + place % page_size. A token whose place is outside the table, or whose page is not in 1 .. num_pages - 1, is
+ * not written, nor are rows in no sequence; two tokens of one slot leave one of them. For each kind:
+ *   x [T, width] bf16 or fp32, rows x_row values apart; width a multiple of 8 up to 1,024;
+ *   norm_weight [norm_width] (null: none; bf16 or fp32 as norm_fp32 says; norm_width a multiple of 8): of the first
+ *     norm_width columns x / sqrt(mean x^2 + eps) * weight, or with norm_bias (x - mean) / sqrt(var + eps) * weight + bias;
+ *   rope_at (-1: none): columns rope_at .. rope_at + 2R - 1 rotated as dsa_rope_rotate does, by positions int32 [n_axes,
+ *     T], or by the token's place where positions is null; rope_at a multiple of 8, R of 4;
+ *   cache [num_pages * page_size, width] e4m3fn, with scale fp32 per slot: s = max(absmax(row), 1e-30) / 448, e4m3fn(clamp(
+ *     row / s, +-fp8_max)), scale[slot] = s; with scale null e4m3fn(clamp(row, +-fp8_max)) (dsa_cache_write's rounding);
+ *     or bf16 (cache_bf16 = 1, scale null).
+ * x, the norm's vectors, the caches and x's rows start at multiples of 16 bytes.
+ */
+typedef struct {
+  const void* x;
+  long long x_row;
+  const void* norm_weight;
+  const void* norm_bias;
+  void* cache;
+  float* scale;
+  int32_t x_fp32, width, rope_at, interleaved, norm_fp32, norm_width, cache_bf16;
+  float eps, fp8_max;
+} dsa_append_rows;
+int dsa_cache_append(const dsa_append_rows* rows, int n_kinds, const int32_t* page_table, const int32_t* ctx_len,
+                     const int32_t* cu_new, const int32_t* positions, const float* inv_freq, const uint8_t* axes, int T,
+                     int B, int R, int n_axes, float factor, int max_pages, int page_size, int num_pages, void* stream);
+
+/*
+ * Verification of drafted tokens against the target's logits from given random numbers (the reference samples on the host,
+ * trnrt/engine). Sequence b's rows are cu[b] .. cu[b + 1] - 1 (int32 [B + 1], ascending, clamped to [0, N]); every row but
+ * its last has a drafted token draft[row], drawn from the draft's distribution probs[row] (null: certain, q = 1 at the
+ * drafted token). With p = softmax(logits[row] / temperature[b]):
+ *   a draft x is taken iff u[row] * q(x) < p(x), up to the first that is not (an id outside [0, V) never is);
+ *   the next token comes from that row: the first i with sum_{k <= i} r(k) > v[b] * sum r, r = max(p - q, 0); from the last
+ *   row, and where r is 0 everywhere, r = p. temperature <= 0 (or NaN): a draft is taken iff it is the first of the row's
+ *   largest logits, which is also the next token.
+ * tokens int32 [N]: the drafts taken, then the next token, then -1; accepted int32 [B]: the drafts taken (0 for a sequence
+ * without rows); logp fp32 [N]: log p of tokens[row] (at temperature 1 for one <= 0), 0 for -1. Rows in no sequence are not
+ * written. A NaN logit is -infinity; among logits of +infinity the largest are equal and the rest impossible; a row with
+ * none above -infinity takes no draft, and gives -1. u, v in [0, 1) and probs >= 0 are the caller's part.
+ *   logits [N, V] bf16 or fp32, rows logits_row values apart, probs likewise; u fp32 [N], v and temperature fp32 [B].
+ * p, the sums and the comparisons are in 64 bits. workspace: dsa_verify_workspace_bytes(N, V, B) (no zero fill needed).
+ */
+size_t dsa_verify_workspace_bytes(int N, int V, int B);
+int dsa_verify(const void* logits, int logits_fp32, long long logits_row, const int32_t* draft, const void* probs,
+               int probs_fp32, long long probs_row, const int32_t* cu, const float* u, const float* v,
+               const float* temperature, int32_t* tokens, int32_t* accepted, float* logp, void* workspace,
+               size_t workspace_bytes, int N, int V, int B, void* stream);
 
 /*
  * Pages of the paged caches (no counterpart among the reference's kernels: its page pool and prefix caches are host

@@ -13,7 +13,7 @@ opened first would pull in ROCm's copy and the later torch import a second one, 
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_longlong, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libdsa_gfx950.so"
@@ -30,9 +30,19 @@ DSA_WS_TOPK = 1
 DSA_WS_ATTENTION = 2
 DSA_WS_LAYER = 3
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 P = c_void_p
+
+
+class AppendRows(ctypes.Structure):
+    """dsa_append_rows."""
+
+    _fields_ = [("x", P), ("x_row", c_longlong), ("norm_weight", P), ("norm_bias", P), ("cache", P), ("scale", P),
+                ("x_fp32", c_int), ("width", c_int), ("rope_at", c_int), ("interleaved", c_int), ("norm_fp32", c_int),
+                ("norm_width", c_int), ("cache_bf16", c_int), ("eps", c_float), ("fp8_max", c_float)]
+
+
 # Every entry point of include/dsa_gfx950.h with its ctypes signature (restype, argtypes).
 SIGNATURES: dict[str, tuple] = {
     "dsa_abi_version": (c_int, []),
@@ -115,6 +125,14 @@ SIGNATURES: dict[str, tuple] = {
     "dsa_expand_latent": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "dsa_expanded_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "dsa_expanded_mla": (c_int, [P, P, P, P, P, P, P, P, P, P, c_size_t, c_int, c_int, c_int, c_int, c_int, c_float, P]),
+    "dsa_expanded_mla_spans": (c_int, [P, P, P, P, P, P, P, P, P, c_float, P, P, P, P, c_size_t, c_int, c_int, c_int, c_int,
+                                       c_int, c_float, P]),
+    "dsa_rope_rotate": (c_int, [P, c_int, c_longlong, c_longlong, P, P, P, P, c_longlong, c_longlong, c_int, c_int, c_int,
+                                c_int, c_int, c_float, c_int, P]),
+    "dsa_cache_append": (c_int, [P, c_int, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_int, P]),
+    "dsa_verify_workspace_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "dsa_verify": (c_int, [P, c_int, c_longlong, P, P, c_int, c_longlong, P, P, P, P, P, P, P, P, c_size_t, c_int, c_int,
+                           c_int, P]),
     "dsa_pages_workspace_bytes": (c_size_t, [c_int, c_int]),
     "dsa_pages_copy": (c_int, [P, P, c_int, P, P, c_int, c_int, P]),
     "dsa_pages_fork": (c_int, [P, P, P, P, P, P, P, P, c_int, P, c_size_t, c_int, c_int, c_int, c_int, c_int, P]),

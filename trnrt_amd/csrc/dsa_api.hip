@@ -3,9 +3,12 @@
 // back to the caller's by events). Nothing here allocates device memory or synchronises the host.
 #include "../../include/dsa_gfx950.h"
 
+#include <cmath>
 #include <mutex>
 
+#include "dsa_append.h"
 #include "dsa_common.h"
+#include "dsa_expand.h"
 
 namespace dsa {
 hipError_t launch_indexer_decode(const uint16_t* q, const float* w, const uint8_t* k, const float* ks,
@@ -125,8 +128,18 @@ hipError_t launch_expand_latent(const uint8_t* kv, const float* kvs, const int* 
 bool expanded_grid_ok(int B, int Tq, int H);
 hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
                                   const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, void* ws,
-                                  int B, int Tq, int Tk, int H, int causal, float scale, int num_cu, hipStream_t s);
+                                  int B, int Tq, int Tk, int H, int causal, float scale, const ExpandedMore* more,
+                                  int num_cu, hipStream_t s);
 size_t expanded_workspace_bytes(int B, int Tq, int Tk, int H, int num_cu);
+hipError_t launch_rope_rotate(const void* x, int fp32, long x_row, long x_head, void* out, long out_row, long out_head,
+                              const RopeAngles& a, int n_tokens, int H, int half, int num_cu, hipStream_t s);
+hipError_t launch_cache_append(const AppendSet& set, const RopeAngles& a, const int* table, const int* ctx_len,
+                               const int* cu, int T, int B, int max_pages, int page_size, int num_pages, hipStream_t s);
+bool verify_grid_ok(int N, int V);
+size_t verify_workspace_bytes(int N, int V, int B);
+hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* draft, const void* probs, int q_fp32,
+                         long q_row, const int* cu, const float* u, const float* v, const float* temperature, int* tokens,
+                         int* accepted, float* logp, void* ws, int N, int V, int B, hipStream_t s);
 size_t pages_fork_bytes(int n);
 size_t pages_compact_bytes(int num_pages);
 bool pages_units_ok(const long long* page_bytes, int n_caches, long n);
@@ -1286,6 +1299,26 @@ static bool aligned16(const P*... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ...) & 15) == 0;
 }
 
+// Both forms of the expanded attention (more null: causal or full alone).
+static int expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
+                        const int32_t* cu_q, const int32_t* cu_k, const dsa::ExpandedMore* more, void* out_bf16,
+                        float* out_f32, float* lse, void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H,
+                        int causal, float scale, void* stream) {
+  if (B < 0 || Tq < 0 || Tk < 0 || H < 1) return DSA_EINVAL;
+  if (!dsa::expanded_grid_ok(B, Tq, H)) return DSA_EUNSUPPORTED;
+  if (B == 0 || Tq == 0) return DSA_OK;
+  // (no keys: k, v and rope_bf16 may be null, and every query sees nothing)
+  if (!q_bf16 || !cu_q || !cu_k || (!out_bf16 && !out_f32) || (Tk > 0 && (!k_bf16 || !v_bf16))) return DSA_EINVAL;
+  if (!aligned16(q_bf16, k_bf16, rope_bf16, v_bf16, out_bf16, out_f32)) return DSA_EINVAL;
+  const size_t need = dsa::expanded_workspace_bytes(B, Tq, Tk, H, num_cu());
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return DSA_EWORKSPACE;
+  return status(dsa::launch_expanded_attend(
+      static_cast<const uint16_t*>(q_bf16), static_cast<const uint16_t*>(k_bf16),
+      static_cast<const uint16_t*>(rope_bf16), static_cast<const uint16_t*>(v_bf16), cu_q, cu_k,
+      static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, Tq, Tk, H, causal != 0, scale, more, num_cu(),
+      static_cast<hipStream_t>(stream)));
+}
+
 extern "C" {
 
 size_t dsa_dense_workspace_bytes(int S, int H) {
@@ -1338,19 +1371,114 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
                      const int32_t* cu_q, const int32_t* cu_k, void* out_bf16, float* out_f32, float* lse,
                      void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal, float scale,
                      void* stream) {
-  if (B < 0 || Tq < 0 || Tk < 0 || H < 1) return DSA_EINVAL;
-  if (!dsa::expanded_grid_ok(B, Tq, H)) return DSA_EUNSUPPORTED;
-  if (B == 0 || Tq == 0) return DSA_OK;
-  // (no keys: k, v and rope_bf16 may be null, and every query sees nothing)
-  if (!q_bf16 || !cu_q || !cu_k || (!out_bf16 && !out_f32) || (Tk > 0 && (!k_bf16 || !v_bf16))) return DSA_EINVAL;
-  if (!aligned16(q_bf16, k_bf16, rope_bf16, v_bf16, out_bf16, out_f32)) return DSA_EINVAL;
-  const size_t need = dsa::expanded_workspace_bytes(B, Tq, Tk, H, num_cu());
-  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return DSA_EWORKSPACE;
-  return status(dsa::launch_expanded_attend(
-      static_cast<const uint16_t*>(q_bf16), static_cast<const uint16_t*>(k_bf16),
-      static_cast<const uint16_t*>(rope_bf16), static_cast<const uint16_t*>(v_bf16), cu_q, cu_k,
-      static_cast<uint16_t*>(out_bf16), out_f32, lse, workspace, B, Tq, Tk, H, causal != 0, scale, num_cu(),
-      static_cast<hipStream_t>(stream)));
+  return expanded_mla(q_bf16, k_bf16, rope_bf16, v_bf16, cu_q, cu_k, nullptr, out_bf16, out_f32, lse, workspace,
+                      workspace_bytes, B, Tq, Tk, H, causal, scale, stream);
+}
+
+int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
+                           const int32_t* cu_q, const int32_t* cu_k, const int32_t* first, const int32_t* last,
+                           const float* slopes, float softcap, void* out_bf16, float* out_f32, float* lse,
+                           void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal,
+                           float scale, void* stream) {
+  if (!(softcap >= 0.0f) || !std::isfinite(softcap)) return DSA_EINVAL;
+  const dsa::ExpandedMore more{first, last, slopes, softcap};
+  return expanded_mla(q_bf16, k_bf16, rope_bf16, v_bf16, cu_q, cu_k, &more, out_bf16, out_f32, lse, workspace,
+                      workspace_bytes, B, Tq, Tk, H, causal, scale, stream);
+}
+
+}  // extern "C"
+
+// -- rotary positions, appends, drafts -----------------------------------------------------------------------------
+
+// The angles' arguments; DSA_OK where they can be taken. (axes: a host array of the R frequencies' axes, or null)
+static int rope_angles(dsa::RopeAngles& a, const int32_t* positions, const float* inv_freq, const uint8_t* axes, int R,
+                       int n_axes, float factor, int inverse) {
+  if (R < 1 || n_axes < 1 || !inv_freq) return DSA_EINVAL;
+  if (R > dsa::RP_MAX_R || n_axes > dsa::RP_MAX_AXES) return DSA_EUNSUPPORTED;
+  if (!axes && n_axes > 1) return DSA_EINVAL;
+  a = dsa::RopeAngles{positions, inv_freq, R, n_axes, factor, inverse ? -1.0f : 1.0f, {}};
+  for (int i = 0; axes && i < R; ++i) {
+    if (axes[i] >= n_axes) return DSA_EINVAL;
+    a.axis[i / 16] |= (uint32_t)axes[i] << (2 * (i % 16));
+  }
+  return DSA_OK;
+}
+
+extern "C" {
+
+int dsa_rope_rotate(const void* x, int x_fp32, long long x_row, long long x_head, const int32_t* positions,
+                    const float* inv_freq, const uint8_t* axes, void* out, long long out_row, long long out_head, int T,
+                    int H, int R, int n_axes, int interleaved, float factor, int inverse, void* stream) {
+  if (T < 0 || H < 1) return DSA_EINVAL;
+  dsa::RopeAngles a;
+  const int st = rope_angles(a, positions, inv_freq, axes, R, n_axes, factor, inverse);
+  if (st != DSA_OK) return st;
+  if (T > 1 << 22 || H > 1 << 16) return DSA_EUNSUPPORTED;
+  if (T == 0) return DSA_OK;
+  if (!x || !out || !positions) return DSA_EINVAL;
+  return status(dsa::launch_rope_rotate(x, x_fp32 != 0, x_row, x_head, out, out_row, out_head, a, T, H, !interleaved,
+                                        num_cu(), static_cast<hipStream_t>(stream)));
+}
+
+int dsa_cache_append(const dsa_append_rows* rows, int n_kinds, const int32_t* page_table, const int32_t* ctx_len,
+                     const int32_t* cu_new, const int32_t* positions, const float* inv_freq, const uint8_t* axes, int T,
+                     int B, int R, int n_axes, float factor, int max_pages, int page_size, int num_pages, void* stream) {
+  if (T < 0 || B < 0 || n_kinds < 1 || !rows || max_pages < 1 || page_size < 1 || num_pages < 1) return DSA_EINVAL;
+  if (n_kinds > dsa::AP_KINDS || (long)T * n_kinds > 1 << 24) return DSA_EUNSUPPORTED;
+  if (!cu_new && T > 0 && (B == 0 || T % B != 0)) return DSA_EINVAL;
+  dsa::AppendSet set{};
+  dsa::RopeAngles a{};
+  set.n = n_kinds;
+  bool rope = false;
+  for (int i = 0; i < n_kinds; ++i) {
+    const dsa_append_rows& r = rows[i];
+    if ((!r.x && T > 0) || !r.cache || r.x_row < r.width || r.width < 1) return DSA_EINVAL;
+    if (r.width % 8 || r.width > dsa::AP_MAX_WIDTH) return DSA_EUNSUPPORTED;
+    const size_t row_bytes = (size_t)r.x_row * (r.x_fp32 ? 4 : 2);
+    if (!aligned16(r.x, r.norm_weight, r.norm_bias) || row_bytes % 16 || reinterpret_cast<uintptr_t>(r.cache) % 16)
+      return DSA_EINVAL;
+    if (r.norm_weight ? r.norm_width < 1 || r.norm_width > r.width || !(r.eps >= 0.0f) : r.norm_bias != nullptr)
+      return DSA_EINVAL;
+    if (r.norm_weight && r.norm_width % 8) return DSA_EUNSUPPORTED;
+    if (r.rope_at >= 0) {
+      if (R < 1 || (long)r.rope_at + 2L * R > r.width) return DSA_EINVAL;
+      if (r.rope_at % 8 || R % 4) return DSA_EUNSUPPORTED;
+      rope = true;
+    }
+    if (r.cache_bf16 ? r.scale != nullptr : !(r.fp8_max > 0.0f && r.fp8_max <= 448.0f)) return DSA_EINVAL;
+    set.rows[i] = dsa::AppendRows{r.x, (long)r.x_row, r.x_fp32 != 0, r.width, r.rope_at, !r.interleaved, r.norm_weight,
+                                  r.norm_bias, r.norm_fp32 != 0, r.norm_width, r.eps, r.fp8_max, r.cache,
+                                  r.cache_bf16 != 0, r.scale};
+  }
+  if (rope) {
+    const int st = rope_angles(a, positions, inv_freq, axes, R, positions ? n_axes : 1, factor, 0);
+    if (st != DSA_OK) return st;
+  }
+  if (T == 0 || B == 0) return DSA_OK;
+  if (!page_table || !ctx_len) return DSA_EINVAL;
+  return status(dsa::launch_cache_append(set, a, page_table, ctx_len, cu_new, T, B, max_pages, page_size, num_pages,
+                                         static_cast<hipStream_t>(stream)));
+}
+
+size_t dsa_verify_workspace_bytes(int N, int V, int B) {
+  if (N < 0 || V < 1 || B < 0) return 0;
+  return align256(dsa::verify_workspace_bytes(N, V, B));
+}
+
+int dsa_verify(const void* logits, int logits_fp32, long long logits_row, const int32_t* draft, const void* probs,
+               int probs_fp32, long long probs_row, const int32_t* cu, const float* u, const float* v,
+               const float* temperature, int32_t* tokens, int32_t* accepted, float* logp, void* workspace,
+               size_t workspace_bytes, int N, int V, int B, void* stream) {
+  if (N < 0 || V < 1 || B < 0) return DSA_EINVAL;
+  if (!dsa::verify_grid_ok(N, V) || !dsa::verify_grid_ok(B, V)) return DSA_EUNSUPPORTED;
+  if (B == 0) return DSA_OK;
+  if (!cu || !v || !temperature || !accepted) return DSA_EINVAL;
+  if (N > 0 && (!logits || !draft || !u || !tokens || !logp || logits_row < V || (probs && probs_row < V)))
+    return DSA_EINVAL;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::verify_workspace_bytes(N, V, B)) return DSA_EWORKSPACE;
+  return status(dsa::launch_verify(logits, logits_fp32 != 0, (long)logits_row, draft, probs, probs_fp32 != 0,
+                                   (long)probs_row, cu, u, v, temperature, tokens, accepted, logp, workspace, N, V, B,
+                                   static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

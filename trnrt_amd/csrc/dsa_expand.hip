@@ -2,6 +2,7 @@
 // rows (expand_latent_kernel), and attention over them (expanded_attend_kernel). Per pair of tokens and head it costs
 // 192 + 128 multiply-adds where the absorbed form's latent products cost 576 + 512.
 #include "dsa_async.h"
+#include "dsa_expand.h"
 #include "dsa_scan.h"
 
 namespace dsa {
@@ -290,12 +291,13 @@ __device__ __forceinline__ void xa_find(int ti, const int* __restrict__ cu_q, in
   __syncthreads();
 }
 
-template <int DQ>
+// MORE: with what ExpandedMore asks for (its branches are the workgroup's, or a tile's).
+template <int DQ, bool MORE>
 __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ kr,
     const uint16_t* __restrict__ v, const int* __restrict__ cu_q, const int* __restrict__ cu_k,
     uint16_t* __restrict__ out, float* __restrict__ out_f32, float* __restrict__ lse_out, float* __restrict__ ws, int B,
-    int Tq, int Tk, int H, int q_tiles, int splits, int causal, float scale) {
+    int Tq, int Tk, int H, int q_tiles, int splits, int causal, float scale, ExpandedMore more) {
   constexpr int STEPS = DQ / 16;
   constexpr int LOADS = DQ > EX_D ? 10 : 8;  // a tile's asynchronous loads per wave
   __shared__ XaShared<DQ> sh;
@@ -320,13 +322,43 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   const int kb = min(max(cu_k[b], 0), Tk), nk = max(min(cu_k[b + 1], Tk) - kb, 0);
   // keys that query i sees
   auto seen = [&](int i) __attribute__((always_inline)) { return causal ? min(nk - nq + i + 1, nk) : nk; };
-  // the tiles of keys, i0 .. nt - 1 of this split's
-  const int all = (max(seen(min(qt + XA_Q, nq) - 1), 0) + XA_K - 1) / XA_K;
-  const int i0 = (int)((long)all * split / splits), nt = (int)((long)all * (split + 1) / splits);
   const int w0 = qt + 32 * wave;  // the wave's first query
-  const int nt_w = w0 < nq ? (max(seen(min(w0 + 32, nq) - 1), 0) + XA_K - 1) / XA_K : 0;
-  const int seen0 = seen(w0);
-  const int qi = min(w0 + j, nq - 1), seen_j = seen(qi);
+  const int qi = min(w0 + j, nq - 1);
+  int low_j = 0, seen_j = seen(qi);  // the keys low_j .. seen_j - 1 are this query's
+  // the tiles of keys, i0 .. nt - 1 of this split's, of them i0_w .. nt_w - 1 the wave's; the keys from full_lo to full_hi
+  // are every query's of the wave
+  int i0, nt, i0_w = 0, nt_w, full_lo = 0, full_hi;
+  if constexpr (MORE) {
+    if (more.first) low_j = min(max(more.first[qb + qi], 0), nk);
+    if (more.last) seen_j = min(seen_j, more.last[qb + qi]);
+    seen_j = max(seen_j, 0);
+    const bool some = low_j < seen_j;  // (a query that sees nothing asks for no tile)
+    int lo = some ? low_j : 0x7fffffff, hi = some ? seen_j : 0;
+    full_lo = low_j, full_hi = seen_j;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      lo = min(lo, __shfl_xor(lo, m, WAVE)), hi = max(hi, __shfl_xor(hi, m, WAVE));
+      full_lo = max(full_lo, __shfl_xor(full_lo, m, WAVE)), full_hi = min(full_hi, __shfl_xor(full_hi, m, WAVE));
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo), hi = __builtin_amdgcn_readfirstlane(hi);
+    full_lo = __builtin_amdgcn_readfirstlane(full_lo), full_hi = __builtin_amdgcn_readfirstlane(full_hi);
+    i0_w = lo / XA_K, nt_w = w0 < nq ? (hi + XA_K - 1) / XA_K : 0;
+    __shared__ int2 span[XA_THREADS / WAVE];
+    if (lane == 0) span[wave] = make_int2(lo, hi);
+    __syncthreads();
+    lo = 0x7fffffff, hi = 0;
+#pragma unroll
+    for (int w = 0; w < XA_THREADS / WAVE; ++w) lo = min(lo, span[w].x), hi = max(hi, span[w].y);
+    lo = __builtin_amdgcn_readfirstlane(lo) / XA_K, hi = (__builtin_amdgcn_readfirstlane(hi) + XA_K - 1) / XA_K;
+    const int all = max(hi - lo, 0);
+    if (all == 0) lo = hi = 0;
+    i0 = lo + (int)((long)all * split / splits), nt = lo + (int)((long)all * (split + 1) / splits);
+  } else {
+    const int all = (max(seen(min(qt + XA_Q, nq) - 1), 0) + XA_K - 1) / XA_K;
+    i0 = (int)((long)all * split / splits), nt = (int)((long)all * (split + 1) / splits);
+    nt_w = w0 < nq ? (max(seen(min(w0 + 32, nq) - 1), 0) + XA_K - 1) / XA_K : 0;
+    full_hi = seen(w0);
+  }
 
   // Waves 0 to 3, the ones with priority, bring the tiles, once they are through with theirs: the loads' issue would
   // delay the others, for whom they wait anyway (8k tokens, 64 heads, on one card: 1,194 us; all waves before
@@ -387,6 +419,12 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     for (int i = 0; i < 4; ++i) voff[i] = 256 * (4 * h + r) + 16 * ((4 * i | p) ^ (4 * r)) + 8 * (lane & 1);
   }
   const float sl2 = scale * XA_LOG2E;
+  [[maybe_unused]] bool fresh = true;  // (MORE) no key of this query's so far
+  [[maybe_unused]] float cap2 = 0.0f, cap_in = 0.0f, slope2 = 0.0f;
+  if constexpr (MORE) {
+    if (more.softcap > 0.0f) cap2 = more.softcap * XA_LOG2E, cap_in = 2.0f * XA_LOG2E * scale / more.softcap;
+    if (more.slopes) slope2 = more.slopes[head] * XA_LOG2E;
+  }
   float m_run = 0.0f, l_run = 0.0f;  // running maximum (base 2), this lane's share of the sum
   f32x16 o[4];                       // dims 32 d + 8 (r / 4) + 4 h + r % 4
 #pragma unroll
@@ -402,7 +440,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         wait_loads<0>();
     }
     lds_barrier();  // tile i is in place, and nobody reads tile i - 1 any more
-    if (i < nt_w) {
+    if (i < nt_w && (!MORE || i >= i0_w)) {
       const uint8_t* const kt = sh.k[stage];
       const uint8_t* const vt = sh.v[stage];
       const uint8_t* const rt = sh.r[DQ > EX_D ? stage : 0];
@@ -415,25 +453,54 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
           s2[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), qf[s], s2[x],
                                                           0, 0, 0);
         }
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s2[x][r] = fmaf(s2[x][r], sl2, -m_run);
-      if ((i + 1) * XA_K > seen0) {  // keys that a query does not see
-        const int lim = seen_j - i * XA_K - 4 * h;
+      if (MORE && cap2 > 0.0f) {
+        // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), here in base 2
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s2[x][r] = 32 * x + 8 * (r >> 2) + (r & 3) < lim ? s2[x][r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(s2[x][r] * cap_in);
+            s2[x][r] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + e), cap2 - m_run);
+          }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s2[x][r] = fmaf(s2[x][r], sl2, -m_run);
+      }
+      if (MORE && more.slopes) {
+        const float from = (float)(nk - nq + qi - i * XA_K - 4 * h);  // (|p - t| < 2^24: exact)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s2[x][r] = fmaf(-slope2, fabsf(from - (float)(32 * x + 8 * (r >> 2) + (r & 3))), s2[x][r]);
+      }
+      if ((i + 1) * XA_K > full_hi || (MORE && i * XA_K < full_lo)) {  // keys that a query does not see
+        const int lim = seen_j - i * XA_K - 4 * h, low = MORE ? low_j - i * XA_K - 4 * h : 0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int t = 32 * x + 8 * (r >> 2) + (r & 3);
+            s2[x][r] = t < lim && (!MORE || t >= low) ? s2[x][r] : -INFINITY;
+          }
       }
       float cm = s2[0][0];
 #pragma unroll
       for (int r = 1; r < 32; ++r) cm = max_nonan(cm, s2[r >> 4][r & 15]);
-      if (i == i0 || __ballot(cm > XA_SLACK) != 0) {
+      if (MORE ? __ballot(fresh || cm > XA_SLACK) != 0 : i == i0 || __ballot(cm > XA_SLACK) != 0) {
         cm = max_nonan(cm, __shfl_xor(cm, 32, WAVE));
-        // a query that sees none of the first tile sees nothing: its maximum stays finite
-        const float up = i == i0 ? max_nonan(cm, -1e30f) : cm > XA_SLACK ? cm : 0.0f;
-        const float alpha = i == i0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+        float up, alpha;
+        if (MORE) {  // the maximum starts at a query's first key, and is 0 until then
+          const bool none = cm == -INFINITY;
+          up = fresh ? none ? 0.0f : cm : cm > XA_SLACK ? cm : 0.0f;
+          alpha = fresh ? 0.0f : __builtin_amdgcn_exp2f(-up);
+          fresh = fresh && none;
+        } else {  // a query that sees none of the first tile sees nothing: its maximum stays finite
+          up = i == i0 ? max_nonan(cm, -1e30f) : cm > XA_SLACK ? cm : 0.0f;
+          alpha = i == i0 ? 0.0f : __builtin_amdgcn_exp2f(-up);
+        }
         m_run += up;
         l_run *= alpha;
 #pragma unroll
@@ -633,12 +700,15 @@ size_t expanded_workspace_bytes(int B, int Tq, int Tk, int H, int num_cu) {
 
 hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const uint16_t* kr, const uint16_t* v,
                                   const int* cu_q, const int* cu_k, uint16_t* out, float* out_f32, float* lse, void* ws,
-                                  int B, int Tq, int Tk, int H, int causal, float scale, int num_cu, hipStream_t s) {
+                                  int B, int Tq, int Tk, int H, int causal, float scale, const ExpandedMore* more,
+                                  int num_cu, hipStream_t s) {
   const int q_tiles = attend_tiles(B, Tq), splits = attend_splits(B, Tq, Tk, H, num_cu);
-  const auto kernel = kr ? expanded_attend_kernel<EX_D + EX_R> : expanded_attend_kernel<EX_D>;
+  const auto kernel = more ? kr ? expanded_attend_kernel<EX_D + EX_R, true> : expanded_attend_kernel<EX_D, true>
+                      : kr ? expanded_attend_kernel<EX_D + EX_R, false>
+                           : expanded_attend_kernel<EX_D, false>;
   const hipError_t e = launch("expanded_attend_kernel", kernel, dim3((unsigned)q_tiles * H * splits), dim3(XA_THREADS), s,
                               q, k, kr, v, cu_q, cu_k, out, out_f32, lse, static_cast<float*>(ws), B, Tq, Tk, H, q_tiles,
-                              splits, causal, scale);
+                              splits, causal, scale, more ? *more : ExpandedMore{});
   if (e != hipSuccess || splits == 1) return e;
   return launch("expanded_combine_kernel", expanded_combine_kernel, dim3((unsigned)q_tiles * H * 4), dim3(XA_THREADS), s,
                 static_cast<const float*>(ws), cu_q, out, out_f32, lse, B, Tq, H, q_tiles, splits);

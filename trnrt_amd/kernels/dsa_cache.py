@@ -9,16 +9,22 @@ indexer-key rows at the step's slot_mapping).
 The HIP kernel (csrc/dsa_cache.hip) converts each row in one wave: fp32 arithmetic with a correctly rounded
 division and round-to-nearest-even into e4m3fn, which is torch's float -> float8_e4m3fn cast.
 
+append takes a step's rows as the projections leave them, norms and rotates them on the way, finds their slots through the
+page table and writes all kinds of them (latent rows, indexer keys) in one launch (csrc/dsa_append.hip).
+
 write_pool_keys is the pooled (GLM) indexer's key write of the same step (trnrt/models/mla.py:1277-1296): each written
 token's pool key, a softmax-gated mean of the pool's cached indexer keys, into the pool-key cache.
 """
 
 from __future__ import annotations
 
+from collections.abc import Sequence
+
 import torch
 
 from .. import _lib
 from . import _common as C
+from .dsa_rope import axis_map
 
 FP8_MAX = 448.0  # the e4m3fn maximum (trnrt/engine/model_runner.py:62-70 off Neuron)
 
@@ -66,6 +72,105 @@ def store(cache: torch.Tensor, slots: torch.Tensor, x: torch.Tensor, fp8_max: fl
     st = _lib.lib().dsa_cache_write(C.ptr(x), x_fp32, C.ptr(slots), C.ptr(cache), C.ptr(scale), T, W, num_slots,
                                     int(scale is not None), float(fp8_max), C.stream_ptr(dev))
     _lib.check(st, "dsa_cache.store")
+
+
+class Rows:
+    """One kind of rows for append: x [T, W] (bf16 or fp32; a view of a wider projection's columns will do) into cache
+    [slots, W] (or [slots, 1, W]; e4m3fn or its uint8 bits, with scale [slots] fp32 or unscaled; or bf16).
+
+    rope_at: the first of the 2R columns that are rotated (None: none), interleaved: their pairs as in dsa_rope.rotate.
+    norm: a weight [n] for the root-mean-square norm of the first n columns, or (weight, bias) for their layer norm (bf16 or
+    fp32), with eps."""
+
+    __slots__ = ("x", "cache", "scale", "rope_at", "interleaved", "norm", "eps", "fp8_max")
+
+    def __init__(self, x: torch.Tensor, cache: torch.Tensor, scale: torch.Tensor | None = None, *,
+                 rope_at: int | None = None, interleaved: bool = True,
+                 norm: torch.Tensor | tuple[torch.Tensor, torch.Tensor] | None = None, eps: float = 1e-6,
+                 fp8_max: float = FP8_MAX):
+        self.x, self.cache, self.scale, self.rope_at, self.interleaved = x, cache, scale, rope_at, interleaved
+        self.norm, self.eps, self.fp8_max = norm, eps, fp8_max
+
+
+def _norm(norm, width: int):
+    """(weight, bias) of one type, starting at multiples of 16 bytes."""
+    w, b = norm if isinstance(norm, (tuple, list)) else (norm, None)
+    if b is not None and (b.shape != w.shape or b.device != w.device):
+        raise ValueError(f"dsa_cache.append: norm weight {tuple(w.shape)} and bias {tuple(b.shape)}")
+    if w.dim() != 1 or not 1 <= w.shape[0] <= width:
+        raise ValueError(f"dsa_cache.append: norm weight {tuple(w.shape)} for rows of {width}")
+    if w.dtype not in (torch.bfloat16, torch.float32) or (b is not None and b.dtype is not w.dtype):
+        w, b = w.float(), None if b is None else b.float()
+    return C.aligned(w.contiguous()), None if b is None else C.aligned(b.contiguous())
+
+
+def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tensor, page_size: int, *,
+           cu_new: torch.Tensor | None = None, positions: torch.Tensor | None = None, inv_freq: torch.Tensor | None = None,
+           axes: Sequence[int] | None = None, factor: float = 1.0) -> None:
+    """The rows of T new tokens of B sequences into the paged caches, in place, on the current stream: sequence b's are rows
+    cu_new[b] .. cu_new[b + 1] - 1 of every x (cu_new [B + 1] int32; None: T / B each) and the last of its ctx_len[b] tokens
+    (ctx_len [B] int32 counts the new ones), through table [B, max_pages] int32. The columns that a kind names are rotated
+    by positions ([T], or [axes, T] with axes, as in dsa_rope.rotate; None: the token's place in its sequence) x inv_freq
+    [R] fp32 x factor. Everything is in fp32 and rounded once, as store rounds. A token whose place is outside the table, or
+    whose page is the null page or outside the pool, is not written, nor are rows in no sequence."""
+    rows = (rows,) if isinstance(rows, Rows) else rows
+    if not rows:
+        raise ValueError("dsa_cache.append: no rows")
+    dev = C.on_gpu(table, ctx_len, cu_new, positions, inv_freq)
+    if table.dim() != 2 or table.shape[1] < 1 or page_size < 1:
+        raise ValueError(f"dsa_cache.append: table {tuple(table.shape)} with pages of {page_size}")
+    B, max_pages = table.shape
+    tb, lens = C.as_i32(table), C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
+    cu = None if cu_new is None else C.need(C.as_i32(cu_new), "cu_new", torch.int32, (B + 1,))
+    if inv_freq is not None:
+        C.need(inv_freq, "inv_freq", torch.float32, (None,))
+    R = 0 if inv_freq is None else inv_freq.shape[0]
+    T = slots = None
+    kinds = (_lib.AppendRows * len(rows))()
+    held = []  # (what a kind's tensors were copied to, until the launch)
+    for r, kind in zip(rows, kinds):
+        x, cache, W = r.x, r.cache, r.cache.shape[-1]
+        if C.on_gpu(x, cache, r.scale) != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {x.device}")
+        if x.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"dsa_cache.append: rows of {x.dtype}, expected bfloat16 or float32")
+        if x.dim() != 2:
+            x = x.reshape(-1, x.shape[-1])
+        if x.shape[1] != W:
+            raise ValueError(f"dsa_cache.append: rows {tuple(x.shape)} for a cache of width {W}")
+        bf = cache.dtype is torch.bfloat16
+        if not bf and cache.dtype not in (C.FP8, torch.uint8):
+            raise NotImplementedError(f"dsa_cache.append: a {cache.dtype} cache; it is float8_e4m3fn or bfloat16")
+        if not cache.is_contiguous() or cache.data_ptr() % 16:
+            raise ValueError("dsa_cache.append: the cache must be contiguous and start at a multiple of 16 bytes")
+        n = cache.numel() // W if W else 0
+        if T is None:
+            T, slots = x.shape[0], n
+        if x.shape[0] != T or n != slots or n < 1 or n % page_size:
+            raise ValueError(f"dsa_cache.append: {x.shape[0]} rows of {T}, {n} cache slots of {slots} in pages of {page_size}")
+        size = x.element_size()
+        if x.stride(1) != 1 or x.data_ptr() % 16 or (x.stride(0) * size % 16 or x.stride(0) < W) and T > 1:
+            x = x.clone(memory_format=torch.contiguous_format)
+            held.append(x)
+        if r.scale is not None:
+            kind.scale = C.need(C.flat(r.scale), "scale", torch.float32, (slots,)).data_ptr()
+        if r.norm is not None:
+            w, b = _norm(r.norm, W)
+            C.on_gpu(x, w, b)
+            held += (w, b)
+            kind.norm_weight, kind.norm_bias = w.data_ptr(), None if b is None else b.data_ptr()
+            kind.norm_fp32, kind.norm_width = w.dtype is torch.float32, w.shape[0]
+        if r.rope_at is not None and not (R and 0 <= r.rope_at <= W - 2 * R):
+            raise ValueError(f"dsa_cache.append: {2 * R} rotated columns from {r.rope_at} on in rows of {W}")
+        kind.x, kind.x_row, kind.x_fp32, kind.width = x.data_ptr(), max(x.stride(0), W), size == 4, W
+        kind.rope_at, kind.interleaved = -1 if r.rope_at is None else r.rope_at, r.interleaved
+        kind.cache, kind.cache_bf16, kind.eps, kind.fp8_max = cache.data_ptr(), bf, r.eps, r.fp8_max
+    if cu is None and T and (not B or T % B):
+        raise ValueError(f"dsa_cache.append: {T} rows for {B} sequences without cu_new")
+    pos, n_axes, which = axis_map(axes, positions, R, T, "dsa_cache.append")
+    st = C.call(dev, _lib.lib().dsa_cache_append, kinds, len(rows), C.ptr(tb), C.ptr(lens), C.ptr(cu), C.ptr(pos),
+                C.ptr(inv_freq), which, T, B, R, n_axes, factor, max_pages, page_size, slots // page_size)
+    _lib.check(st, "dsa_cache.append")
 
 
 def write_pool_keys(pool_key: torch.Tensor, rows: torch.Tensor, positions: torch.Tensor, table: torch.Tensor,

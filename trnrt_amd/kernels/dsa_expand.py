@@ -2,7 +2,8 @@
 from the cached latent rows, and ragged causal attention over them.
 
     expand(kv_cache, kv_scale, table, cu_len, total, page_size, w)   k, k_rope, v of the sequences' cached tokens
-    attend(q, k, k_rope, v, cu_q, cu_k, scale)                       o, lse of the queries
+    attend(q, k, k_rope, v, cu_q, cu_k, scale)                       o, lse of the queries; with first, last: a range of keys
+                                                                     for each query; softcap, slopes: scores changed
 
 Per pair of tokens and head this costs 192 + 128 multiply-adds where the absorbed form (dsa_dense.attend) costs 576 + 512,
 so it is the form for many queries a sequence; for one or a few, whose time is the cache's stream, it is dsa_dense.attend.
@@ -75,13 +76,19 @@ def expand(kv_cache: torch.Tensor, kv_scale: torch.Tensor | None, table: torch.T
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: torch.Tensor, cu_q: torch.Tensor,
-           cu_k: torch.Tensor, scale: float, *, causal: bool = True, lse: bool = True, out_dtype=torch.bfloat16,
-           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
+           cu_k: torch.Tensor, scale: float, *, causal: bool = True, first: torch.Tensor | None = None,
+           last: torch.Tensor | None = None, softcap: float = 0.0, slopes: torch.Tensor | None = None, lse: bool = True,
+           out_dtype=torch.bfloat16, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None):
     """o [Tq, H, 128] in out_dtype (bf16 or fp32) and lse [Tq, H] fp32 (o alone without lse) of ragged sequences: q
     [Tq, H, 192] bf16 with k_rope [Tk, 64] bf16 shared by the heads, or [Tq, H, 128] without (k_rope None); k, v
     [Tk, H, 128] bf16; cu_q, cu_k [B + 1] int32 on the device: sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1,
     its keys rows cu_k[b] .. . causal: query i of nq sees the first nk - nq + i + 1 of the nk keys (the last sees all);
     otherwise every key. A query that sees no key has o = 0 and lse NEG_INF; rows of q in no sequence are not written.
+    first, last [Tq] int32: a query sees only keys first <= t < last of its sequence (either may be None), besides causal:
+    documents packed into one sequence are first = the document's start; a prefix that its own tokens see both ways is last =
+    max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. Only the
+    tiles of 64 keys that a query tile sees are read. softcap > 0: scores become softcap tanh(s / softcap). slopes [H] fp32:
+    slopes[h] |p - t| is taken off them.
     workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
     dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
@@ -104,15 +111,27 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     C.need(out, "out", (torch.bfloat16, torch.float32), (Tq, H, DH))
     ls = q.new_empty((Tq, H), dtype=torch.float32) if lse else None
     bf = out.dtype == torch.bfloat16
+    more = first is not None or last is not None or slopes is not None or softcap != 0.0
+    if more:
+        C.on_gpu(q, first, last, slopes)
+        if not 0.0 <= softcap < float("inf"):
+            raise ValueError(f"dsa_expand: softcap {softcap}")
+        first = None if first is None else C.need(C.as_i32(first), "first", torch.int32, (Tq,))
+        last = None if last is None else C.need(C.as_i32(last), "last", torch.int32, (Tq,))
+        slopes = None if slopes is None else C.need(C.as_f32(slopes), "slopes", torch.float32, (H,))
     lib, B = _lib.lib(), cu_q.numel() - 1
     if workspace is not None:
         ws = C.given(workspace, "dsa_expand")
     else:
         need = int(lib.dsa_expanded_workspace_bytes(B, Tq, Tk, H))
         ws = C.scratch(dev, need, "expanded") if need else None
-    st = C.call(dev, lib.dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),
-                C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), C.ptr(ws),
-                0 if ws is None else ws.numel() * ws.element_size(), B, Tq, Tk, H,
-                int(bool(causal)), float(scale))
+    size = 0 if ws is None else ws.numel() * ws.element_size()
+    o = (C.ptr(out) if bf else None, None if bf else C.ptr(out), C.ptr(ls), C.ptr(ws), size, B, Tq, Tk, H, int(bool(causal)),
+         float(scale))
+    if more:
+        st = C.call(dev, lib.dsa_expanded_mla_spans, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck),
+                    C.ptr(first), C.ptr(last), C.ptr(slopes), float(softcap), *o)
+    else:
+        st = C.call(dev, lib.dsa_expanded_mla, C.ptr(q), C.ptr(k), C.ptr(r), C.ptr(v), C.ptr(cq), C.ptr(ck), *o)
     _lib.check(st, "dsa_expand.attend")
     return (out, ls) if lse else out
