@@ -1,6 +1,7 @@
 """Verification of drafts (trnrt_amd/kernels/dsa_verify.py) against a loop over rows in numpy's float64: tokens and counts
-equal, the log probabilities within 2^-24 of themselves and 2^-40 (they are computed in 64 bits and rounded once; exp2, log and
-sums there are good to far less than 2^-40)."""
+equal, the log probabilities within 2^-24 of themselves (they are rounded once) and 2^-18: a row's sum is of 32-bit exponentials
+whose exponents are off by 2^-23 of themselves, 20 at the weights' mean at most (20 x 2^-23 ln 2 = 1.7e-6), exp2 by 2^-23, and a
+term goes through 16 roundings on its way into the sum (1e-6): 2.8e-6, less than 2^-18 = 3.8e-6."""
 
 import math
 
@@ -82,7 +83,7 @@ def check(logits, draft, cu, u, v, temperature, probs=None, got=None):
     a, z = int(cu[0]), int(cu[-1])
     assert (tokens.cpu().numpy()[a:z] == rt[a:z]).all(), (tokens.cpu().numpy()[a:z], rt[a:z])
     err = np.abs(logp.double().cpu().numpy()[a:z] - rl[a:z])
-    assert (err <= 2.0 ** -24 * np.abs(rl[a:z]) + 2.0 ** -40).all()
+    assert (err <= 2.0 ** -24 * np.abs(rl[a:z]) + 2.0 ** -18).all()
     assert tokens.shape == logp.shape == (N,)
     return tokens, accepted, logp
 
@@ -167,6 +168,29 @@ def test_edges_of_the_random_numbers():
     sure[:, 12345] = 3.0
     check(sure, torch.full_like(draft, 12345), cu, u, v, temperature)
     check(sure, torch.full_like(draft, 12344), cu, u, v, temperature)
+
+
+@pytest.mark.parametrize("V", [3, 700, 40000])
+def test_decisions_that_32_bits_do_not_make(V):
+    """u q within an fp32 rounding of p, on either side; and a draft whose probabilities are the target's own, rounded, refused
+    all the same: what is left over is roundings, and the token is the one that they give in 64 bits."""
+    say("verify close", V)
+    for dtype in (torch.bfloat16, torch.float32):
+        logits, draft, cu, u, v, temperature, _ = make([3] * 40, V, dtype, None, V)
+        temperature = temperature.clamp(min=0.7)
+        seq = torch.arange(40).repeat_interleave(3)
+        p = torch.softmax(logits.cpu().double() / temperature.double()[seq][:, None], -1)
+        q = p.float()
+        px = p.gather(1, draft.long()[:, None])[:, 0]
+        half = q.clone()
+        half.scatter_(1, draft.long()[:, None], (2 * px).float()[:, None])
+        _, accepted, _ = check(logits, draft, cu, torch.full_like(u, 0.5), v, temperature, half.cuda())
+        assert (accepted > 0).any() and (accepted < 2).any()
+        above = q.clone()  # q just above p at the drafted token, so that u just under 1 refuses it
+        above.scatter_(1, draft.long()[:, None], (px * (1 + 2.0 ** -20)).float()[:, None])
+        _, accepted, _ = check(logits, draft, cu, torch.full_like(u, 1 - 2.0 ** -24), v, temperature, above.cuda())
+        assert (accepted < 2).any()
+        check(logits, draft, cu, torch.full_like(u, 1 - 2.0 ** -24), v, temperature, (q * (1 + 3e-6)).cuda())
 
 
 def test_views_and_rows_outside():
