@@ -12,10 +12,11 @@
 // w = q z by less than VF_NEAR are too near to say, their r is at most VF_NEAR q z each, and where the sum of those bounds
 // could move the token (or where r would be 0) the row is gone through once more with the 64-bit sum.
 //
-// Two launches. verify_rows_kernel: a wave takes 512 to 2,048 logits of a row to (maximum, sum, place of the maximum),
-// without LDS. verify_pick_kernel: every workgroup of a sequence finds the stop row from those alike; each sums a chunk of it,
-// and the last to be done (a count per sequence, cleared by the first launch) looks for the token.
-#include "dsa_common.h"
+// Three launches. verify_rows_kernel: a wave takes 512 to 2,048 logits of a row to (maximum, sum, place of the maximum),
+// without LDS. verify_stop_kernel: a workgroup a sequence, a wave a row, takes the drafts and finds the stop row.
+// verify_pick_kernel: a workgroup sums a chunk of a stop row, the last of a sequence's to be done (a count that the second
+// launch cleared) looks for the token.
+#include "dsa_async.h"
 
 namespace dsa {
 
@@ -40,7 +41,7 @@ struct VerifyArgs {
   long l_row, q_row;
   int l_fp32, q_fp32;
   int N, V, B;
-  int parts, chunks;   // of a row, for the two launches
+  int parts, chunks;   // of a row, for the first launch and the last
 };
 
 struct VerifyPart {
@@ -50,9 +51,17 @@ struct VerifyPart {
   int pad;
 };
 
-struct VerifyChunk {  // of the stop row
+struct VerifyStop {  // a sequence's stop row
+  double sum;
+  float max;
+  int row;            // -1: nothing is drawn from it
+  int last;           // the sequence's last row: r = p
+  int done;           // chunks that are summed
+};
+
+struct VerifyChunk {  // sums over a chunk of the stop row
   double all;         // w
-  double over, q;     // w and q where w > q z
+  double rest, q;     // w - q z, and q, where that is above 0
   double near;        // bound of what is too near to say
 };
 
@@ -99,13 +108,36 @@ __device__ __forceinline__ double vf_exponent(float l, float m, double k) {
   return x <= 0.0 && l > -INFINITY ? x : -INFINITY;
 }
 
-__device__ __forceinline__ double vf_weight(float l, float m, double k) { return exp2(vf_exponent(l, m, k)); }
+
+// 2^x for x <= 0 (x < -1022: 2^-1022), by the series of e^(f ln 2) about the nearest whole number; the first term left out is
+// 2e-13 of it at most. The whole number is found, and put into the exponent, through the low bits of x + 1.5 2^52.
+__device__ __forceinline__ double vf_exp2(double x) {
+  x = fmax(x, -1022.0);
+  const double big = 6755399441055744.0, n = x + big, f = x - (n - big);
+  double p = 7.0549116208011233299e-9;  // (ln 2)^k / k!
+  p = fma(p, f, 1.0178086009239699728e-7);
+  p = fma(p, f, 1.3215486790144309488e-6);
+  p = fma(p, f, 1.5252733804059840280e-5);
+  p = fma(p, f, 1.5403530393381609954e-4);
+  p = fma(p, f, 1.3333558146428443423e-3);
+  p = fma(p, f, 9.6181291076284771620e-3);
+  p = fma(p, f, 5.5504108664821579953e-2);
+  p = fma(p, f, 2.4022650695910071233e-1);
+  p = fma(p, f, 6.9314718055994530942e-1);
+  p = fma(p, f, 1.0);
+  const long long u = __builtin_bit_cast(long long, p);
+  const int hi = (int)(u >> 32) + ((int)__builtin_bit_cast(long long, n) << 20);
+  return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)u);
+}
+
+__device__ __forceinline__ double vf_weight(float l, float m, double k) {
+  const double x = vf_exponent(l, m, k);
+  return x > -1022.0 ? vf_exp2(x) : 0.0;
+}
 
 __device__ __forceinline__ double vf_rate(float temperature) {
   return 1.4426950408889634074 / (temperature > 0.0f ? (double)temperature : 1.0);
 }
-
-__device__ __forceinline__ int vf_row(const VerifyArgs& a, int b) { return min(max(a.cu[b], 0), a.N); }
 
 // The sum over the wave, in every lane.
 __device__ __forceinline__ double vf_swap(double x, int ctrl) {
@@ -132,25 +164,6 @@ __device__ __forceinline__ double vf_wave_sum(double x) {
   return (vf_lane(x, 0) + vf_lane(x, 16)) + (vf_lane(x, 32) + vf_lane(x, 48));
 }
 
-// 2^x for x <= 0, by the series of e^(x ln 2) about the nearest whole number: the first term left out is 6e-15 of it.
-__device__ __forceinline__ double vf_exp2(double x) {
-  x = fmax(x, -1100.0);  // (2^-1100 is 0)
-  const double n = rint(x), t = (x - n) * 0.69314718055994530942;
-  double p = 1.0 / 39916800.0;
-  p = fma(p, t, 1.0 / 3628800.0);
-  p = fma(p, t, 1.0 / 362880.0);
-  p = fma(p, t, 1.0 / 40320.0);
-  p = fma(p, t, 1.0 / 5040.0);
-  p = fma(p, t, 1.0 / 720.0);
-  p = fma(p, t, 1.0 / 120.0);
-  p = fma(p, t, 1.0 / 24.0);
-  p = fma(p, t, 1.0 / 6.0);
-  p = fma(p, t, 0.5);
-  p = fma(p, t, 1.0);
-  p = fma(p, t, 1.0);
-  return ldexp(p, (int)n);
-}
-
 // The number of sequences that end by `row` (cu ascends), the same in every lane of the wave; B: past the last.
 __device__ __forceinline__ int vf_sequence(const int* __restrict__ cu, int B, int row) {
   const int lane = threadIdx.x & (WAVE - 1);
@@ -168,21 +181,22 @@ __device__ __forceinline__ int vf_sequence(const int* __restrict__ cu, int B, in
 // A wave per unit: LOADS x 512 logits of a row. Not even a comparison is spent on NaN or infinities: they make the sum NaN,
 // and the unit is then done again with care.
 template <typename T, int LOADS>
-__global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a, VerifyPart* __restrict__ parts,
-                                                                 int* __restrict__ done) {
+__global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a,
+                                                                 VerifyPart* __restrict__ parts) {
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int unit = blockIdx.x * VF_WAVES + wave;
-  for (int b = blockIdx.x * VF_THREADS + threadIdx.x; b < a.B; b += gridDim.x * VF_THREADS) done[b] = 0;
   const int row = unit / a.parts, part = unit - row * a.parts;
   if (row >= a.N) return;
   const int i0 = (part * LOADS * WAVE + lane) * VF_VEC;
+  // (the sequences' ends are on their way before the logits, and the temperature while those are)
+  const int end = a.cu[min(lane + 1, a.B)];
   float x[LOADS][VF_VEC];
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
     vf_load(static_cast<const T*>(a.logits) + (size_t)row * a.l_row, i0 + i * WAVE * VF_VEC, a.V, -INFINITY, x[i]);
-  if (row < a.cu[0]) return;
-  const int b = vf_sequence(a.cu, a.B, row);
-  if (b >= a.B) return;
+  int b = __popcll(__ballot(lane < a.B && end <= row));
+  if (b == WAVE) b = vf_sequence(a.cu, a.B, row);
+  if (b >= a.B || row < a.cu[0]) return;
   const float temperature = a.temperature[b];
   const double k = vf_rate(temperature);
   float m = -INFINITY;
@@ -201,21 +215,13 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a, V
       s[e & 3] += __builtin_amdgcn_exp2f(fmaf(d, kh, d * kl));
     }
   float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  const int from = part * LOADS * WAVE * VF_VEC, to = min(from + LOADS * WAVE * VF_VEC, a.V);
   if (!(sum >= 0.0f)) {
     m = -INFINITY;
-    double t = 0.0;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-      for (int e = 0; e < VF_VEC; ++e) {
-        x[i][e] = x[i][e] > -INFINITY ? x[i][e] : -INFINITY;
-        m = fmaxf(m, x[i][e]);
-      }
+    for (int i = from + lane; i < to; i += WAVE) m = fmaxf(m, vf_logit(a, row, i));
     m = wave_max(m);
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i)
-#pragma unroll
-      for (int e = 0; e < VF_VEC; ++e) t += vf_weight(x[i][e], m, k);
+    double t = 0.0;
+    for (int i = from + lane; i < to; i += WAVE) t += vf_weight(vf_logit(a, row, i), m, k);
     sum = (float)vf_wave_sum(t);
   }
   uint32_t first = 0x7fffffffu;
@@ -227,6 +233,10 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a, V
     first = wave_min_u32(first);
   }
   if (lane == 0) parts[unit] = VerifyPart{m, sum, (int)first, 0};
+}
+
+__device__ __forceinline__ float vf_logp(float l, float m, double sum, double k) {
+  return (float)(vf_exponent(l, m, k) * 0.69314718055994530942 - log(sum));
 }
 
 struct VerifyRow {
@@ -269,283 +279,269 @@ __device__ __forceinline__ double vf_exact_sum(const VerifyArgs& a, int row, flo
   return vf_wave_sum(s);
 }
 
-// Whether row's drafted token is taken.
-__device__ __forceinline__ bool vf_taken(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int row, bool warm,
-                                         double k) {
-  const int x = a.draft[row];
-  if ((unsigned)x >= (unsigned)a.V) return false;
-  const double q = !warm || !a.probs ? 1.0
-                   : a.q_fp32 ? (double)static_cast<const float*>(a.probs)[(size_t)row * a.q_row + x]
-                              : (double)vf_value(static_cast<const uint16_t*>(a.probs)[(size_t)row * a.q_row + x]);
-  const float l = vf_logit(a, row, x);
-  const VerifyRow r = vf_join(a, parts, row, k);
-  if (!warm) return r.max > -INFINITY && x == r.first;
-  const double uq = (double)a.u[row] * q, w = vf_weight(l, r.max, k);
-  if (fabs(uq * r.sum - w) > VF_NEAR * w) return uq * r.sum < w;  // (false for a q that is NaN)
-  return uq * vf_exact_sum(a, row, r.max, k) < w;
-}
+// One workgroup a sequence: its drafts, its stop row, and all that is written but the token drawn from that.
+constexpr int VF_STOP_THREADS = 512;
 
-// The row that sequence b's next token comes from (the first whose draft is not taken, or the last), by the workgroup.
-__device__ __forceinline__ int vf_stop(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int r0, int r1, bool warm,
-                                       double k, int* found) {
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  if (threadIdx.x == 0) *found = r1 - 1;
+__global__ __launch_bounds__(VF_STOP_THREADS) void verify_stop_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
+                                                                      VerifyStop* __restrict__ stops) {
+  __shared__ int found;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
+  const float temperature = a.temperature[b];
+  const bool warm = temperature > 0.0f;
+  const double k = vf_rate(temperature);
+  if (r1 <= r0) {
+    if (tid == 0) a.accepted[b] = 0, stops[b].row = -1;
+    return;
+  }
+  if (tid == 0) found = r1 - 1;
   __syncthreads();
-  for (int row = r0 + wave; row < r1 - 1; row += VF_WAVES)
-    if (!vf_taken(a, parts, row, warm, k)) {
-      if ((threadIdx.x & (WAVE - 1)) == 0) atomicMin(found, row);
-      break;
+  // a wave's rows until one whose draft is not taken; that one, or the last row, stays in r, row
+  VerifyRow r{0.0, -INFINITY, 0};
+  int row = r0 + wave;
+  for (; row < r1; row += VF_STOP_THREADS / WAVE) {
+    const bool last = row == r1 - 1;
+    const int x = last ? 0 : a.draft[row], i = min(max(x, 0), a.V - 1);
+    const float u = last ? 0.0f : a.u[row];
+    const float l = vf_logit(a, row, i);
+    double q = 1.0;
+    if (warm && a.probs)
+      q = a.q_fp32 ? (double)static_cast<const float*>(a.probs)[(size_t)row * a.q_row + i]
+                   : (double)vf_value(static_cast<const uint16_t*>(a.probs)[(size_t)row * a.q_row + i]);
+    r = vf_join(a, parts, row, k);
+    if (last || x != i) break;
+    bool taken = x == r.first && r.max > -INFINITY;
+    if (warm) {
+      const double uq = (double)u * q, w = vf_weight(l, r.max, k);
+      // (not near, or u q that is NaN: decided here)
+      taken = uq * (fabs(uq * r.sum - w) <= VF_NEAR * w ? vf_exact_sum(a, row, r.max, k) : r.sum) < w;
     }
+    if (!taken) break;
+    if (lane == 0) a.tokens[row] = x, a.logp[row] = vf_logp(l, r.max, r.sum, k);
+  }
+  if (lane == 0 && row < r1) atomicMin(&found, row);
   __syncthreads();
-  return __builtin_amdgcn_readfirstlane(*found);
+  const int stop = found;
+  if (row == stop && lane == 0) {
+    const bool none = !(r.max > -INFINITY), drawn = warm && !none;
+    stops[b] = VerifyStop{r.sum, r.max, drawn ? stop : -1, stop == r1 - 1, 0};
+    a.accepted[b] = stop - r0;
+    if (!drawn) a.tokens[stop] = none ? -1 : r.first, a.logp[stop] = none ? 0.0f : vf_logp(r.max, r.max, r.sum, k);
+  }
+  for (int i = stop + 1 + tid; i < r1; i += VF_STOP_THREADS) a.tokens[i] = -1, a.logp[i] = 0.0f;
 }
 
-// Weights w and draft's probabilities q of tokens i .. i + 7 of the stop row, 0 past the last: r = max(w - q sum, 0). (A
-// draft that is certain takes its token's weight out.)
-__device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool last, float m, double k, int i,
-                                            double (&w)[VF_VEC], float (&q)[VF_VEC]) {
-  float x[VF_VEC];
-  vf_logits(a, row, i, x);
+// Logits x and the draft's probabilities q (0 where there are none) of tokens i .. i + 7 of the stop row. A draft that is
+// certain, d, cannot come (-1: there is no such draft).
+__device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool with_q, int d, int i, float (&x)[VF_VEC],
+                                            float (&q)[VF_VEC]) {
+  if (a.l_fp32)
+    vf_load(static_cast<const float*>(a.logits) + (size_t)row * a.l_row, i, a.V, -INFINITY, x);
+  else
+    vf_load(static_cast<const uint16_t*>(a.logits) + (size_t)row * a.l_row, i, a.V, -INFINITY, x);
+  if (d >= i && d < i + VF_VEC) {
+#pragma unroll
+    for (int e = 0; e < VF_VEC; ++e) x[e] = i + e == d ? -INFINITY : x[e];
+  }
 #pragma unroll
   for (int e = 0; e < VF_VEC; ++e) q[e] = 0.0f;
-  if (!last && a.probs) {
+  if (with_q) {
     if (a.q_fp32)
       vf_load(static_cast<const float*>(a.probs) + (size_t)row * a.q_row, i, a.V, 0.0f, q);
     else
       vf_load(static_cast<const uint16_t*>(a.probs) + (size_t)row * a.q_row, i, a.V, 0.0f, q);
   }
-  if (m < INFINITY) {
-#pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) w[e] = vf_exp2(((double)x[e] - (double)m) * k);
-  } else {
-#pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) w[e] = vf_weight(x[e], m, k);
-  }
-  if (!last && !a.probs) {
-    const int d = a.draft[row];
-#pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) w[e] = i + e == d ? 0.0 : w[e];
-  }
 }
 
-// v's inclusive prefix sum over the workgroup; tot: VF_WAVES doubles of LDS.
-__device__ __forceinline__ double vf_scan(double v, double* tot) {
-  const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
-#pragma unroll
-  for (int d = 1; d < WAVE; d *= 2) {
-    const long long u = __builtin_bit_cast(long long, v);
-    const int lo = __shfl_up((int)u, d, WAVE), hi = __shfl_up((int)(u >> 32), d, WAVE);
-    if (lane >= d) v += __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
-  }
-  __syncthreads();
-  if (lane == WAVE - 1) tot[wave] = v;
-  __syncthreads();
-  double before = 0.0;
-  for (int w = 0; w < wave; ++w) before += tot[w];
-  return before + v;
+// A weight of the stop row.
+__device__ __forceinline__ double vf_stop_weight(float x, float m, double k) {
+  const double w = m < INFINITY ? vf_exp2(((double)x - (double)m) * k) : x == m ? 1.0 : 0.0;
+  return x > -INFINITY ? w : 0.0;
 }
 
-__device__ __forceinline__ float vf_logp(float l, float m, double sum, double k) {
-  return (float)(vf_exponent(l, m, k) * 0.69314718055994530942 - log(sum));
+// v's inclusive prefix sum over the wave.
+__device__ __forceinline__ double vf_wave_scan(double v) {
+  const auto step = [&](auto lo, auto hi) { v += __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo); };
+#define VF_STEP(...)                                                       \
+  {                                                                        \
+    const long long u = __builtin_bit_cast(long long, v);                  \
+    step(dpp<__VA_ARGS__>((int)u), dpp<__VA_ARGS__>((int)(u >> 32)));      \
+  }
+  VF_STEP(0x111) VF_STEP(0x112) VF_STEP(0x114) VF_STEP(0x118) VF_STEP(0x142, 0xa, false) VF_STEP(0x143, 0xc, false)
+#undef VF_STEP
+  return v;
 }
 
-// What a workgroup sums of the stop row: chunk's tokens, those of one thread side by side where `inner` (for the search).
-struct VerifySearch {
-  double tot[VF_WAVES];
-  int found, passed, positive, pick;
-  int last;
-  double at, r;  // (of the token that was found: the sum before it, and its r)
-  VerifyChunk part[VF_WAVES];
-};
+// A sequence's workgroups sum PER chunks of its stop row each; the last of them looks for the token.
+constexpr int VF_CHUNK = VF_THREADS * VF_VEC;
 
-// Looks for the target in a chunk whose tokens come after a sum of `before`; the whole workgroup. pick: the token, -1: r is 0
-// throughout.
-template <int LOADS>
-__device__ __forceinline__ void vf_search(const VerifyArgs& a, VerifySearch& sh, int stop, bool last, float m, double z,
-                                          double k, int chunk, double before, double target) {
-  constexpr int PER = LOADS * VF_VEC;
-  const int tid = threadIdx.x, i0 = (chunk * VF_THREADS + tid) * PER;
-  __syncthreads();
-  if (tid == 0) sh.passed = VF_THREADS, sh.positive = -1, sh.pick = -1;
-  double w[PER], mine = 0.0;
-#pragma unroll
-  for (int i = 0; i < PER; i += VF_VEC) {
-    double x[VF_VEC];
-    float q[VF_VEC];
-    vf_stop_row(a, stop, last, m, k, i0 + i, x, q);
-#pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) mine += w[i + e] = fmax(x[e] - (double)q[e] * z, 0.0);
-  }
-  const double upto = before + vf_scan(mine, sh.tot);
-  if (mine > 0.0) {
-    atomicMax(&sh.positive, tid);
-    if (upto > target) atomicMin(&sh.passed, tid);
-  }
-  __syncthreads();
-  if (tid == (sh.passed < VF_THREADS ? sh.passed : sh.positive)) {  // (where rounding has it pass nowhere: the last token)
-    double x = upto - mine, at = x, r = 0.0;
-    int y = -1;
-    bool open = true;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-      if (open && w[e] > 0.0) y = i0 + e, at = x, r = w[e];
-      x += w[e];
-      open = open && !(w[e] > 0.0 && x > target);
-    }
-    sh.pick = y, sh.at = at, sh.r = r;
-  }
-  __syncthreads();
-}
-
-// Workgroups 0 .. chunks - 1 of a sequence sum a chunk of its stop row each, the last of them looks for the token; workgroup
-// `chunks` writes what the rows before and behind it get (and, at T = 0, the stop row).
-template <int LOADS>
-__global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
-                                                                 VerifyChunk* __restrict__ sums, int* __restrict__ done) {
-  __shared__ VerifySearch sh;
-  const int b = blockIdx.x / (a.chunks + 1), chunk = blockIdx.x - b * (a.chunks + 1), tid = threadIdx.x;
+template <int PER>
+__global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, VerifyStop* __restrict__ stops,
+                                                                 VerifyChunk* __restrict__ sums) {
+  __shared__ VerifyChunk part[PER][VF_WAVES];
+  __shared__ double tot[VF_WAVES], found_at, found_r;
+  __shared__ float found_x;
+  __shared__ int is_last, passed, positive, found;
+  const int groups = (a.chunks + PER - 1) / PER;
+  const int b = blockIdx.x / groups, chunk = (blockIdx.x - b * groups) * PER, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int r0 = vf_row(a, b), r1 = vf_row(a, b + 1);
-  const float temperature = a.temperature[b];
-  const bool warm = temperature > 0.0f;
-  if (r1 <= r0) {
-    if (chunk == a.chunks && tid == 0) a.accepted[b] = 0;
-    return;
-  }
-  if (!warm && chunk < a.chunks) return;
-  const double k = vf_rate(temperature);
-  const int stop = vf_stop(a, parts, r0, r1, warm, k, &sh.found);
-  if (chunk == a.chunks) {
-    if (tid == 0) a.accepted[b] = stop - r0;
-    for (int row = r0 + wave; row < r1; row += VF_WAVES) {
-      if (row > stop) {
-        if (lane == 0) a.tokens[row] = -1, a.logp[row] = 0.0f;
-        continue;
-      }
-      const VerifyRow r = vf_join(a, parts, row, k);
-      const bool none = !(r.max > -INFINITY);
-      if (lane || (row == stop && warm && !none)) continue;
-      const int y = row < stop ? a.draft[row] : none ? -1 : r.first;
-      a.tokens[row] = y;
-      a.logp[row] = y < 0 ? 0.0f : vf_logp(vf_logit(a, row, y), r.max, r.sum, k);
-    }
-    return;
-  }
-  const VerifyRow r = vf_join(a, parts, stop, k);
-  if (!(r.max > -INFINITY)) return;
-  const bool last = stop == r1 - 1;
-  VerifyChunk mine{0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    double w[VF_VEC];
-    float q[VF_VEC];
-    vf_stop_row(a, stop, last, r.max, k, ((chunk * LOADS + i) * VF_THREADS + tid) * VF_VEC, w, q);
-#pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) {
-      const double qz = (double)q[e] * r.sum;
-      mine.all += w[e];
-      if (w[e] > qz) mine.over += w[e], mine.q += (double)q[e];
-      if (fabs(w[e] - qz) <= VF_NEAR * qz) mine.near += VF_NEAR * qz;
-    }
-  }
-  mine.all = vf_wave_sum(mine.all), mine.over = vf_wave_sum(mine.over);
-  mine.q = vf_wave_sum(mine.q), mine.near = vf_wave_sum(mine.near);
-  if (lane == 0) sh.part[wave] = mine;
-  __syncthreads();
+  const int stop = stops[b].row;
+  if (stop < 0) return;
+  const float m = stops[b].max;
+  const double z0 = stops[b].sum, k = vf_rate(a.temperature[b]);
+  const float zf = (float)z0;
+  const bool last = stops[b].last;
+  const int d = last || a.probs ? -1 : a.draft[stop];
   VerifyChunk* const row_sums = sums + (size_t)b * a.chunks;
-  if (tid == 0) {
-    VerifyChunk t = sh.part[0];
-    for (int w = 1; w < VF_WAVES; ++w)
-      t.all += sh.part[w].all, t.over += sh.part[w].over, t.q += sh.part[w].q, t.near += sh.part[w].near;
-    double* const to = &row_sums[chunk].all;
-    __hip_atomic_store(to, t.all, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(to + 1, t.over, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(to + 2, t.q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __hip_atomic_store(to + 3, t.near, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    sh.last = __hip_atomic_fetch_add(&done[b], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+  float xd = -INFINITY;
+  {
+    float x[PER][VF_VEC], q[PER][VF_VEC];
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      vf_stop_row(a, stop, !last && a.probs, d, (chunk + p) * VF_CHUNK + VF_VEC * tid, x[p], q[p]);
+    if (d >= 0 && d < a.V) xd = vf_logit(a, stop, d);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      double all = 0.0, rest = 0.0;
+      float taken = 0.0f, near = 0.0f;
+#pragma unroll
+      for (int e = 0; e < VF_VEC; ++e) {
+        const double w = vf_stop_weight(x[p][e], m, k), r = fma(-(double)q[p][e], z0, w);
+        const float edge = (float)VF_NEAR * q[p][e] * zf;
+        all += w, rest += fmax(r, 0.0);
+        taken += r > 0.0 ? q[p][e] : 0.0f;
+        near += fabsf((float)r) <= edge ? edge : 0.0f;
+      }
+      all = vf_wave_sum(all), rest = vf_wave_sum(rest);
+      taken = wave_sum(taken), near = wave_sum(near);
+      if (lane == 0) part[p][wave] = VerifyChunk{all, rest, (double)taken, 1.01 * (double)near};
+    }
   }
   __syncthreads();
-  if (!sh.last) return;
+  if (tid < 4 * PER && chunk + (tid >> 2) < a.chunks) {  // (a number each: wave 0, which counts the workgroup below)
+    const double* const from = &part[tid >> 2][0].all + (tid & 3);
+    double t = from[0];
+    for (int w = 1; w < VF_WAVES; ++w) t += from[4 * w];
+    __hip_atomic_store(&row_sums[chunk + (tid >> 2)].all + (tid & 3), t, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (wave == 0) {
+    // The sums are stored and loaded past the L2s, and are there before the count rises: no cache has to be written back or
+    // emptied for them (a release and acquire here, which do that, made the launch 108 us for 29).
+    wait_loads<0>();
+    if (lane == 0)
+      is_last = __hip_atomic_fetch_add(&stops[b].done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+  }
+  __syncthreads();
+  if (!is_last) return;
 
-  // the whole row's sums, every wave alike, 64 chunks at a time
-  const auto sum_of = [&](int c) {
+  // The whole row's sums, every wave alike, 64 chunks at a time (the first of them stay in registers).
+  const auto load = [&](int c) {
     VerifyChunk t{0.0, 0.0, 0.0, 0.0};
     if (c < a.chunks) {
       const double* const from = &row_sums[c].all;
       t.all = __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      t.over = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      t.rest = __hip_atomic_load(from + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       t.q = __hip_atomic_load(from + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       t.near = __hip_atomic_load(from + 3, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     return t;
   };
-  VerifyChunk whole{0.0, 0.0, 0.0, 0.0};
-  for (int c0 = 0; c0 < a.chunks; c0 += WAVE) {
-    const VerifyChunk t = sum_of(c0 + lane);
-    whole.all += t.all, whole.over += t.over, whole.q += t.q, whole.near += t.near;
+  const VerifyChunk front = load(lane);
+  double z = front.all, near = front.near;
+  for (int c0 = WAVE; c0 < a.chunks; c0 += WAVE) {
+    const VerifyChunk t = load(c0 + lane);
+    z += t.all, near += t.near;
   }
-  whole.all = vf_wave_sum(whole.all), whole.over = vf_wave_sum(whole.over);
-  whole.q = vf_wave_sum(whole.q), whole.near = vf_wave_sum(whole.near);
-  // (a certain draft's own weight is not in `all`: the row's sum has it)
-  double z = whole.all;
-  if (!last && !a.probs && (unsigned)a.draft[stop] < (unsigned)a.V) z += vf_weight(vf_logit(a, stop, a.draft[stop]), r.max, k);
+  // (a certain draft's own weight is not in `all`)
+  z = vf_wave_sum(z) + vf_stop_weight(xd, m, k), near = vf_wave_sum(near);
+  // r's sum at z: it moves by q for every one that z does
+  const auto rest_of = [&](const VerifyChunk& t) { return fmax(fma(z0 - z, t.q, t.rest), 0.0); };
+  double rest = rest_of(front);
+  for (int c0 = WAVE; c0 < a.chunks; c0 += WAVE) {
+    const VerifyChunk t = load(c0 + lane);
+    rest += rest_of(t);
+  }
+  rest = vf_wave_sum(rest);
+  // The chunk in which the sum passes the target (if rounding has it pass nowhere: the last that has anything).
   const double v = (double)a.v[b];
-  double rest = whole.over - whole.q * z;
-  bool sure = whole.near == 0.0 ? true : rest > 0.0;
-  int token = -1;
-  if (sure && rest > 0.0) {
-    const double target = v * rest;
-    double before = 0.0, at = 0.0;
-    int in = 0;
-    for (int c0 = 0, go = 1; go && c0 < a.chunks; c0 += WAVE) {
-      const VerifyChunk t = sum_of(c0 + lane);
-      const double x = t.over - t.q * z;
-      for (int c = 0; c < WAVE && c0 + c < a.chunks; ++c) {
-        const double y = vf_lane(x, c);
-        if (y > 0.0) {
-          in = c0 + c, before = at;
-          if (at + y > target) {
-            go = 0;
-            break;
-          }
-        }
-        at += y;
-      }
+  double target = v * rest, before = 0.0;
+  int c = -1;
+  {
+    double at = 0.0;
+    VerifyChunk t = front;
+    for (int c0 = 0;;) {
+      const double y = rest_of(t), upto = at + vf_wave_scan(y);
+      const uint64_t some = __ballot(y > 0.0), hit = __ballot(y > 0.0 && upto > target);
+      const int l = hit ? __builtin_ctzll(hit) : some ? 63 - __builtin_clzll(some) : -1;
+      if (l >= 0) c = c0 + l, before = vf_lane(upto - y, l);
+      if (hit || (c0 += WAVE) >= a.chunks) break;
+      at = vf_lane(upto, WAVE - 1);
+      t = load(c0 + lane);
     }
-    vf_search<LOADS>(a, sh, stop, last, r.max, z, k, in, before, target);
-    token = sh.pick;
-    // r's sums up to either side of the token are off by less than `near` from what the 64-bit sum gives
-    sure = whole.near == 0.0 || (token >= 0 && target - sh.at > 2.0 * whole.near && sh.at + sh.r - target > 2.0 * whole.near);
   }
-  if (!sure || token < 0) {  // once more, chunk after chunk; from p where r is 0
-    bool from_p = false;
-    for (int pass = 0; pass < 2; ++pass) {
-      double total = 0.0;
-      for (int c = 0; c < a.chunks; ++c) {
-        vf_search<LOADS>(a, sh, stop, last || from_p, r.max, z, k, c, 0.0, INFINITY);
-        double s = 0.0;
-        for (int w = 0; w < VF_WAVES; ++w) s += sh.tot[w];
-        total += s;
-      }
-      if (total > 0.0) {
-        const double target = v * total;
-        double before = 0.0;
-        for (int c = 0; c < a.chunks; ++c) {
-          vf_search<LOADS>(a, sh, stop, last || from_p, r.max, z, k, c, before, target);
-          if (sh.pick >= 0) token = sh.pick;
-          if (sh.passed < VF_THREADS) break;
-          double s = 0.0;
-          for (int w = 0; w < VF_WAVES; ++w) s += sh.tot[w];
-          before += s;
-        }
-        break;
-      }
-      from_p = true;
+  // The token in it, first from these sums; where the tokens that were too near to say might move it, or r is 0 throughout,
+  // chunk after chunk: r's sum, then its place, of max(w - q z, 0) and if that is 0 of w.
+  enum { QUICK, SUM, PLACE } way = c >= 0 ? QUICK : SUM;
+  if (way == SUM) c = 0, before = 0.0, target = INFINITY;
+  bool from_p = false;
+  int token = -1;
+  for (;;) {
+    __syncthreads();
+    if (tid == 0) passed = VF_THREADS, positive = -1, found = -1;
+    const int i0 = c * VF_CHUNK + VF_VEC * tid;
+    double w[VF_VEC], mine = 0.0;
+    float x[VF_VEC], q[VF_VEC];
+    vf_stop_row(a, stop, !last && !from_p && a.probs, from_p ? -1 : d, i0, x, q);
+#pragma unroll
+    for (int e = 0; e < VF_VEC; ++e) mine += w[e] = fmax(fma(-(double)q[e], z, vf_stop_weight(x[e], m, k)), 0.0);
+    double upto = vf_wave_scan(mine);
+    if (lane == WAVE - 1) tot[wave] = upto;
+    __syncthreads();
+    double sum = 0.0;
+    for (int y = 0; y < VF_WAVES; ++y) {
+      if (y == wave) upto += before + sum;
+      sum += tot[y];
     }
+    if (mine > 0.0) {
+      atomicMax(&positive, tid);
+      if (upto > target) atomicMin(&passed, tid);
+    }
+    __syncthreads();
+    const int who = passed < VF_THREADS ? passed : positive;
+    if (tid == who) {
+      double at = upto - mine, at_y = at, r = 0.0;
+      float xy = 0.0f;
+      int y = -1;
+      bool open = true;
+#pragma unroll
+      for (int e = 0; e < VF_VEC; ++e) {
+        if (open && w[e] > 0.0) y = i0 + e, at_y = at, r = w[e], xy = x[e];
+        at += w[e];
+        open = open && !(w[e] > 0.0 && at > target);
+      }
+      found = y, found_at = at_y, found_r = r, found_x = xy;
+    }
+    __syncthreads();
+    if (who >= 0) token = found;
+    if (way == QUICK) {
+      // (the chunks' sums, and with them the target, are off by `near` at most)
+      if (who >= 0 && (near == 0.0 || (target - found_at > 2.0 * near && found_at + found_r - target > 2.0 * near))) break;
+      way = SUM, c = 0, before = 0.0, target = INFINITY, token = -1;
+      continue;
+    }
+    if (way == PLACE && passed < VF_THREADS) break;
+    before += sum;
+    if (++c < a.chunks) continue;
+    if (way == PLACE) break;
+    if (before > 0.0) way = PLACE, target = v * before, token = -1;
+    else if (from_p) break;
+    else from_p = true;
+    c = 0, before = 0.0;
   }
   if (tid == 0) {
     a.tokens[stop] = token;
-    a.logp[stop] = token < 0 ? 0.0f : vf_logp(vf_logit(a, stop, token), r.max, z, k);
+    a.logp[stop] = token < 0 ? 0.0f : vf_logp(found_x, m, z, k);
   }
 }
 
@@ -555,41 +551,46 @@ static int verify_loads(long n, int num_cu) {  // loads of a thread: 4 where eno
 }
 static int verify_units(int V, int per) { return (V + per - 1) / per; }
 
-bool verify_grid_ok(int N, int V) { return (long)N * (verify_units(V, WAVE * VF_VEC) + 1L) <= 0xffffffL; }
+bool verify_grid_ok(int N, int V) { return (long)N * verify_units(V, WAVE * VF_VEC) <= 0xffffffL; }
 
 size_t verify_workspace_bytes(int N, int V, int B, int num_cu) {
   const int parts = verify_units(V, WAVE * VF_VEC * verify_loads((long)N * V, num_cu));
-  const int chunks = verify_units(V, VF_THREADS * VF_VEC * verify_loads((long)B * V, num_cu));
-  return (size_t)N * parts * sizeof(VerifyPart) + (size_t)B * chunks * sizeof(VerifyChunk) + (size_t)B * sizeof(int);
+  return (size_t)N * parts * sizeof(VerifyPart) + (size_t)B * (verify_units(V, VF_CHUNK) * sizeof(VerifyChunk) + sizeof(VerifyStop));
 }
 
 hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* draft, const void* probs, int q_fp32,
                          long q_row, const int* cu, const float* u, const float* v, const float* temperature, int* tokens,
                          int* accepted, float* logp, void* ws, int N, int V, int B, int num_cu, hipStream_t s) {
-  const int rows = verify_loads((long)N * V, num_cu), pick = verify_loads((long)B * V, num_cu);
+  const int loads = verify_loads((long)N * V, num_cu);
   VerifyArgs a{logits, probs, draft, cu, u, v, temperature, tokens, accepted, logp, l_row, q_row, l_fp32, q_fp32,
-               N, V, B, verify_units(V, WAVE * VF_VEC * rows), verify_units(V, VF_THREADS * VF_VEC * pick)};
+               N, V, B, verify_units(V, WAVE * VF_VEC * loads), verify_units(V, VF_CHUNK)};
   VerifyPart* const parts = static_cast<VerifyPart*>(ws);
   VerifyChunk* const sums = reinterpret_cast<VerifyChunk*>(parts + (size_t)N * a.parts);
-  int* const done = reinterpret_cast<int*>(sums + (size_t)B * a.chunks);
+  VerifyStop* const stops = reinterpret_cast<VerifyStop*>(sums + (size_t)B * a.chunks);
   const unsigned groups = (unsigned)(((long)N * a.parts + VF_WAVES - 1) / VF_WAVES);
-  const auto first = [&](auto kernel) {
-    return launch("verify_rows_kernel", kernel, dim3(groups), dim3(VF_THREADS), s, a, parts, done);
-  };
-  const auto second = [&](auto kernel) {
-    return launch("verify_pick_kernel", kernel, dim3((unsigned)B * (a.chunks + 1)), dim3(VF_THREADS), s, a, parts, sums, done);
+  const auto rows = [&](auto kernel) {
+    return launch("verify_rows_kernel", kernel, dim3(groups), dim3(VF_THREADS), s, a, parts);
   };
   hipError_t e = hipSuccess;
   if (N > 0 && l_fp32)
-    e = rows == 4   ? first(verify_rows_kernel<float, 4>)
-        : rows == 2 ? first(verify_rows_kernel<float, 2>)
-                    : first(verify_rows_kernel<float, 1>);
+    e = loads == 4   ? rows(verify_rows_kernel<float, 4>)
+        : loads == 2 ? rows(verify_rows_kernel<float, 2>)
+                     : rows(verify_rows_kernel<float, 1>);
   else if (N > 0)
-    e = rows == 4   ? first(verify_rows_kernel<uint16_t, 4>)
-        : rows == 2 ? first(verify_rows_kernel<uint16_t, 2>)
-                    : first(verify_rows_kernel<uint16_t, 1>);
-  if (e != hipSuccess) return e;
-  return pick == 4 ? second(verify_pick_kernel<4>) : pick == 2 ? second(verify_pick_kernel<2>) : second(verify_pick_kernel<1>);
+    e = loads == 4   ? rows(verify_rows_kernel<uint16_t, 4>)
+        : loads == 2 ? rows(verify_rows_kernel<uint16_t, 2>)
+                     : rows(verify_rows_kernel<uint16_t, 1>);
+  if (e == hipSuccess)
+    e = launch("verify_stop_kernel", verify_stop_kernel, dim3(B), dim3(VF_STOP_THREADS), s, a, parts, stops);
+  if (e != hipSuccess || N == 0) return e;
+  // as many chunks a workgroup as leave them all at once on the CUs (4 each), 4 at most
+  const long at_once = 4L * num_cu, all = (long)B * a.chunks;
+  const int per = all >= 4 * at_once ? 4 : all >= 2 * at_once ? 2 : 1;
+  const auto pick = [&](auto kernel) {
+    return launch("verify_pick_kernel", kernel, dim3((unsigned)(B * verify_units(a.chunks, per))), dim3(VF_THREADS), s, a,
+                  stops, sums);
+  };
+  return per == 4 ? pick(verify_pick_kernel<4>) : per == 2 ? pick(verify_pick_kernel<2>) : pick(verify_pick_kernel<1>);
 }
 
 }  // namespace dsa
