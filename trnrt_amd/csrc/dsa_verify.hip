@@ -82,7 +82,10 @@ __device__ __forceinline__ void vf_load(const T* row, int i, int V, float none, 
     for (int e = 0; e < VF_VEC; ++e) x[e] = vf_value(u.x[e]);
   } else {
 #pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) x[e] = i + e < V ? vf_value(row[i + e]) : none;
+    for (int e = 0; e < VF_VEC; ++e) {
+      const float y = vf_value(row[min(i + e, V - 1)]);
+      x[e] = i + e < V ? y : none;
+    }
   }
 }
 
@@ -114,17 +117,15 @@ __device__ __forceinline__ double vf_exponent(float l, float m, double k) {
 __device__ __forceinline__ double vf_exp2(double x) {
   x = fmax(x, -1022.0);
   const double big = 6755399441055744.0, n = x + big, f = x - (n - big);
-  double p = 7.0549116208011233299e-9;  // (ln 2)^k / k!
-  p = fma(p, f, 1.0178086009239699728e-7);
-  p = fma(p, f, 1.3215486790144309488e-6);
-  p = fma(p, f, 1.5252733804059840280e-5);
-  p = fma(p, f, 1.5403530393381609954e-4);
-  p = fma(p, f, 1.3333558146428443423e-3);
-  p = fma(p, f, 9.6181291076284771620e-3);
-  p = fma(p, f, 5.5504108664821579953e-2);
-  p = fma(p, f, 2.4022650695910071233e-1);
-  p = fma(p, f, 6.9314718055994530942e-1);
-  p = fma(p, f, 1.0);
+  // (ln 2)^k / k!, in scalar registers: as literals each would be moved into the accumulator's first
+  double c[11] = {1.0, 6.9314718055994530942e-1, 2.4022650695910071233e-1, 5.5504108664821579953e-2, 9.6181291076284771620e-3,
+                  1.3333558146428443423e-3, 1.5403530393381609954e-4, 1.5252733804059840280e-5, 1.3215486790144309488e-6,
+                  1.0178086009239699728e-7, 7.0549116208011233299e-9};
+#pragma unroll
+  for (int i = 0; i <= 10; ++i) asm("" : "+s"(c[i]));
+  double p = c[10];
+#pragma unroll
+  for (int i = 9; i >= 0; --i) p = fma(p, f, c[i]);
   const long long u = __builtin_bit_cast(long long, p);
   const int hi = (int)(u >> 32) + ((int)__builtin_bit_cast(long long, n) << 20);
   return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)u);
@@ -334,8 +335,8 @@ __global__ __launch_bounds__(VF_STOP_THREADS) void verify_stop_kernel(VerifyArgs
 
 // Logits x and the draft's probabilities q (0 where there are none) of tokens i .. i + 7 of the stop row. A draft that is
 // certain, d, cannot come (-1: there is no such draft).
-__device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool with_q, int d, int i, float (&x)[VF_VEC],
-                                            float (&q)[VF_VEC]) {
+__device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool with_q, int d, bool infinite, int i,
+                                            float (&x)[VF_VEC], float (&q)[VF_VEC]) {
   if (a.l_fp32)
     vf_load(static_cast<const float*>(a.logits) + (size_t)row * a.l_row, i, a.V, -INFINITY, x);
   else
@@ -343,6 +344,10 @@ __device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool w
   if (d >= i && d < i + VF_VEC) {
 #pragma unroll
     for (int e = 0; e < VF_VEC; ++e) x[e] = i + e == d ? -INFINITY : x[e];
+  }
+  if (infinite) {  // (one of several: as many times 0)
+#pragma unroll
+    for (int e = 0; e < VF_VEC; ++e) x[e] = x[e] == INFINITY ? 0.0f : -INFINITY;
   }
 #pragma unroll
   for (int e = 0; e < VF_VEC; ++e) q[e] = 0.0f;
@@ -354,9 +359,9 @@ __device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool w
   }
 }
 
-// A weight of the stop row.
+// A weight of the stop row (m is finite there).
 __device__ __forceinline__ double vf_stop_weight(float x, float m, double k) {
-  const double w = m < INFINITY ? vf_exp2(((double)x - (double)m) * k) : x == m ? 1.0 : 0.0;
+  const double w = vf_exp2(((double)x - (double)m) * k);
   return x > -INFINITY ? w : 0.0;
 }
 
@@ -382,13 +387,14 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
   __shared__ VerifyChunk part[PER][VF_WAVES];
   __shared__ double tot[VF_WAVES], found_at, found_r;
   __shared__ float found_x;
-  __shared__ int is_last, passed, positive, found;
+  __shared__ int is_last, found, first[VF_WAVES], end[VF_WAVES];
   const int groups = (a.chunks + PER - 1) / PER;
   const int b = blockIdx.x / groups, chunk = (blockIdx.x - b * groups) * PER, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int stop = stops[b].row;
   if (stop < 0) return;
-  const float m = stops[b].max;
+  const bool infinite = stops[b].max == INFINITY;
+  const float m = infinite ? 0.0f : stops[b].max;
   const double z0 = stops[b].sum, k = vf_rate(a.temperature[b]);
   const float zf = (float)z0;
   const bool last = stops[b].last;
@@ -399,8 +405,11 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
     float x[PER][VF_VEC], q[PER][VF_VEC];
 #pragma unroll
     for (int p = 0; p < PER; ++p)
-      vf_stop_row(a, stop, !last && a.probs, d, (chunk + p) * VF_CHUNK + VF_VEC * tid, x[p], q[p]);
-    if (d >= 0 && d < a.V) xd = vf_logit(a, stop, d);
+      vf_stop_row(a, stop, !last && a.probs, d, infinite, (chunk + p) * VF_CHUNK + VF_VEC * tid, x[p], q[p]);
+    if (d >= 0 && d < a.V) {
+      xd = vf_logit(a, stop, d);
+      if (infinite) xd = xd == INFINITY ? 0.0f : -INFINITY;
+    }
 #pragma unroll
     for (int p = 0; p < PER; ++p) {
       double all = 0.0, rest = 0.0;
@@ -487,12 +496,10 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
   bool from_p = false;
   int token = -1;
   for (;;) {
-    __syncthreads();
-    if (tid == 0) passed = VF_THREADS, positive = -1, found = -1;
     const int i0 = c * VF_CHUNK + VF_VEC * tid;
     double w[VF_VEC], mine = 0.0;
     float x[VF_VEC], q[VF_VEC];
-    vf_stop_row(a, stop, !last && !from_p && a.probs, from_p ? -1 : d, i0, x, q);
+    vf_stop_row(a, stop, !last && !from_p && a.probs, from_p ? -1 : d, infinite, i0, x, q);
 #pragma unroll
     for (int e = 0; e < VF_VEC; ++e) mine += w[e] = fmax(fma(-(double)q[e], z, vf_stop_weight(x[e], m, k)), 0.0);
     double upto = vf_wave_scan(mine);
@@ -503,12 +510,15 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
       if (y == wave) upto += before + sum;
       sum += tot[y];
     }
-    if (mine > 0.0) {
-      atomicMax(&positive, tid);
-      if (upto > target) atomicMin(&passed, tid);
+    const uint64_t some = __ballot(mine > 0.0), hit = __ballot(mine > 0.0 && upto > target);
+    if (lane == 0) {
+      first[wave] = hit ? tid + __builtin_ctzll(hit) : VF_THREADS;
+      end[wave] = some ? tid + 63 - __builtin_clzll(some) : -1;
     }
     __syncthreads();
-    const int who = passed < VF_THREADS ? passed : positive;
+    int passed = VF_THREADS, who = -1;
+    for (int y = VF_WAVES - 1; y >= 0; --y) passed = min(passed, first[y]), who = max(who, end[y]);
+    if (passed < VF_THREADS) who = passed;
     if (tid == who) {
       double at = upto - mine, at_y = at, r = 0.0;
       float xy = 0.0f;
