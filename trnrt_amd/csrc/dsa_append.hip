@@ -4,13 +4,24 @@
 //   2R of y's columns rotated by the token's positions (dsa_rope.h);
 //   s = max(absmax(y), 1e-30) / 448, cache[slot] = e4m3(clamp(y / s)), scale[slot] = s.
 // Everything between the row's load and its store is in fp32 and is rounded once.
+//
+// 16 lanes have a row (a row of the DPP network: its sums and maxima never leave it), 8 of its columns at a time each, so that
+// rows of 576 and of 128 columns both leave few lanes idle; a wave has the rows of one kind of 4 tokens. What bounds it is
+// vector issue, about 300 instructions a token and wave, then the rows' bytes.
 #include "dsa_append.h"
 
 namespace dsa {
 
 constexpr int AP_WAVES = 4;
-constexpr int AP_GROUPS = AP_MAX_WIDTH / (8 * WAVE);  // of 8 columns that a lane holds
+constexpr int AP_LANES = 16;                            // of a row
+constexpr int AP_TOKENS = WAVE / AP_LANES;              // of a wave
 constexpr float AP_FP8_MAX = 448.0f;
+
+template <int R>
+struct ApWave {  // LDS of a wave: its tokens' (cos, sin), and the rotated columns where pairs lie apart
+  float2 cs[AP_TOKENS][R];
+  float x[AP_TOKENS][2 * R];
+};
 
 __device__ __forceinline__ void ap_load8(const void* p, int fp32, long at, float (&v)[8]) {
   if (fp32) {
@@ -28,76 +39,82 @@ __device__ __forceinline__ void ap_load8(const void* p, int fp32, long at, float
   }
 }
 
-// The number of sequences that end by row t (cu ascends), the same in every lane.
+__device__ __forceinline__ void ap_wave_sync() {  // (LDS accesses of a wave are in order; so must the compiler's be)
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The number of sequences that end by token t (cu ascends), each row of 16 lanes its own t.
 __device__ __forceinline__ int ap_sequence(const int* __restrict__ cu, int B, int t) {
-  const int lane = threadIdx.x & (WAVE - 1);
+  const int lane = threadIdx.x & (WAVE - 1), j = lane & (AP_LANES - 1);
   int lo = 0, hi = B;  // the answer is in [lo, hi]
-  while (hi > lo) {
-    const int step = (hi - lo + WAVE - 1) / WAVE, at = min(lo + (lane + 1) * step, hi);
-    const int n = __popcll(__ballot(lo + (lane + 1) * step <= hi && cu[at] <= t));
-    const int to = lo + n * step;  // (cu[to] <= t)
+  while (__ballot(hi > lo)) {
+    const int step = max((hi - lo + AP_LANES - 1) / AP_LANES, 1), at = lo + (j + 1) * step;
+    const uint64_t below = __ballot(at <= hi && cu[min(at, hi)] <= t);
+    const int to = lo + step * __popc((uint32_t)(below >> (lane & ~(AP_LANES - 1))) & 0xffffu);
     hi = min(hi, to + step - 1);
     lo = to;
   }
   return lo;
 }
 
-// One wave per token and kind of rows.
-__global__ __launch_bounds__(AP_WAVES* WAVE) void cache_append_kernel(AppendSet set, RopeAngles a,
-                                                                      const int* __restrict__ table,
-                                                                      const int* __restrict__ ctx_len,
-                                                                      const int* __restrict__ cu, int T, int B,
-                                                                      int max_pages, int page_size, int num_pages) {
-  __shared__ float stage[AP_WAVES][2 * RP_MAX_R];
-  const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const long unit = (long)blockIdx.x * AP_WAVES + wave;
-  const int t = (int)(unit / set.n), kind = (int)(unit - (long)t * set.n);
-  if (t >= T) return;
-  const AppendRows& r = set.rows[kind];
-  const int G = r.width / 8;
-  float v[AP_GROUPS][8];
-#pragma unroll
-  for (int i = 0; i < AP_GROUPS; ++i)  // (lanes past the row load its last columns)
-    ap_load8(r.x, r.fp32, (long)t * r.x_row + 8 * min(lane + WAVE * i, G - 1), v[i]);
-
-  // the token's place and slot
+// A token's slot, -1 where it is not written; place: where it stands in its sequence.
+__device__ __forceinline__ long ap_slot(const int* __restrict__ table, const int* __restrict__ ctx_len,
+                                        const int* __restrict__ cu, int t, int T, int B, int max_pages, int page_size,
+                                        int num_pages, int& place) {
   int b, j, n;
   if (cu) {
-    if (t < cu[0]) return;
     b = ap_sequence(cu, B, t);
-    if (b >= B) return;  // (rows past the last sequence)
+    if (b >= B || t < cu[0]) return -1;  // (in no sequence)
     j = t - cu[b], n = cu[b + 1] - cu[b];
   } else {
     n = T / B, b = t / n, j = t - b * n;
   }
-  const long place = (long)ctx_len[b] - n + j;
-  if (place < 0 || place >= (long)max_pages * page_size) return;
-  const int page = table[(size_t)b * max_pages + place / page_size];
-  if (page < 1 || page >= num_pages) return;
-  const long slot = (long)page * page_size + place % page_size;
+  const long at = (long)ctx_len[b] - n + j;
+  if (at < 0 || at >= (long)max_pages * page_size) return -1;
+  place = (int)at;
+  const int page = table[(size_t)b * max_pages + at / page_size];
+  return page < 1 || page >= num_pages ? -1 : (long)page * page_size + at % page_size;
+}
+
+// Rows of up to 128 NG columns: group i of a lane is columns 8 (16 i + j) .. + 7.
+template <int NG, int R>
+__device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a, const int* __restrict__ table,
+                                        const int* __restrict__ ctx_len, const int* __restrict__ cu, int t0, int T, int B,
+                                        int max_pages, int page_size, int num_pages, ApWave<R>& sh) {
+  const int lane = threadIdx.x & (WAVE - 1), j = lane & (AP_LANES - 1), tok = lane / AP_LANES;
+  const int t = min(t0 + tok, T - 1), G = r.width / 8;
+  float v[NG][8];
+#pragma unroll
+  for (int i = 0; i < NG; ++i)  // (lanes past the row load its last columns)
+    if (AP_LANES * i < G) ap_load8(r.x, r.fp32, (long)t * r.x_row + 8 * min(j + AP_LANES * i, G - 1), v[i]);
+  int place = 0;
+  long slot = ap_slot(table, ctx_len, cu, t, T, B, max_pages, page_size, num_pages, place);
+  if (t0 + tok >= T) slot = -1;
 
   if (r.weight) {
-    const int NG = r.norm_width / 8;
+    const int N = r.norm_width / 8;
+    const float count = 1.0f / (float)r.norm_width;
     float sum = 0.0f, mean = 0.0f;
     if (r.bias) {
 #pragma unroll
-      for (int i = 0; i < AP_GROUPS; ++i)
-        if (lane + WAVE * i < NG)
+      for (int i = 0; i < NG; ++i)
+        if (j + AP_LANES * i < N)
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum += v[i][e];
-      mean = wave_sum(sum) / (float)r.norm_width;
+      mean = row_sum(sum) * count;
     }
     sum = 0.0f;
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i)
-      if (lane + WAVE * i < NG)
+    for (int i = 0; i < NG; ++i)
+      if (j + AP_LANES * i < N)
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e] - mean, v[i][e] - mean, sum);
-    const float inv = 1.0f / sqrtf(wave_sum(sum) / (float)r.norm_width + r.eps);
+    const float inv = 1.0f / sqrtf(fmaf(row_sum(sum), count, r.eps));
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i) {
-      const int g = lane + WAVE * i;
-      if (g >= NG) break;
+    for (int i = 0; i < NG; ++i) {
+      const int g = j + AP_LANES * i;
+      if (g >= N) continue;
       float w[8], c[8] = {};
       ap_load8(r.weight, r.norm_fp32, 8 * g, w);
       if (r.bias) ap_load8(r.bias, r.norm_fp32, 8 * g, c);
@@ -106,66 +123,84 @@ __global__ __launch_bounds__(AP_WAVES* WAVE) void cache_append_kernel(AppendSet 
     }
   }
 
-  if (r.rope_at >= 0) {  // the rotated columns through LDS, a pair a lane
-    float* const st = stage[wave];
+  if (r.rope_at >= 0) {
     const int g0 = r.rope_at / 8, ng = a.R / 4;
+    for (int f = j; f < a.R; f += AP_LANES)
+      sh.cs[tok][f] = rope_angle(a, a.positions ? a.positions[(size_t)rope_axis(a, f) * T + t] : place, f);
+    if (r.half) {
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i) {
-      const int g = lane + WAVE * i - g0;
-      if (g >= 0 && g < ng)
+      for (int i = 0; i < NG; ++i) {
+        const int g = j + AP_LANES * i - g0;
+        if (g >= 0 && g < ng)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) st[8 * g + e] = v[i][e];
+          for (int e = 0; e < 8; ++e) sh.x[tok][8 * g + e] = v[i][e];
+      }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    for (int f = lane; f < a.R; f += WAVE) {
-      const int pos = a.positions ? a.positions[(size_t)rope_axis(a, f) * T + t] : (int)place;
-      const float2 cs = rope_angle(a, pos, f);
-      const int p = r.half ? f : 2 * f, q = r.half ? f + a.R : 2 * f + 1;
-      float x = st[p], y = st[q];
-      turn_pair(x, y, cs);
-      st[p] = x, st[q] = y;
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    ap_wave_sync();
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i) {
-      const int g = lane + WAVE * i - g0;
-      if (g >= 0 && g < ng)
+    for (int i = 0; i < NG; ++i) {
+      const int g = j + AP_LANES * i - g0;
+      if (g < 0 || g >= ng) continue;
+      if (r.half) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[i][e] = st[8 * g + e];
+        for (int e = 0; e < 8; ++e) {  // (column c: of pair c, or c - R)
+          const int c = 8 * g + e;
+          float x = c < a.R ? v[i][e] : sh.x[tok][c - a.R], y = c < a.R ? sh.x[tok][c + a.R] : v[i][e];
+          turn_pair(x, y, sh.cs[tok][c < a.R ? c : c - a.R]);
+          v[i][e] = c < a.R ? x : y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) turn_pair(v[i][e], v[i][e + 1], sh.cs[tok][4 * g + e / 2]);
+      }
     }
   }
 
   if (r.cache_bf16) {
+    if (slot < 0) return;
     uint16_t* const row = static_cast<uint16_t*>(r.cache) + (size_t)slot * r.width;
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i) {
-      const int g = lane + WAVE * i;
+    for (int i = 0; i < NG; ++i) {
+      const int g = j + AP_LANES * i;
       if (g < G)
         *reinterpret_cast<u32x4*>(row + 8 * g) = u32x4{bf16_pack(v[i][0], v[i][1]), bf16_pack(v[i][2], v[i][3]),
                                                        bf16_pack(v[i][4], v[i][5]), bf16_pack(v[i][6], v[i][7])};
     }
     return;
   }
+  // The quotient by s, correctly rounded as store's is: the product with the (correctly rounded) reciprocal, corrected by the
+  // remainder, which is exact; only a divisor whose mantissa is all ones needs the division itself, and an infinite one no
+  // correction. (A division a value took 44 of the kernel's NNN us.)
   float s = 1.0f;
   if (r.scale) {
     float amax = 0.0f;
 #pragma unroll
-    for (int i = 0; i < AP_GROUPS; ++i)
+    for (int i = 0; i < NG; ++i)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = lane + WAVE * i < G ? fmaxf(amax, fabsf(v[i][e])) : amax;
-    s = fmaxf(wave_max(amax), 1e-30f) / AP_FP8_MAX;
-    if (lane == 0) r.scale[slot] = s;
+      for (int e = 0; e < 8; ++e) amax = j + AP_LANES * i < G ? fmaxf(amax, fabsf(v[i][e])) : amax;
+    s = fmaxf(row_max(amax), 1e-30f) / AP_FP8_MAX;
+    if (slot >= 0 && j == 0) r.scale[slot] = s;
   }
+  if (slot < 0) return;
+  const float inv = 1.0f / s;
+  const bool ones = (__float_as_uint(s) & 0x7fffffu) == 0x7fffffu, correct = s < INFINITY;
   uint8_t* const row = static_cast<uint8_t*>(r.cache) + (size_t)slot * r.width;
 #pragma unroll
-  for (int i = 0; i < AP_GROUPS; ++i) {
-    const int g = lane + WAVE * i;
-    if (g >= G) break;
+  for (int i = 0; i < NG; ++i) {
+    const int g = j + AP_LANES * i;
+    if (g >= G) continue;
     float q[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(v[i][e] / s, -r.fp8_max), r.fp8_max);
+    for (int e = 0; e < 8; ++e) {
+      const float p = v[i][e] * inv;
+      q[e] = correct ? fmaf(fmaf(-p, s, v[i][e]), inv, p) : p;
+    }
+    if (ones) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = v[i][e] / s;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], -r.fp8_max), r.fp8_max);
     int lo = 0, hi = 0;
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
@@ -175,11 +210,35 @@ __global__ __launch_bounds__(AP_WAVES* WAVE) void cache_append_kernel(AppendSet 
   }
 }
 
+// For rows of up to 128 NG columns and R frequencies.
+template <int NG, int R>
+__global__ __launch_bounds__(AP_WAVES* WAVE) void cache_append_kernel(AppendSet set, RopeAngles a,
+                                                                      const int* __restrict__ table,
+                                                                      const int* __restrict__ ctx_len,
+                                                                      const int* __restrict__ cu, int T, int B,
+                                                                      int max_pages, int page_size, int num_pages) {
+  __shared__ ApWave<R> sh[AP_WAVES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const long unit = (long)blockIdx.x * AP_WAVES + wave;
+  const int four = (int)(unit / set.n), t0 = four * AP_TOKENS;
+  if (t0 >= T) return;
+  const AppendRows& r = set.rows[unit - (long)four * set.n];
+  if (r.width <= 128)
+    ap_rows<1>(r, a, table, ctx_len, cu, t0, T, B, max_pages, page_size, num_pages, sh[wave]);
+  else
+    ap_rows<NG>(r, a, table, ctx_len, cu, t0, T, B, max_pages, page_size, num_pages, sh[wave]);
+}
+
 hipError_t launch_cache_append(const AppendSet& set, const RopeAngles& a, const int* table, const int* ctx_len,
                                const int* cu, int T, int B, int max_pages, int page_size, int num_pages, hipStream_t s) {
-  const long units = (long)T * set.n;
-  return launch("cache_append_kernel", cache_append_kernel, dim3((unsigned)((units + AP_WAVES - 1) / AP_WAVES)),
-                dim3(AP_WAVES * WAVE), s, set, a, table, ctx_len, cu, T, B, max_pages, page_size, num_pages);
+  const long units = ((long)T + AP_TOKENS - 1) / AP_TOKENS * set.n;
+  int width = 0;
+  for (int i = 0; i < set.n; ++i) width = width > set.rows[i].width ? width : set.rows[i].width;
+  const auto go = [&](auto kernel) {
+    return launch("cache_append_kernel", kernel, dim3((unsigned)((units + AP_WAVES - 1) / AP_WAVES)), dim3(AP_WAVES * WAVE), s,
+                  set, a, table, ctx_len, cu, T, B, max_pages, page_size, num_pages);
+  };
+  return width <= 640 && a.R <= 64 ? go(cache_append_kernel<5, 64>) : go(cache_append_kernel<AP_MAX_WIDTH / 128, RP_MAX_R>);
 }
 
 }  // namespace dsa
