@@ -1,7 +1,7 @@
 """Rotary positions (trnrt_amd/kernels/dsa_rope.py) against their definition in float64.
 
 Tolerance, from the arithmetic: the reduced angle is rounded once to fp32 in turns (at most 2^-26 of them, 1e-7 radians),
-sincospi is good to 4 units of 2^-24 (2.4e-7), so cos and sin are off by less than 4e-7 each, times the factor's two roundings;
+the series for cos and sin are good to 2^-23 (1.2e-7), so these are off by less than 2.3e-7 each, times the factor's roundings;
 a result is one product and one fma of them (2^-23 of the sizes): less than 6e-7 factor (|x0| + |x1|) in all, for which 1e-6 is
 taken, then the output's rounding (2^-8 or 2^-24 of the value)."""
 

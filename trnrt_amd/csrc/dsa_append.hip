@@ -23,14 +23,16 @@ struct ApWave {  // LDS of a wave: its tokens' (cos, sin), and the rotated colum
   float x[AP_TOKENS][2 * R];
 };
 
-__device__ __forceinline__ void ap_load8(const void* p, int fp32, long at, float (&v)[8]) {
-  if (fp32) {
-    const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + at);
+// Eight values of type T from p + n on; p is a lane's own address, n the same in every lane.
+template <typename T>
+__device__ __forceinline__ void ap_load8(const T* p, int n, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4* q = reinterpret_cast<const f32x4*>(p + n);
     const f32x4 a = q[0], b = q[1];
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = a[e], v[4 + e] = b[e];
   } else {
-    const u32x4 u = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + at);
+    const u32x4 u = *reinterpret_cast<const u32x4*>(p + n);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[2 * e] = __uint_as_float(u[e] << 16);
@@ -73,8 +75,9 @@ __device__ __forceinline__ long ap_slot(const int* __restrict__ table, const int
   const long at = (long)ctx_len[b] - n + j;
   if (at < 0 || at >= (long)max_pages * page_size) return -1;
   place = (int)at;
-  const int page = table[(size_t)b * max_pages + at / page_size];
-  return page < 1 || page >= num_pages ? -1 : (long)page * page_size + at % page_size;
+  const uint32_t col = (uint32_t)place / (uint32_t)page_size;
+  const int page = table[(size_t)b * max_pages + col];
+  return page < 1 || page >= num_pages ? -1 : (long)page * page_size + (place - (int)col * page_size);
 }
 
 // Rows of up to 128 NG columns: group i of a lane is columns 8 (16 i + j) .. + 7.
@@ -84,10 +87,22 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
                                         int max_pages, int page_size, int num_pages, ApWave<R>& sh) {
   const int lane = threadIdx.x & (WAVE - 1), j = lane & (AP_LANES - 1), tok = lane / AP_LANES;
   const int t = min(t0 + tok, T - 1), G = r.width / 8;
+  const int full = G / AP_LANES, rest = G % AP_LANES;  // groups of every lane, and lanes with one more
   float v[NG][8];
+  const auto load = [&](auto* x) {
+    x += (long)t * r.x_row + 8 * j;
 #pragma unroll
-  for (int i = 0; i < NG; ++i)  // (lanes past the row load its last columns)
-    if (AP_LANES * i < G) ap_load8(r.x, r.fp32, (long)t * r.x_row + 8 * min(j + AP_LANES * i, G - 1), v[i]);
+    for (int i = 0; i < NG; ++i) {
+      if (i < full) ap_load8(x, 8 * AP_LANES * i, v[i]);
+      if (i == full) {  // (the other lanes' are 0)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
+        if (j < rest) ap_load8(x, 8 * AP_LANES * i, v[i]);
+      }
+    }
+  };
+  if (r.fp32) load(static_cast<const float*>(r.x));
+  else load(static_cast<const uint16_t*>(r.x));
   int place = 0;
   long slot = ap_slot(table, ctx_len, cu, t, T, B, max_pages, page_size, num_pages, place);
   if (t0 + tok >= T) slot = -1;
@@ -95,38 +110,55 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
   if (r.weight) {
     const int N = r.norm_width / 8;
     const float count = 1.0f / (float)r.norm_width;
-    float sum = 0.0f, mean = 0.0f;
     if (r.bias) {
+      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < NG; ++i)
         if (j + AP_LANES * i < N)
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum += v[i][e];
-      mean = row_sum(sum) * count;
+      const float mean = row_sum(sum) * count;
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+        if (j + AP_LANES * i < N)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] -= mean;
     }
-    sum = 0.0f;
+    float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NG; ++i)
       if (j + AP_LANES * i < N)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e] - mean, v[i][e] - mean, sum);
+        for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e], v[i][e], sum);
     const float inv = 1.0f / sqrtf(fmaf(row_sum(sum), count, r.eps));
+    const auto apply = [&](auto* w, auto* c) {
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const int g = j + AP_LANES * i;
-      if (g >= N) continue;
-      float w[8], c[8] = {};
-      ap_load8(r.weight, r.norm_fp32, 8 * g, w);
-      if (r.bias) ap_load8(r.bias, r.norm_fp32, 8 * g, c);
+      for (int i = 0; i < NG; ++i) {
+        if (j + AP_LANES * i >= N) continue;
+        float x[8];
+        ap_load8(w + 8 * j, 8 * AP_LANES * i, x);
+        if (c) {
+          float y[8];
+          ap_load8(c + 8 * j, 8 * AP_LANES * i, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[i][e] = fmaf((v[i][e] - mean) * inv, w[e], c[e]);
-    }
+          for (int e = 0; e < 8; ++e) v[i][e] = fmaf(v[i][e] * inv, x[e], y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * inv * x[e];
+        }
+      }
+    };
+    if (r.norm_fp32) apply(static_cast<const float*>(r.weight), static_cast<const float*>(r.bias));
+    else apply(static_cast<const uint16_t*>(r.weight), static_cast<const uint16_t*>(r.bias));
   }
 
   if (r.rope_at >= 0) {
     const int g0 = r.rope_at / 8, ng = a.R / 4;
-    for (int f = j; f < a.R; f += AP_LANES)
-      sh.cs[tok][f] = rope_angle(a, a.positions ? a.positions[(size_t)rope_axis(a, f) * T + t] : place, f);
+    for (int f = j, n = 0; f < a.R; f += AP_LANES, ++n) {
+      static_assert(AP_LANES == 16, "frequencies whose axes one word holds");
+      const uint32_t axis = (a.axis[n] >> (2 * j)) & 3;
+      sh.cs[tok][f] = rope_angle(a, a.positions ? a.positions[axis * (uint32_t)T + (uint32_t)t] : place, f);
+    }
     if (r.half) {
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
@@ -173,18 +205,20 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
   // correction. (A division a value took 44 of the kernel's NNN us.)
   float s = 1.0f;
   if (r.scale) {
-    float amax = 0.0f;
+    float amax = 0.0f;  // (columns past the row are 0)
 #pragma unroll
     for (int i = 0; i < NG; ++i)
+      if (AP_LANES * i < G)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) amax = j + AP_LANES * i < G ? fmaxf(amax, fabsf(v[i][e])) : amax;
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(v[i][e]));
     s = fmaxf(row_max(amax), 1e-30f) / AP_FP8_MAX;
     if (slot >= 0 && j == 0) r.scale[slot] = s;
   }
   if (slot < 0) return;
   const float inv = 1.0f / s;
-  const bool ones = (__float_as_uint(s) & 0x7fffffu) == 0x7fffffu, correct = s < INFINITY;
-  uint8_t* const row = static_cast<uint8_t*>(r.cache) + (size_t)slot * r.width;
+  const bool ones = (__float_as_uint(s) & 0x7fffffu) == 0x7fffffu;
+  const float by = s < INFINITY ? s : 0.0f;
+  uint8_t* const row = static_cast<uint8_t*>(r.cache) + (size_t)slot * r.width + 8 * j;
 #pragma unroll
   for (int i = 0; i < NG; ++i) {
     const int g = j + AP_LANES * i;
@@ -193,20 +227,20 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const float p = v[i][e] * inv;
-      q[e] = correct ? fmaf(fmaf(-p, s, v[i][e]), inv, p) : p;
+      q[e] = fmaf(fmaf(-p, by, v[i][e]), inv, p);
     }
     if (ones) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[e] = v[i][e] / s;
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = fminf(fmaxf(q[e], -r.fp8_max), r.fp8_max);
+    for (int e = 0; e < 8; ++e) q[e] = __builtin_amdgcn_fmed3f(q[e], -r.fp8_max, r.fp8_max);  // (NaN: -)
     int lo = 0, hi = 0;
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
     hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
-    *reinterpret_cast<uint2*>(row + 8 * g) = make_uint2((uint32_t)lo, (uint32_t)hi);
+    *reinterpret_cast<uint2*>(row + 8 * AP_LANES * i) = make_uint2((uint32_t)lo, (uint32_t)hi);
   }
 }
 
@@ -219,10 +253,9 @@ __global__ __launch_bounds__(AP_WAVES* WAVE) void cache_append_kernel(AppendSet 
                                                                       int max_pages, int page_size, int num_pages) {
   __shared__ ApWave<R> sh[AP_WAVES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const long unit = (long)blockIdx.x * AP_WAVES + wave;
-  const int four = (int)(unit / set.n), t0 = four * AP_TOKENS;
+  const int unit = blockIdx.x * AP_WAVES + wave, four = unit / set.n, t0 = four * AP_TOKENS;
   if (t0 >= T) return;
-  const AppendRows& r = set.rows[unit - (long)four * set.n];
+  const AppendRows& r = set.rows[unit - four * set.n];
   if (r.width <= 128)
     ap_rows<1>(r, a, table, ctx_len, cu, t0, T, B, max_pages, page_size, num_pages, sh[wave]);
   else
