@@ -40,6 +40,14 @@ def test_refusals():
     assert call(T=0, table=None) == _lib.DSA_OK and call(B=0, T=0) == _lib.DSA_OK
 
 
+def test_packed_layout():
+    """append packs dsa_append_rows by itself: the same bytes as the structure's."""
+    k = kind(x=1 << 40, x_row=-5, norm_weight=7, norm_bias=9, cache=11, scale=13, norm_fp32=1, norm_width=3, cache_bf16=1)
+    assert dsa_cache._KIND.size == ctypes.sizeof(k)
+    packed = dsa_cache._KIND.pack(1 << 40, -5, 7, 9, 11, 13, 0, 576, 512, 1, 1, 3, 1, 1e-6, 448.0)
+    assert packed[:84] == bytes(k)[:84]  # (then 4 bytes of padding)
+
+
 def test_host_tensors_raise():
     z = torch.zeros(64, 576, dtype=torch.uint8)
     with pytest.raises(RuntimeError, match="GPU only"):

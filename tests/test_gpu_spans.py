@@ -4,7 +4,8 @@ last, softcap, slopes) against its definition in float64.
 Tolerances, from the arithmetic. A score's error e[t]: the products' fp32 sum, D 2^-24 times the sum of |q k|; with a cap the
 tanh's, less than cap 2^-20 (the exponent's argument y = 2 s / cap is off by 2^-23 of itself, which moves tanh by at most y (1 -
 tanh^2) 2^-23 < 2^-23; exp2 and the reciprocal are good to 2^-22 each of a term of at most 2; the last product and sum 2^-23:
-together below 2^-20); the bias, the running maximum and the factor of log2 e each 2^-23 of the sizes that they are added to. A
+together below 2^-20); the bias, the running maximum and the factor of log2 e each 2^-23 of the sizes that they are added to (the bias of a tile of 64 keys is
+one sum of two, off by 64 of them). A
 weight moves by e[t] relative, so an output by sum p e |v| + (sum p e) sum p |v|, and lse by sum p e, to first order (1.01 for
 the rest). Weights are rounded to bf16 in their product (2^-8 of sum p |v|), sums are fp32 (2^-20), a bf16 output is rounded
 once more (2^-8)."""
@@ -48,7 +49,7 @@ def reference(q, k, r, v, lq, lk, scale, causal, first, last, cap, slopes):
                 e = e + cap * 2.0 ** -20
             if slopes is not None:
                 s = s - slopes[h].double() * (place - t).abs()
-                e = e + slopes[h].double().abs() * (place - t).abs() * 2.0 ** -22
+                e = e + slopes[h].double().abs() * ((place - t).abs() + 64) * 2.0 ** -22
             e = e + s.abs() * 2.0 ** -22
             ok = see.any(1)
             if nk == 0 or not ok.any():
@@ -131,7 +132,7 @@ def test_ranges(lq, lk, H, rope, kind):
     compare(out, lse, reference(q, k, r, v, lq, lk, 192 ** -0.5, causal, first, last, 0.0, None))
 
 
-@pytest.mark.parametrize("cap,bias", [(20.0, False), (0.0, True), (5.0, True), (0.5, False), (1e6, False)])
+@pytest.mark.parametrize("cap,bias", [(20.0, False), (0.0, True), (5.0, True), (0.5, False), (50.0, False), (1e6, False)])
 @pytest.mark.parametrize("kind", ["causal", "prefix", "any"])
 @pytest.mark.parametrize("rope", [True, False])
 @pytest.mark.parametrize("lq,lk,H", SHAPES)

@@ -18,6 +18,7 @@ token's pool key, a softmax-gated mean of the pool's cached indexer keys, into t
 
 from __future__ import annotations
 
+import struct
 from collections.abc import Sequence
 
 import torch
@@ -26,6 +27,8 @@ from .. import _lib
 from . import _common as C
 from .dsa_rope import axis_map
 
+_KIND = struct.Struct("PqPPPP7i2f4x")  # dsa_append_rows
+_SIZES = {torch.bfloat16: 2, torch.float32: 4}
 FP8_MAX = 448.0  # the e4m3fn maximum (trnrt/engine/model_runner.py:62-70 off Neuron)
 
 
@@ -122,53 +125,60 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
     B, max_pages = table.shape
     tb, lens = C.as_i32(table), C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
     cu = None if cu_new is None else C.need(C.as_i32(cu_new), "cu_new", torch.int32, (B + 1,))
+    R = 0
     if inv_freq is not None:
-        C.need(inv_freq, "inv_freq", torch.float32, (None,))
-    R = 0 if inv_freq is None else inv_freq.shape[0]
+        R = C.need(inv_freq, "inv_freq", torch.float32, (None,)).shape[0]
     T = slots = None
-    kinds = (_lib.AppendRows * len(rows))()
-    held = []  # (what a kind's tensors were copied to, until the launch)
-    for r, kind in zip(rows, kinds):
-        x, cache, W = r.x, r.cache, r.cache.shape[-1]
-        if C.on_gpu(x, cache, r.scale) != dev:
-            raise ValueError(f"tensors on different devices: {dev} and {x.device}")
-        if x.dtype not in (torch.bfloat16, torch.float32):
+    kinds = b""  # (a step's call of a few us is bound by this function: packed, with few tensor attributes asked twice)
+    held = []  # what tensors were copied to, until the launch
+    on = table.get_device()
+    for r in rows:
+        x, cache, scale, norm, at = r.x, r.cache, r.scale, r.norm, r.rope_at
+        if x.get_device() != on or cache.get_device() != on or (scale is not None and scale.get_device() != on):
+            C.on_gpu(table, x, cache, scale)
+        size = _SIZES.get(x.dtype)
+        if size is None:
             raise ValueError(f"dsa_cache.append: rows of {x.dtype}, expected bfloat16 or float32")
         if x.dim() != 2:
             x = x.reshape(-1, x.shape[-1])
-        if x.shape[1] != W:
-            raise ValueError(f"dsa_cache.append: rows {tuple(x.shape)} for a cache of width {W}")
+        t, W = x.shape
+        if cache.shape[-1] != W or W == 0:
+            raise ValueError(f"dsa_cache.append: rows {tuple(x.shape)} for a cache of width {cache.shape[-1]}")
         bf = cache.dtype is torch.bfloat16
-        if not bf and cache.dtype not in (C.FP8, torch.uint8):
+        if not bf and cache.dtype is not C.FP8 and cache.dtype is not torch.uint8:
             raise NotImplementedError(f"dsa_cache.append: a {cache.dtype} cache; it is float8_e4m3fn or bfloat16")
-        if not cache.is_contiguous() or cache.data_ptr() % 16:
+        to = cache.data_ptr()
+        if not cache.is_contiguous() or to % 16:
             raise ValueError("dsa_cache.append: the cache must be contiguous and start at a multiple of 16 bytes")
-        n = cache.numel() // W if W else 0
+        n = cache.shape[0] if cache.dim() == 2 else cache.numel() // W
         if T is None:
-            T, slots = x.shape[0], n
-        if x.shape[0] != T or n != slots or n < 1 or n % page_size:
-            raise ValueError(f"dsa_cache.append: {x.shape[0]} rows of {T}, {n} cache slots of {slots} in pages of {page_size}")
-        size = x.element_size()
-        if x.stride(1) != 1 or x.data_ptr() % 16 or (x.stride(0) * size % 16 or x.stride(0) < W) and T > 1:
+            T, slots = t, n
+        if t != T or n != slots or n < 1 or n % page_size:
+            raise ValueError(f"dsa_cache.append: {t} rows of {T}, {n} cache slots of {slots} in pages of {page_size}")
+        row, col = x.stride()
+        if col != 1 or x.data_ptr() % 16 or (T > 1 and (row * size % 16 or row < W)):
             x = x.clone(memory_format=torch.contiguous_format)
             held.append(x)
-        if r.scale is not None:
-            kind.scale = C.need(C.flat(r.scale), "scale", torch.float32, (slots,)).data_ptr()
-        if r.norm is not None:
-            w, b = _norm(r.norm, W)
-            C.on_gpu(x, w, b)
-            held += (w, b)
-            kind.norm_weight, kind.norm_bias = w.data_ptr(), None if b is None else b.data_ptr()
-            kind.norm_fp32, kind.norm_width = w.dtype is torch.float32, w.shape[0]
-        if r.rope_at is not None and not (R and 0 <= r.rope_at <= W - 2 * R):
-            raise ValueError(f"dsa_cache.append: {2 * R} rotated columns from {r.rope_at} on in rows of {W}")
-        kind.x, kind.x_row, kind.x_fp32, kind.width = x.data_ptr(), max(x.stride(0), W), size == 4, W
-        kind.rope_at, kind.interleaved = -1 if r.rope_at is None else r.rope_at, r.interleaved
-        kind.cache, kind.cache_bf16, kind.eps, kind.fp8_max = cache.data_ptr(), bf, r.eps, r.fp8_max
+            row = W
+        if at is None:
+            at = -1
+        elif not (R and 0 <= at <= W - 2 * R):
+            raise ValueError(f"dsa_cache.append: {2 * R} rotated columns from {at} on in rows of {W}")
+        if scale is not None:
+            scale = C.need(C.flat(scale), "scale", torch.float32, (slots,)).data_ptr()
+        w = b = norm_fp32 = norm_width = 0
+        if norm is not None:
+            norm = _norm(norm, W)
+            C.on_gpu(table, *norm)
+            held.append(norm)
+            w, b = norm[0].data_ptr(), 0 if norm[1] is None else norm[1].data_ptr()
+            norm_fp32, norm_width = norm[0].dtype is torch.float32, norm[0].shape[0]
+        kinds += _KIND.pack(x.data_ptr(), max(row, W), w, b, to, scale or 0, size == 4, W, at, bool(r.interleaved), norm_fp32,
+                            norm_width, bf, r.eps, r.fp8_max)
     if cu is None and T and (not B or T % B):
         raise ValueError(f"dsa_cache.append: {T} rows for {B} sequences without cu_new")
     pos, n_axes, which = axis_map(axes, positions, R, T, "dsa_cache.append")
-    st = C.call(dev, _lib.lib().dsa_cache_append, kinds, len(rows), C.ptr(tb), C.ptr(lens), C.ptr(cu), C.ptr(pos),
+    st = C.call(dev, _lib.lib().dsa_cache_append, kinds, len(rows), tb.data_ptr(), lens.data_ptr(), C.ptr(cu), C.ptr(pos),
                 C.ptr(inv_freq), which, T, B, R, n_axes, factor, max_pages, page_size, slots // page_size)
     _lib.check(st, "dsa_cache.append")
 
