@@ -6,6 +6,7 @@
 namespace dsa {
 
 constexpr int RT_THREADS = 256;
+constexpr int RT_AT_ONCE = 4;
 
 template <typename T>
 struct RopeVec;  // 16 bytes of values
@@ -56,39 +57,63 @@ __global__ __launch_bounds__(RT_THREADS) void rope_rotate_kernel(const T* x, lon
   const int tg = blockIdx.x / head_groups, hg = blockIdx.x - tg * head_groups;
   const int t0 = tg * tokens, h0 = hg * heads;
   const int nt = min(tokens, n_tokens - t0), nh = min(heads, H - h0);
+  // A thread has the same item of every `step`-th row (token t, head h). RT_AT_ONCE rows' loads go out before the first store
+  // (which may be to the same memory), the first of them before the angles are computed.
+  const int per = VEC ? (HALF ? R / N : 2 * R / N) : R;  // items of a row
+  const int step = RT_THREADS / per, row0 = tid / per, c = tid - row0 * per;
+  const int dt = step / nh, dh = step - dt * nh;
+  int t = row0 / nh, h = row0 - t * nh;
+  if (row0 >= step) t = nt;  // (no item)
+  constexpr int V = VEC ? N : 1;
+  T* yr[RT_AT_ONCE];
+  int tok[RT_AT_ONCE];
+  float u[RT_AT_ONCE][V], v[RT_AT_ONCE][V];
+  const auto load = [&]() {
+#pragma unroll
+    for (int k = 0; k < RT_AT_ONCE; ++k) {
+      tok[k] = t;
+      if (t < nt) {
+        const T* const xr = x + (size_t)(t0 + t) * x_row + (size_t)(h0 + h) * x_head;
+        yr[k] = out + (size_t)(t0 + t) * out_row + (size_t)(h0 + h) * out_head;
+        if constexpr (VEC) {
+          RopeVec<T>::load(xr + N * c, u[k]);
+          if (HALF) RopeVec<T>::load(xr + R + N * c, v[k]);
+        } else {
+          u[k][0] = RopeVec<T>::get(xr + (HALF ? c : 2 * c));
+          v[k][0] = RopeVec<T>::get(xr + (HALF ? c + R : 2 * c + 1));
+        }
+      }
+      t += dt, h += dh;
+      if (h >= nh) h -= nh, ++t;
+    }
+  };
+  load();
   for (int i = tid; i < nt * R; i += RT_THREADS) {
-    const int t = i / R, f = i - t * R;
-    cs[i] = rope_angle(a, a.positions[(size_t)rope_axis(a, f) * n_tokens + t0 + t], f);
+    const int y = i / R, f = i - y * R;
+    cs[i] = rope_angle(a, a.positions[(size_t)rope_axis(a, f) * n_tokens + t0 + y], f);
   }
   __syncthreads();
-  const int per = VEC ? (HALF ? R / N : 2 * R / N) : R;  // items of a row
-  const int items = nt * nh * per;
-  for (int it = tid; it < items; it += RT_THREADS) {
-    const int row = it / per, c = it - row * per, t = row / nh, h = row - t * nh;
-    const T* xr = x + (size_t)(t0 + t) * x_row + (size_t)(h0 + h) * x_head;
-    T* yr = out + (size_t)(t0 + t) * out_row + (size_t)(h0 + h) * out_head;
-    const float2* w = cs + t * R;
-    if (VEC && HALF) {
-      float u[N], v[N];
-      RopeVec<T>::load(xr + N * c, u);
-      RopeVec<T>::load(xr + R + N * c, v);
+  for (;;) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) turn_pair(u[e], v[e], w[N * c + e]);
-      RopeVec<T>::store(yr + N * c, u);
-      RopeVec<T>::store(yr + R + N * c, v);
-    } else if (VEC) {
-      float u[N];
-      RopeVec<T>::load(xr + N * c, u);
+    for (int k = 0; k < RT_AT_ONCE; ++k) {
+      if (tok[k] >= nt) return;
+      const float2* const w = cs + tok[k] * R;
+      if constexpr (!VEC) {
+        turn_pair(u[k][0], v[k][0], w[c]);
+        RopeVec<T>::put(yr[k] + (HALF ? c : 2 * c), u[k][0]);
+        RopeVec<T>::put(yr[k] + (HALF ? c + R : 2 * c + 1), v[k][0]);
+      } else if constexpr (HALF) {
 #pragma unroll
-      for (int e = 0; e < N; e += 2) turn_pair(u[e], u[e + 1], w[(N * c + e) / 2]);
-      RopeVec<T>::store(yr + N * c, u);
-    } else {
-      const int i = HALF ? c : 2 * c, j = HALF ? c + R : 2 * c + 1;
-      float u = RopeVec<T>::get(xr + i), v = RopeVec<T>::get(xr + j);
-      turn_pair(u, v, w[c]);
-      RopeVec<T>::put(yr + i, u);
-      RopeVec<T>::put(yr + j, v);
+        for (int e = 0; e < N; ++e) turn_pair(u[k][e], v[k][e], w[N * c + e]);
+        RopeVec<T>::store(yr[k] + N * c, u[k]);
+        RopeVec<T>::store(yr[k] + R + N * c, v[k]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; e += 2) turn_pair(u[k][e], u[k][e + 1], w[(N * c + e) / 2]);
+        RopeVec<T>::store(yr[k] + N * c, u[k]);
+      }
     }
+    load();
   }
 }
 
