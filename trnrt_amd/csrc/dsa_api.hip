@@ -136,7 +136,7 @@ hipError_t launch_rope_rotate(const void* x, int fp32, long x_row, long x_head, 
 hipError_t launch_cache_append(const AppendSet& set, const RopeAngles& a, const int* table, const int* ctx_len,
                                const int* cu, int T, int B, int max_pages, int page_size, int num_pages, hipStream_t s);
 bool verify_grid_ok(int N, int V);
-size_t verify_workspace_bytes(int N, int V, int B, int num_cu);
+size_t verify_workspace_bytes(int N, int V, int B);
 hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* draft, const void* probs, int q_fp32,
                          long q_row, const int* cu, const float* u, const float* v, const float* temperature, int* tokens,
                          int* accepted, float* logp, void* ws, int N, int V, int B, int num_cu, hipStream_t s);
@@ -1462,7 +1462,7 @@ int dsa_cache_append(const dsa_append_rows* rows, int n_kinds, const int32_t* pa
 
 size_t dsa_verify_workspace_bytes(int N, int V, int B) {
   if (N < 0 || V < 1 || B < 0) return 0;
-  return align256(dsa::verify_workspace_bytes(N, V, B, num_cu()));
+  return align256(dsa::verify_workspace_bytes(N, V, B));
 }
 
 int dsa_verify(const void* logits, int logits_fp32, long long logits_row, const int32_t* draft, const void* probs,
@@ -1475,7 +1475,7 @@ int dsa_verify(const void* logits, int logits_fp32, long long logits_row, const 
   if (!cu || !v || !temperature || !accepted) return DSA_EINVAL;
   if (N > 0 && (!logits || !draft || !u || !tokens || !logp || logits_row < V || (probs && probs_row < V)))
     return DSA_EINVAL;
-  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::verify_workspace_bytes(N, V, B, num_cu())) return DSA_EWORKSPACE;
+  if (!workspace || !aligned16(workspace) || workspace_bytes < dsa::verify_workspace_bytes(N, V, B)) return DSA_EWORKSPACE;
   return status(dsa::launch_verify(logits, logits_fp32 != 0, (long)logits_row, draft, probs, probs_fp32 != 0,
                                    (long)probs_row, cu, u, v, temperature, tokens, accepted, logp, workspace, N, V, B,
                                    num_cu(), static_cast<hipStream_t>(stream)));

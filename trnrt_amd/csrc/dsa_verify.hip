@@ -12,10 +12,10 @@
 // w = q z by less than VF_NEAR are too near to say, their r is at most VF_NEAR q z each, and where the sum of those bounds
 // could move the token (or where r would be 0) the row is gone through once more with the 64-bit sum.
 //
-// Three launches. verify_rows_kernel: a wave takes 512 to 2,048 logits of a row to (maximum, sum, place of the maximum),
-// without LDS. verify_stop_kernel: a workgroup a sequence, a wave a row, takes the drafts and finds the stop row.
-// verify_pick_kernel: a workgroup sums a chunk of a stop row, the last of a sequence's to be done (a count that the second
-// launch cleared) looks for the token.
+// Two launches, or three. verify_rows_kernel: a workgroup of 16 waves takes up to 32,768 logits of a row to (maximum, sum,
+// place of the maximum), so that a row has few parts. verify_pick_kernel: every workgroup of a sequence finds its stop row
+// alike, a lane a row (in large batches verify_stop_kernel has found them), and sums a chunk of that; the last of them to be
+// done (a count that the first launch cleared) looks for the token.
 #include "dsa_async.h"
 
 namespace dsa {
@@ -41,7 +41,7 @@ struct VerifyArgs {
   long l_row, q_row;
   int l_fp32, q_fp32;
   int N, V, B;
-  int parts, chunks;   // of a row, for the first launch and the last
+  int parts, chunks;   // of a row, for the two launches
 };
 
 struct VerifyPart {
@@ -51,12 +51,10 @@ struct VerifyPart {
   int pad;
 };
 
-struct VerifyStop {  // a sequence's stop row
-  double sum;
-  float max;
-  int row;            // -1: nothing is drawn from it
-  int last;           // the sequence's last row: r = p
-  int done;           // chunks that are summed
+// The count of a sequence's chunks that are summed, in a cache line of its own: the adds to a line wait for each other (32
+// sequences a line: the pick of 64 rows of 131,072 34 us for 19).
+struct VerifyCount {
+  int n, pad[31];
 };
 
 struct VerifyChunk {  // sums over a chunk of the stop row
@@ -179,16 +177,19 @@ __device__ __forceinline__ int vf_sequence(const int* __restrict__ cu, int B, in
   return lo;
 }
 
-// A wave per unit: LOADS x 512 logits of a row. Not even a comparison is spent on NaN or infinities: they make the sum NaN,
-// and the unit is then done again with care.
+constexpr int VF_ROW_THREADS = 1024;
+constexpr int VF_ROW_WAVES = VF_ROW_THREADS / WAVE;
+
+// A workgroup's part of a row: LOADS x 8,192 logits, a wave's side by side. Not even a comparison is spent on NaN or
+// infinities: they make a wave's sum NaN, and its logits are then gone through again with care.
 template <typename T, int LOADS>
-__global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a,
-                                                                 VerifyPart* __restrict__ parts) {
+__global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs a, VerifyPart* __restrict__ parts,
+                                                                     VerifyCount* __restrict__ done) {
+  __shared__ VerifyPart wave_part[VF_ROW_WAVES];
   const int lane = threadIdx.x & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int unit = blockIdx.x * VF_WAVES + wave;
-  const int row = unit / a.parts, part = unit - row * a.parts;
-  if (row >= a.N) return;
-  const int i0 = (part * LOADS * WAVE + lane) * VF_VEC;
+  for (int b = blockIdx.x * VF_ROW_THREADS + threadIdx.x; b < a.B; b += gridDim.x * VF_ROW_THREADS) done[b].n = 0;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  const int from = (part * VF_ROW_WAVES + wave) * LOADS * WAVE * VF_VEC, i0 = from + lane * VF_VEC;
   // (the sequences' ends are on their way before the logits, and the temperature while those are)
   const int end = a.cu[min(lane + 1, a.B)];
   float x[LOADS][VF_VEC];
@@ -216,8 +217,8 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a,
       s[e & 3] += __builtin_amdgcn_exp2f(fmaf(d, kh, d * kl));
     }
   float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
-  const int from = part * LOADS * WAVE * VF_VEC, to = min(from + LOADS * WAVE * VF_VEC, a.V);
   if (!(sum >= 0.0f)) {
+    const int to = min(from + LOADS * WAVE * VF_VEC, a.V);
     m = -INFINITY;
     for (int i = from + lane; i < to; i += WAVE) m = fmaxf(m, vf_logit(a, row, i));
     m = wave_max(m);
@@ -233,39 +234,19 @@ __global__ __launch_bounds__(VF_THREADS) void verify_rows_kernel(VerifyArgs a,
       for (int e = VF_VEC - 1; e >= 0; --e) first = x[i][e] == m ? (uint32_t)(i0 + i * WAVE * VF_VEC + e) : first;
     first = wave_min_u32(first);
   }
-  if (lane == 0) parts[unit] = VerifyPart{m, sum, (int)first, 0};
+  if (lane == 0) wave_part[wave] = VerifyPart{m, sum, (int)first, 0};
+  __syncthreads();
+  if (wave) return;
+  VerifyPart w{-INFINITY, 0.0f, 0x7fffffff, 0};
+  if (lane < VF_ROW_WAVES) w = wave_part[lane];
+  m = wave_max(w.max);
+  const double all = vf_wave_sum((double)w.sum * vf_weight(w.max, m, k));
+  first = wave_min_u32(w.max == m ? (uint32_t)w.first : 0x7fffffffu);
+  if (lane == 0) parts[blockIdx.x] = VerifyPart{m, (float)all, (int)first, 0};
 }
 
 __device__ __forceinline__ float vf_logp(float l, float m, double sum, double k) {
   return (float)(vf_exponent(l, m, k) * 0.69314718055994530942 - log(sum));
-}
-
-struct VerifyRow {
-  double sum;
-  float max;
-  int first;
-};
-
-// A row from its parts, in every lane of the wave.
-__device__ __forceinline__ VerifyRow vf_join(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int row, double k) {
-  const int lane = threadIdx.x & (WAVE - 1);
-  const VerifyPart* const p = parts + (size_t)row * a.parts;
-  VerifyRow r{0.0, -INFINITY, 0};
-  uint32_t first = 0x7fffffffu;
-  for (int c = lane; c < a.parts; c += WAVE) {
-    const VerifyPart x = p[c];
-    if (x.max > r.max) {
-      r.sum = r.sum * vf_weight(r.max, x.max, k) + (double)x.sum;
-      r.max = x.max, first = (uint32_t)x.first;
-    } else {
-      r.sum += (double)x.sum * vf_weight(x.max, r.max, k);
-    }
-  }
-  const float m = wave_max(r.max);
-  r.sum = vf_wave_sum(r.sum * vf_weight(r.max, m, k));
-  r.first = (int)wave_min_u32(r.max == m ? first : 0x7fffffffu);
-  r.max = m;
-  return r;
 }
 
 // The row's sum in 64 bits, by the wave alone.
@@ -280,57 +261,72 @@ __device__ __forceinline__ double vf_exact_sum(const VerifyArgs& a, int row, flo
   return vf_wave_sum(s);
 }
 
-// One workgroup a sequence: its drafts, its stop row, and all that is written but the token drawn from that.
-constexpr int VF_STOP_THREADS = 512;
+struct VerifyStop {  // a sequence's stop row
+  double sum;
+  float max;
+  int row;  // -1: nothing is drawn from it
+};
 
-__global__ __launch_bounds__(VF_STOP_THREADS) void verify_stop_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
-                                                                      VerifyStop* __restrict__ stops) {
-  __shared__ int found;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & (WAVE - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
-  const float temperature = a.temperature[b];
-  const bool warm = temperature > 0.0f;
-  const double k = vf_rate(temperature);
-  if (r1 <= r0) {
-    if (tid == 0) a.accepted[b] = 0, stops[b].row = -1;
-    return;
-  }
-  if (tid == 0) found = r1 - 1;
-  __syncthreads();
-  // a wave's rows until one whose draft is not taken; that one, or the last row, stays in r, row
-  VerifyRow r{0.0, -INFINITY, 0};
-  int row = r0 + wave;
-  for (; row < r1; row += VF_STOP_THREADS / WAVE) {
+// The stop row of rows r0 .. r1 - 1, by a wave, a lane a row; `write`: and all that is written but the token drawn from it.
+__device__ __forceinline__ VerifyStop vf_stop(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int b, int r0, int r1,
+                                              bool warm, double k, bool write) {
+  const int lane = threadIdx.x & (WAVE - 1);
+  for (int row0 = r0;; row0 += WAVE) {
+    const int row = min(row0 + lane, r1 - 1);
     const bool last = row == r1 - 1;
-    const int x = last ? 0 : a.draft[row], i = min(max(x, 0), a.V - 1);
-    const float u = last ? 0.0f : a.u[row];
-    const float l = vf_logit(a, row, i);
+    const VerifyPart* const p = parts + (size_t)row * a.parts;
+    VerifyPart part = p[0];
+    const int x = a.draft[row], i = min(max(x, 0), a.V - 1);
+    const float u = a.u[row], l = vf_logit(a, row, i);
     double q = 1.0;
     if (warm && a.probs)
       q = a.q_fp32 ? (double)static_cast<const float*>(a.probs)[(size_t)row * a.q_row + i]
                    : (double)vf_value(static_cast<const uint16_t*>(a.probs)[(size_t)row * a.q_row + i]);
-    r = vf_join(a, parts, row, k);
-    if (last || x != i) break;
-    bool taken = x == r.first && r.max > -INFINITY;
-    if (warm) {
-      const double uq = (double)u * q, w = vf_weight(l, r.max, k);
-      // (not near, or u q that is NaN: decided here)
-      taken = uq * (fabs(uq * r.sum - w) <= VF_NEAR * w ? vf_exact_sum(a, row, r.max, k) : r.sum) < w;
+    double sum = (double)part.sum;
+    float m = part.max;
+    int first = part.first;
+    for (int c = 1; c < a.parts; ++c) {
+      part = p[c];
+      const float to = fmaxf(m, part.max);
+      const double w = vf_weight(fminf(m, part.max), to, k);  // (the larger one's is 1)
+      sum = part.max > m ? sum * w + (double)part.sum : sum + (double)part.sum * w;
+      first = part.max > m ? part.first : first;
+      m = to;
     }
-    if (!taken) break;
-    if (lane == 0) a.tokens[row] = x, a.logp[row] = vf_logp(l, r.max, r.sum, k);
+    const bool none = !(m > -INFINITY);
+    bool taken = !last && x == i && !none;
+    if (warm) {
+      const double uq = (double)u * q, w = vf_weight(l, m, k);
+      const bool near = taken && fabs(uq * sum - w) <= VF_NEAR * w;
+      double s = sum;
+      for (uint64_t todo = __ballot(near); todo; todo &= todo - 1) {
+        const int who = __builtin_ctzll(todo);
+        const double e = vf_exact_sum(a, __builtin_amdgcn_readlane(row, who),
+                                      __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), who)), k);
+        if (lane == who) s = e;
+      }
+      taken = taken && uq * s < w;  // (not for a u q that is NaN)
+    } else {
+      taken = taken && x == first;
+    }
+    const uint64_t refused = __ballot(!taken);  // (at the last row at the latest)
+    const int stop = refused ? __builtin_ctzll(refused) : WAVE;
+    const bool drawn = warm && !none;
+    if (write && row0 + lane < r1) {
+      const int y = lane < stop ? x : lane > stop || none ? -1 : first;
+      if (lane != stop || !drawn) {
+        a.tokens[row] = y;
+        a.logp[row] = y < 0 ? 0.0f : vf_logp(lane < stop ? l : m, m, sum, k);
+      }
+    }
+    if (stop == WAVE) continue;
+    if (write) {
+      if (lane == 0) a.accepted[b] = row0 + stop - r0;
+      for (int r = row0 + WAVE + lane; r < r1; r += WAVE) a.tokens[r] = -1, a.logp[r] = 0.0f;
+    }
+    return VerifyStop{vf_lane(sum, stop), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), stop)),
+                      __builtin_amdgcn_readlane((int)drawn, stop) ? row0 + stop : -1};
   }
-  if (lane == 0 && row < r1) atomicMin(&found, row);
-  __syncthreads();
-  const int stop = found;
-  if (row == stop && lane == 0) {
-    const bool none = !(r.max > -INFINITY), drawn = warm && !none;
-    stops[b] = VerifyStop{r.sum, r.max, drawn ? stop : -1, stop == r1 - 1, 0};
-    a.accepted[b] = stop - r0;
-    if (!drawn) a.tokens[stop] = none ? -1 : r.first, a.logp[stop] = none ? 0.0f : vf_logp(r.max, r.max, r.sum, k);
-  }
-  for (int i = stop + 1 + tid; i < r1; i += VF_STOP_THREADS) a.tokens[i] = -1, a.logp[i] = 0.0f;
 }
 
 // Logits x and the draft's probabilities q (0 where there are none) of tokens i .. i + 7 of the stop row. A draft that is
@@ -378,25 +374,57 @@ __device__ __forceinline__ double vf_wave_scan(double v) {
   return v;
 }
 
+// The stop rows in a launch of their own, a wave a sequence.
+__global__ __launch_bounds__(WAVE) void verify_stop_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
+                                                           VerifyStop* __restrict__ stops) {
+  const int b = blockIdx.x, r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
+  const float temperature = a.temperature[b];
+  VerifyStop s{0.0, 0.0f, -1};
+  if (r1 > r0) s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, vf_rate(temperature), true);
+  else if (threadIdx.x == 0) a.accepted[b] = 0;
+  if (threadIdx.x == 0) stops[b] = s;
+}
+
 // A sequence's workgroups sum a chunk of its stop row each; the last of them looks for the token. (Two or four chunks a
-// workgroup, with all workgroups on the CUs at once: 64 rows of 131,072 20.0 and 22.8 us for 20.2.)
+// workgroup, with all workgroups on the CUs at once: 64 rows of 131,072 20.0 and 22.8 us for 20.2.) FOUND: the stop rows are
+// in stops, else the first wave finds its sequence's.
 constexpr int VF_CHUNK = VF_THREADS * VF_VEC;
 
-__global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, VerifyStop* __restrict__ stops,
-                                                                 VerifyChunk* __restrict__ sums) {
+template <bool FOUND>
+__global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
+                                                                 const VerifyStop* __restrict__ stops,
+                                                                 VerifyChunk* __restrict__ sums, VerifyCount* __restrict__ done) {
+  __shared__ VerifyStop stop_row;
   __shared__ VerifyChunk part[VF_WAVES];
   __shared__ double tot[VF_WAVES], found_at, found_r;
   __shared__ float found_x;
   __shared__ int is_last, found, first[VF_WAVES], end[VF_WAVES];
   const int b = blockIdx.x / a.chunks, chunk = blockIdx.x - b * a.chunks, tid = threadIdx.x;
   const int lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
-  const int stop = stops[b].row;
+  const int r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
+  const float temperature = a.temperature[b];
+  const double k = vf_rate(temperature);
+  VerifyStop at_stop;
+  if (FOUND) {
+    at_stop = stops[b];
+  } else {
+    if (r1 <= r0 || (chunk > 0 && !(temperature > 0.0f))) {
+      if (r1 <= r0 && chunk == 0 && tid == 0) a.accepted[b] = 0;
+      return;
+    }
+    if (wave == 0) {
+      const VerifyStop s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, k, chunk == 0);
+      if (lane == 0) stop_row = s;
+    }
+    __syncthreads();
+    at_stop = stop_row;
+  }
+  const int stop = __builtin_amdgcn_readfirstlane(at_stop.row);
   if (stop < 0) return;
-  const bool infinite = stops[b].max == INFINITY;
-  const float m = infinite ? 0.0f : stops[b].max;
-  const double z0 = stops[b].sum, k = vf_rate(a.temperature[b]);
+  const bool last = stop == r1 - 1, infinite = at_stop.max == INFINITY;
+  const float m = infinite ? 0.0f : at_stop.max;
+  const double z0 = at_stop.sum;
   const float zf = (float)z0;
-  const bool last = stops[b].last;
   const int d = last || a.probs ? -1 : a.draft[stop];
   VerifyChunk* const row_sums = sums + (size_t)b * a.chunks;
   float xd = -INFINITY;  // a certain draft's logit
@@ -433,7 +461,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
     // emptied for them (a release and acquire here, which do that, made the launch 108 us for 29).
     wait_loads<0>();
     if (lane == 0)
-      is_last = __hip_atomic_fetch_add(&stops[b].done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
+      is_last = __hip_atomic_fetch_add(&done[b].n, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1;
   }
   __syncthreads();
   if (!is_last) return;
@@ -549,31 +577,32 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, V
   }
 }
 
-static int verify_loads(long n, int num_cu) {  // loads of a thread: 4 where enough of them are left to fill the CUs
-  const long at_once = 8L * VF_WAVES * num_cu * WAVE * VF_VEC;
-  return n >= 4 * at_once ? 4 : n >= 2 * at_once ? 2 : 1;
-}
+// Loads of a thread of the first launch: few, so that a small vocabulary is spread out, as long as a row has at most 8 parts.
+static int verify_loads(int V) { return V > 16 * VF_ROW_THREADS * VF_VEC ? 4 : V > 8 * VF_ROW_THREADS * VF_VEC ? 2 : 1; }
 static int verify_units(int V, int per) { return (V + per - 1) / per; }
 
-bool verify_grid_ok(int N, int V) { return (long)N * verify_units(V, WAVE * VF_VEC) <= 0xffffffL; }
+bool verify_grid_ok(int N, int V) {
+  return (long)N * verify_units(V, VF_CHUNK) <= 0xffffffL && (long)N * verify_units(V, VF_ROW_THREADS * VF_VEC) <= 0x3fffffL;
+}
 
-size_t verify_workspace_bytes(int N, int V, int B, int num_cu) {
-  const int parts = verify_units(V, WAVE * VF_VEC * verify_loads((long)N * V, num_cu));
-  return (size_t)N * parts * sizeof(VerifyPart) + (size_t)B * (verify_units(V, VF_CHUNK) * sizeof(VerifyChunk) + sizeof(VerifyStop));
+size_t verify_workspace_bytes(int N, int V, int B) {
+  const int parts = verify_units(V, VF_ROW_THREADS * VF_VEC * verify_loads(V)), chunks = verify_units(V, VF_CHUNK);
+  return (size_t)B * sizeof(VerifyCount) + (size_t)N * parts * sizeof(VerifyPart) +
+         (size_t)B * (chunks * sizeof(VerifyChunk) + sizeof(VerifyStop));
 }
 
 hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* draft, const void* probs, int q_fp32,
                          long q_row, const int* cu, const float* u, const float* v, const float* temperature, int* tokens,
                          int* accepted, float* logp, void* ws, int N, int V, int B, int num_cu, hipStream_t s) {
-  const int loads = verify_loads((long)N * V, num_cu);
-  VerifyArgs a{logits, probs, draft, cu, u, v, temperature, tokens, accepted, logp, l_row, q_row, l_fp32, q_fp32,
-               N, V, B, verify_units(V, WAVE * VF_VEC * loads), verify_units(V, VF_CHUNK)};
-  VerifyPart* const parts = static_cast<VerifyPart*>(ws);
+  const int loads = verify_loads(V);
+  const VerifyArgs a{logits, probs, draft, cu, u, v, temperature, tokens, accepted, logp, l_row, q_row, l_fp32, q_fp32,
+                     N, V, B, verify_units(V, VF_ROW_THREADS * VF_VEC * loads), verify_units(V, VF_CHUNK)};
+  VerifyCount* const done = static_cast<VerifyCount*>(ws);
+  VerifyPart* const parts = reinterpret_cast<VerifyPart*>(done + B);
   VerifyChunk* const sums = reinterpret_cast<VerifyChunk*>(parts + (size_t)N * a.parts);
   VerifyStop* const stops = reinterpret_cast<VerifyStop*>(sums + (size_t)B * a.chunks);
-  const unsigned groups = (unsigned)(((long)N * a.parts + VF_WAVES - 1) / VF_WAVES);
   const auto rows = [&](auto kernel) {
-    return launch("verify_rows_kernel", kernel, dim3(groups), dim3(VF_THREADS), s, a, parts);
+    return launch("verify_rows_kernel", kernel, dim3((unsigned)(N * a.parts)), dim3(VF_ROW_THREADS), s, a, parts, done);
   };
   hipError_t e = hipSuccess;
   if (N > 0 && l_fp32)
@@ -584,10 +613,15 @@ hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* 
     e = loads == 4   ? rows(verify_rows_kernel<uint16_t, 4>)
         : loads == 2 ? rows(verify_rows_kernel<uint16_t, 2>)
                      : rows(verify_rows_kernel<uint16_t, 1>);
-  if (e == hipSuccess)
-    e = launch("verify_stop_kernel", verify_stop_kernel, dim3(B), dim3(VF_STOP_THREADS), s, a, parts, stops);
-  if (e != hipSuccess || N == 0) return e;
-  return launch("verify_pick_kernel", verify_pick_kernel, dim3((unsigned)(B * a.chunks)), dim3(VF_THREADS), s, a, stops, sums);
+  if (e != hipSuccess) return e;
+  const auto pick = [&](auto kernel) {
+    return launch("verify_pick_kernel", kernel, dim3((unsigned)(B * a.chunks)), dim3(VF_THREADS), s, a, parts, stops, sums, done);
+  };
+  // Where the workgroups do not all run at once (5 a CU), each finding its stop row costs more than a launch that does: 64
+  // sequences of 131,072 42 us for 5 + 20, 13 of 100,003 13.6 for 5 + 9.6.
+  if ((long)B * a.chunks <= 5L * num_cu) return pick(verify_pick_kernel<false>);
+  e = launch("verify_stop_kernel", verify_stop_kernel, dim3(B), dim3(WAVE), s, a, parts, stops);
+  return e == hipSuccess ? pick(verify_pick_kernel<true>) : e;
 }
 
 }  // namespace dsa

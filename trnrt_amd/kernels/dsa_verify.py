@@ -33,7 +33,7 @@ def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch
            workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(tokens [N] int32, accepted [B] int32, logp [N] fp32) of B sequences whose rows of logits [N, V] (bf16 or fp32, rows
     may be views) are cu[b] .. cu[b + 1] - 1 (cu [B + 1] int32 on the device). Every row but a sequence's last has a drafted
-    token draft [N] int32 (the last rows' entries are not read), drawn from draft_probs [N, V] (bf16 or fp32), or certain
+    token draft [N] int32 (the last rows' entries are not used), drawn from draft_probs [N, V] (bf16 or fp32), or certain
     (None: greedy or n-gram drafts). u [N] and v [B] fp32 in [0, 1), temperature [B] fp32 (0: the largest logit, the first
     of equals, is taken and comes next). tokens: a sequence's taken drafts, then its next token, then -1; accepted: how many
     were taken; logp: each token's log probability under the target (at temperature 1 for 0; 0 where tokens is -1). A draft
