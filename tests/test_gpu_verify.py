@@ -1,7 +1,7 @@
 """Verification of drafts (trnrt_amd/kernels/dsa_verify.py) against a loop over rows in numpy's float64: tokens and counts
-equal, the log probabilities within 2^-24 of themselves (they are rounded once) and 2^-18: a row's sum is of 32-bit exponentials
-whose exponents are off by 2^-23 of themselves, 20 at the weights' mean at most (20 x 2^-23 ln 2 = 1.7e-6), exp2 by 2^-23, and a
-term goes through 16 roundings on its way into the sum (1e-6): 2.8e-6, less than 2^-18 = 3.8e-6."""
+equal, the log probabilities within 2^-24 of themselves (they are rounded once) and 2^-17: a row's sum is of 32-bit exponentials
+whose exponents are off by 1.5 x 2^-23 of themselves, 20 at the weights' mean at most (20 x 1.5 x 2^-23 ln 2 = 2.5e-6), exp2 by
+2^-23, and a term goes through 16 roundings on its way into the sum (1e-6): 3.6e-6, less than 2^-17 = 7.6e-6."""
 
 import math
 
@@ -83,7 +83,7 @@ def check(logits, draft, cu, u, v, temperature, probs=None, got=None):
     a, z = int(cu[0]), int(cu[-1])
     assert (tokens.cpu().numpy()[a:z] == rt[a:z]).all(), (tokens.cpu().numpy()[a:z], rt[a:z])
     err = np.abs(logp.double().cpu().numpy()[a:z] - rl[a:z])
-    assert (err <= 2.0 ** -24 * np.abs(rl[a:z]) + 2.0 ** -18).all()
+    assert (err <= 2.0 ** -24 * np.abs(rl[a:z]) + 2.0 ** -17).all()
     assert tokens.shape == logp.shape == (N,)
     return tokens, accepted, logp
 

@@ -23,8 +23,9 @@ namespace dsa {
 constexpr int VF_THREADS = 256;
 constexpr int VF_WAVES = VF_THREADS / WAVE;
 constexpr int VF_VEC = 8;  // logits of a load
-// Bound of a row's sum's error: exponents (l - max) k in two terms, 2^-23 of themselves, 20 at the weights' mean (2^17 logits)
-// at most: 1.7e-6; exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; the part's sum in 32 bits 2^-24.
+// Bound of a row's sum's error: exponents (l - max) k with three roundings, 1.5 2^-23 of themselves, 20 at the weights' mean
+// (2^17 logits) at most: 2.5e-6; exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; the part's sum in 32 bits
+// 2^-24.
 constexpr double VF_NEAR = 1e-5;
 
 struct VerifyArgs {
@@ -205,17 +206,14 @@ __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs 
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
 #pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) m = fmaxf(m, x[i][e]);
+    for (int e = 0; e < VF_VEC; ++e) m = max_nonan(m, x[i][e]);  // (a NaN: as it was)
   m = wave_max(m);
-  const float kh = (float)k, kl = (float)(k - (double)kh);
+  const float rate = (float)k;
   float s[4] = {};
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
 #pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) {
-      const float d = x[i][e] - m;
-      s[e & 3] += __builtin_amdgcn_exp2f(fmaf(d, kh, d * kl));
-    }
+    for (int e = 0; e < VF_VEC; ++e) s[e & 3] += __builtin_amdgcn_exp2f((x[i][e] - m) * rate);
   float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
   if (!(sum >= 0.0f)) {
     const int to = min(from + LOADS * WAVE * VF_VEC, a.V);
