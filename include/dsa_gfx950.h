@@ -484,12 +484,12 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
 /*
  * dsa_expanded_mla with more asked of the scores (the rest, the workspace among it, as there). Query i of a sequence stands
  * at place p = nk - nq + i among its nk keys; first, last int32 [Tq] (either may be null: 0 and nk), slopes fp32 [H] or
- * null, softcap >= 0 (0: none):
+ * null, softcap 0 (none) or at least 1e-30 (its scores are off by softcap 2^-20 at most):
  *   z[t] = scale * (q . k[t]),  z = softcap * tanh(z / softcap),  z -= slopes[h] * |p - t|,
  *   over the keys first[i] <= t < last[i] of the query's sequence, and t <= p where causal != 0.
  * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
  * document's start; a window: first = p - window + 1. Only the tiles of 64 keys that some query of a workgroup's 256 sees
- * are read. DSA_EINVAL for a softcap that is negative, infinite or NaN.
+ * are read. DSA_EINVAL for another softcap.
  */
 int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
                            const int32_t* cu_q, const int32_t* cu_k, const int32_t* first, const int32_t* last,
@@ -555,7 +555,8 @@ int dsa_cache_append(const dsa_append_rows* rows, int n_kinds, const int32_t* pa
  * written. A NaN logit is -infinity; among logits of +infinity the largest are equal and the rest impossible; a row with
  * none above -infinity takes no draft, and gives -1. u, v in [0, 1) and probs >= 0 are the caller's part.
  *   logits [N, V] bf16 or fp32, rows logits_row values apart, probs likewise; u fp32 [N], v and temperature fp32 [B].
- * p, the sums and the comparisons are in 64 bits. workspace: dsa_verify_workspace_bytes(N, V, B) (no zero fill needed).
+ * Tokens and counts are those of 64-bit probabilities, sums and comparisons; logp is off by 2^-17 at most beside its rounding
+ * (a row's sum in 32 bits). workspace: dsa_verify_workspace_bytes(N, V, B) (no zero fill needed).
  */
 size_t dsa_verify_workspace_bytes(int N, int V, int B);
 int dsa_verify(const void* logits, int logits_fp32, long long logits_row, const int32_t* draft, const void* probs,

@@ -206,6 +206,25 @@ def test_rows_of_zeros_and_infinities():
     assert (a[slot[0]].float() == 448).all() and sa[slot[0]] == torch.tensor(1.0 / 448)
 
 
+def test_large_cache():
+    """Slots whose rows lie past 2^32 bytes, and rows of x past 2^31 values."""
+    say("append large cache")
+    pages = 130_000
+    cache, scale = torch.zeros(pages * 64, 576, dtype=FP8, device="cuda"), torch.zeros(pages * 64, device="cuda")
+    table = torch.tensor([[pages - 1, 3], [7, pages - 2]], dtype=torch.int32).cuda()
+    ctx, row = torch.tensor([64, 70], dtype=torch.int32).cuda(), 800_000_000
+    big = torch.empty(3 * row + 576, dtype=torch.bfloat16, device="cuda")
+    x = torch.as_strided(big, (4, 576), (row, 1))
+    x.copy_(torch.randn(4, 576, generator=torch.Generator().manual_seed(5)))
+    dsa_cache.append(Rows(x, cache, scale), table, ctx, 64)
+    slot = torch.tensor([(pages - 1) * 64 + 62, (pages - 1) * 64 + 63, (pages - 2) * 64 + 4, (pages - 2) * 64 + 5]).cuda()
+    y = x.cpu().double()
+    s = y.abs().amax(1) / 448
+    assert ((scale[slot].cpu().double() - s).abs() <= 6e-6 * s).all() and int((scale != 0).sum()) == 4
+    code = y / s[:, None]
+    assert ((cache[slot].cpu().double() - code).abs() <= (code.abs() * 2.0 ** -4).clamp(min=2.0 ** -10) + 448 * 6e-6).all()
+
+
 def test_streams_and_graph():
     say("append graph")
     cu, ctx, table, slots, slot, _ = setup([2, 2], [70, 5], 64, 4)
@@ -246,7 +265,7 @@ def test_refusals():
     call()
     for kw in (dict(rows=[]), dict(table=table[0]), dict(ctx=ctx[:1]), dict(ps=0), dict(ps=63), dict(cu_new=cu[:2]),
                dict(inv_freq=None), dict(inv_freq=freqs(65)), dict(positions=torch.zeros(3, **i32)),
-               dict(positions=torch.zeros(2, 4, **i32)), dict(axes=[1] * 32), dict(rows=Rows(x, kv, s[1:])),
+               dict(positions=torch.zeros(2, 4, **i32)), dict(axes=[1] * 32), dict(rows=Rows(x, kv, s[1:])), dict(rows=Rows(x, kv, s.repeat(2)[::2][:, None])),
                dict(rows=Rows(x[:, :120], kv, s)), dict(rows=Rows(x.half(), kv, s)), dict(rows=Rows(x, kv, s, rope_at=72)),
                dict(rows=[Rows(x, kv, s), Rows(x[:3], kv, s)]), dict(rows=Rows(x, kv, s, norm=f[None])),
                dict(rows=Rows(x, kv, s, norm=torch.ones(136, device="cuda"))), dict(rows=Rows(x, kv, s, norm=(f, f[:8]))),

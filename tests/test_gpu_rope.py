@@ -127,6 +127,20 @@ def test_inverse_is_the_gradient(half):
         assert abs(change - gx[t, h, c].double()) <= 4e-6 * g.double().abs().max()
 
 
+def test_rows_far_apart():
+    """Rows whose offsets pass 2^31 values and 2^32 bytes, read and written."""
+    say("rotate far apart")
+    row = 1_200_000_000
+    big = torch.empty(2 * row + 300, dtype=torch.bfloat16, device="cuda")
+    x = torch.as_strided(big, (3, 2, 64), (row, 64, 1))
+    x.copy_(torch.randn(3, 2, 64, generator=torch.Generator().manual_seed(4)))
+    pos = torch.tensor([5, 70, 900], dtype=torch.int32).cuda()
+    ref, size = reference(x, pos, freqs(32), None, False)
+    close(dsa_rope.rotate(x, pos, freqs(32)), ref, size)
+    dsa_rope.rotate(x, pos, freqs(32), out=x)
+    close(x, ref, size)
+
+
 def test_streams_and_graph():
     """On a side stream, and captured and replayed with other inputs between eager calls."""
     say("rotate graph")

@@ -206,6 +206,16 @@ def test_views_and_rows_outside():
     check(logits, draft, inner, u, v[:3], temperature[:3], q)
 
 
+def test_rows_far_apart():
+    """Rows of logits and probabilities whose offsets pass 2^31 values."""
+    say("verify far apart")
+    logits, draft, cu, u, v, temperature, q = make([3, 1], 5000, torch.bfloat16, torch.bfloat16, 8)
+    row = 900_000_000
+    far, qf = (torch.as_strided(torch.empty(3 * row + 5000, dtype=torch.bfloat16, device="cuda"), (4, 5000), (row, 1)) for _ in "ab")
+    far.copy_(logits), qf.copy_(q)
+    check(far, draft, cu, u, v, temperature, qf)
+
+
 def test_no_rows():
     say("verify no rows")
     z = torch.zeros(0, device="cuda")

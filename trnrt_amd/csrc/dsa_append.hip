@@ -202,7 +202,7 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
   }
   // The quotient by s, correctly rounded as store's is: the product with the (correctly rounded) reciprocal, corrected by the
   // remainder, which is exact; only a divisor whose mantissa is all ones needs the division itself, and an infinite one no
-  // correction. (A division a value took 44 of the kernel's NNN us.)
+  // correction.
   float s = 1.0f;
   if (r.scale) {
     float amax = 0.0f;  // (columns past the row are 0)

@@ -164,8 +164,8 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
             at = -1
         elif not (R and 0 <= at <= W - 2 * R):
             raise ValueError(f"dsa_cache.append: {2 * R} rotated columns from {at} on in rows of {W}")
-        if scale is not None:
-            scale = C.need(C.flat(scale), "scale", torch.float32, (slots,)).data_ptr()
+        if scale is not None:  # (written in place: no copy of one that is not contiguous)
+            scale = C.need(C.flat(C.need(scale, "scale", torch.float32)), "scale", torch.float32, (slots,)).data_ptr()
         w = b = norm_fp32 = norm_width = 0
         if norm is not None:
             norm = _norm(norm, W)

@@ -6,8 +6,8 @@ back by the drafts that were not taken, whose cached rows the next dsa_cache.app
 
 With p = softmax(logits / temperature), a draft x of row j is taken iff u[j] q(x) < p(x), up to the first that is not; the
 next token is drawn from max(p - q, 0) of that row (from p of the last row, once all are taken) by v: what comes out is
-distributed as the target's own samples are. Probabilities, sums and comparisons are in 64 bits, in an order that does not
-vary. The HIP kernels are in csrc/dsa_verify.hip.
+distributed as the target's own samples are. Tokens and counts are those of 64-bit probabilities, sums and comparisons, and do
+not vary from run to run; logp is off by 2^-17 at most beside its rounding. The HIP kernels are in csrc/dsa_verify.hip.
 """
 
 from __future__ import annotations
