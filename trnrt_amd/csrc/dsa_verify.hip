@@ -14,7 +14,7 @@
 //
 // Two launches, or three. verify_rows_kernel: a workgroup of 16 waves takes up to 32,768 logits of a row to (maximum, sum,
 // place of the maximum), so that a row has few parts. verify_pick_kernel: every workgroup of a sequence finds its stop row
-// alike, a lane a row (in large batches verify_stop_kernel has found them), and sums a chunk of that; the last of them to be
+// alike, 8 lanes a row (in large batches verify_stop_kernel has found them), and sums a chunk of that; the last of them to be
 // done (a count that the first launch cleared) looks for the token.
 #include "dsa_async.h"
 
@@ -265,65 +265,78 @@ struct VerifyStop {  // a sequence's stop row
   int row;  // -1: nothing is drawn from it
 };
 
-// The stop row of rows r0 .. r1 - 1, by a wave, a lane a row; `write`: and all that is written but the token drawn from it.
+// The stop row of rows r0 .. r1 - 1, by a wave, 8 lanes a row, a lane a part (or every 8th); `write`: and all that is written
+// but the token drawn from it.
+constexpr int VF_ROW_LANES = 8;
+constexpr int VF_STOP_ROWS = WAVE / VF_ROW_LANES;
+
 __device__ __forceinline__ VerifyStop vf_stop(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int b, int r0, int r1,
                                               bool warm, double k, bool write) {
-  const int lane = threadIdx.x & (WAVE - 1);
-  for (int row0 = r0;; row0 += WAVE) {
-    const int row = min(row0 + lane, r1 - 1);
+  const int lane = threadIdx.x & (WAVE - 1), j = lane & (VF_ROW_LANES - 1);
+#pragma unroll 1
+  for (int row0 = r0;; row0 += VF_STOP_ROWS) {
+    const int mine = row0 + lane / VF_ROW_LANES, row = min(mine, r1 - 1);
     const bool last = row == r1 - 1;
     const VerifyPart* const p = parts + (size_t)row * a.parts;
-    VerifyPart part = p[0];
+    VerifyPart part{-INFINITY, 0.0f, 0x7fffffff, 0};
+    if (j < a.parts) part = p[j];
     const int x = a.draft[row], i = min(max(x, 0), a.V - 1);
     const float u = a.u[row], l = vf_logit(a, row, i);
     double q = 1.0;
     if (warm && a.probs)
       q = a.q_fp32 ? (double)static_cast<const float*>(a.probs)[(size_t)row * a.q_row + i]
                    : (double)vf_value(static_cast<const uint16_t*>(a.probs)[(size_t)row * a.q_row + i]);
-    double sum = (double)part.sum;
     float m = part.max;
-    int first = part.first;
-    for (int c = 1; c < a.parts; ++c) {
+    for (int c = j + VF_ROW_LANES; c < a.parts; c += VF_ROW_LANES) m = fmaxf(m, p[c].max);
+    m = fmaxf(m, __int_as_float(dpp<0xb1>(__float_as_int(m))));
+    m = fmaxf(m, __int_as_float(dpp<0x4e>(__float_as_int(m))));
+    m = fmaxf(m, __int_as_float(dpp<0x141>(__float_as_int(m))));
+    double sum = 0.0;
+    uint32_t first = 0x7fffffffu;  // (the parts' first places ascend)
+    for (int c = j;;) {
+      sum += (double)part.sum * vf_weight(part.max, m, k);
+      if (part.max == m) first = min(first, (uint32_t)part.first);
+      if ((c += VF_ROW_LANES) >= a.parts) break;
       part = p[c];
-      const float to = fmaxf(m, part.max);
-      const double w = vf_weight(fminf(m, part.max), to, k);  // (the larger one's is 1)
-      sum = part.max > m ? sum * w + (double)part.sum : sum + (double)part.sum * w;
-      first = part.max > m ? part.first : first;
-      m = to;
     }
+    sum += vf_swap(sum, 0);
+    sum += vf_swap(sum, 1);
+    sum += vf_swap(sum, 2);
+    first = min(first, (uint32_t)dpp<0xb1>((int)first));
+    first = min(first, (uint32_t)dpp<0x4e>((int)first));
+    first = min(first, (uint32_t)dpp<0x141>((int)first));
     const bool none = !(m > -INFINITY);
     bool taken = !last && x == i && !none;
     if (warm) {
       const double uq = (double)u * q, w = vf_weight(l, m, k);
-      const bool near = taken && fabs(uq * sum - w) <= VF_NEAR * w;
       double s = sum;
-      for (uint64_t todo = __ballot(near); todo; todo &= todo - 1) {
-        const int who = __builtin_ctzll(todo);
+      uint64_t todo = __ballot(taken && fabs(uq * sum - w) <= VF_NEAR * w);
+      while (todo) {
+        const int who = __builtin_ctzll(todo) & ~(VF_ROW_LANES - 1);
+        todo &= ~(0xffull << who);
         const double e = vf_exact_sum(a, __builtin_amdgcn_readlane(row, who),
                                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), who)), k);
-        if (lane == who) s = e;
+        if ((lane & ~(VF_ROW_LANES - 1)) == who) s = e;
       }
       taken = taken && uq * s < w;  // (not for a u q that is NaN)
     } else {
-      taken = taken && x == first;
+      taken = taken && x == (int)first;
     }
     const uint64_t refused = __ballot(!taken);  // (at the last row at the latest)
-    const int stop = refused ? __builtin_ctzll(refused) : WAVE;
+    const int at = refused ? __builtin_ctzll(refused) : WAVE, stop = row0 + at / VF_ROW_LANES;
     const bool drawn = warm && !none;
-    if (write && row0 + lane < r1) {
-      const int y = lane < stop ? x : lane > stop || none ? -1 : first;
-      if (lane != stop || !drawn) {
-        a.tokens[row] = y;
-        a.logp[row] = y < 0 ? 0.0f : vf_logp(lane < stop ? l : m, m, sum, k);
-      }
+    if (write && mine < r1 && j == 0 && (row != stop || !drawn)) {
+      const int y = row < stop ? x : row > stop || none ? -1 : (int)first;
+      a.tokens[row] = y;
+      a.logp[row] = y < 0 ? 0.0f : vf_logp(row < stop ? l : m, m, sum, k);
     }
-    if (stop == WAVE) continue;
+    if (at == WAVE) continue;
     if (write) {
-      if (lane == 0) a.accepted[b] = row0 + stop - r0;
-      for (int r = row0 + WAVE + lane; r < r1; r += WAVE) a.tokens[r] = -1, a.logp[r] = 0.0f;
+      if (lane == 0) a.accepted[b] = stop - r0;
+      for (int r = row0 + VF_STOP_ROWS + lane; r < r1; r += WAVE) a.tokens[r] = -1, a.logp[r] = 0.0f;
     }
-    return VerifyStop{vf_lane(sum, stop), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), stop)),
-                      __builtin_amdgcn_readlane((int)drawn, stop) ? row0 + stop : -1};
+    return VerifyStop{vf_lane(sum, at), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), at)),
+                      __builtin_amdgcn_readlane((int)drawn, at) ? stop : -1};
   }
 }
 
