@@ -105,6 +105,7 @@ def make(rows, V, dtype, probs, seed, near=0.5):
 @pytest.mark.parametrize("rows,V", [
     ([1], 1), ([4], 2), ([2, 1, 5, 0, 3], 7), ([5] * 13, 1000), ([1, 8, 2, 9], 8191), ([3, 3], 8192), ([2, 4, 1], 8193),
     ([5, 5, 2], 65537), ([3] * 200, 33), ([300, 2], 64), ([2, 3], 600001),
+    ([4, 1, 0, 9] * 11, 65537), ([70] * 3, 70000),
 ])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("probs", [None, torch.float32, torch.bfloat16])
@@ -170,7 +171,7 @@ def test_edges_of_the_random_numbers():
     check(sure, torch.full_like(draft, 12344), cu, u, v, temperature)
 
 
-@pytest.mark.parametrize("V", [3, 700, 40000])
+@pytest.mark.parametrize("V", [3, 700, 40000, 100000])  # (the last with the stop rows in a launch of their own)
 def test_decisions_that_32_bits_do_not_make(V):
     """u q within an fp32 rounding of p, on either side; and a draft whose probabilities are the target's own, rounded, refused
     all the same: what is left over is roundings, and the token is the one that they give in 64 bits."""

@@ -8,9 +8,10 @@
 // Which token comes does not depend on roundings in 32 bits, though nearly all rows are only summed in 32: a row's sum of
 // exp((l - max) / T) is taken in 32 bits (off by VF_NEAR of itself at most), and only where that decides nothing, with u q
 // and p that close, again in 64. The stop row's sums are in 64 bits: with w the weights and z the 32-bit sum, a pass over it
-// sums w, and w and q where w > q z. r's sum is then the latter two's difference at the 64-bit sum; tokens on either side of
-// w = q z by less than VF_NEAR are too near to say, their r is at most VF_NEAR q z each, and where the sum of those bounds
-// could move the token (or where r would be 0) the row is gone through once more with the 64-bit sum.
+// sums w, and w - q z and q where that is above 0. r's sum at the 64-bit sum z' of w is then theirs plus (z - z') times q's
+// (for which 32 bits do); tokens on either side of w = q z by less than VF_NEAR are too near to say, their r is off by q |z' -
+// z| each, and where the sum of those bounds could move the token (or where r would be 0) the row is gone through once more
+// with z'.
 //
 // Two launches, or three. verify_rows_kernel: a workgroup of 16 waves takes up to 32,768 logits of a row to (maximum, sum,
 // place of the maximum), so that a row has few parts. verify_pick_kernel: every workgroup of a sequence finds its stop row
@@ -24,9 +25,9 @@ constexpr int VF_THREADS = 256;
 constexpr int VF_WAVES = VF_THREADS / WAVE;
 constexpr int VF_VEC = 8;  // logits of a load
 // Bound of a row's sum's error: exponents (l - max) k with three roundings, 1.5 2^-23 of themselves, 20 at the weights' mean
-// (2^17 logits) at most: 2.5e-6; exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; the part's sum in 32 bits
-// 2^-24.
-constexpr double VF_NEAR = 1e-5;
+// (2^17 logits) at most: 2.5e-6; two times exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; its product with a
+// wave's weight and the part's sum in 32 bits 2^-24 each: 3.9e-6.
+constexpr double VF_NEAR = 4e-6;
 
 struct VerifyArgs {
   const void* logits;  // [N, V], rows l_row values apart, bf16 or fp32
@@ -110,21 +111,22 @@ __device__ __forceinline__ double vf_exponent(float l, float m, double k) {
   return x <= 0.0 && l > -INFINITY ? x : -INFINITY;
 }
 
-
 // 2^x for x <= 0 (x < -1022: 2^-1022), by the series of e^(f ln 2) about the nearest whole number; the first term left out is
-// 2e-13 of it at most. The whole number is found, and put into the exponent, through the low bits of x + 1.5 2^52.
+// 2e-16 of it at most. (With two terms less, 2e-13, tokens moved where a draft's probabilities were the target's own.) The whole
+// number is found, and put into the exponent, through the low bits of x + 1.5 2^52.
 __device__ __forceinline__ double vf_exp2(double x) {
   x = fmax(x, -1022.0);
   const double big = 6755399441055744.0, n = x + big, f = x - (n - big);
   // (ln 2)^k / k!, in scalar registers: as literals each would be moved into the accumulator's first
-  double c[11] = {1.0, 6.9314718055994530942e-1, 2.4022650695910071233e-1, 5.5504108664821579953e-2, 9.6181291076284771620e-3,
-                  1.3333558146428443423e-3, 1.5403530393381609954e-4, 1.5252733804059840280e-5, 1.3215486790144309488e-6,
-                  1.0178086009239699728e-7, 7.0549116208011233299e-9};
+  double c[13] = {1.0, 6.9314718055994530942e-1, 2.4022650695910071233e-1, 5.5504108664821579953e-2,
+                  9.6181291076284771619e-3, 1.3333558146428443423e-3, 1.5403530393381609954e-4, 1.5252733804059840280e-5,
+                  1.3215486790144309488e-6, 1.0178086009239699728e-7, 7.0549116208011233299e-9, 4.4455382718708114976e-10,
+                  2.5678435993488205142e-11};
 #pragma unroll
-  for (int i = 0; i <= 10; ++i) asm("" : "+s"(c[i]));
-  double p = c[10];
+  for (int i = 0; i <= 12; ++i) asm("" : "+s"(c[i]));
+  double p = c[12];
 #pragma unroll
-  for (int i = 9; i >= 0; --i) p = fma(p, f, c[i]);
+  for (int i = 11; i >= 0; --i) p = fma(p, f, c[i]);
   const long long u = __builtin_bit_cast(long long, p);
   const int hi = (int)(u >> 32) + ((int)__builtin_bit_cast(long long, n) << 20);
   return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)u);
@@ -178,6 +180,11 @@ __device__ __forceinline__ int vf_sequence(const int* __restrict__ cu, int B, in
   return lo;
 }
 
+// vf_weight in 32 bits. (In 64, though few lanes come to it, 320 rows of 131,072 took 28.4 us for 21.6.)
+__device__ __forceinline__ float vf_weight32(float l, float m, float k) {
+  return l == m ? (l > -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f((l - m) * k);
+}
+
 constexpr int VF_ROW_THREADS = 1024;
 constexpr int VF_ROW_WAVES = VF_ROW_THREADS / WAVE;
 
@@ -201,14 +208,13 @@ __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs 
   if (b == WAVE) b = vf_sequence(a.cu, a.B, row);
   if (b >= a.B || row < a.cu[0]) return;
   const float temperature = a.temperature[b];
-  const double k = vf_rate(temperature);
+  const float rate = (float)vf_rate(temperature);
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
 #pragma unroll
     for (int e = 0; e < VF_VEC; ++e) m = max_nonan(m, x[i][e]);  // (a NaN: as it was)
   m = wave_max(m);
-  const float rate = (float)k;
   float s[4] = {};
 #pragma unroll
   for (int i = 0; i < LOADS; ++i)
@@ -221,7 +227,7 @@ __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs 
     for (int i = from + lane; i < to; i += WAVE) m = fmaxf(m, vf_logit(a, row, i));
     m = wave_max(m);
     double t = 0.0;
-    for (int i = from + lane; i < to; i += WAVE) t += vf_weight(vf_logit(a, row, i), m, k);
+    for (int i = from + lane; i < to; i += WAVE) t += (double)vf_weight32(vf_logit(a, row, i), m, rate);
     sum = (float)vf_wave_sum(t);
   }
   uint32_t first = 0x7fffffffu;
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs 
   VerifyPart w{-INFINITY, 0.0f, 0x7fffffff, 0};
   if (lane < VF_ROW_WAVES) w = wave_part[lane];
   m = wave_max(w.max);
-  const double all = vf_wave_sum((double)w.sum * vf_weight(w.max, m, k));
+  const double all = vf_wave_sum((double)(w.sum * vf_weight32(w.max, m, rate)));
   first = wave_min_u32(w.max == m ? (uint32_t)w.first : 0x7fffffffu);
   if (lane == 0) parts[blockIdx.x] = VerifyPart{m, (float)all, (int)first, 0};
 }
@@ -247,16 +253,47 @@ __device__ __forceinline__ float vf_logp(float l, float m, double sum, double k)
   return (float)(vf_exponent(l, m, k) * 0.69314718055994530942 - log(sum));
 }
 
-// The row's sum in 64 bits, by the wave alone.
-__device__ __forceinline__ double vf_exact_sum(const VerifyArgs& a, int row, float m, double k) {
+// A row's sum in 64 bits is asked for by the workgroup's first wave, which has found that it needs it (one row in 100,000),
+// and computed by all: the others wait for questions (vf_answer) until there are no more (vf_no_more).
+struct VerifyAsk {
+  int row;  // -1: no more
+  float m;
+  double part[16];
+};
+
+__device__ __forceinline__ void vf_exact_part(const VerifyArgs& a, VerifyAsk& ask, double k) {
   double s = 0.0;
-  for (int i = (threadIdx.x & (WAVE - 1)) * VF_VEC; i < a.V; i += WAVE * VF_VEC) {
+  for (int i = threadIdx.x * VF_VEC; i < a.V; i += blockDim.x * VF_VEC) {
     float x[VF_VEC];
-    vf_logits(a, row, i, x);
+    vf_logits(a, ask.row, i, x);
 #pragma unroll
-    for (int e = 0; e < VF_VEC; ++e) s += vf_weight(x[e], m, k);
+    for (int e = 0; e < VF_VEC; ++e) s += vf_weight(x[e], ask.m, k);
   }
-  return vf_wave_sum(s);
+  s = vf_wave_sum(s);
+  if ((threadIdx.x & (WAVE - 1)) == 0) ask.part[threadIdx.x / WAVE] = s;
+  __syncthreads();
+}
+
+__device__ __forceinline__ double vf_exact_sum(const VerifyArgs& a, VerifyAsk& ask, int row, float m, double k) {
+  if (threadIdx.x == 0) ask.row = row, ask.m = m;
+  __syncthreads();
+  vf_exact_part(a, ask, k);
+  double s = 0.0;
+  for (int w = 0; w < (int)blockDim.x / WAVE; ++w) s += ask.part[w];
+  return s;
+}
+
+__device__ __forceinline__ void vf_no_more(VerifyAsk& ask) {
+  if (threadIdx.x == 0) ask.row = -1;
+  __syncthreads();
+}
+
+__device__ __forceinline__ void vf_answer(const VerifyArgs& a, VerifyAsk& ask, double k) {
+  for (;;) {
+    __syncthreads();
+    if (ask.row < 0) return;
+    vf_exact_part(a, ask, k);
+  }
 }
 
 struct VerifyStop {  // a sequence's stop row
@@ -271,7 +308,7 @@ constexpr int VF_ROW_LANES = 8;
 constexpr int VF_STOP_ROWS = WAVE / VF_ROW_LANES;
 
 __device__ __forceinline__ VerifyStop vf_stop(const VerifyArgs& a, const VerifyPart* __restrict__ parts, int b, int r0, int r1,
-                                              bool warm, double k, bool write) {
+                                              bool warm, double k, bool write, VerifyAsk& ask) {
   const int lane = threadIdx.x & (WAVE - 1), j = lane & (VF_ROW_LANES - 1);
 #pragma unroll 1
   for (int row0 = r0;; row0 += VF_STOP_ROWS) {
@@ -314,7 +351,7 @@ __device__ __forceinline__ VerifyStop vf_stop(const VerifyArgs& a, const VerifyP
       while (todo) {
         const int who = __builtin_ctzll(todo) & ~(VF_ROW_LANES - 1);
         todo &= ~(0xffull << who);
-        const double e = vf_exact_sum(a, __builtin_amdgcn_readlane(row, who),
+        const double e = vf_exact_sum(a, ask, __builtin_amdgcn_readlane(row, who),
                                       __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m), who)), k);
         if ((lane & ~(VF_ROW_LANES - 1)) == who) s = e;
       }
@@ -385,14 +422,24 @@ __device__ __forceinline__ double vf_wave_scan(double v) {
   return v;
 }
 
-// The stop rows in a launch of their own, a wave a sequence.
-__global__ __launch_bounds__(WAVE) void verify_stop_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
-                                                           VerifyStop* __restrict__ stops) {
+// The stop rows in a launch of their own, a workgroup a sequence (for its first wave).
+constexpr int VF_STOP_THREADS = 1024;
+
+__global__ __launch_bounds__(VF_STOP_THREADS) void verify_stop_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
+                                                                      VerifyStop* __restrict__ stops) {
+  __shared__ VerifyAsk ask;
   const int b = blockIdx.x, r0 = min(max(a.cu[b], 0), a.N), r1 = min(max(a.cu[b + 1], 0), a.N);
   const float temperature = a.temperature[b];
+  const double k = vf_rate(temperature);
   VerifyStop s{0.0, 0.0f, -1};
-  if (r1 > r0) s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, vf_rate(temperature), true);
-  else if (threadIdx.x == 0) a.accepted[b] = 0;
+  if (r1 <= r0) {
+    if (threadIdx.x == 0) a.accepted[b] = 0;
+  } else if (threadIdx.x >= WAVE) {
+    vf_answer(a, ask, k);
+  } else {
+    s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, k, true, ask);
+    vf_no_more(ask);
+  }
   if (threadIdx.x == 0) stops[b] = s;
 }
 
@@ -406,6 +453,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
                                                                  const VerifyStop* __restrict__ stops,
                                                                  VerifyChunk* __restrict__ sums, VerifyCount* __restrict__ done) {
   __shared__ VerifyStop stop_row;
+  __shared__ VerifyAsk ask;
   __shared__ VerifyChunk part[VF_WAVES];
   __shared__ double tot[VF_WAVES], found_at, found_r;
   __shared__ float found_x;
@@ -424,10 +472,12 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
       return;
     }
     if (wave == 0) {
-      const VerifyStop s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, k, chunk == 0);
+      const VerifyStop s = vf_stop(a, parts, b, r0, r1, temperature > 0.0f, k, chunk == 0, ask);
       if (lane == 0) stop_row = s;
+      vf_no_more(ask);
+    } else {
+      vf_answer(a, ask, k);
     }
-    __syncthreads();
     at_stop = stop_row;
   }
   const int stop = __builtin_amdgcn_readfirstlane(at_stop.row);
@@ -496,7 +546,9 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
     z += t.all, near += t.near;
   }
   // (a certain draft's own weight is not in `all`)
-  z = vf_wave_sum(z) + vf_stop_weight(xd, m, k), near = vf_wave_sum(near);
+  z = vf_wave_sum(z) + vf_stop_weight(xd, m, k);
+  // (the bounds were for a z off by VF_NEAR of itself; by now it is known by how much)
+  near = vf_wave_sum(near) * (fabs(z - z0) / (VF_NEAR * z0));
   // r's sum at z: it moves by q for every one that z does
   const auto rest_of = [&](const VerifyChunk& t) { return fmax(fma(z0 - z, t.q, t.rest), 0.0); };
   double rest = rest_of(front);
@@ -631,7 +683,7 @@ hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* 
   // Where the workgroups do not all run at once (5 a CU), each finding its stop row costs more than a launch that does: 64
   // sequences of 131,072 42 us for 5 + 20, 13 of 100,003 13.6 for 5 + 9.6.
   if ((long)B * a.chunks <= 5L * num_cu) return pick(verify_pick_kernel<false>);
-  e = launch("verify_stop_kernel", verify_stop_kernel, dim3(B), dim3(WAVE), s, a, parts, stops);
+  e = launch("verify_stop_kernel", verify_stop_kernel, dim3(B), dim3(VF_STOP_THREADS), s, a, parts, stops);
   return e == hipSuccess ? pick(verify_pick_kernel<true>) : e;
 }
 
