@@ -221,7 +221,7 @@ __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs 
 #pragma unroll
     for (int e = 0; e < VF_VEC; ++e) s[e & 3] += __builtin_amdgcn_exp2f((x[i][e] - m) * rate);
   float sum = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
-  if (!(sum >= 0.0f)) {
+  if (__builtin_expect(!(sum >= 0.0f), 0)) {
     const int to = min(from + LOADS * WAVE * VF_VEC, a.V);
     m = -INFINITY;
     for (int i = from + lane; i < to; i += WAVE) m = fmaxf(m, vf_logit(a, row, i));
@@ -291,7 +291,7 @@ __device__ __forceinline__ void vf_no_more(VerifyAsk& ask) {
 __device__ __forceinline__ void vf_answer(const VerifyArgs& a, VerifyAsk& ask, double k) {
   for (;;) {
     __syncthreads();
-    if (ask.row < 0) return;
+    if (__builtin_expect(ask.row < 0, 1)) return;
     vf_exact_part(a, ask, k);
   }
 }
@@ -348,7 +348,7 @@ __device__ __forceinline__ VerifyStop vf_stop(const VerifyArgs& a, const VerifyP
       const double uq = (double)u * q, w = vf_weight(l, m, k);
       double s = sum;
       uint64_t todo = __ballot(taken && fabs(uq * sum - w) <= VF_NEAR * w);
-      while (todo) {
+      while (__builtin_expect(todo != 0, 0)) {
         const int who = __builtin_ctzll(todo) & ~(VF_ROW_LANES - 1);
         todo &= ~(0xffull << who);
         const double e = vf_exact_sum(a, ask, __builtin_amdgcn_readlane(row, who),
