@@ -172,6 +172,19 @@ def test_four_kinds_even_batches_and_axes():
         check(c, s, torch.zeros_like(c), slot, y)
 
 
+def test_rows_of_batches_that_do_not_merge():
+    """x [B, S, W] out of [B, S + 1, W], several kinds of one size: each kind's copy lives until the launch."""
+    say("append, batches that do not merge")
+    cu, ctx, table, slots, slot, place = setup([3] * 5, [40] * 5, 64, 4)
+    g = torch.Generator().manual_seed(8)
+    x = [torch.randn(5, 4, 128, generator=g).bfloat16().cuda() for _ in range(3)]
+    a, b = [[torch.zeros(slots, 128, dtype=torch.bfloat16).cuda() for _ in x] for _ in range(2)]
+    dsa_cache.append([Rows(y[:, :3], c) for y, c in zip(x, a)], table, ctx, 64, cu_new=cu)
+    dsa_cache.append([Rows(y[:, :3].reshape(15, 128).contiguous(), c) for y, c in zip(x, b)], table, ctx, 64, cu_new=cu)
+    for y, c, d in zip(x, a, b):
+        assert torch.equal(c, d) and torch.equal(c.cpu()[slot], y[:, :3].reshape(15, 128).cpu())
+
+
 def test_what_is_not_written():
     """Places outside the table, the null page, pages outside the pool, a length shorter than the new tokens, no sequence."""
     say("append not written")

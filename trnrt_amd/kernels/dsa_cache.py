@@ -139,8 +139,9 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
         size = _SIZES.get(x.dtype)
         if size is None:
             raise ValueError(f"dsa_cache.append: rows of {x.dtype}, expected bfloat16 or float32")
-        if x.dim() != 2:
+        if x.dim() != 2:  # (a copy, where the strides do not merge)
             x = x.reshape(-1, x.shape[-1])
+            held.append(x)
         t, W = x.shape
         if cache.shape[-1] != W or W == 0:
             raise ValueError(f"dsa_cache.append: rows {tuple(x.shape)} for a cache of width {cache.shape[-1]}")
