@@ -185,6 +185,16 @@ def test_rows_of_batches_that_do_not_merge():
         assert torch.equal(c, d) and torch.equal(c.cpu()[slot], y[:, :3].reshape(15, 128).cpu())
 
 
+@pytest.mark.parametrize("stride", [0, 8, 577, 580])
+def test_one_row_of_any_stride(stride):
+    say("append, a row of stride", stride)
+    cu, ctx, table, slots, slot, place = setup([1], [70], 64, 4)
+    x = torch.randn(600, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    cache = torch.zeros(slots, 576, dtype=torch.bfloat16).cuda()
+    dsa_cache.append(Rows(x.as_strided((1, 576), (stride, 1)), cache), table, ctx, 64)
+    assert torch.equal(cache.cpu()[slot], x[None, :576].cpu())
+
+
 def test_what_is_not_written():
     """Places outside the table, the null page, pages outside the pool, a length shorter than the new tokens, no sequence."""
     say("append not written")

@@ -161,6 +161,8 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
             x = x.clone(memory_format=torch.contiguous_format)
             held.append(x)
             row = W
+        elif T <= 1:  # (a single row's stride says nothing)
+            row = W
         if at is None:
             at = -1
         elif not (R and 0 <= at <= W - 2 * R):
@@ -174,7 +176,7 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
             held.append(norm)
             w, b = norm[0].data_ptr(), 0 if norm[1] is None else norm[1].data_ptr()
             norm_fp32, norm_width = norm[0].dtype is torch.float32, norm[0].shape[0]
-        kinds += _KIND.pack(x.data_ptr(), max(row, W), w, b, to, scale or 0, size == 4, W, at, bool(r.interleaved), norm_fp32,
+        kinds += _KIND.pack(x.data_ptr(), row, w, b, to, scale or 0, size == 4, W, at, bool(r.interleaved), norm_fp32,
                             norm_width, bf, r.eps, r.fp8_max)
     if cu is None and T and (not B or T % B):
         raise ValueError(f"dsa_cache.append: {T} rows for {B} sequences without cu_new")
