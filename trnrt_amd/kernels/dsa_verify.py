@@ -20,12 +20,17 @@ from . import _common as C
 _TYPES = (torch.bfloat16, torch.float32)
 
 
-def _rows(t: torch.Tensor, name: str, shape: tuple) -> torch.Tensor:
+def _rows(t: torch.Tensor, name: str, shape: tuple) -> tuple[torch.Tensor, int]:
+    """The rows, copied where a row's values do not lie side by side or rows overlap, and their stride."""
     if t.dtype not in _TYPES:
         raise ValueError(f"dsa_verify: {name} of {t.dtype}, expected bfloat16 or float32")
     if t.shape != shape:
         raise ValueError(f"dsa_verify: {name} {tuple(t.shape)}, expected {tuple(shape)}")
-    return t if t.stride(1) == 1 and t.stride(0) >= shape[1] else t.contiguous()
+    N, V = shape
+    row, col = t.stride()
+    if (col != 1 and V > 1) or (row < V and N > 1):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t, max(t.stride(0), V)  # (a single row's stride says nothing)
 
 
 def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch.Tensor, v: torch.Tensor,
@@ -44,9 +49,8 @@ def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError(f"dsa_verify: logits {tuple(logits.shape)}, expected [N, V]")
     N, V = logits.shape
-    logits = _rows(logits, "logits", logits.shape)
-    if draft_probs is not None:
-        draft_probs = _rows(draft_probs, "draft_probs", logits.shape)
+    logits, l_row = _rows(logits, "logits", logits.shape)
+    q, q_row = (None, 0) if draft_probs is None else _rows(draft_probs, "draft_probs", logits.shape)
     if cu.dim() != 1 or cu.numel() < 1:
         raise ValueError(f"dsa_verify: cu {tuple(cu.shape)}, expected [B + 1]")
     B = cu.numel() - 1
@@ -61,9 +65,8 @@ def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch
         ws = C.given(workspace, "dsa_verify")
     else:
         ws = C.scratch(dev, int(lib.dsa_verify_workspace_bytes(N, V, B)), "verify")
-    q = draft_probs
-    st = C.call(dev, lib.dsa_verify, logits.data_ptr(), logits.dtype is torch.float32, logits.stride(0), draft.data_ptr(),
-                C.ptr(q), q is not None and q.dtype is torch.float32, 0 if q is None else q.stride(0), cu.data_ptr(),
+    st = C.call(dev, lib.dsa_verify, logits.data_ptr(), logits.dtype is torch.float32, l_row, draft.data_ptr(),
+                C.ptr(q), q is not None and q.dtype is torch.float32, q_row, cu.data_ptr(),
                 u.data_ptr(), v.data_ptr(), temperature.data_ptr(), tokens.data_ptr(), accepted.data_ptr(),
                 logp.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), N, V, B)
     _lib.check(st, "dsa_verify")
