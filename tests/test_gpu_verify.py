@@ -1,7 +1,8 @@
 """Verification of drafts (trnrt_amd/kernels/dsa_verify.py) against a loop over rows in numpy's float64: tokens and counts
 equal, the log probabilities within 2^-24 of themselves (they are rounded once) and 2^-17: a row's sum is of 32-bit exponentials
 whose exponents are off by 1.5 x 2^-23 of themselves, 20 at the weights' mean at most (20 x 1.5 x 2^-23 ln 2 = 2.5e-6), exp2 by
-2^-23, and a term goes through 16 roundings on its way into the sum (1e-6): 3.6e-6, less than 2^-17 = 7.6e-6."""
+2^-23 twice (a logit's and its wave's), a term goes through 16 roundings on its way into the sum (1e-6) and the sum through two
+more: 3.9e-6, less than 2^-17 = 7.6e-6."""
 
 import math
 
@@ -22,7 +23,8 @@ def softmax(logits, temperature):
     if m == -np.inf:
         return np.zeros_like(x), np.full_like(x, -np.inf)
     t = float(temperature) if temperature > 0 else 1.0
-    e = np.where(x == m, 0.0, -np.inf) if m == np.inf else (x - m) / t
+    with np.errstate(invalid="ignore"):  # (-infinity over an infinite temperature)
+        e = np.where(x == m, 0.0, -np.inf if m == np.inf else np.where(x > -np.inf, (x - m) / t, -np.inf))
     p = np.exp(e)
     return p / p.sum(), e - math.log(p.sum())
 
@@ -148,6 +150,18 @@ def test_masks_ties_and_strange_logits():
         check(logits, draft, cu, u, v, heat)
     low = logits.bfloat16()
     check(low, draft, cu, u, v, temperature, q.bfloat16())
+
+
+@pytest.mark.parametrize("V", [300, 40000])
+def test_strange_temperatures(V):
+    """Infinite ones (all tokens that can come alike), the least and the largest, beside masked and infinite logits."""
+    say("verify, strange temperatures", V)
+    temperature = torch.tensor([math.inf, 1e30, 1e-30, 1e-45, 3e38, math.nan, -1.0, math.inf])
+    logits, draft, cu, u, v, _, q = make([4] * 8, V, torch.float32, torch.float32, 5)
+    logits[:, V // 3:V // 2] = -math.inf
+    logits[29:, 7] = math.inf
+    check(logits, draft, cu, u, v, temperature, q)
+    check(logits, draft, cu, u, v, temperature)
 
 
 def test_edges_of_the_random_numbers():

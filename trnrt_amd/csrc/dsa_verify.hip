@@ -182,7 +182,8 @@ __device__ __forceinline__ int vf_sequence(const int* __restrict__ cu, int B, in
 
 // vf_weight in 32 bits. (In 64, though few lanes come to it, 320 rows of 131,072 took 28.4 us for 21.6.)
 __device__ __forceinline__ float vf_weight32(float l, float m, float k) {
-  return l == m ? (l > -INFINITY ? 1.0f : 0.0f) : __builtin_amdgcn_exp2f((l - m) * k);
+  const float x = l == m ? 0.0f : (l - m) * k;
+  return x <= 0.0f && l > -INFINITY ? __builtin_amdgcn_exp2f(x) : 0.0f;
 }
 
 constexpr int VF_ROW_THREADS = 1024;
