@@ -484,9 +484,10 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
 /*
  * dsa_expanded_mla with more asked of the scores (the rest, the workspace among it, as there). Query i of a sequence stands
  * at place p = nk - nq + i among its nk keys; first, last int32 [Tq] (either may be null: 0 and nk), slopes fp32 [H] or
- * null, softcap 0 (none) or at least 1e-30 (its scores are off by softcap 2^-20 at most):
+ * null, softcap 0 (none) or 1e-30 to 1e30 (its scores are off by softcap 2^-20 at most):
  *   z[t] = scale * (q . k[t]),  z = softcap * tanh(z / softcap),  z -= slopes[h] * |p - t|,
  *   over the keys first[i] <= t < last[i] of the query's sequence, and t <= p where causal != 0.
+ * (slopes[h] * |p - t| is taken off in 32 bits, by 2^-22 of itself wrong at most.)
  * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
  * document's start; a window: first = p - window + 1. Only the tiles of 64 keys that some query of a workgroup's 256 sees
  * are read. DSA_EINVAL for another softcap.

@@ -16,7 +16,7 @@ def test_refusals():
         return _lib.lib().dsa_expanded_mla_spans(q, k, None, P, P, P, None, None, None, cap, out, None, P, ws, size, B, Tq, Tk,
                                                  H, 1, 0.1, None)
 
-    for kw in (dict(cap=-1.0), dict(cap=1e-31), dict(cap=float("inf")), dict(cap=float("nan")), dict(q=None), dict(k=None), dict(out=None),
+    for kw in (dict(cap=-1.0), dict(cap=1e-31), dict(cap=float("inf")), dict(cap=1e31), dict(cap=float("nan")), dict(q=None), dict(k=None), dict(out=None),
                dict(B=-1), dict(H=0), dict(q=ctypes.c_void_p(264))):
         assert call(**kw) == _lib.DSA_EINVAL, kw
     assert call(Tq=1 << 30, H=1 << 10) == _lib.DSA_EUNSUPPORTED

@@ -3,7 +3,6 @@
 // back to the caller's by events). Nothing here allocates device memory or synchronises the host.
 #include "../../include/dsa_gfx950.h"
 
-#include <cmath>
 #include <mutex>
 
 #include "dsa_append.h"
@@ -1380,7 +1379,7 @@ int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* r
                            const float* slopes, float softcap, void* out_bf16, float* out_f32, float* lse,
                            void* workspace, size_t workspace_bytes, int B, int Tq, int Tk, int H, int causal,
                            float scale, void* stream) {
-  if (!(softcap == 0.0f || softcap >= 1e-30f) || !std::isfinite(softcap)) return DSA_EINVAL;
+  if (!(softcap == 0.0f || (softcap >= 1e-30f && softcap <= 1e30f))) return DSA_EINVAL;
   const dsa::ExpandedMore more{first, last, slopes, softcap};
   return expanded_mla(q_bf16, k_bf16, rope_bf16, v_bf16, cu_q, cu_k, &more, out_bf16, out_f32, lse, workspace,
                       workspace_bytes, B, Tq, Tk, H, causal, scale, stream);

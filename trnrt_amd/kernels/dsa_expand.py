@@ -87,8 +87,9 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     first, last [Tq] int32: a query sees only keys first <= t < last of its sequence (either may be None), besides causal:
     documents packed into one sequence are first = the document's start; a prefix that its own tokens see both ways is last =
     max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. Only the
-    tiles of 64 keys that a query tile sees are read. softcap (0, or 1e-30 and more): scores become softcap tanh(s / softcap),
-    off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them.
+    tiles of 64 keys that a query tile sees are read. softcap (0, or 1e-30 to 1e30): scores become softcap tanh(s / softcap),
+    off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits,
+    off by 2^-22 of itself at most).
     workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
     dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
@@ -114,7 +115,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     more = first is not None or last is not None or slopes is not None or softcap != 0.0
     if more:
         C.on_gpu(q, first, last, slopes)
-        if softcap != 0.0 and not 1e-30 <= softcap < float("inf"):
+        if softcap != 0.0 and not 1e-30 <= softcap <= 1e30:
             raise ValueError(f"dsa_expand: softcap {softcap}")
         first = None if first is None else C.need(C.as_i32(first), "first", torch.int32, (Tq,))
         last = None if last is None else C.need(C.as_i32(last), "last", torch.int32, (Tq,))
