@@ -224,8 +224,9 @@ def test_views_and_rows_outside():
 def test_rows_of_any_stride():
     """A single row whose stride is below its width, a vocabulary of one token, one row for all, columns apart."""
     say("verify, strides")
-    x, q = torch.randn(900, generator=torch.Generator().manual_seed(3)).cuda(), torch.full((900,), 0.01).cuda()
-    for N, V, strides in [(1, 700, (0, 1)), (1, 700, (5, 1)), (1, 1, (1, 7)), (4, 1, (3, 7)), (4, 300, (0, 1)), (4, 300, (2, 3))]:
+    x, q = torch.randn(904, generator=torch.Generator().manual_seed(3)).cuda(), torch.full((904,), 0.01).cuda()
+    for N, V, strides in [(1, 700, (0, 1)), (1, 700, (5, 1)), (1, 1, (1, 7)), (4, 1, (3, 7)), (4, 300, (0, 1)),
+                          (4, 300, (2, 3))]:
         logits, probs = x.as_strided((N, V), strides), q.as_strided((N, V), strides)
         rand = torch.Generator().manual_seed(N + V)
         check(logits, torch.randint(0, V, (N,), generator=rand, dtype=torch.int32), torch.tensor([0, N], dtype=torch.int32),
