@@ -291,8 +291,11 @@ __device__ __forceinline__ void xa_find(int ti, const int* __restrict__ cu_q, in
   __syncthreads();
 }
 
-// MORE: with what ExpandedMore asks for (its branches are the workgroup's, or a tile's).
-template <int DQ, bool MORE>
+// MORE: 1 with the ranges of ExpandedMore, 2 with all that it asks for; its branches are the workgroup's, or a tile's. 8,192
+// causal tokens, 32 heads (610 us without): with first = 0 throughout 617 (as 2: 626), a window of 1,000 220, distances 685,
+// caps 705, both 788. What the ranges cost is tiles of 64 keys and 256 queries that they cut (a window of 1,000: 1.4 times
+// the pairs); caps and distances are vector issue beside the products.
+template <int DQ, int MORE>
 __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ kr,
     const uint16_t* __restrict__ v, const int* __restrict__ cu_q, const int* __restrict__ cu_k,
@@ -420,9 +423,16 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   }
   const float sl2 = scale * XA_LOG2E;
   [[maybe_unused]] bool fresh = true;  // (MORE) no key of this query's so far
-  [[maybe_unused]] float cap2 = 0.0f, cap_in = 0.0f, slope2 = 0.0f;
-  if constexpr (MORE) {
-    if (more.softcap > 0.0f) cap2 = more.softcap * XA_LOG2E, cap_in = 2.0f * XA_LOG2E * scale / more.softcap;
+  [[maybe_unused]] float cap2 = 0.0f, cap_in = 0.0f, slope2 = 0.0f, near_s = -1.0f, near_c[4];
+  if constexpr (MORE == 2) {
+    if (more.softcap > 0.0f) {
+      cap2 = more.softcap * XA_LOG2E, cap_in = 2.0f * XA_LOG2E * scale / more.softcap;
+      // tanh(x) / x for |x| <= 1/2 as a polynomial of x^2 (least largest error, 5.5e-7 of it), here of the score's square
+      const float by = scale / more.softcap, y = by * by;
+      if (fabsf(by) < 1e4f) near_s = fminf(0.5f / fabsf(by), 1e15f);
+      near_c[0] = 0.99999946f * sl2, near_c[1] = -0.33326318f * sl2 * y;
+      near_c[2] = 0.13190297f * sl2 * y * y, near_c[3] = -0.044402226f * sl2 * y * y * y;
+    }
     if (more.slopes) slope2 = more.slopes[head] * XA_LOG2E;
   }
   float m_run = 0.0f, l_run = 0.0f;  // running maximum (base 2), this lane's share of the sum
@@ -453,23 +463,37 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
           s2[x] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(*reinterpret_cast<const uint4*>(at)), qf[s], s2[x],
                                                           0, 0, 0);
         }
-      const float from = MORE ? (float)(nk - nq + qi - i * XA_K - 4 * h) : 0.0f;  // (|p - t| < 2^24: exact)
-      if (MORE && cap2 > 0.0f) {
-        // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), here in base 2
+      const float from = MORE == 2 ? (float)(nk - nq + qi - i * XA_K - 4 * h) : 0.0f;  // (|p - t| < 2^24: exact)
+      if (MORE == 2 && cap2 > 0.0f) {
+        float top = fabsf(s2[0][0]);
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int r = 1; r < 32; ++r) top = max_nonan(top, fabsf(s2[r >> 4][r & 15]));
+        // Where the tile's scores are all below half the cap, as most are, no exponential and reciprocal (705 us for 728 of
+        // the call below; scores of up to the cap 745 for 730).
+        if (__ballot(!(top <= near_s)) == 0) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const float e = __builtin_amdgcn_exp2f(s2[x][r] * cap_in);
-            s2[x][r] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + e), cap2 - m_run);
-          }
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float s = s2[x][r], y = s * s;
+              s2[x][r] = fmaf(s, fmaf(y, fmaf(y, fmaf(y, near_c[3], near_c[2]), near_c[1]), near_c[0]), -m_run);
+            }
+        } else {  // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), here in base 2
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const float e = __builtin_amdgcn_exp2f(s2[x][r] * cap_in);
+              s2[x][r] = fmaf(-2.0f * cap2, __builtin_amdgcn_rcpf(1.0f + e), cap2 - m_run);
+            }
+        }
         if (more.slopes)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               s2[x][r] = fmaf(-slope2, fabsf(from - (float)(32 * x + 8 * (r >> 2) + (r & 3))), s2[x][r]);
-      } else if (MORE && more.slopes && (i + 1) * XA_K - 1 <= nk - nq + w0) {
+      } else if (MORE == 2 && more.slopes && (i + 1) * XA_K - 1 <= nk - nq + w0) {
         // No key of the tile is behind a query of the wave: slope (p - t) is the tile's own, as large as its weights are
         // small, less slope times the key's place in it (8k tokens, 32 heads: 692 us for 702).
         const float base = fmaf(-slope2, from, -m_run);
@@ -483,7 +507,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s2[x][r] = fmaf(s2[x][r], sl2, -m_run);
-        if (MORE && more.slopes)
+        if (MORE == 2 && more.slopes)
 #pragma unroll
           for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -717,9 +741,11 @@ hipError_t launch_expanded_attend(const uint16_t* q, const uint16_t* k, const ui
                                   int B, int Tq, int Tk, int H, int causal, float scale, const ExpandedMore* more,
                                   int num_cu, hipStream_t s) {
   const int q_tiles = attend_tiles(B, Tq), splits = attend_splits(B, Tq, Tk, H, num_cu);
-  const auto kernel = more ? kr ? expanded_attend_kernel<EX_D + EX_R, true> : expanded_attend_kernel<EX_D, true>
-                      : kr ? expanded_attend_kernel<EX_D + EX_R, false>
-                           : expanded_attend_kernel<EX_D, false>;
+  const auto kernel = !more ? kr ? expanded_attend_kernel<EX_D + EX_R, 0> : expanded_attend_kernel<EX_D, 0>
+                      : more->softcap == 0.0f && !more->slopes
+                          ? kr ? expanded_attend_kernel<EX_D + EX_R, 1> : expanded_attend_kernel<EX_D, 1>
+                      : kr ? expanded_attend_kernel<EX_D + EX_R, 2>
+                           : expanded_attend_kernel<EX_D, 2>;
   const hipError_t e = launch("expanded_attend_kernel", kernel, dim3((unsigned)q_tiles * H * splits), dim3(XA_THREADS), s,
                               q, k, kr, v, cu_q, cu_k, out, out_f32, lse, static_cast<float*>(ws), B, Tq, Tk, H, q_tiles,
                               splits, causal, scale, more ? *more : ExpandedMore{});
