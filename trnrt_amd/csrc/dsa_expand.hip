@@ -293,7 +293,7 @@ __device__ __forceinline__ void xa_find(int ti, const int* __restrict__ cu_q, in
 
 // MORE: 1 with the ranges of ExpandedMore, 2 with all that it asks for; its branches are the workgroup's, or a tile's. 8,192
 // causal tokens, 32 heads (610 us without): with first = 0 throughout 617 (as 2: 626), a window of 1,000 220, distances 685,
-// caps 705, both 788. What the ranges cost is tiles of 64 keys and 256 queries that they cut (a window of 1,000: 1.4 times
+// caps 705, both 788. What the ranges cost is tiles of 64 keys and 256 queries that they cut (a window of 1,000: 1.3 times
 // the pairs); caps and distances are vector issue beside the products.
 template <int DQ, int MORE>
 __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
