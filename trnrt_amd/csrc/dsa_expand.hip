@@ -292,9 +292,9 @@ __device__ __forceinline__ void xa_find(int ti, const int* __restrict__ cu_q, in
 }
 
 // MORE: 1 with the ranges of ExpandedMore, 2 with all that it asks for; its branches are the workgroup's, or a tile's. 8,192
-// causal tokens, 32 heads (610 us without): with first = 0 throughout 617 (as 2: 626), a window of 1,000 220, distances 685,
-// caps 705, both 788. What the ranges cost is tiles of 64 keys and 256 queries that they cut (a window of 1,000: 1.3 times
-// the pairs); caps and distances are vector issue beside the products.
+// causal tokens, 32 heads on one card (601 us without): with first = 0 throughout 608 (as 2: 626 for 617 on another), a window
+// of 1,000 215, distances 632, caps 702, both 733. What the ranges cost is the tiles of 64 keys and 256 queries that they cut
+// (a window of 1,000: 1.3 times the pairs); caps and distances are vector issue beside the products.
 template <int DQ, int MORE>
 __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k, const uint16_t* __restrict__ kr,
@@ -388,7 +388,10 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                        8 * ((lane & 7) ^ ((8 * x + (lane >> 3)) >> 1)),
                    r_lds + XA_K * 128 * to + 1024 * x);
   };
-  if (brings && nt > i0) issue(i0, 0);
+  // The tile that comes n-th. With distances the last one comes first: its scores are the largest, so that the maximum hardly
+  // moves after it (8,192 tokens, 32 heads 632 us for 675; 2,048 of 10,240 309 for 339).
+  auto tile = [&](int n) __attribute__((always_inline)) { return MORE == 2 ? nt - 1 - (n - i0) : n; };
+  if (brings && nt > i0) issue(tile(i0), 0);
   // the queries through LDS, over the stages that tiles 1 and 2 take: columns 64 p .. + 63 of the wave's 32 rows are 4
   // KiB of k, v or r, laid out as rope rows. (Read straight into the operands' layout, 32 bytes of 32 rows at a time,
   // they took 5,000 cycles more.)
@@ -410,7 +413,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
                                                         16 * ((2 * (s & 3) + h) ^ ((j >> 1) & 7))));
   }
   lds_barrier();  // the queries are read
-  if (brings && nt > i0 + 1) issue(i0 + 1, 1);
+  if (brings && nt > i0 + 1) issue(tile(i0 + 1), 1);
   int koff[8], roff[4], voff[4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) koff[i] = 256 * j + 16 * ((2 * i | h) ^ (j & 15));
@@ -442,14 +445,15 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
   if (wave < 4) __builtin_amdgcn_s_setprio(1);
   int stage = 0;
 #pragma unroll 1
-  for (int i = i0; i < nt; ++i) {
+  for (int n = i0; n < nt; ++n) {
+    const int i = tile(n);
     if (brings) {
-      if (i + 1 < nt)
+      if (n + 1 < nt)
         wait_loads<LOADS>();
       else
         wait_loads<0>();
     }
-    lds_barrier();  // tile i is in place, and nobody reads tile i - 1 any more
+    lds_barrier();  // tile i is in place, and nobody reads the one before any more
     if (i < nt_w && (!MORE || i >= i0_w)) {
       const uint8_t* const kt = sh.k[stage];
       const uint8_t* const vt = sh.v[stage];
@@ -468,8 +472,8 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         float top = fabsf(s2[0][0]);
 #pragma unroll
         for (int r = 1; r < 32; ++r) top = max_nonan(top, fabsf(s2[r >> 4][r & 15]));
-        // Where the tile's scores are all below half the cap, as most are, no exponential and reciprocal (705 us for 728 of
-        // the call below; scores of up to the cap 745 for 730).
+        // Where the tile's scores are all below half the cap, as most are, no exponential and reciprocal (8,192 tokens,
+        // 32 heads: 705 us for 728; scores of up to the cap 745 for 730).
         if (__ballot(!(top <= near_s)) == 0) {
 #pragma unroll
           for (int x = 0; x < 2; ++x)
@@ -495,7 +499,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
               s2[x][r] = fmaf(-slope2, fabsf(from - (float)(32 * x + 8 * (r >> 2) + (r & 3))), s2[x][r]);
       } else if (MORE == 2 && more.slopes && (i + 1) * XA_K - 1 <= nk - nq + w0) {
         // No key of the tile is behind a query of the wave: slope (p - t) is the tile's own, as large as its weights are
-        // small, less slope times the key's place in it (8k tokens, 32 heads: 692 us for 702).
+        // small, less slope times the key's place in it (8,192 tokens, 32 heads: 692 us for 702 then).
         const float base = fmaf(-slope2, from, -m_run);
 #pragma unroll
         for (int x = 0; x < 2; ++x)
@@ -576,7 +580,7 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
         }
       }
     }
-    if (brings && i + 2 < nt) issue(i + 2, stage == 0 ? 2 : stage - 1);  // (where tile i - 1 was)
+    if (brings && n + 2 < nt) issue(tile(n + 2), stage == 0 ? 2 : stage - 1);  // (where the one before was)
     stage = stage == XA_STAGES - 1 ? 0 : stage + 1;
   }
   __syncthreads();  // the stages are free
