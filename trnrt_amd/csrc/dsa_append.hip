@@ -7,7 +7,11 @@
 //
 // 16 lanes have a row (a row of the DPP network: its sums and maxima never leave it), 8 of its columns at a time each, so that
 // rows of 576 and of 128 columns both leave few lanes idle; a wave has the rows of one kind of 4 tokens. What bounds it is
-// vector issue, about 300 instructions a token and wave, then the rows' bytes.
+// vector issue (13 of the 23 us of 21,456 tokens with norms and three axes, whose 46 MB a copy would move in 9), then loads
+// that one wave's four tokens do not cover; 8 tokens 4.4 us: a launch and three dependent reads (lengths, page, row). Not
+// kept, of those 23 us: every kind's rows in one wave 23.2; registers for 5 or 6 waves a SIMD 22.8 and 32; workgroups of 1
+// and 2 waves 27 and 24; a wave a row, which
+// divides by s, 40.
 #include "dsa_append.h"
 
 namespace dsa {
@@ -271,6 +275,7 @@ hipError_t launch_cache_append(const AppendSet& set, const RopeAngles& a, const 
     return launch("cache_append_kernel", kernel, dim3((unsigned)((units + AP_WAVES - 1) / AP_WAVES)), dim3(AP_WAVES * WAVE), s,
                   set, a, table, ctx_len, cu, T, B, max_pages, page_size, num_pages);
   };
+  // (the wider one for the same rows: 39 us for 23)
   return width <= 640 && a.R <= 64 ? go(cache_append_kernel<5, 64>) : go(cache_append_kernel<AP_MAX_WIDTH / 128, RP_MAX_R>);
 }
 
