@@ -517,7 +517,8 @@ int dsa_rope_rotate(const void* x, int x_fp32, long long x_row, long long x_head
  * cu_new[b] .. cu_new[b + 1] - 1 of every x (int32 [B + 1], ascending; null: T / B each), the last of its ctx_len[b] tokens
  * (int32 [B], the new ones counted): token j of n has place ctx_len[b] - n + j, slot page_table[b][place / page_size] *
  * page_size + place % page_size. A token whose place is outside the table, or whose page is not in 1 .. num_pages - 1, is
- * not written, nor are rows in no sequence; two tokens of one slot leave one of them. For each kind:
+ * not written, nor are rows in no sequence; no two tokens of a call may have one slot (its row would be parts of both). For
+ * each kind:
  *   x [T, width] bf16 or fp32, rows x_row values apart; width a multiple of 8 up to 1,024;
  *   norm_weight [norm_width] (null: none; bf16 or fp32 as norm_fp32 says; norm_width a multiple of 8): of the first
  *     norm_width columns x / sqrt(mean x^2 + eps) * weight, or with norm_bias (x - mean) / sqrt(var + eps) * weight + bias;

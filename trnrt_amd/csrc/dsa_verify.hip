@@ -117,8 +117,8 @@ __device__ __forceinline__ double vf_exponent(float l, float m, double k) {
 }
 
 // 2^x for x <= 0 (x < -1022: 2^-1022), by the series of e^(f ln 2) about the nearest whole number; the first term left out is
-// 2e-16 of it at most. (With two terms less, 2e-13, tokens moved where a draft's probabilities were the target's own.) The whole
-// number is found, and put into the exponent, through the low bits of x + 1.5 2^52.
+// 2e-16 of it at most. (With two terms less, 2e-13, tokens moved where a draft's probabilities were the target's own.) The
+// whole number is found, and put into the exponent, through the low bits of x + 1.5 2^52.
 __device__ __forceinline__ double vf_exp2(double x) {
   x = fmax(x, -1022.0);
   const double big = 6755399441055744.0, n = x + big, f = x - (n - big);

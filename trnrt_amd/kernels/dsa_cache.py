@@ -115,7 +115,8 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
     (ctx_len [B] int32 counts the new ones), through table [B, max_pages] int32. The columns that a kind names are rotated
     by positions ([T], or [axes, T] with axes, as in dsa_rope.rotate; None: the token's place in its sequence) x inv_freq
     [R] fp32 x factor. Everything is in fp32 and rounded once, as store rounds. A token whose place is outside the table, or
-    whose page is the null page or outside the pool, is not written, nor are rows in no sequence."""
+    whose page is the null page or outside the pool, is not written, nor are rows in no sequence. No two tokens of a call may
+    have one slot."""
     rows = (rows,) if isinstance(rows, Rows) else rows
     if not rows:
         raise ValueError("dsa_cache.append: no rows")
