@@ -195,6 +195,17 @@ def test_one_row_of_any_stride(stride):
     assert torch.equal(cache.cpu()[slot], x[None, :576].cpu())
 
 
+def test_no_rotation_beside_positions_and_axes():
+    """Rows without rotated columns in a program that has positions of three axes for its other layers."""
+    say("append, axes without frequencies")
+    cu, ctx, table, slots, slot, place = setup([3, 40], [40, 7], 64, 4)
+    x = torch.randn(43, 512, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    cache = torch.zeros(slots, 512, dtype=torch.bfloat16).cuda()
+    pos = torch.zeros(3, 43, dtype=torch.int32).cuda()
+    dsa_cache.append(Rows(x, cache), table, ctx, 64, cu_new=cu, positions=pos, axes=[i % 3 for i in range(32)], factor=1.1)
+    assert torch.equal(cache.cpu()[slot], x.cpu())
+
+
 def test_what_is_not_written():
     """Places outside the table, the null page, pages outside the pool, a length shorter than the new tokens, no sequence."""
     say("append not written")

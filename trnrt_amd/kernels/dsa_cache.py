@@ -114,9 +114,9 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
     cu_new[b] .. cu_new[b + 1] - 1 of every x (cu_new [B + 1] int32; None: T / B each) and the last of its ctx_len[b] tokens
     (ctx_len [B] int32 counts the new ones), through table [B, max_pages] int32. The columns that a kind names are rotated
     by positions ([T], or [axes, T] with axes, as in dsa_rope.rotate; None: the token's place in its sequence) x inv_freq
-    [R] fp32 x factor. Everything is in fp32 and rounded once, as store rounds. A token whose place is outside the table, or
-    whose page is the null page or outside the pool, is not written, nor are rows in no sequence. No two tokens of a call may
-    have one slot."""
+    [R] fp32 x factor (without inv_freq no kind is rotated, and positions and axes are not used). Everything is in fp32 and
+    rounded once, as store rounds. A token whose place is outside the table, or whose page is the null page or outside the
+    pool, is not written, nor are rows in no sequence. No two tokens of a call may have one slot."""
     rows = (rows,) if isinstance(rows, Rows) else rows
     if not rows:
         raise ValueError("dsa_cache.append: no rows")
@@ -181,7 +181,7 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
                             norm_width, bf, r.eps, r.fp8_max)
     if cu is None and T and (not B or T % B):
         raise ValueError(f"dsa_cache.append: {T} rows for {B} sequences without cu_new")
-    pos, n_axes, which = axis_map(axes, positions, R, T, "dsa_cache.append")
+    pos, n_axes, which = axis_map(axes, positions, R, T, "dsa_cache.append") if R else (None, 1, None)
     st = C.call(dev, _lib.lib().dsa_cache_append, kinds, len(rows), tb.data_ptr(), lens.data_ptr(), C.ptr(cu), C.ptr(pos),
                 C.ptr(inv_freq), which, T, B, R, n_axes, factor, max_pages, page_size, slots // page_size)
     _lib.check(st, "dsa_cache.append")
