@@ -490,7 +490,8 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
  * (slopes[h] * |p - t| is taken off in 32 bits, by 2^-22 of itself wrong at most.)
  * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
  * document's start; a window: first = p - window + 1. Only the tiles of 64 keys that some query of a workgroup's 256 sees
- * are read. DSA_EINVAL for another softcap.
+ * are read. A hidden key's NaN or infinity stays hidden; a value's reaches every query of its sequence whose 32 share a tile
+ * of 64 keys with it, as 0 x NaN, also queries of another document. DSA_EINVAL for another softcap.
  */
 int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
                            const int32_t* cu_q, const int32_t* cu_k, const int32_t* first, const int32_t* last,

@@ -88,8 +88,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     documents packed into one sequence are first = the document's start; a prefix that its own tokens see both ways is last =
     max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. Only the
     tiles of 64 keys that a query tile sees are read. softcap (0, or 1e-30 to 1e30): scores become softcap tanh(s / softcap),
-    off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits,
-    off by 2^-22 of itself at most).
+    off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits, off by 2^-22 of itself at
+    most). A value's NaN or infinity may reach queries that do not see it (0 x NaN), a key's does not.
     workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
     dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
