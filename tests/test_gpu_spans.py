@@ -205,6 +205,25 @@ def test_strange_values_in_hidden_keys():
     assert torch.equal(out[:240], clean[0][:240]) and lse[240:250, 0].isnan().all()
 
 
+@pytest.mark.parametrize("cap,bias", [(50.0, False), (0.5, False), (0.0, True), (50.0, True)])
+def test_strange_values_in_hidden_keys_beside_caps_and_distances(cap, bias):
+    """The same where scores are changed. A hidden score may decide how its neighbours' caps are computed, within what those are
+    off by (cap 2^-20 on both sides, 2^-13 of a weight at most here): the outputs then move by that, by two roundings of each
+    weight and by the outputs' own, so by less than 2^-7 + 2^-8 + 2^-12 of the largest value; the lse by 2^-13 and 2^-23 of it."""
+    say("spans hidden NaN, scores", cap, bias)
+    lq = lk = [500]
+    q, k, r, v = inputs(lq, lk, 2, True, 6)
+    first = torch.where(torch.arange(500) < 250, 0, 250).to(torch.int32).cuda()
+    kw = dict(first=first, softcap=cap, slopes=torch.tensor([0.01, 0.5]).cuda() if bias else None)
+    clean = dsa_expand.attend(q, k, r, v, cu_of(lq).cuda(), cu_of(lk).cuda(), 0.07, **kw)
+    k[240, 0, 3], k[245, :, 9], r[247] = torch.nan, torch.inf, -torch.inf
+    out, lse = dsa_expand.attend(q, k, r, v, cu_of(lq).cuda(), cu_of(lk).cuda(), 0.07, **kw)
+    for a, b in ((250, 500), (0, 240)):
+        assert ((out - clean[0])[a:b].abs() <= (2.0 ** -7 + 2.0 ** -8 + 2.0 ** -12) * v.abs().max()).all()
+        assert ((lse - clean[1])[a:b].abs() <= 2.0 ** -13 + 2.0 ** -23 * lse[a:b].abs()).all()
+    assert lse[240:250, 0].isnan().all()
+
+
 def test_graph():
     say("spans graph")
     lq, lk, H = [40, 100], [3000, 100], 2

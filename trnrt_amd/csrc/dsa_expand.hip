@@ -473,7 +473,8 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
 #pragma unroll
         for (int r = 1; r < 32; ++r) top = max_nonan(top, fabsf(s2[r >> 4][r & 15]));
         // Where the tile's scores are all below half the cap, as most are, no exponential and reciprocal (8,192 tokens,
-        // 32 heads: 705 us for 728; scores of up to the cap 745 for 730).
+        // 32 heads: 705 us for 728; scores of up to the cap 745 for 730). The two differ by the cap's 2^-20 at most, so that a
+        // query's bits may depend on its wave's other queries.
         if (__ballot(!(top <= near_s)) == 0) {
 #pragma unroll
           for (int x = 0; x < 2; ++x)

@@ -457,7 +457,8 @@ constexpr int VF_CHUNK = VF_THREADS * VF_VEC;
 template <bool FOUND>
 __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, const VerifyPart* __restrict__ parts,
                                                                  const VerifyStop* __restrict__ stops,
-                                                                 VerifyChunk* __restrict__ sums, VerifyCount* __restrict__ done) {
+                                                                 VerifyChunk* __restrict__ sums,
+                                                                 VerifyCount* __restrict__ done) {
   __shared__ VerifyStop stop_row;
   __shared__ VerifyAsk ask;
   __shared__ VerifyChunk part[VF_WAVES];
@@ -685,7 +686,8 @@ hipError_t launch_verify(const void* logits, int l_fp32, long l_row, const int* 
                      : rows(verify_rows_kernel<uint16_t, 1>);
   if (e != hipSuccess) return e;
   const auto pick = [&](auto kernel) {
-    return launch("verify_pick_kernel", kernel, dim3((unsigned)(B * a.chunks)), dim3(VF_THREADS), s, a, parts, stops, sums, done);
+    return launch("verify_pick_kernel", kernel, dim3((unsigned)(B * a.chunks)), dim3(VF_THREADS), s, a, parts, stops, sums,
+                  done);
   };
   // Where the workgroups do not all run at once (5 a CU), each finding its stop row costs more than a launch that does: 64
   // sequences of 131,072 42 us for 5 + 20, 13 of 100,003 13.6 for 5 + 9.6.
