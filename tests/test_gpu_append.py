@@ -314,3 +314,26 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="GPU only"):
         call(rows=Rows(x.cpu(), kv, s))
     call(rows=Rows(x[:0], kv, s), cu_new=torch.zeros(3, **i32))  # no tokens
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("fp8_max", [448.0, 240.0])
+@pytest.mark.parametrize("W", [128, 576])
+def test_infinities_without_a_scale(dtype, fp8_max, W):
+    """+infinity is clamped to the largest code, -infinity and NaN to the least: store's bytes, from rows and out of a norm."""
+    say("append infinities, unscaled", dtype, fp8_max, W)
+    cu, ctx, table, slots, slot, _ = setup([5], [60], 64, 2)
+    x = torch.randn(5, W, generator=torch.Generator().manual_seed(W)).to(dtype).cuda()
+    x[0, 5], x[1, 7], x[2, 0], x[3, W - 1], x[3, 1] = torch.inf, -torch.inf, torch.nan, torch.inf, -torch.inf
+    x[4, 3], x[4, 9] = 3e38, -3e38
+    a, b = (torch.ones(slots, W, device="cuda").to(FP8) for _ in range(2))
+    dsa_cache.append(Rows(x, a, fp8_max=fp8_max), table, ctx, 64, cu_new=cu)
+    dsa_cache.store(b, slot.cuda(), x, fp8_max)
+    assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    got = a[slot.cuda()].float()
+    assert got[0, 5] == got[3, W - 1] == got[4, 3] == fp8_max and got[1, 7] == got[3, 1] == got[4, 9] == -fp8_max
+    w = torch.full((W,), 1e38, device="cuda")  # (normed values of 2 and more overflow)
+    y = torch.zeros(1, W, device="cuda")
+    y[0, 0], y[0, 1] = 1.0, -1.0
+    dsa_cache.append(Rows(y, a, norm=w, fp8_max=fp8_max), table, ctx, 64)
+    assert a[slot[4].cuda(), :2].float().tolist() == [fp8_max, -fp8_max] and (a[slot[4].cuda(), 2:].float() == 0).all()

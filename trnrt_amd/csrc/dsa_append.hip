@@ -206,7 +206,7 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
   }
   // The quotient by s, correctly rounded as store's is: the product with the (correctly rounded) reciprocal, corrected by the
   // remainder, which is exact; only a divisor whose mantissa is all ones needs the division itself, and an infinite one no
-  // correction.
+  // correction. Without a scale nothing is divided (an infinity's remainder by 1 would be NaN, which is clamped to -).
   float s = 1.0f;
   if (r.scale) {
     float amax = 0.0f;  // (columns past the row are 0)
@@ -236,6 +236,10 @@ __device__ __forceinline__ void ap_rows(const AppendRows& r, const RopeAngles& a
     if (ones) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) q[e] = v[i][e] / s;
+    }
+    if (!r.scale) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) q[e] = v[i][e];
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) q[e] = __builtin_amdgcn_fmed3f(q[e], -r.fp8_max, r.fp8_max);  // (NaN: -)
