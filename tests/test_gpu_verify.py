@@ -333,3 +333,31 @@ def test_refusals():
             dsa_verify.verify(**{**base, **kw})
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_verify.verify(**{**base, "u": u.cpu()})
+
+
+@pytest.mark.parametrize("B,V", [(1, 6), (9, 3000), (3, 70000), (40, 70000)])  # (the last with a launch for the stop rows)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_that_are_nothing_in_64_bits(B, V, dtype):
+    """Low temperatures, at which all but few tokens' probabilities are 0 in 64 bits (e^-1000 and less): with v = 0 the first token
+    whose is not comes; and where the draft's probabilities leave nothing over of those few (r = 0), it comes from p."""
+    say("verify, weights that are nothing", B, V, dtype)
+    g = torch.Generator().manual_seed(V)
+    rows = [3] * B
+    N = 3 * B
+    cu = torch.tensor([0] + rows).cumsum(0).to(torch.int32)
+    main = torch.randint(V // 2, V, (N,), generator=g)
+    logits = torch.randint(-3, 1, (N, V), generator=g).float()
+    logits[torch.arange(N), main] = 10.0
+    logits = logits.to(dtype).cuda()
+    q = torch.zeros(N, V)
+    q[torch.arange(N), main] = 1.0
+    q[:, 2], q[:, 0] = 1e-30, 1e-38  # (drafts of these are refused: their p is 0)
+    u, zero, most = torch.rand(N, generator=g), torch.zeros(B), torch.full((B,), 1 - 2.0 ** -24)
+    for heat in (1e-3, 1e-2):
+        temperature = torch.full((B,), heat)
+        for v in (zero, most):
+            for draft in (torch.full((N,), -1, dtype=torch.int32), torch.full((N,), 2, dtype=torch.int32), main.to(torch.int32)):
+                for probs in (None, q.cuda(), q.to(torch.bfloat16).cuda()):
+                    tokens, _, _ = check(logits, draft, cu, u, v, temperature, probs)
+                    drawn = tokens.cpu()[tokens.cpu() >= 0].long()
+                    assert torch.isin(drawn, main).all()

@@ -409,10 +409,11 @@ __device__ __forceinline__ void vf_stop_row(const VerifyArgs& a, int row, bool w
   }
 }
 
-// A weight of the stop row (m is finite there).
+// A weight of the stop row (m is finite there): 0 where vf_weight's is, so that no token comes whose probability is 0.
+// (-infinity: exponent -infinity, or NaN at an infinite temperature)
 __device__ __forceinline__ double vf_stop_weight(float x, float m, double k) {
-  const double w = vf_exp2(((double)x - (double)m) * k);
-  return x > -INFINITY ? w : 0.0;
+  const double e = ((double)x - (double)m) * k, w = vf_exp2(e);
+  return e > -1022.0 ? w : 0.0;
 }
 
 // v's inclusive prefix sum over the wave.

@@ -6,8 +6,9 @@ back by the drafts that were not taken, whose cached rows the next dsa_cache.app
 
 With p = softmax(logits / temperature), a draft x of row j is taken iff u[j] q(x) < p(x), up to the first that is not; the
 next token is drawn from max(p - q, 0) of that row (from p of the last row, once all are taken) by v: what comes out is
-distributed as the target's own samples are. Tokens and counts are those of 64-bit probabilities, sums and comparisons, and do
-not vary from run to run; logp is off by 2^-17 at most beside its rounding. The HIP kernels are in csrc/dsa_verify.hip.
+distributed as the target's own samples are. Tokens and counts are those of 64-bit probabilities, sums and comparisons (a
+probability of no more than 2^-1022 of the row's largest is 0), and do not vary from run to run; logp is off by 2^-17 at most
+beside its rounding. The HIP kernels are in csrc/dsa_verify.hip.
 """
 
 from __future__ import annotations
