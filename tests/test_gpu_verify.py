@@ -361,3 +361,46 @@ def test_weights_that_are_nothing_in_64_bits(B, V, dtype):
                     tokens, _, _ = check(logits, draft, cu, u, v, temperature, probs)
                     drawn = tokens.cpu()[tokens.cpu() >= 0].long()
                     assert torch.isin(drawn, main).all()
+
+
+def test_targets_beside_a_tokens_edge():
+    """v within 2e-12 to 4e-11 of where the running sum passes a token's end: r is (1e-5 of p, so that no token is too near to
+    say) and its sums are such that the 32-bit row sum's error and a 32-bit sum of q together move them by more than that. In 64
+    bits they are off by less than 1e-12: r by 3e-16 of p, 3e-11 of itself, at random over 100,000 tokens. The reference is in
+    80 bits. The temperature is one whose reciprocal rounds badly, so that the 32-bit sum is off by 4e-7."""
+    say("verify, edges")
+    V, B = 100_000, 128
+    rng = np.random.default_rng(5)
+    heats = np.float32(0.9) + np.arange(4000, dtype=np.float32) * np.float32(2.0 ** -16)
+    k = 1.4426950408889634 / heats.astype(np.float64)
+    heat = heats[np.argmax(k.astype(np.float32) / k)]
+    l = (np.round(rng.standard_normal(V) * 2 * 256) / 256).astype(np.float32)  # (differences exact in 32 bits)
+    e = np.exp((l.astype(np.longdouble) - l.max()) / np.longdouble(heat))
+    p = e / e.sum()
+    q = (p * (1 + np.longdouble(1e-5) * np.where(rng.random(V) < 0.5, 1, -1))).astype(np.float32)
+    r = np.maximum(p - q, 0)
+    c = np.cumsum(r)
+    c /= c[-1]
+    ends = c[r > 0]
+    vs = []
+    for v in (ends.astype(np.float32), np.nextafter(ends.astype(np.float32), np.float32(0)),
+              np.nextafter(ends.astype(np.float32), np.float32(1))):
+        gap = np.abs(v - ends)
+        vs.append(v[(gap > 2e-12) & (gap < 4e-11) & (v > 0) & (v < 1)])
+    v = np.unique(np.concatenate(vs))
+    assert len(v) >= 32
+    v = rng.choice(v, B)
+    want = np.array([int(np.nonzero(c > np.longdouble(x))[0][0]) for x in v])
+    x = int(np.argmax(np.where(q > p, p, 0)))  # (u q > p: refused)
+    row, probs = torch.tensor(l).cuda(), torch.tensor(q).cuda()
+    for few in (4, B):  # (the stop rows found by the pick itself, and in a launch of their own)
+        tokens = []
+        for at in range(0, B, few):
+            n = 2 * few
+            tokens.append(dsa_verify.verify(
+                row.expand(n, V).contiguous(), torch.full((n,), x, dtype=torch.int32).cuda(),
+                torch.arange(0, n + 1, 2, dtype=torch.int32).cuda(), torch.full((n,), 1 - 2.0 ** -24).cuda(),
+                torch.tensor(v[at:at + few]).cuda(), torch.full((few,), float(heat)).cuda(),
+                draft_probs=probs.expand(n, V).contiguous())[0][0::2].cpu())
+        got = torch.cat(tokens).numpy()
+        assert (got == want).all(), (int((got != want).sum()), got[got != want], want[got != want])

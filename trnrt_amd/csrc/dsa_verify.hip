@@ -8,10 +8,10 @@
 // Which token comes does not depend on roundings in 32 bits, though nearly all rows are only summed in 32: a row's sum of
 // exp((l - max) / T) is taken in 32 bits (off by VF_NEAR of itself at most), and only where that decides nothing, with u q
 // and p that close, again in 64. The stop row's sums are in 64 bits: with w the weights and z the 32-bit sum, a pass over it
-// sums w, and w - q z and q where that is above 0. r's sum at the 64-bit sum z' of w is then theirs plus (z - z') times q's
-// (for which 32 bits do); tokens on either side of w = q z by less than VF_NEAR are too near to say, their r is off by q |z' -
-// z| each, and where the sum of those bounds could move the token (or where r would be 0) the row is gone through once more
-// with z'.
+// sums w, and w - q z and q where that is above 0. r's sum at the 64-bit sum z' of w is then theirs plus (z - z') times q's,
+// which is summed in 32 bits, off by 2^-20 of itself at most; tokens on either side of w = q z by less than VF_NEAR are too near
+// to say, their r is off by q |z' - z| each. Where the sum of those bounds could move the token (or where r would be 0) the row
+// is gone through once more with z'.
 //
 // Two launches, or three. verify_rows_kernel: a workgroup of 16 waves takes up to 32,768 logits of a row to (maximum, sum,
 // place of the maximum), so that a row has few parts. verify_pick_kernel: every workgroup of a sequence finds its stop row
@@ -555,16 +555,17 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
   }
   // (a certain draft's own weight is not in `all`)
   z = vf_wave_sum(z) + vf_stop_weight(xd, m, k);
-  // (the bounds were for a z off by VF_NEAR of itself; by now it is known by how much)
-  near = vf_wave_sum(near) * (fabs(z - z0) / (VF_NEAR * z0));
   // r's sum at z: it moves by q for every one that z does
   const auto rest_of = [&](const VerifyChunk& t) { return fmax(fma(z0 - z, t.q, t.rest), 0.0); };
-  double rest = rest_of(front);
+  double rest = rest_of(front), taken = front.q;
   for (int c0 = WAVE; c0 < a.chunks; c0 += WAVE) {
     const VerifyChunk t = load(c0 + lane);
-    rest += rest_of(t);
+    rest += rest_of(t), taken += t.q;
   }
   rest = vf_wave_sum(rest);
+  // The bounds were for a z off by VF_NEAR of itself; by now it is known by how much. And the chunks' q are sums in 32 bits,
+  // 14 roundings of 2^-24 on a term's way into them.
+  near = fabs(z - z0) * (vf_wave_sum(near) / (VF_NEAR * z0) + 0x1p-20 * vf_wave_sum(taken));
   // The chunk in which the sum passes the target (if rounding has it pass nowhere: the last that has anything).
   const double v = (double)a.v[b];
   double target = v * rest, before = 0.0;
@@ -628,7 +629,7 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
     __syncthreads();
     if (who >= 0) token = found;
     if (way == QUICK) {
-      // (the chunks' sums, and with them the target, are off by `near` at most)
+      // (the chunks' sums, and with them the target, are off by `near` at most: 0 where there is no q)
       if (who >= 0 && (near == 0.0 || (target - found_at > 2.0 * near && found_at + found_r - target > 2.0 * near))) break;
       way = SUM, c = 0, before = 0.0, target = INFINITY, token = -1;
       continue;
