@@ -557,7 +557,8 @@ int dsa_cache_append(const dsa_append_rows* rows, int n_kinds, const int32_t* pa
  * without rows); logp fp32 [N]: log p of tokens[row] (at temperature 1 for one <= 0), 0 for -1. Rows in no sequence are not
  * written. A NaN logit is -infinity; among logits of +infinity the largest are equal and the rest impossible; a row with
  * none above -infinity takes no draft, and gives -1. u, v in [0, 1) and probs >= 0 are the caller's part.
- *   logits [N, V] bf16 or fp32, rows logits_row values apart, probs likewise; u fp32 [N], v and temperature fp32 [B].
+ *   logits [N, V] bf16 or fp32, V up to 2^30 (DSA_EUNSUPPORTED past it), rows logits_row values apart, probs likewise; u fp32
+ *   [N], v and temperature fp32 [B].
  * Tokens and counts are those of 64-bit probabilities, sums and comparisons (a probability of no more than 2^-1022 of the row's
  * largest is 0); logp is off by 2^-17 at most beside its rounding (a row's sum in 32 bits). workspace: dsa_verify_workspace_bytes(N, V, B) (no zero fill needed).
  */

@@ -35,3 +35,14 @@ def test_host_tensors_raise():
     f, i = torch.zeros(1), torch.zeros(1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_verify.verify(torch.zeros(1, 5), i, torch.tensor([0, 1], dtype=torch.int32), f, f, f)
+
+
+def test_rows_of_too_many_logits_are_refused():
+    """Past 2^30 logits a row an index would pass 2^31: nothing is launched, and there is no size of a workspace."""
+    need, call = _lib.lib().dsa_verify_workspace_bytes, _lib.lib().dsa_verify
+    for V in ((1 << 30) + 1, (1 << 31) - 2048, (1 << 31) - 1):
+        assert need(1, V, 1) == 0
+        for f32 in (0, 1):
+            st = call(P, f32, V, P, None, 0, 0, P, P, P, P, P, P, P, P, ctypes.c_size_t(1 << 40), 1, V, 1, None)
+            assert st == _lib.DSA_EUNSUPPORTED
+    assert need(1, 1 << 30, 1) > 0

@@ -29,6 +29,7 @@ namespace dsa {
 constexpr int VF_THREADS = 256;
 constexpr int VF_WAVES = VF_THREADS / WAVE;
 constexpr int VF_VEC = 8;  // logits of a load
+constexpr int VF_MAX_V = 1 << 30;
 // Bound of a row's sum's error: exponents (l - max) k with three roundings, 1.5 2^-23 of themselves, 20 at the weights' mean
 // (2^17 logits) at most: 2.5e-6; two times exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; its product with a
 // wave's weight and the part's sum in 32 bits 2^-24 each: 3.9e-6.
@@ -654,11 +655,13 @@ __global__ __launch_bounds__(VF_THREADS) void verify_pick_kernel(VerifyArgs a, c
 static int verify_loads(int V) { return V > 16 * VF_ROW_THREADS * VF_VEC ? 4 : V > 8 * VF_ROW_THREADS * VF_VEC ? 2 : 1; }
 static int verify_units(int V, int per) { return (V + per - 1) / per; }
 
+// (a row's tiles end less than 2^16 logits past it: their indices are ints)
 bool verify_grid_ok(int N, int V) {
-  return (long)N * verify_units(V, VF_CHUNK) <= 0xffffffL && (long)N * verify_units(V, VF_ROW_THREADS * VF_VEC) <= 0x3fffffL;
+  return V <= VF_MAX_V && (long)N * verify_units(V, VF_CHUNK) <= 0xffffffL && (long)N * verify_units(V, VF_ROW_THREADS * VF_VEC) <= 0x3fffffL;
 }
 
 size_t verify_workspace_bytes(int N, int V, int B) {
+  if (V > VF_MAX_V) return 0;
   const int parts = verify_units(V, VF_ROW_THREADS * VF_VEC * verify_loads(V)), chunks = verify_units(V, VF_CHUNK);
   return (size_t)B * sizeof(VerifyCount) + (size_t)N * parts * sizeof(VerifyPart) +
          (size_t)B * (chunks * sizeof(VerifyChunk) + sizeof(VerifyStop));
