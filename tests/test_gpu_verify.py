@@ -404,3 +404,42 @@ def test_targets_beside_a_tokens_edge():
                 draft_probs=probs.expand(n, V).contiguous())[0][0::2].cpu())
         got = torch.cat(tokens).numpy()
         assert (got == want).all(), (int((got != want).sum()), got[got != want], want[got != want])
+
+
+def test_long_rows():
+    """Rows past 2^25 logits, nearly all of them equal and 15 below one: their exponents are 20 in the weights' mean, as large as
+    they can be, and each rounds alike (at the temperature of 4,000 whose reciprocal rounds worst). The drafts' u are the two fp32
+    numbers on either side of p. Their sum by hand: one weight of 1 and V - 1 of e^(-15 / T)."""
+    say("verify, long rows")
+    V = (1 << 25) + 5
+    heats = np.float32(0.99) + np.arange(4000, dtype=np.float32) * np.float32(2.0 ** -20)
+    k = 1.4426950408889634 / heats.astype(np.float64)
+    heat = float(heats[np.argmax(np.abs(k.astype(np.float32) / k - 1))])
+    at = 31_234_567
+    row = torch.full((V,), -15.0, device="cuda")
+    row[at] = 0.0
+    w = math.exp(-15.0 / heat)
+    z = 1 + (V - 1) * w
+    p = 1 / z
+    below = np.float32(p)
+    if float(below) >= p:
+        below = np.nextafter(below, np.float32(0))
+    above = np.nextafter(below, np.float32(1))
+    logits = row.expand(4, V).contiguous()
+    cu = torch.tensor([0, 2, 4], dtype=torch.int32).cuda()
+    u = torch.tensor([below, 0.0, above, 0.0]).cuda()
+    v = torch.tensor([0.25, 0.75]).cuda()
+    draft = torch.full((4,), at, dtype=torch.int32).cuda()
+    tokens, accepted, logp = (t.cpu() for t in dsa_verify.verify(logits, draft, cu, u, v, torch.full((2,), heat).cuda()))
+    assert accepted.tolist() == [1, 0]
+    assert tokens[0] == at and tokens[3] == -1
+    # the second row: the first i whose running sum of weights is above 0.25 z; the third: without the draft, above 0.75
+    assert tokens[1] == math.floor(0.25 * z / w) or abs(0.25 * z / w - round(0.25 * z / w)) < 1e-6
+    # 0.75 (V - 1) is a whole number n: the running sum of the first n weights (token n - 1's end) is the target itself, and whether
+    # it is above it is a matter of the 64-bit sums' roundings. Those are below 1e-13 of the target, and a weight is 4e-8 of it:
+    # it is that token or the next.
+    n = 3 * (V - 1) // 4
+    assert 4 * n == 3 * (V - 1) and n < at
+    assert tokens[2] in (n - 1, n)
+    want = torch.tensor([math.log(p), -15.0 / heat - math.log(z), -15.0 / heat - math.log(z), 0.0], dtype=torch.float64)
+    assert ((logp.double() - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -17).all()

@@ -30,10 +30,11 @@ constexpr int VF_THREADS = 256;
 constexpr int VF_WAVES = VF_THREADS / WAVE;
 constexpr int VF_VEC = 8;  // logits of a load
 constexpr int VF_MAX_V = 1 << 30;
-// Bound of a row's sum's error: exponents (l - max) k with three roundings, 1.5 2^-23 of themselves, 20 at the weights' mean
-// (2^17 logits) at most: 2.5e-6; two times exp2 2^-23; 16 roundings of a term on its way into the sum, 1e-6; its product with a
-// wave's weight and the part's sum in 32 bits 2^-24 each: 3.9e-6.
-constexpr double VF_NEAR = 4e-6;
+// Bound of a row's sum's error: exponents (l - max) k with three roundings, 1.5 2^-23 of themselves, which are 25 in the weights'
+// mean at most (2^30 logits: their entropy less that of the largest alone; 13 for 2^17): 3.1e-6; two times exp2 2^-23; 16
+// roundings of a term on its way into the sum, 1e-6; its product with a wave's weight and the part's sum in 32 bits 2^-24 each:
+// 4.4e-6.
+constexpr double VF_NEAR = 5e-6;
 
 struct VerifyArgs {
   const void* logits;  // [N, V], rows l_row values apart, bf16 or fp32
