@@ -504,7 +504,8 @@ int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* r
  * < R of each row turns by the angle positions[axes[i]][t] * inv_freq[i], taken in 64 bits:
  *   (y0, y1) = factor * (x0 cos - x1 sin, x1 cos + x0 sin)   (inverse != 0: by the negative angle)
  * with (x0, x1) columns (2i, 2i + 1) (interleaved != 0) or (i, i + R).
- *   x, out [T, H, 2R] bf16 (x_fp32 = 0) or fp32, rows x_row and heads x_head values apart (out likewise; out may be x);
+ *   x, out [T, H, 2R] bf16 (x_fp32 = 0) or fp32, rows x_row and heads x_head values apart (out likewise, no row
+ *   over another; out may be x, with its strides);
  *   positions int32 [n_axes, T]; inv_freq fp32 [R]; axes: a host array of R axes < n_axes, or null with one axis.
  *   R <= 256, n_axes <= 4, H <= 65,536, T <= 4,194,304 (DSA_EUNSUPPORTED past them).
  */

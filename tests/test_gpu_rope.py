@@ -177,3 +177,22 @@ def test_refusals():
         dsa_rope.rotate(torch.zeros(1, 600, device="cuda"), pos[:1], freqs(300))
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_rope.rotate(x, pos.cpu(), freq)
+
+
+def test_outputs_whose_rows_overlap_are_refused():
+    """Rows 32 of 64 values apart, heads that run into the next token's; rows between each other's are taken."""
+    say("rotate overlap")
+    x, pos, freq = torch.randn(6, 3, 64, device="cuda"), torch.arange(6, dtype=torch.int32, device="cuda"), freqs(32)
+    big = torch.zeros(4096, device="cuda")
+    for strides in ((192, 32, 1), (128, 64, 1), (96, 576, 1), (0, 64, 1)):
+        if strides == (96, 576, 1):  # (apart)
+            dsa_rope.rotate(x, pos, freq, out=big.as_strided((6, 3, 64), strides))
+            assert torch.equal(big.as_strided((6, 3, 64), strides), dsa_rope.rotate(x, pos, freq))
+            continue
+        with pytest.raises(ValueError, match="no row over another"):
+            dsa_rope.rotate(x, pos, freq, out=big.as_strided((6, 3, 64), strides))
+    with pytest.raises(ValueError, match="no row over another"):
+        dsa_rope.rotate(x[:, 0], pos, freq, out=big.as_strided((6, 64), (60, 1)))
+    y = big.as_strided((1, 3, 64), (1, 64, 1))  # (one token: its stride says nothing)
+    dsa_rope.rotate(x[:1], pos[:1], freq, out=y)
+    assert torch.equal(y, dsa_rope.rotate(x[:1], pos[:1], freq))

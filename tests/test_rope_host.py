@@ -37,3 +37,19 @@ def test_axis_map():
 def test_host_tensors_raise():
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_rope.rotate(torch.zeros(2, 8), torch.zeros(2, dtype=torch.int32), torch.ones(4))
+
+
+def test_rows_of_outputs_that_overlap():
+    """Against every pair of rows; the wrapper refuses outputs whose rows share values (two workgroups would write them)."""
+    def slowly(T, H, row, head, W):
+        at = sorted(t * row + h * head for t in range(T) for h in range(H))
+        return all(b - a >= W for a, b in zip(at, at[1:]))
+
+    for T in (0, 1, 2, 3, 5):
+        for H in (1, 2, 4):
+            for row in (0, 1, 3, 4, 5, 8, 9, 12, 13, 16, 20):
+                for head in (0, 2, 4, 6, 8, 10, 12, 16, 21):
+                    for W in (2, 4):
+                        assert dsa_rope.rows_apart(T, H, row, head, W) == slowly(T, H, row, head, W), (T, H, row, head, W)
+    assert dsa_rope.rows_apart(8192, 64, 64 * 192, 192, 64) and dsa_rope.rows_apart(1 << 22, 65536, 64, 64 << 22, 64)
+    assert not dsa_rope.rows_apart(8192, 64, 63 * 64, 64, 64)

@@ -42,6 +42,23 @@ def axis_map(axes: Sequence[int] | None, positions: torch.Tensor | None, R: int,
     return C.as_i32(positions), n, axes
 
 
+def rows_apart(T: int, H: int, row: int, head: int, width: int) -> bool:
+    """Whether no two of T x H rows of `width` values, `row` and `head` values apart, share one."""
+    if row >= head * (H - 1) + width and (head >= width or H < 2):
+        return True  # (a token's heads, then the next token's)
+    (n, a), (m, b) = sorted(((T, row), (H, head)), key=lambda x: x[1] if x[0] > 1 else 0)
+    if T < 1 or (n < 2 or a >= width) and (m < 2 or b >= a * (n - 1) * (n > 1) + width):
+        return True  # (one dimension's rows within a step of the other: every ordinary layout)
+    if (n > 1 and a < width) or (m > 1 and b < width):
+        return False
+    (k, c), (l, d) = sorted(((n, a), (m, b)))  # (fewer rows first)
+    for i in range(1, k):  # i steps of it against the nearest numbers of steps of the other
+        j = min(i * c // d, l - 1)
+        if i * c - j * d < width or (j + 1 < l and (j + 1) * d - i * c < width):
+            return False
+    return True
+
+
 def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, axes: Sequence[int] | None = None,
            interleaved: bool = True, factor: float = 1.0, inverse: bool = False,
            out: torch.Tensor | None = None) -> torch.Tensor:
@@ -69,7 +86,7 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
     if xs[-1] != 1:
         x = x.contiguous()
         xs = x.stride()
-    if os[-1] != 1 or (T > 1 and os[0] == 0) or (H > 1 and os[1] == 0):
+    if os[-1] != 1 or not rows_apart(T, H, os[0], os[1] if H > 1 else 0, 2 * R):
         raise ValueError(f"dsa_rope.rotate: out with strides {os}: its columns must lie side by side, no row over another")
     st = C.call(dev, _lib.lib().dsa_rope_rotate, x.data_ptr(), x.dtype is torch.float32, xs[0], xs[1] if H > 1 else 0,
                 pos.data_ptr(), inv_freq.data_ptr(), which, out.data_ptr(), os[0], os[1] if H > 1 else 0, T, H, R, n_axes,
