@@ -71,6 +71,15 @@ def as_i32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
+def whole(t: torch.Tensor, name: str) -> torch.Tensor:
+    """Whole numbers as contiguous int32, wider ones past its ends as its ends; ValueError for other types."""
+    if t.dtype in (torch.int64, torch.uint32):
+        t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
+    elif t.dtype.is_floating_point or t.dtype.is_complex or t.dtype in (torch.bool, torch.uint64):
+        raise ValueError(f"{name}: dtype {t.dtype}, expected int32 (or int64)")
+    return as_i32(t)
+
+
 def as_f32(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float32 and t.is_contiguous() else t.float().contiguous()
 

@@ -84,7 +84,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     [Tk, H, 128] bf16; cu_q, cu_k [B + 1] int32 on the device: sequence b's queries are rows cu_q[b] .. cu_q[b + 1] - 1,
     its keys rows cu_k[b] .. . causal: query i of nq sees the first nk - nq + i + 1 of the nk keys (the last sees all);
     otherwise every key. A query that sees no key has o = 0 and lse NEG_INF; rows of q in no sequence are not written.
-    first, last [Tq] int32: a query sees only keys first <= t < last of its sequence (either may be None), besides causal:
+    first, last [Tq] int32 (or int64, values past int32's ends as these): a query sees only keys first <= t < last of its
+    sequence (either may be None), besides causal:
     documents packed into one sequence are first = the document's start; a prefix that its own tokens see both ways is last =
     max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. Only the
     tiles of 64 keys that a query tile sees are read. softcap (0, or 1e-30 to 1e30): scores become softcap tanh(s / softcap),
@@ -117,8 +118,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
         C.on_gpu(q, first, last, slopes)
         if softcap != 0.0 and not 1e-30 <= softcap <= 1e30:
             raise ValueError(f"dsa_expand: softcap {softcap}")
-        first = None if first is None else C.need(C.as_i32(first), "first", torch.int32, (Tq,))
-        last = None if last is None else C.need(C.as_i32(last), "last", torch.int32, (Tq,))
+        first = None if first is None else C.need(C.whole(first, "first"), "first", torch.int32, (Tq,))
+        last = None if last is None else C.need(C.whole(last, "last"), "last", torch.int32, (Tq,))
         slopes = None if slopes is None else C.need(C.as_f32(slopes), "slopes", torch.float32, (H,))
     lib, B = _lib.lib(), cu_q.numel() - 1
     if workspace is not None:

@@ -43,7 +43,7 @@ def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch
     (None: greedy or n-gram drafts). u [N] and v [B] fp32 in [0, 1), temperature [B] fp32 (0: the largest logit, the first
     of equals, is taken and comes next). tokens: a sequence's taken drafts, then its next token, then -1; accepted: how many
     were taken; logp: each token's log probability under the target (at temperature 1 for 0; 0 where tokens is -1). A draft
-    outside [0, V) is not taken; a row without a logit above -infinity takes none and gives -1. Rows in no sequence are not
+    outside [0, V) is not taken (draft and cu may be int64: values past int32's ends are these); a row without a logit above -infinity takes none and gives -1. Rows in no sequence are not
     written. workspace: dsa_verify_workspace_bytes(N, V, B) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
     dev = C.on_gpu(logits, draft, cu, u, v, temperature, draft_probs, workspace)
@@ -55,8 +55,8 @@ def verify(logits: torch.Tensor, draft: torch.Tensor, cu: torch.Tensor, u: torch
     if cu.dim() != 1 or cu.numel() < 1:
         raise ValueError(f"dsa_verify: cu {tuple(cu.shape)}, expected [B + 1]")
     B = cu.numel() - 1
-    cu = C.as_i32(cu)
-    draft = C.need(C.as_i32(draft), "draft", torch.int32, (N,))
+    cu = C.whole(cu, "cu")
+    draft = C.need(C.whole(draft, "draft"), "draft", torch.int32, (N,))
     u, v = C.need(u, "u", torch.float32, (N,)), C.need(v, "v", torch.float32, (B,))
     temperature = C.need(C.as_f32(temperature), "temperature", torch.float32, (B,))
     tokens, accepted = draft.new_empty(N), draft.new_empty(B)
