@@ -489,9 +489,11 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
  *   over the keys first[i] <= t < last[i] of the query's sequence, and t <= p where causal != 0.
  * (slopes[h] * |p - t| is taken off in 32 bits, by 2^-22 of itself wrong at most.)
  * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
- * document's start; a window: first = p - window + 1. Only the tiles of 64 keys that some query of a workgroup's 256 sees
- * are read. A hidden key's NaN or infinity stays hidden; a value's reaches every query of its sequence whose 32 share a tile
- * of 64 keys with it, as 0 x NaN, also queries of another document. DSA_EINVAL for another softcap.
+ * document's start; a window: first = p - window + 1. A workgroup's 256 queries (those of a sequence from its first on) read
+ * the tiles of 64 keys from the first that one of them sees to the last, and 32 of them multiply those from their own first to
+ * their own last: ranges that lie far apart within them cost what lies between. A hidden key's NaN or infinity stays hidden; a
+ * value's reaches, as 0 x NaN, every query whose 32 go through its tile, also where none of them sees it, and queries of another
+ * document. DSA_EINVAL for another softcap.
  */
 int dsa_expanded_mla_spans(const void* q_bf16, const void* k_bf16, const void* rope_bf16, const void* v_bf16,
                            const int32_t* cu_q, const int32_t* cu_k, const int32_t* first, const int32_t* last,

@@ -252,3 +252,36 @@ def test_refusals():
             dsa_expand.attend(q, k, r, v, cu, cu, 0.1, **kw)
     with pytest.raises(RuntimeError, match="GPU only"):
         dsa_expand.attend(q, k, r, v, cu, cu, 0.1, first=i.cpu())
+
+
+@pytest.mark.parametrize("cached", [0, 3000])
+@pytest.mark.parametrize("H,bias", [(2, False), (3, True)])
+def test_how_far_a_hidden_value_reaches(cached, H, bias):
+    """A value's NaN stays with the queries whose 32 go through its tile of 64 keys: every other one is as it was, bit for bit,
+    and those that see it are NaN. Ranges at random places, some empty, in blocks of 32 that lie far apart."""
+    say("spans hidden values", cached, H, bias)
+    lq, lk = [700, 65], [700 + cached, 65]
+    q, k, r, v = inputs(lq, lk, H, True, 7)
+    g = torch.Generator().manual_seed(cached + H)
+    block = torch.randint(0, lk[0], (22,), generator=g).repeat_interleave(32)[:700]
+    first = torch.cat([block + torch.randint(0, 40, (700,), generator=g), torch.zeros(65, dtype=torch.int64)])
+    last = first + torch.randint(-3, 200, (765,), generator=g)
+    last[700:] = torch.arange(1, 66)
+    a, z = first.to(torch.int32).cuda(), last.to(torch.int32).cuda()
+    kw = dict(causal=False, first=a, last=z, slopes=torch.full((H,), 0.01).cuda() if bias else None)
+    clean = dsa_expand.attend(q, k, r, v, cu_of(lq).cuda(), cu_of(lk).cuda(), 0.07, **kw)
+    lo, hi = first[:700].clamp(0, lk[0]), last[:700].clamp(max=lk[0])
+    for key in torch.randint(0, lk[0], (6,), generator=g).tolist() + [int(block[40])]:
+        w = v.clone()
+        w[key] = torch.nan
+        out, lse = dsa_expand.attend(q, k, r, w, cu_of(lq).cuda(), cu_of(lk).cuda(), 0.07, **kw)
+        reached = torch.zeros(765, dtype=torch.bool)
+        for i in range(0, 700, 32):
+            some = lo[i:i + 32] < hi[i:i + 32]
+            if some.any():
+                begin, end = int(lo[i:i + 32][some].min()) // 64 * 64, -(-int(hi[i:i + 32][some].max()) // 64) * 64
+                reached[i:min(i + 32, 700)] = begin <= key < end
+        assert torch.equal(out.cpu()[~reached], clean[0].cpu()[~reached]) and torch.equal(lse, clean[1])
+        sees = torch.zeros(765, dtype=torch.bool)
+        sees[:700] = (lo <= key) & (key < hi)
+        assert out.cpu()[sees].isnan().all()

@@ -87,10 +87,12 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     first, last [Tq] int32 (or int64, values past int32's ends as these): a query sees only keys first <= t < last of its
     sequence (either may be None), besides causal:
     documents packed into one sequence are first = the document's start; a prefix that its own tokens see both ways is last =
-    max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. Only the
-    tiles of 64 keys that a query tile sees are read. softcap (0, or 1e-30 to 1e30): scores become softcap tanh(s / softcap),
-    off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits, off by 2^-22 of itself at
-    most). A value's NaN or infinity may reach queries that do not see it (0 x NaN), a key's does not.
+    max(p + 1, prefix) with causal False (p = nk - nq + i, the query's place); a window is first = p - window + 1. 256 queries
+    (a sequence's, from its first on) read the keys from the first that one of them sees to the last, in tiles of 64, and 32 of
+    them multiply theirs: ranges far apart within them cost what lies between. softcap (0, or 1e-30 to 1e30): scores become
+    softcap tanh(s / softcap), off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits,
+    off by 2^-22 of itself at most). A value's NaN or infinity may reach queries
+    that do not see it (0 x NaN: all of the 32 that go through its tile), a key's does not.
     workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
     dev = C.on_gpu(q, k, k_rope, v, cu_q, cu_k, out, workspace)
