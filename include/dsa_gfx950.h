@@ -487,7 +487,8 @@ int dsa_expanded_mla(const void* q_bf16, const void* k_bf16, const void* rope_bf
  * null, softcap 0 (none) or 1e-30 to 1e30 (its scores are off by softcap 2^-20 at most):
  *   z[t] = scale * (q . k[t]),  z = softcap * tanh(z / softcap),  z -= slopes[h] * |p - t|,
  *   over the keys first[i] <= t < last[i] of the query's sequence, and t <= p where causal != 0.
- * (slopes[h] * |p - t| is taken off in 32 bits, by 2^-22 of itself wrong at most.)
+ * (slopes[h] * |p - t| is taken off in 32 bits, wrong by slopes[h] * (|p - t| + 64) * 2^-22 at most beside the score's rounding
+ * and the running maximum's.)
  * A prefix seen both ways: causal = 0, last = max(p + 1, prefix); documents in one sequence: causal = 1, first = the
  * document's start; a window: first = p - window + 1. A workgroup's 256 queries (those of a sequence from its first on) read
  * the tiles of 64 keys from the first that one of them sees to the last, and 32 of them multiply those from their own first to

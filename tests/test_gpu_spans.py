@@ -285,3 +285,16 @@ def test_how_far_a_hidden_value_reaches(cached, H, bias):
         sees = torch.zeros(765, dtype=torch.bool)
         sees[:700] = (lo <= key) & (key < hi)
         assert out.cpu()[sees].isnan().all()
+
+
+@pytest.mark.parametrize("rope", [True, False])
+@pytest.mark.parametrize("lq,lk,H", [([700], [1400], 4), ([300, 1, 0, 257], [300, 65, 4, 600], 3), ([20], [9000], 2)])
+def test_steep_distances(lq, lk, H, rope):
+    """Slopes of up to 16 a token, at which a bias is off by more than 2^-22 of itself: by slope (|p - t| + 64) 2^-22 at most."""
+    say("spans steep", len(lq), sum(lq), sum(lk), H, rope)
+    q, k, r, v = inputs(lq, lk, H, rope, H + 5)
+    for slopes in (torch.linspace(2.0, 16.0, H).cuda(), torch.linspace(-0.5, -4.0, H).cuda()):
+        for cap in (0.0, 30.0):
+            out, lse = dsa_expand.attend(q, k, r, v, cu_of(lq).cuda(), cu_of(lk).cuda(), 192 ** -0.5, softcap=cap, slopes=slopes,
+                                         out_dtype=torch.float32)
+            compare(out, lse, reference(q, k, r, v, lq, lk, 192 ** -0.5, True, None, None, cap, slopes))

@@ -499,8 +499,8 @@ __global__ __launch_bounds__(XA_THREADS, 1) void expanded_attend_kernel(
             for (int r = 0; r < 16; ++r)
               s2[x][r] = fmaf(-slope2, fabsf(from - (float)(32 * x + 8 * (r >> 2) + (r & 3))), s2[x][r]);
       } else if (MORE == 2 && more.slopes && (i + 1) * XA_K - 1 <= nk - nq + w0) {
-        // No key of the tile is behind a query of the wave: slope (p - t) is the tile's own, as large as its weights are
-        // small, less slope times the key's place in it (8,192 tokens, 32 heads: 692 us for 702 then).
+        // No key of the tile is behind a query of the wave: slope (p - t) is the tile's own, less slope times the key's place in
+        // it: off by up to 64 slopes' roundings more than of |p - t| alone (8,192 tokens, 32 heads: 692 us for 702 then).
         const float base = fmaf(-slope2, from, -m_run);
 #pragma unroll
         for (int x = 0; x < 2; ++x)

@@ -91,7 +91,7 @@ def attend(q: torch.Tensor, k: torch.Tensor, k_rope: torch.Tensor | None, v: tor
     (a sequence's, from its first on) read the keys from the first that one of them sees to the last, in tiles of 64, and 32 of
     them multiply theirs: ranges far apart within them cost what lies between. softcap (0, or 1e-30 to 1e30): scores become
     softcap tanh(s / softcap), off by softcap 2^-20 at most. slopes [H] fp32: slopes[h] |p - t| is taken off them (in 32 bits,
-    off by 2^-22 of itself at most). A value's NaN or infinity may reach queries
+    off by slopes[h] (|p - t| + 64) 2^-22 at most beside the score's own rounding). A value's NaN or infinity may reach queries
     that do not see it (0 x NaN: all of the 32 that go through its tile), a key's does not.
     workspace: dsa_expanded_workspace_bytes(B, Tq, Tk, H) bytes, or None for one kept per stream and host thread (a
     captured graph has its own)."""
