@@ -5,7 +5,7 @@ import torch
 
 from tests._helpers import say
 from trnrt_amd.kernels import _common as C
-from trnrt_amd.kernels import dsa_expand, dsa_verify
+from trnrt_amd.kernels import dsa_cache, dsa_expand, dsa_verify
 
 
 def test_whole():
@@ -60,3 +60,19 @@ def test_drafts_and_ends():
         dsa_verify.verify(logits, torch.tensor([5.0, 0.0]).cuda(), cu, *args)
     with pytest.raises(ValueError, match="dtype"):
         dsa_verify.verify(logits, torch.tensor([5, 0]).cuda(), cu.float(), *args)
+
+
+@pytest.mark.gpu
+def test_pages_and_lengths():
+    """A page or a length of 2^32 + 1 is outside the pool or the table (and not page 1 or a length of 1): nothing is written."""
+    say("int64 pages")
+    x = torch.ones(1, 64, device="cuda")
+    for page, n, written in ((1, 1, True), (2 ** 32 + 1, 1, False), (1 - 2 ** 32, 1, False), (1, 2 ** 32 + 1, False),
+                             (1, -2 ** 32 + 1, False)):
+        cache = torch.zeros(32, 64, dtype=torch.bfloat16, device="cuda")
+        table, ctx = torch.tensor([[page, 0]]).cuda(), torch.tensor([n]).cuda()
+        dsa_cache.append(dsa_cache.Rows(x, cache), table, ctx, 16, cu_new=torch.tensor([0, 1]).cuda())
+        assert bool((cache[16] == 1).all()) == written and (cache.sum() == 64 * written).all()
+    for kw in (dict(table=table.float()), dict(ctx_len=ctx.float()), dict(cu_new=torch.tensor([0.0, 1.0]).cuda())):
+        with pytest.raises(ValueError, match="dtype"):
+            dsa_cache.append(dsa_cache.Rows(x, cache), **{**dict(table=table, ctx_len=ctx, page_size=16), **kw})

@@ -73,6 +73,8 @@ def as_i32(t: torch.Tensor) -> torch.Tensor:
 
 def whole(t: torch.Tensor, name: str) -> torch.Tensor:
     """Whole numbers as contiguous int32, wider ones past its ends as its ends; ValueError for other types."""
+    if t.dtype is torch.int32:
+        return as_i32(t)
     if t.dtype in (torch.int64, torch.uint32):
         t = t.to(torch.int64).clamp(-(1 << 31), (1 << 31) - 1)
     elif t.dtype.is_floating_point or t.dtype.is_complex or t.dtype in (torch.bool, torch.uint64):

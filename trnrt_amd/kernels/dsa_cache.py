@@ -116,7 +116,8 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
     by positions ([T], or [axes, T] with axes, as in dsa_rope.rotate; None: the token's place in its sequence) x inv_freq
     [R] fp32 x factor (without inv_freq no kind is rotated, and positions and axes are not used). Everything is in fp32 and
     rounded once, as store rounds. A token whose place is outside the table, or whose page is the null page or outside the
-    pool, is not written, nor are rows in no sequence. No two tokens of a call may have one slot."""
+    pool, is not written, nor are rows in no sequence. No two tokens of a call may have one slot. (table, ctx_len and cu_new
+    may be int64: values past int32's ends are these.)"""
     rows = (rows,) if isinstance(rows, Rows) else rows
     if not rows:
         raise ValueError("dsa_cache.append: no rows")
@@ -124,8 +125,8 @@ def append(rows: Rows | Sequence[Rows], table: torch.Tensor, ctx_len: torch.Tens
     if table.dim() != 2 or table.shape[1] < 1 or page_size < 1:
         raise ValueError(f"dsa_cache.append: table {tuple(table.shape)} with pages of {page_size}")
     B, max_pages = table.shape
-    tb, lens = C.as_i32(table), C.need(C.as_i32(ctx_len), "ctx_len", torch.int32, (B,))
-    cu = None if cu_new is None else C.need(C.as_i32(cu_new), "cu_new", torch.int32, (B + 1,))
+    tb, lens = C.whole(table, "table"), C.need(C.whole(ctx_len, "ctx_len"), "ctx_len", torch.int32, (B,))
+    cu = None if cu_new is None else C.need(C.whole(cu_new, "cu_new"), "cu_new", torch.int32, (B + 1,))
     R = 0
     if inv_freq is not None:
         R = C.need(inv_freq, "inv_freq", torch.float32, (None,)).shape[0]

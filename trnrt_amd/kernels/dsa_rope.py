@@ -63,10 +63,10 @@ def rotate(x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, *, 
            interleaved: bool = True, factor: float = 1.0, inverse: bool = False,
            out: torch.Tensor | None = None) -> torch.Tensor:
     """x [T, H, 2R] or [T, 2R] (bf16 or fp32; a view of the rope columns of wider rows will do) rotated by positions [T], or
-    [axes, T] with axes the axis of each of the R frequencies inv_freq [R] fp32; positions int32. interleaved: the pairs are
-    columns (2i, 2i + 1), else (i, i + R). factor multiplies the result; inverse turns back (with factor, that is the
-    gradient of rotate). out: a tensor or view of x's shape and type to write, x itself for a rotation in place (no other
-    overlap); None for a new one."""
+    [axes, T] with axes the axis of each of the R frequencies inv_freq [R] fp32; positions int32 (int64 ones within its
+    range). interleaved: the pairs are columns (2i, 2i + 1), else (i, i + R). factor multiplies the result; inverse turns back
+    (with factor, that is the gradient of rotate). out: a tensor or view of x's shape and type to write, x itself for a
+    rotation in place (no other overlap); None for a new one."""
     dev = C.on_gpu(x, positions, inv_freq, out)
     if x.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError(f"dsa_rope.rotate: x of {x.dtype}, expected bfloat16 or float32")
