@@ -18,6 +18,7 @@ token's pool key, a softmax-gated mean of the pool's cached indexer keys, into t
 
 from __future__ import annotations
 
+import ctypes
 import struct
 from collections.abc import Sequence
 
@@ -27,7 +28,8 @@ from .. import _lib
 from . import _common as C
 from .dsa_rope import axis_map
 
-_KIND = struct.Struct("PqPPPP7i2f4x")  # dsa_append_rows
+_FORMAT = "".join(t._type_ for _, t in _lib.AppendRows._fields_)  # (packed in 0.4 us, where ctypes fills one in 1.3)
+_KIND = struct.Struct(f"{_FORMAT}{ctypes.sizeof(_lib.AppendRows) - struct.calcsize(_FORMAT)}x")
 _SIZES = {torch.bfloat16: 2, torch.float32: 4}
 FP8_MAX = 448.0  # the e4m3fn maximum (trnrt/engine/model_runner.py:62-70 off Neuron)
 
