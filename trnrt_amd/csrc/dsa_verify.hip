@@ -18,10 +18,12 @@
 // alike, 8 lanes a row (in large batches verify_stop_kernel has found them), and sums a chunk of that; the last of them to be
 // done (a count that the first launch cleared) looks for the token.
 //
-// The first launch is bound by the logits' bytes, the others by their chains of dependent reads (lengths, parts, the draft's
-// logit, a chunk, the count, the sums, the chunk again) and by 64-bit operations, 30 a logit of the stop row. 64 sequences of
-// 5 rows of 131,072 logits (bf16) 46 us: 22 (3.8 TB/s) + 5 + 20; 13 ragged ones of up to 8 rows of 100,003 (fp32) 17.8: 7.2 +
-// 11.5; one of 4 rows of 32,768 14: 3.3 + 9.4.
+// The first launch is bound by the logits' bytes, where a wave's logits are not all masked (its sum is then NaN, and it goes
+// through them twice more: with all but 50 of 131,072 at -infinity 56 us for 22). The others are bound by their chains of
+// dependent reads (lengths, parts, the draft's logit, a chunk, the count, the sums, the chunk again) in short workgroups; vector
+// instructions, a good part of them the stop row's 30 64-bit operations a logit, issue in half of the pick's time. 64 sequences
+// of 5 rows of 131,072 logits (bf16) 45 to 46 us: 22 (3.8 TB/s) + 5 + 20; 13 ragged ones of up to 8 rows of 100,003 (fp32) 17.9
+// to 18.4: 7.2 to 8.3 + 11.8; one of 4 rows of 32,768 13.7 to 14.8: 3.3 + 9.5.
 #include "dsa_async.h"
 
 namespace dsa {
@@ -197,7 +199,8 @@ constexpr int VF_ROW_THREADS = 1024;
 constexpr int VF_ROW_WAVES = VF_ROW_THREADS / WAVE;
 
 // A workgroup's part of a row: LOADS x 8,192 logits, a wave's side by side. Not even a comparison is spent on NaN or
-// infinities: they make a wave's sum NaN, and its logits are then gone through again with care.
+// infinities: they (and a wave whose logits are all -infinity) make a wave's sum NaN, and its logits are then gone through again
+// with care.
 template <typename T, int LOADS>
 __global__ __launch_bounds__(VF_ROW_THREADS) void verify_rows_kernel(VerifyArgs a, VerifyPart* __restrict__ parts,
                                                                      VerifyCount* __restrict__ done) {
